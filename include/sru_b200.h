@@ -309,6 +309,48 @@ int sru_b200_layer_norm_backward(
     int64_t rows, int64_t n, int x_dtype, int y_dtype,
     void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * Gated linear recurrence: the SRU's state update with a forget gate that does not look at the state (weight_c = 0,
+ * the `v1` gates of sru/modules.py:211-215), so that time can be scanned in parallel:
+ *
+ *   f_t = sigmoid(g_t + bias),  c_t = f_t c_{t-1} + (1 - f_t) x_t,  h_t = c_t
+ *
+ *   u        (L, B, d, 2) pairs (x, g), gate index innermost (the SRU's U with k = 2); SRU_F32, SRU_F16 or SRU_BF16.
+ *            Strides of L and B are given in elements (even; the pairs themselves contiguous and aligned to their size)
+ *   h        out (L, B, d) contiguous, u's type; 0 at padded positions
+ *   c_last   out float (B, d), may be NULL;  c_init  float (B, d) or NULL (zeros);  bias  float[d] or NULL
+ *   states   out, ..._states_bytes() bytes, for the backward pass; may be NULL (inference)
+ *   mask_pad (L, B) bytes or NULL, non-zero = padded: the state passes through, u is not looked at there
+ *   reverse  non-zero: time runs from L-1 down to 0
+ * The reference has no such operator; with SRU_F64 the call gives SRU_ERR_UNSUPPORTED.
+ */
+size_t sru_b200_linear_recurrence_states_bytes(int64_t length, int64_t batch, int64_t hidden);
+
+int sru_b200_linear_recurrence_forward(
+    void *h, float *c_last, void *states, const void *u, const float *bias, const float *c_init,
+    const uint8_t *mask_pad, int64_t length, int64_t batch, int64_t hidden,
+    int64_t u_stride_t, int64_t u_stride_b, int reverse, int dtype, void *stream);
+
+/* Scratch of the backward pass (partial sums of grad_bias); needed only with a grad_bias. */
+size_t sru_b200_linear_recurrence_backward_workspace_bytes(int64_t length, int64_t batch, int64_t hidden);
+
+/*
+ * Backward of the above.  With dc_t the whole gradient of c_t (dc_t = grad_h_t + f_{t+1} dc_{t+1}, grad_last added at
+ * the last step):  dx_t = (1 - f_t) dc_t,  dg_t = dc_t (c_{t-1} - x_t) f_t (1 - f_t);  both 0 at padded positions.
+ *
+ *   grad_u     out (L, B, d, 2) contiguous, u's type
+ *   grad_bias  out float[d] or NULL: dg summed over L and B in a fixed order (no atomics)
+ *   grad_init  out float (B, d) or NULL
+ *   u, bias, mask_pad, sizes, strides, reverse   as in the forward call;  states   what it left
+ *   grad_h     (L, B, d) in u's type with the given strides, or NULL (zeros);  grad_last  float (B, d) or NULL (zeros)
+ */
+int sru_b200_linear_recurrence_backward(
+    void *grad_u, float *grad_bias, float *grad_init, const void *u, const float *bias, const void *states,
+    const uint8_t *mask_pad, const void *grad_h, const float *grad_last,
+    int64_t length, int64_t batch, int64_t hidden, int64_t u_stride_t, int64_t u_stride_b,
+    int64_t gh_stride_t, int64_t gh_stride_b, int reverse, int dtype,
+    void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

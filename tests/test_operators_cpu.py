@@ -1,0 +1,37 @@
+"""Refusals of the operators around the recurrent layers, without a GPU: bad arguments end as errors on the host."""
+import ctypes
+
+import pytest
+import torch
+
+from sru_b200 import _lib
+
+
+def last_error():
+    return _lib.lib().sru_b200_last_error().decode()
+
+
+def test_linear_recurrence_refuses_cpu_tensors():
+    from sru_b200 import gated_linear_recurrence
+    with pytest.raises(_lib.SruB200Error, match="no CPU path"):
+        gated_linear_recurrence(torch.zeros(2, 1, 8))
+
+
+def test_linear_recurrence_c_arguments():
+    L = _lib.lib()
+    one = ctypes.c_void_p(16)      # never dereferenced: every call below is refused on the host
+    f = L.sru_b200_linear_recurrence_forward
+    assert f(None, None, None, None, None, None, None, 4, 2, 8, 32, 16, 0, _lib.SRU_F32, None) == -1
+    assert "must not be null" in last_error()
+    assert f(one, None, None, one, None, None, None, -1, 2, 8, 32, 16, 0, _lib.SRU_F32, None) == -1
+    assert f(one, None, None, one, None, None, None, 4, 2, 0, 32, 16, 0, _lib.SRU_F32, None) == -1
+    assert f(one, None, None, one, None, None, None, 4, 2, 8, 32, 16, 0, _lib.SRU_F64, None) == -2
+    assert f(one, None, None, one, None, None, None, 4, 2, 8, 31, 16, 0, _lib.SRU_F32, None) == -1
+    assert "aligned" in last_error()
+    assert f(one, None, None, ctypes.c_void_p(18), None, None, None, 4, 2, 8, 32, 16, 0, _lib.SRU_BF16, None) == -1
+    assert f(one, None, None, one, None, None, None, 0, 2, 8, 32, 16, 0, _lib.SRU_F32, None) == 0      # nothing to do
+    g = L.sru_b200_linear_recurrence_backward
+    assert g(one, None, None, one, None, None, None, None, None, 4, 2, 8, 32, 16, 16, 8, 0, 0, None, 0, None) == -1
+    assert g(one, one, None, one, one, one, None, None, None, 4, 2, 8, 32, 16, 16, 8, 0, 0, None, 0, None) == -3
+    assert L.sru_b200_linear_recurrence_states_bytes(17, 3, 5) == 2 * 3 * 5 * 4
+    assert L.sru_b200_linear_recurrence_states_bytes(0, 3, 5) == 0
