@@ -55,8 +55,8 @@ const char *sru_b200_last_error(void);
 
 /*
  * Synchronises `stream` and returns SRU_ERR_DEVICE if any kernel since the last
- * call gave up a bounded wait (an mbarrier that never completed); the flag is
- * cleared.  Kernels never spin without a limit, so a lost copy shows up here as
+ * call gave up a bounded wait (an mbarrier that never completed) or met a token
+ * outside its table (sru_b200_embedding_*); the flag is cleared.  Kernels never spin without a limit, so a lost copy shows up here as
  * an error code instead of a hang.
  */
 int sru_b200_check_device_error(void *stream);
@@ -349,6 +349,33 @@ int sru_b200_linear_recurrence_backward(
     const uint8_t *mask_pad, const void *grad_h, const float *grad_last,
     int64_t length, int64_t batch, int64_t hidden, int64_t u_stride_t, int64_t u_stride_b,
     int64_t gh_stride_t, int64_t gh_stride_b, int reverse, int dtype,
+    void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Scaled lookup in a table of token vectors: y[i, :] = scale * table[tokens[i], :] for n tokens.  The reference reads
+ * its tokens through the framework's embedding (language_model/train_enwik8.py:56-62); here the scale and the
+ * conversion to the type of the first projection happen on the way.
+ *   tokens      n integers of token_bytes (4 or 8) bytes
+ *   table       (vocabulary, hidden), rows table_stride elements apart; SRU_F32, SRU_F16 or SRU_BF16
+ *   y           (n, hidden) contiguous, in the table's type, or SRU_F16 / SRU_BF16 over an SRU_F32 table
+ * A token outside the table reads nothing, gives a row of zeros and raises the device error flag.
+ */
+int sru_b200_embedding_forward(
+    void *y, const void *tokens, const void *table, int64_t n, int64_t vocabulary, int64_t hidden,
+    int64_t table_stride, double scale, int token_bytes, int table_dtype, int y_dtype, void *stream);
+
+/* Scratch of the gradient: the sorted (token, position) pairs twice, and partial rows of runs that cross tiles. */
+size_t sru_b200_embedding_backward_workspace_bytes(int64_t n, int64_t vocabulary, int64_t hidden);
+
+/*
+ * grad_table[v, :] = scale * sum over {i : tokens[i] = v} of grad_y[i, :], every row written (0 where v does not occur
+ * or is padding_idx; padding_idx < 0: none).  Sums are float32 in the order of the positions, without atomics:
+ * repeated calls give identical bits.  grad_table (vocabulary, hidden) contiguous in the table's type, grad_y
+ * (n, hidden) contiguous in y's type, workspace 16-byte aligned.
+ */
+int sru_b200_embedding_backward(
+    void *grad_table, const void *tokens, const void *grad_y, int64_t n, int64_t vocabulary, int64_t hidden,
+    int64_t padding_idx, double scale, int token_bytes, int table_dtype, int y_dtype,
     void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus

@@ -6,10 +6,11 @@ reference's constructor arguments, call signature and ``state_dict`` layout; the
 of ``include/sru_b200.h`` (``sru_b200/lib/libsru_b200.so``); there is no CPU or PyTorch fallback.
 """
 from . import _lib
+from .embedding import embedding_lookup
 from .linear_recurrence import gated_linear_recurrence
 from .ops import (ElementwiseRecurrence, elementwise_recurrence_forward, elementwise_recurrence_gpu,
                   get_amp_mode, set_amp_mode, set_c_hist_dtype)
 
 __version__ = "0.1.0"
 __all__ = ["ElementwiseRecurrence", "elementwise_recurrence_forward", "elementwise_recurrence_gpu",
-           "gated_linear_recurrence", "set_amp_mode", "get_amp_mode", "set_c_hist_dtype"]
+           "embedding_lookup", "gated_linear_recurrence", "set_amp_mode", "get_amp_mode", "set_c_hist_dtype"]

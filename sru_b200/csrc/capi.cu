@@ -142,6 +142,7 @@ int sru_b200_check_device_error(void *stream) {
     if (v != 0) {
         SRUB_CUDA_CHECK(cudaMemsetAsync(flag, 0, sizeof(int), st));
         SRUB_CUDA_CHECK(cudaStreamSynchronize(st));
+        if (v == kSiteToken) return set_error(SRU_ERR_DEVICE, "a token is outside its embedding table");
         return set_error(SRU_ERR_DEVICE, "a kernel gave up a bounded wait (site %d)", v);
     }
     return 0;

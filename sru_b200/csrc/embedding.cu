@@ -1,0 +1,422 @@
+// Scaled lookup in a table of token vectors, and its gradient.
+//
+//   forward    y[n, :] = scale * W[token_n, :]
+//   backward   dW[v, :] = scale * sum over {n : token_n = v} of dy[n, :],   0 for tokens that do not occur
+//
+// Both are bound by HBM: the rows read and written, and for the gradient the dense dW.
+//
+// The gradient is formed by sorted tokens, so that it needs no floating-point atomics and repeated calls give identical
+// bits: a stable radix sort of (token, position) by one cluster of eight CTAs, then sums over tiles of kTile sorted
+// positions.  Token frequencies are uneven (one word may be a twentieth of all positions), so the unit of work is a
+// tile of positions, not a token: a run of equal tokens inside a tile goes straight to dW; a run that crosses tiles
+// leaves one float32 partial row per tile, and a last kernel adds those up in order.
+//
+// A token outside the table reads nothing: its row of y is zero, it adds nothing to the gradient, and the device error
+// flag is raised (sru_b200_check_device_error).
+#include <algorithm>
+#include <cstring>
+
+#include "common.cuh"
+
+namespace srub {
+
+namespace {
+
+constexpr int kSortCtas = 8, kSortWarps = 32, kBins = 256;
+constexpr int kTile = 32;             // sorted positions per tile: one per lane of the warp that reads their keys
+
+struct EmbArgs {
+    const void *tokens, *src;         // src: table (forward) or dy (backward)
+    void *dst;                        // y (forward) or dW (backward)
+    float *part;                      // backward: (tiles, 2, d): sums of a tile's first and last run where they cross it
+    uint2 *sorted, *spare;            // (token, position)
+    int64_t n, v, ld;
+    int64_t padding;
+    int d;
+    int passes;
+    float scale;
+    int *err;
+};
+
+template <typename TK> __device__ __forceinline__ int64_t token_at(const void *tokens, int64_t i) {
+    return static_cast<int64_t>(static_cast<const TK *>(tokens)[i]);
+}
+
+// ---- forward ----------------------------------------------------------------------------------------------------
+// One warp per (row, block of 32 * VEC * REP columns): REP loads of VEC elements per lane in flight.
+template <typename TK, typename TI, typename TO, int VEC, int REP>
+__global__ void __launch_bounds__(256) embedding_fwd_kernel(const EmbArgs a, int blocks_per_row) {
+    const int lane = threadIdx.x & 31;
+    const int64_t units = a.n * blocks_per_row, step = (int64_t)gridDim.x * 8;
+    for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < units; w += step) {
+        const int64_t row = w / blocks_per_row;
+        const int c0 = (int)(w - row * blocks_per_row) * (32 * VEC * REP) + lane * VEC;
+        const int64_t t = token_at<TK>(a.tokens, row);
+        const bool ok = t >= 0 && t < a.v;
+        const TI *src = static_cast<const TI *>(a.src) + (ok ? t : 0) * a.ld;
+        TO *dst = static_cast<TO *>(a.dst) + row * a.d;
+        Pack<TI, VEC> in[REP];
+#pragma unroll
+        for (int r = 0; r < REP; ++r) {
+            const int c = c0 + r * 32 * VEC;
+            if (ok && c < a.d) in[r] = *reinterpret_cast<const Pack<TI, VEC> *>(src + c);
+            else memset(&in[r], 0, sizeof(in[r]));
+        }
+#pragma unroll
+        for (int r = 0; r < REP; ++r) {
+            const int c = c0 + r * 32 * VEC;
+            Pack<TO, VEC> out;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) out.v[k] = Cvt<TO>::from_f(Cvt<TI>::to_f(in[r].v[k]) * a.scale);
+            if (c < a.d) *reinterpret_cast<Pack<TO, VEC> *>(dst + c) = out;
+        }
+        if (!ok && lane == 0) atomicExch(a.err, kSiteToken);
+    }
+}
+
+// ---- sort -------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t rank, uint32_t v) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
+}
+
+// Key of position i: the token, or v (behind all tokens) where the position adds nothing to the gradient.
+template <typename TK> __device__ __forceinline__ uint32_t key_at(const EmbArgs &a, int64_t i) {
+    const int64_t t = token_at<TK>(a.tokens, i);
+    if (t < 0 || t >= a.v) { atomicExch(a.err, kSiteToken); return (uint32_t)a.v; }
+    return (uint32_t)(t == a.padding ? a.v : t);
+}
+
+// Stable radix sort, 8 bits a pass, by ONE cluster: every warp owns a contiguous part of the positions and a histogram of
+// its own; counts become starting offsets by a prefix over (digit, CTA, warp), the CTAs' totals travelling through
+// distributed shared memory; then every warp writes its entries in order.  Counts are integers: no order matters.
+template <typename TK>
+__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortWarps * 32)
+embedding_sort_kernel(const EmbArgs a) {
+    __shared__ uint32_t hist[kSortWarps][kBins];
+    __shared__ uint32_t totals[kSortCtas][kBins];
+    __shared__ uint32_t offs[kBins];
+    __shared__ uint32_t warp_sum[8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int64_t per = ((a.n + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps) + 31) / 32 * 32;
+    const int64_t i0 = min(a.n, ((int64_t)rank * kSortWarps + warp) * per), i1 = min(a.n, i0 + per);
+
+    for (int pass = 0; pass < a.passes; ++pass) {
+        const int shift = 8 * pass;
+        // the last pass ends in a.sorted
+        uint2 *out = ((a.passes - pass) & 1) ? a.sorted : a.spare;
+        const uint2 *in = ((a.passes - pass) & 1) ? a.spare : a.sorted;
+        auto entry = [&](int64_t i) -> uint2 {
+            if (pass == 0) return make_uint2(key_at<TK>(a, i), (uint32_t)i);
+            return __ldcg(in + i);         // written by other SMs of the cluster: past L1
+        };
+        for (int k = lane; k < kBins; k += 32) hist[warp][k] = 0;
+        __syncwarp();
+        for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&hist[warp][(entry(i).x >> shift) & 255u], 1u);
+        __syncthreads();
+        if (threadIdx.x < kBins) {
+            uint32_t s = 0;
+#pragma unroll 8
+            for (int w = 0; w < kSortWarps; ++w) {
+                const uint32_t c = hist[w][threadIdx.x];
+                hist[w][threadIdx.x] = s;
+                s += c;
+            }
+            for (uint32_t r = 0; r < kSortCtas; ++r) store_cluster(smem_u32(&totals[rank][threadIdx.x]), r, s);
+        }
+        cluster_barrier();
+        uint32_t all = 0, below = 0, incl = 0;
+        if (threadIdx.x < kBins) {
+#pragma unroll
+            for (uint32_t r = 0; r < kSortCtas; ++r) {
+                const uint32_t c = totals[r][threadIdx.x];
+                below += r < rank ? c : 0u;
+                all += c;
+            }
+            incl = all;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += x;
+            }
+            if (lane == 31) warp_sum[warp] = incl;
+        }
+        __syncthreads();
+        if (threadIdx.x < kBins) {
+            uint32_t base = incl - all;
+            for (int w = 0; w < warp; ++w) base += warp_sum[w];
+            offs[threadIdx.x] = base + below;
+        }
+        __syncthreads();
+        for (int64_t i = i0; i < i1; i += 32) {
+            const bool on = i + lane < i1;
+            const uint2 e = on ? entry(i + lane) : make_uint2(0u, 0u);
+            const uint32_t digit = (e.x >> shift) & 255u;
+            const unsigned same = __match_any_sync(0xffffffffu, on ? digit : 256u + lane);
+            const uint32_t at = on ? hist[warp][digit] : 0u;
+            __syncwarp();
+            if (on) {
+                if ((same >> lane) == 1u) hist[warp][digit] = at + __popc(same);     // the last lane with this digit
+                out[offs[digit] + at + __popc(same & ((1u << lane) - 1u))] = e;
+            }
+            __syncwarp();
+        }
+        __threadfence();
+        cluster_barrier();
+    }
+}
+
+// ---- sums over sorted positions ---------------------------------------------------------------------------------
+// Columns of this lane: c0 + r * 32 * VEC + k, r < REP, k < VEC.
+template <typename TO, int VEC, int REP>
+__device__ __forceinline__ void store_sum(TO *row, int c0, int d, const float (&acc)[REP][VEC], float scale) {
+#pragma unroll
+    for (int r = 0; r < REP; ++r) {
+        const int c = c0 + r * 32 * VEC;
+        if (c >= d) continue;
+        Pack<TO, VEC> o;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) o.v[k] = Cvt<TO>::from_f(acc[r][k] * scale);
+        *reinterpret_cast<Pack<TO, VEC> *>(row + c) = o;
+    }
+}
+
+template <typename TI, typename TO, int VEC, int REP>
+__global__ void __launch_bounds__(128) embedding_sum_kernel(const EmbArgs a, int blocks_per_row) {
+    const int lane = threadIdx.x & 31;
+    const int64_t tiles = (a.n + kTile - 1) / kTile, units = tiles * blocks_per_row, step = (int64_t)gridDim.x * 4;
+    for (int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); w < units; w += step) {
+        const int64_t tile = w / blocks_per_row, i0 = tile * kTile;
+        const int c0 = (int)(w - tile * blocks_per_row) * (32 * VEC * REP) + lane * VEC;
+        const uint32_t none = (uint32_t)a.v;                // key of positions that add nothing
+        const uint2 mine = (i0 + lane < a.n) ? a.sorted[i0 + lane] : make_uint2(none, 0u);
+        const uint32_t before = i0 > 0 ? a.sorted[i0 - 1].x : none;
+        const uint32_t after = i0 + kTile < a.n ? a.sorted[i0 + kTile].x : none;
+        if (__shfl_sync(0xffffffffu, mine.x, 0) == none) continue;      // sorted: nothing follows
+        float acc[REP][VEC];
+#pragma unroll
+        for (int r = 0; r < REP; ++r)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc[r][k] = 0.0f;
+        bool whole_head = true;                             // the current run reaches back to the tile's first entry
+        constexpr int G = 4;                                // rows requested together
+        for (int e0 = 0; e0 < kTile; e0 += G) {
+            Pack<TI, VEC> in[G][REP];
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const uint32_t key = __shfl_sync(0xffffffffu, mine.x, e0 + g), pos = __shfl_sync(0xffffffffu, mine.y, e0 + g);
+                const TI *row = static_cast<const TI *>(a.src) + (int64_t)pos * a.d;
+#pragma unroll
+                for (int r = 0; r < REP; ++r) {
+                    const int c = c0 + r * 32 * VEC;
+                    if (key != none && c < a.d) in[g][r] = *reinterpret_cast<const Pack<TI, VEC> *>(row + c);
+                    else memset(&in[g][r], 0, sizeof(in[g][r]));
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int e = e0 + g;
+                const uint32_t key = __shfl_sync(0xffffffffu, mine.x, e);
+                const uint32_t next = e + 1 < kTile ? __shfl_sync(0xffffffffu, mine.x, e + 1 & 31) : after;
+#pragma unroll
+                for (int r = 0; r < REP; ++r)
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) acc[r][k] += Cvt<TI>::to_f(in[g][r].v[k]);
+                if (key == none) continue;
+                const bool crosses_in = whole_head && key == before;
+                if (next != key || e == kTile - 1) {
+                    if (crosses_in)
+                        store_sum<float, VEC, REP>(a.part + (tile * 2) * a.d, c0, a.d, acc, 1.0f);
+                    else if (next == key)
+                        store_sum<float, VEC, REP>(a.part + (tile * 2 + 1) * a.d, c0, a.d, acc, 1.0f);
+                    else
+                        store_sum<TO, VEC, REP>(static_cast<TO *>(a.dst) + (int64_t)key * a.d, c0, a.d, acc, a.scale);
+#pragma unroll
+                    for (int r = 0; r < REP; ++r)
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) acc[r][k] = 0.0f;
+                    whole_head = false;
+                }
+            }
+        }
+    }
+}
+
+// Runs that cross tiles: the warp of the tile in which the run starts adds the tiles' partial rows in order.
+template <typename TO, int VEC, int REP>
+__global__ void __launch_bounds__(128) embedding_join_kernel(const EmbArgs a, int blocks_per_row) {
+    const int lane = threadIdx.x & 31;
+    const int64_t tiles = (a.n + kTile - 1) / kTile, units = tiles * blocks_per_row, step = (int64_t)gridDim.x * 4;
+    for (int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); w < units; w += step) {
+        const int64_t tile = w / blocks_per_row, i0 = tile * kTile, i1 = i0 + kTile;
+        if (i1 >= a.n) continue;
+        const uint32_t key = a.sorted[i1 - 1].x;
+        if (key == (uint32_t)a.v || a.sorted[i1].x != key) continue;                       // nothing continues
+        if (i0 > 0 && a.sorted[i0].x == key && a.sorted[i0 - 1].x == key) continue;         // it started earlier
+        const int c0 = (int)(w - tile * blocks_per_row) * (32 * VEC * REP) + lane * VEC;
+        float acc[REP][VEC];
+#pragma unroll
+        for (int r = 0; r < REP; ++r) {
+            const int c = c0 + r * 32 * VEC;
+            Pack<float, VEC> p;
+            memset(&p, 0, sizeof(p));
+            if (c < a.d) p = *reinterpret_cast<const Pack<float, VEC> *>(a.part + (tile * 2 + 1) * a.d + c);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc[r][k] = p.v[k];
+        }
+        for (int64_t u0 = tile + 1;; u0 += 32) {
+            // how many of the next 32 tiles begin inside this run
+            const int64_t u = u0 + lane;
+            const bool in = u < tiles && a.sorted[u * kTile].x == key;
+            const unsigned m = __ballot_sync(0xffffffffu, in);
+            const int count = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
+#pragma unroll 4
+            for (int q = 0; q < count; ++q) {
+#pragma unroll
+                for (int r = 0; r < REP; ++r) {
+                    const int c = c0 + r * 32 * VEC;
+                    if (c >= a.d) continue;
+                    const Pack<float, VEC> p = *reinterpret_cast<const Pack<float, VEC> *>(a.part + (u0 + q) * 2 * a.d + c);
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) acc[r][k] += p.v[k];
+                }
+            }
+            if (count < 32) break;
+        }
+        store_sum<TO, VEC, REP>(static_cast<TO *>(a.dst) + (int64_t)key * a.d, c0, a.d, acc, a.scale);
+    }
+}
+
+int check_embedding(int64_t n, int64_t v, int64_t d, int64_t ld, int token_bytes, int table_dtype, int y_dtype) {
+    if (n < 0 || v < 1 || d < 1 || ld < d || n > 0x7fffffff || v > 0x7fffffff || d > (1 << 24))
+        return set_error(SRU_ERR_BAD_ARG, "bad sizes: %lld tokens, table (%lld, %lld) with row stride %lld", (long long)n,
+                         (long long)v, (long long)d, (long long)ld);
+    if (token_bytes != 4 && token_bytes != 8) return set_error(SRU_ERR_BAD_ARG, "tokens must be 4 or 8 bytes wide");
+    const bool t16 = table_dtype == SRU_F16 || table_dtype == SRU_BF16, y16 = y_dtype == SRU_F16 || y_dtype == SRU_BF16;
+    if (!(table_dtype == y_dtype && (t16 || table_dtype == SRU_F32)) && !(table_dtype == SRU_F32 && y16))
+        return set_error(SRU_ERR_UNSUPPORTED, "embedding: y must have the table's type (float32, float16, bfloat16) or be "
+                         "16-bit over a float32 table, got %d over %d", y_dtype, table_dtype);
+    return 0;
+}
+
+bool aligned16(const void *p, int64_t row_bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row_bytes % 16 == 0; }
+
+template <typename TK, typename TI, typename TO> int launch_forward(const EmbArgs &a, cudaStream_t st) {
+    constexpr int VEC = 16 / sizeof(TO);
+    const bool wide = aligned16(a.src, a.ld * sizeof(TI)) && aligned16(a.dst, a.d * sizeof(TO));
+    auto go = [&](auto vec, auto rep) {
+        constexpr int V = decltype(vec)::value, R = decltype(rep)::value;
+        const int per_row = (a.d + 32 * V * R - 1) / (32 * V * R);
+        const int64_t blocks = std::min<int64_t>((a.n * per_row + 7) / 8, 148 * 64);
+        embedding_fwd_kernel<TK, TI, TO, V, R><<<(unsigned)blocks, 256, 0, st>>>(a, per_row);
+    };
+    if (wide) go(std::integral_constant<int, VEC>(), std::integral_constant<int, 2>());
+    else go(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
+    SRUB_CUDA_CHECK(cudaGetLastError());
+    return 0;
+}
+
+template <typename TI, typename TO> int launch_sums(const EmbArgs &a, cudaStream_t st) {
+    constexpr int VEC = 16 / sizeof(TI);
+    const bool wide = aligned16(a.src, a.d * sizeof(TI)) && aligned16(a.dst, a.d * sizeof(TO));
+    auto go = [&](auto vec, auto rep) {
+        constexpr int V = decltype(vec)::value, R = decltype(rep)::value;
+        const int per_row = (a.d + 32 * V * R - 1) / (32 * V * R);
+        const int64_t units = (a.n + kTile - 1) / kTile * per_row;
+        const int64_t blocks = std::min<int64_t>((units + 3) / 4, 148 * 64);
+        embedding_sum_kernel<TI, TO, V, R><<<(unsigned)blocks, 128, 0, st>>>(a, per_row);
+        embedding_join_kernel<TO, V, R><<<(unsigned)blocks, 128, 0, st>>>(a, per_row);
+    };
+    if (wide) go(std::integral_constant<int, VEC>(), std::integral_constant<int, 1>());
+    else go(std::integral_constant<int, 1>(), std::integral_constant<int, 4>());
+    SRUB_CUDA_CHECK(cudaGetLastError());
+    return 0;
+}
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+size_t sort_bytes(int64_t n) { return round256((size_t)n * sizeof(uint2)); }
+
+}  // namespace
+
+}  // namespace srub
+
+using namespace srub;
+
+extern "C" {
+
+int sru_b200_embedding_forward(void *y, const void *tokens, const void *table, int64_t n, int64_t vocabulary,
+                               int64_t hidden, int64_t table_stride, double scale, int token_bytes, int table_dtype,
+                               int y_dtype, void *stream) {
+    int rc = check_embedding(n, vocabulary, hidden, table_stride, token_bytes, table_dtype, y_dtype);
+    if (rc) return rc;
+    if (n == 0) return 0;
+    if (!y || !tokens || !table) return set_error(SRU_ERR_BAD_ARG, "embedding: a required pointer is null");
+    EmbArgs a;
+    memset(&a, 0, sizeof(a));
+    a.tokens = tokens; a.src = table; a.dst = y;
+    a.n = n; a.v = vocabulary; a.d = (int)hidden; a.ld = table_stride; a.scale = (float)scale;
+    a.err = device_error_flag();
+    if (!a.err) return set_error(SRU_ERR_CUDA, "device error flag unavailable");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    auto go = [&](auto tk) -> int {
+        using TK = decltype(tk);
+        if (table_dtype == SRU_F32 && y_dtype == SRU_F32) return launch_forward<TK, float, float>(a, st);
+        if (table_dtype == SRU_F32 && y_dtype == SRU_F16) return launch_forward<TK, float, __half>(a, st);
+        if (table_dtype == SRU_F32) return launch_forward<TK, float, __nv_bfloat16>(a, st);
+        if (table_dtype == SRU_F16) return launch_forward<TK, __half, __half>(a, st);
+        return launch_forward<TK, __nv_bfloat16, __nv_bfloat16>(a, st);
+    };
+    return token_bytes == 4 ? go(int32_t()) : go(int64_t());
+}
+
+size_t sru_b200_embedding_backward_workspace_bytes(int64_t n, int64_t vocabulary, int64_t hidden) {
+    (void)vocabulary;
+    if (n < 1 || hidden < 1) return 0;
+    return 2 * sort_bytes(n) + (size_t)((n + kTile - 1) / kTile) * 2 * (size_t)hidden * sizeof(float);
+}
+
+int sru_b200_embedding_backward(void *grad_table, const void *tokens, const void *grad_y, int64_t n, int64_t vocabulary,
+                                int64_t hidden, int64_t padding_idx, double scale, int token_bytes, int table_dtype,
+                                int y_dtype, void *workspace, size_t workspace_bytes, void *stream) {
+    int rc = check_embedding(n, vocabulary, hidden, hidden, token_bytes, table_dtype, y_dtype);
+    if (rc) return rc;
+    if (!grad_table || (n > 0 && (!tokens || !grad_y))) return set_error(SRU_ERR_BAD_ARG, "embedding: a required pointer is null");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const size_t need = sru_b200_embedding_backward_workspace_bytes(n, vocabulary, hidden);
+    if (n > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+        return set_error(SRU_ERR_WORKSPACE, "16-byte aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    SRUB_CUDA_CHECK(cudaMemsetAsync(grad_table, 0, (size_t)vocabulary * hidden * dtype_size(table_dtype), st));
+    if (n == 0) return 0;
+    EmbArgs a;
+    memset(&a, 0, sizeof(a));
+    char *ws = static_cast<char *>(workspace);
+    a.tokens = tokens; a.src = grad_y; a.dst = grad_table;
+    a.sorted = reinterpret_cast<uint2 *>(ws);
+    a.spare = reinterpret_cast<uint2 *>(ws + sort_bytes(n));
+    a.part = reinterpret_cast<float *>(ws + 2 * sort_bytes(n));
+    a.n = n; a.v = vocabulary; a.d = (int)hidden; a.padding = padding_idx < 0 ? -1 : padding_idx; a.scale = (float)scale;
+    a.passes = 1;
+    while (a.passes < 4 && (vocabulary >> (8 * a.passes)) != 0) ++a.passes;     // the largest key is `vocabulary`
+    a.err = device_error_flag();
+    if (!a.err) return set_error(SRU_ERR_CUDA, "device error flag unavailable");
+    if (token_bytes == 4) embedding_sort_kernel<int32_t><<<kSortCtas, kSortWarps * 32, 0, st>>>(a);
+    else embedding_sort_kernel<int64_t><<<kSortCtas, kSortWarps * 32, 0, st>>>(a);
+    SRUB_CUDA_CHECK(cudaGetLastError());
+    if (table_dtype == SRU_F32 && y_dtype == SRU_F32) return launch_sums<float, float>(a, st);
+    if (table_dtype == SRU_F32 && y_dtype == SRU_F16) return launch_sums<__half, float>(a, st);
+    if (table_dtype == SRU_F32) return launch_sums<__nv_bfloat16, float>(a, st);
+    if (table_dtype == SRU_F16) return launch_sums<__half, __half>(a, st);
+    return launch_sums<__nv_bfloat16, __nv_bfloat16>(a, st);
+}
+
+}  // extern "C"

@@ -35,3 +35,28 @@ def test_linear_recurrence_c_arguments():
     assert g(one, one, None, one, one, one, None, None, None, 4, 2, 8, 32, 16, 16, 8, 0, 0, None, 0, None) == -3
     assert L.sru_b200_linear_recurrence_states_bytes(17, 3, 5) == 2 * 3 * 5 * 4
     assert L.sru_b200_linear_recurrence_states_bytes(0, 3, 5) == 0
+
+
+def test_embedding_refuses_cpu_tensors():
+    from sru_b200 import embedding_lookup
+    with pytest.raises(_lib.SruB200Error, match="no CPU path"):
+        embedding_lookup(torch.zeros(3, dtype=torch.long), torch.zeros(5, 8))
+
+
+def test_embedding_c_arguments():
+    L = _lib.lib()
+    one = ctypes.c_void_p(16)      # never dereferenced: every call below is refused on the host
+    f, g = L.sru_b200_embedding_forward, L.sru_b200_embedding_backward
+    assert f(None, one, one, 3, 5, 8, 8, 1.0, 8, 0, 0, None) == -1
+    assert f(one, one, one, 3, 0, 8, 8, 1.0, 8, 0, 0, None) == -1
+    assert f(one, one, one, 3, 5, 8, 7, 1.0, 8, 0, 0, None) == -1
+    assert f(one, one, one, 3, 5, 8, 8, 1.0, 2, 0, 0, None) == -1
+    assert f(one, one, one, 1 << 31, 5, 8, 8, 1.0, 8, 0, 0, None) == -1
+    assert f(one, one, one, 3, 1 << 31, 8, 8, 1.0, 8, 0, 0, None) == -1
+    assert f(one, one, one, 3, 5, 8, 8, 1.0, 8, _lib.SRU_BF16, _lib.SRU_F32, None) == -2
+    assert f(one, one, one, 3, 5, 8, 8, 1.0, 8, _lib.SRU_F64, _lib.SRU_F64, None) == -2
+    assert f(None, None, None, 0, 5, 8, 8, 1.0, 8, 0, 0, None) == 0
+    assert g(None, one, one, 3, 5, 8, -1, 1.0, 8, 0, 0, None, 0, None) == -1
+    assert g(one, one, one, 3, 5, 8, -1, 1.0, 8, 0, 0, None, 0, None) == -3
+    assert g(one, one, one, 3, 5, 8, -1, 1.0, 8, 0, 0, ctypes.c_void_p(8), 1 << 20, None) == -3
+    assert "aligned" in last_error()
