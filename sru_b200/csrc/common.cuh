@@ -17,7 +17,7 @@ namespace srub {
 // ---------------------------------------------------------------------------------------
 int set_error(int code, const char *fmt, ...);
 int *device_error_flag();  // device int, set non-zero by a kernel whose bounded wait gave up
-constexpr int kSiteToken = 21;   // flag value of a token outside its embedding table; other values: a wait's site
+constexpr int kSiteToken = 101;   // flag value of a token outside its embedding table; below 100: the site of a wait
 int ensure_context();      // binds the device's primary context to this thread if it has none; 0 or SRU_ERR_CUDA
 
 // Tuning / diagnostic options (sru_b200_set_option).  Each starts from the environment variable
