@@ -378,6 +378,28 @@ int sru_b200_embedding_backward(
     int64_t padding_idx, double scale, int token_bytes, int table_dtype, int y_dtype,
     void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * Orthogonalised update of weight matrices by Newton-Schulz steps (the Muon optimiser's): per matrix
+ *
+ *   X_0 = G / (|G|_F + eps),   `steps` times  X <- a X + (b A + c A A) X,  A = X X^T     (X the smaller side first)
+ *
+ * on the tensor cores, with fp16 iterates and float32 accumulation (about 1e-3 off the exact steps with the usual
+ * a, b, c = 3.4445, -4.7750, 2.0315; coefficients that let the iterates leave fp16's range give infinities).
+ *   grad   `batch` matrices (rows, cols), SRU_F32, SRU_F16 or SRU_BF16, element (z, i, j) at
+ *          z * stride_batch + i * stride_row + j * stride_col, one of stride_row, stride_col being 1
+ *   out    (batch, rows, cols) contiguous, SRU_F16 or SRU_BF16
+ *   workspace   256-byte aligned, ..._workspace_bytes(); calls that share one must be stream-ordered
+ * The norm is summed in 64 bits in a fixed order: repeated calls give identical bits.  The reference has no such
+ * operator; its applications step plain SGD and Adam (language_model/train_enwik8.py).
+ */
+size_t sru_b200_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
+
+int sru_b200_orthogonalize(
+    void *out, const void *grad, int64_t batch, int64_t rows, int64_t cols,
+    int64_t stride_batch, int64_t stride_row, int64_t stride_col, int steps,
+    double a, double b, double c, double eps, int grad_dtype, int out_dtype,
+    void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,9 +8,11 @@ of ``include/sru_b200.h`` (``sru_b200/lib/libsru_b200.so``); there is no CPU or 
 from . import _lib
 from .embedding import embedding_lookup
 from .linear_recurrence import gated_linear_recurrence
+from .orthogonalize import orthogonalize
 from .ops import (ElementwiseRecurrence, elementwise_recurrence_forward, elementwise_recurrence_gpu,
                   get_amp_mode, set_amp_mode, set_c_hist_dtype)
 
 __version__ = "0.1.0"
 __all__ = ["ElementwiseRecurrence", "elementwise_recurrence_forward", "elementwise_recurrence_gpu",
-           "embedding_lookup", "gated_linear_recurrence", "set_amp_mode", "get_amp_mode", "set_c_hist_dtype"]
+           "embedding_lookup", "gated_linear_recurrence", "orthogonalize",
+           "set_amp_mode", "get_amp_mode", "set_c_hist_dtype"]

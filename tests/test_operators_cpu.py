@@ -60,3 +60,29 @@ def test_embedding_c_arguments():
     assert g(one, one, one, 3, 5, 8, -1, 1.0, 8, 0, 0, None, 0, None) == -3
     assert g(one, one, one, 3, 5, 8, -1, 1.0, 8, 0, 0, ctypes.c_void_p(8), 1 << 20, None) == -3
     assert "aligned" in last_error()
+
+
+def test_orthogonalize_refuses_cpu_tensors():
+    from sru_b200 import orthogonalize
+    with pytest.raises(_lib.SruB200Error, match="no CPU path"):
+        orthogonalize(torch.zeros(3, 4))
+
+
+def test_orthogonalize_c_arguments():
+    L = _lib.lib()
+    one = ctypes.c_void_p(256)     # never dereferenced: every call below is refused on the host
+    f = L.sru_b200_orthogonalize
+    tail = (3.4, -4.7, 2.0, 1e-7)
+    big = 1 << 30
+    assert f(one, one, -1, 4, 5, 20, 5, 1, 5, *tail, 0, 2, one, big, None) == -1
+    assert f(one, one, 1, 1 << 21, 5, 20, 5, 1, 5, *tail, 0, 2, one, big, None) == -1
+    assert f(one, one, 1, 4, 5, 20, 5, 1, -1, *tail, 0, 2, one, big, None) == -1
+    assert f(one, one, 1, 4, 5, 20, 5, 1, 5, 3.4, -4.7, 2.0, -1.0, 0, 2, one, big, None) == -1
+    assert f(one, one, 1, 4, 5, 20, 5, 1, 5, 3.4, -4.7, 2.0, float("nan"), 0, 2, one, big, None) == -1
+    assert f(one, one, 1, 4, 5, 20, 5, 1, 5, *tail, _lib.SRU_F64, 2, one, big, None) == -2
+    assert f(one, one, 1, 4, 5, 20, 5, 1, 5, *tail, 0, _lib.SRU_F32, one, big, None) == -2
+    assert f(None, one, 1, 4, 5, 20, 5, 1, 5, *tail, 0, 2, one, big, None) == -1
+    assert f(one, one, 1, 4, 5, 20, 10, 2, 5, *tail, 0, 2, one, big, None) == -1
+    assert f(one, one, 1, 4, 5, 20, 5, 1, 5, *tail, 0, 2, None, 0, None) == -3
+    assert f(one, one, 1, 4, 5, 20, 5, 1, 5, *tail, 0, 2, ctypes.c_void_p(16), big, None) == -3
+    assert f(one, one, 0, 4, 5, 20, 5, 1, 5, *tail, 0, 2, None, 0, None) == 0
