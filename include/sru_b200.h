@@ -80,6 +80,7 @@ int sru_b200_check_device_error(void *stream);
  *   gemm_dynamic                       1: the pair GEMM hands out its tiles dynamically (needs the
  *                                      workspace form of the call); for products that share the GPU with
  *                                      a collective
+ *   linrec_slices                      parts of time that one column's gated linear recurrence is cut into (1..64)
  * Unknown names give SRU_ERR_BAD_ARG.  sru_b200_get_option returns the value, or -1 when not set.
  */
 int sru_b200_set_option(const char *name, int value);

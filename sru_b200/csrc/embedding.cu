@@ -111,6 +111,7 @@ embedding_sort_kernel(const EmbArgs a) {
     const int64_t per = ((a.n + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps) + 31) / 32 * 32;
     const int64_t i0 = min(a.n, ((int64_t)rank * kSortWarps + warp) * per), i1 = min(a.n, i0 + per);
 
+    cluster_barrier();       // every CTA has started before another writes to its shared memory
     for (int pass = 0; pass < a.passes; ++pass) {
         const int shift = 8 * pass;
         // the last pass ends in a.sorted

@@ -27,6 +27,12 @@ namespace {
 
 constexpr int kT = 16;          // steps per chunk, and between two saved states
 
+// Slices of time per column: warps of a CTA, times CTAs of a cluster.
+struct Slices {
+    int warps, ranks;
+    int count() const { return warps * ranks; }
+};
+
 struct LinRecArgs {
     void *h;                    // forward: (L, B, d); backward: grad_u (L, B, d, 2)
     float *last;                // forward: c_last (B, d); backward: grad of c0 (B, d); may be NULL
@@ -48,11 +54,11 @@ __device__ __forceinline__ float min_nan(float a, float b) {     // NaN if eithe
     return r;
 }
 
-// One step's V pairs of u, as loaded.
-template <typename TT, int V> struct PairLoad {
-    Pack<TT, 2 * V> p;
-    __device__ __forceinline__ float x(int v) const { return Cvt<TT>::to_f(p.v[2 * v]); }
-    __device__ __forceinline__ float g(int v) const { return Cvt<TT>::to_f(p.v[2 * v + 1]); }
+// One step's pair of u, as loaded.
+template <typename TT> struct PairLoad {
+    Pack<TT, 2> p;
+    __device__ __forceinline__ float x() const { return Cvt<TT>::to_f(p.v[0]); }
+    __device__ __forceinline__ float g() const { return Cvt<TT>::to_f(p.v[1]); }
 };
 
 template <typename P> __device__ __forceinline__ P zero_pack() {
@@ -61,25 +67,25 @@ template <typename P> __device__ __forceinline__ P zero_pack() {
     return p;
 }
 
-// kT steps of a strided stream of N elements per lane and step; steps from `n` on are left zero and not read.
-template <typename TT, int N>
-__device__ __forceinline__ void load_steps(Pack<TT, N> (&r)[kT], const TT *p, int64_t stride, int n, bool on) {
-    if (on && n >= kT) {
+// T steps of a strided stream of N elements per lane and step; steps from `n` on are left zero and not read.
+template <typename TT, int N, int T>
+__device__ __forceinline__ void load_steps(Pack<TT, N> (&r)[T], const TT *p, int64_t stride, int64_t n, bool on) {
+    if (on && n >= T) {
 #pragma unroll
-        for (int i = 0; i < kT; ++i) r[i] = *reinterpret_cast<const Pack<TT, N> *>(p + i * stride);
+        for (int i = 0; i < T; ++i) r[i] = *reinterpret_cast<const Pack<TT, N> *>(p + i * stride);
     } else {
 #pragma unroll
-        for (int i = 0; i < kT; ++i)
+        for (int i = 0; i < T; ++i)
             r[i] = (on && i < n) ? *reinterpret_cast<const Pack<TT, N> *>(p + i * stride) : zero_pack<Pack<TT, N>>();
     }
 }
 
 // Bit i: step i of the chunk is padded or lies behind the end.  The whole warp works on one sequence, so the flags are
 // uniform; lane i fetches step i's byte.
-__device__ __forceinline__ unsigned load_flags(const uint8_t *mask, int64_t stride, int64_t n, int lane) {
+template <int T> __device__ __forceinline__ unsigned load_flags(const uint8_t *mask, int64_t stride, int64_t n, int lane) {
     bool pad = lane >= n;
-    if (mask && lane < kT && lane < n) pad = mask[lane * stride] != 0;
-    return __ballot_sync(0xffffffffu, pad) & ((1u << kT) - 1u);
+    if (mask && lane < T && lane < n) pad = mask[lane * stride] != 0;
+    return __ballot_sync(0xffffffffu, pad);
 }
 
 // f and 1 - f from the gate's logit; nb = -bias * log2(e)
@@ -89,146 +95,240 @@ __device__ __forceinline__ void gate(float g, float nb, float *f, float *keep) {
     *keep = e * *f;
 }
 
-template <typename TT, int V>
-__global__ void __launch_bounds__(64)
-linear_recurrence_fwd_kernel(const LinRecArgs a) {
-    const int lane = threadIdx.x & 31;
-    const int64_t wid = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int64_t b = wid / a.groups;
-    if (b >= a.B) return;
-    const int j = (int)(wid - b * a.groups) * 32 * V + lane * V;
-    const bool on = j < a.d;
-    const int64_t col = b * a.d + j;
-    const TT *u = static_cast<const TT *>(a.u) + b * a.u_b + 2 * j;
-    TT *h = static_cast<TT *>(a.h) + col;
-    const uint8_t *mask = a.mask ? a.mask + b : nullptr;
-    float nb[V], c[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        nb[v] = (on && a.bias) ? a.bias[j + v] * kNegLog2e : 0.0f;
-        c[v] = (on && a.first) ? a.first[col + v] : 0.0f;
+// Where a warp stands: its sequence and column, and which of the `slices` interleaved parts of time it works on.  Slices are
+// the warps of a CTA and the CTAs of a cluster; chunk k of a column belongs to slice k mod slices.
+struct Place {
+    int lane, warp, warps;          // of the CTA
+    uint32_t rank, ranks;           // of the cluster
+    int64_t b, col;
+    int j;
+    bool on;
+};
+
+template <bool SPLIT> __device__ __forceinline__ bool find_place(const LinRecArgs &a, Place *p) {
+    p->lane = threadIdx.x & 31;
+    p->warp = threadIdx.x >> 5;
+    p->warps = blockDim.x >> 5;
+    p->rank = 0; p->ranks = 1;
+    int64_t wid;
+    if (SPLIT) {
+        asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(p->rank));
+        asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(p->ranks));
+        wid = blockIdx.x / p->ranks;
+    } else {
+        wid = (int64_t)blockIdx.x * p->warps + p->warp;
     }
-    Pack<TT, 2 * V> next[kT];
-    unsigned next_flags;
-    auto fetch = [&](int64_t t0) {
-        load_steps<TT, 2 * V>(next, u + t0 * a.u_t, a.u_t, (int)min((int64_t)kT, a.L - t0), on);
-        next_flags = load_flags(mask ? mask + t0 * a.m_t : nullptr, a.m_t, a.L - t0, lane);
-    };
-    fetch(0);
-    for (int64_t t0 = 0; t0 < a.L; t0 += kT) {
-        PairLoad<TT, V> cur[kT];
-#pragma unroll
-        for (int i = 0; i < kT; ++i) cur[i].p = next[i];
-        const unsigned flags = next_flags;
-        if (t0 + kT < a.L) fetch(t0 + kT);
-        if (a.states && on) {
-            Pack<float, V> s;
-#pragma unroll
-            for (int v = 0; v < V; ++v) s.v[v] = c[v];
-            *reinterpret_cast<Pack<float, V> *>(a.states + (t0 / kT) * a.B * a.d + col) = s;
-        }
-#pragma unroll
-        for (int i = 0; i < kT; ++i) {
-            const bool pad = (flags >> i) & 1u;
-            Pack<TT, V> out;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float f, keep;
-                gate(cur[i].g(v), nb[v], &f, &keep);
-                const float n = fmaf(f, c[v], keep * cur[i].x(v));
-                c[v] = pad ? c[v] : n;
-                out.v[v] = Cvt<TT>::from_f(pad ? 0.0f : n);
-            }
-            if (on && t0 + i < a.L) *reinterpret_cast<Pack<TT, V> *>(h + (t0 + i) * a.h_t) = out;
-        }
-    }
-    if (on && a.last) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) a.last[col + v] = c[v];
-    }
+    p->b = wid / a.groups;
+    p->j = (int)(wid - p->b * a.groups) * 32 + p->lane;
+    p->on = p->j < a.d;
+    p->col = p->b * a.d + p->j;
+    return p->b < a.B;
 }
 
-template <typename TT, int V>
-__global__ void __launch_bounds__(64)
-linear_recurrence_bwd_kernel(const LinRecArgs a) {
-    const int lane = threadIdx.x & 31;
-    const int64_t wid = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int64_t b = wid / a.groups;
-    if (b >= a.B) return;
-    const int j = (int)(wid - b * a.groups) * 32 * V + lane * V;
-    const bool on = j < a.d;
-    const int64_t col = b * a.d + j;
-    const TT *u = static_cast<const TT *>(a.u) + b * a.u_b + 2 * j;
-    const TT *gh = a.grad_h ? static_cast<const TT *>(a.grad_h) + b * a.gh_b + j : nullptr;
-    TT *gu = static_cast<TT *>(a.h) + 2 * col;
-    const uint8_t *mask = a.mask ? a.mask + b : nullptr;
-    float nb[V], dc[V], db[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        nb[v] = (on && a.bias) ? a.bias[j + v] * kNegLog2e : 0.0f;
-        dc[v] = (on && a.first) ? a.first[col + v] : 0.0f;
-        db[v] = 0.0f;
+// The affine maps s -> P s + C of all slices' chunks, exchanged: returns the value in front of this warp's chunk and moves
+// *carry behind the last one.  `back`: the slices follow each other from the last to the first.  One buffer is written while
+// the other may still be read, so one barrier per round is enough.
+constexpr int kMaxWarps = 8, kMaxRanks = 8;
+struct Exchange {
+    float2 warp[2][kMaxWarps][32];
+    float2 cta[2][kMaxRanks][32];
+};
+
+__device__ __forceinline__ float exchange(Exchange &x, int buf, const Place &p, float P, float C, bool back, float *carry) {
+    x.warp[buf][p.warp][p.lane] = make_float2(P, C);
+    __syncthreads();
+    float start = *carry;
+    if (p.ranks > 1) {
+        if (p.warp == 0) {
+            float tp = 1.0f, tc = 0.0f;
+            for (int k = 0; k < p.warps; ++k) {
+                const float2 m = x.warp[buf][back ? p.warps - 1 - k : k][p.lane];
+                tc = fmaf(m.x, tc, m.y);
+                tp *= m.x;
+            }
+            const uint32_t here = smem_u32(&x.cta[buf][p.rank][p.lane]);
+            for (uint32_t r = 0; r < p.ranks; ++r) {
+                uint32_t there;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(r));
+                asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(tp), "f"(tc) : "memory");
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        float s = *carry;
+        for (uint32_t k = 0; k < p.ranks; ++k) {
+            const uint32_t r = back ? p.ranks - 1 - k : k;
+            if (r == p.rank) start = s;
+            const float2 m = x.cta[buf][r][p.lane];
+            s = fmaf(m.x, s, m.y);
+        }
+        *carry = s;
     }
-    Pack<TT, 2 * V> next_u[kT];
-    Pack<TT, V> next_g[kT];
-    Pack<float, V> next_c = zero_pack<Pack<float, V>>();
+    float s = start, mine = start;
+    for (int k = 0; k < p.warps; ++k) {
+        const int w = back ? p.warps - 1 - k : k;
+        if (w == p.warp) mine = s;
+        const float2 m = x.warp[buf][w][p.lane];
+        s = fmaf(m.x, s, m.y);
+    }
+    if (p.ranks == 1) *carry = s;
+    return mine;
+}
+
+// No CTA of a cluster writes to another's shared memory before that one has started.
+__device__ __forceinline__ void cluster_started(const Place &p) {
+    if (p.ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// SPLIT: the slices' chunks are scanned locally, c_t = C_t + P_t c_in, and finished once c_in is known.
+template <typename TT, int T, bool SPLIT>
+__global__ void __launch_bounds__(SPLIT ? 256 : 64, SPLIT ? 3 : 8)
+linear_recurrence_fwd_kernel(const LinRecArgs a) {
+    __shared__ Exchange x[1];
+    Place p;
+    if (!find_place<SPLIT>(a, &p)) return;
+    const TT *u = static_cast<const TT *>(a.u) + p.b * a.u_b + 2 * p.j;
+    TT *h = static_cast<TT *>(a.h) + p.col;
+    const uint8_t *mask = a.mask ? a.mask + p.b : nullptr;
+    const float nb = (p.on && a.bias) ? a.bias[p.j] * kNegLog2e : 0.0f;
+    float carry = (p.on && a.first) ? a.first[p.col] : 0.0f;
+    const int slices = SPLIT ? p.warps * (int)p.ranks : 1;
+    const int slice = SPLIT ? (int)p.rank * p.warps + p.warp : 0;
+    const int64_t round = (int64_t)slices * T;
+    Pack<TT, 2> next[T];
     unsigned next_flags;
     auto fetch = [&](int64_t t0) {
-        const int n = (int)min((int64_t)kT, a.L - t0);
-        if (on) next_c = *reinterpret_cast<const Pack<float, V> *>(a.states + (t0 / kT) * a.B * a.d + col);
-        load_steps<TT, 2 * V>(next_u, u + t0 * a.u_t, a.u_t, n, on);
-        load_steps<TT, V>(next_g, gh + t0 * a.gh_t, a.gh_t, n, on && gh);
-        next_flags = load_flags(mask ? mask + t0 * a.m_t : nullptr, a.m_t, a.L - t0, lane);
+        load_steps<TT, 2, T>(next, u + t0 * a.u_t, a.u_t, a.L - t0, p.on);
+        next_flags = load_flags<T>(mask ? mask + t0 * a.m_t : nullptr, a.m_t, a.L - t0, p.lane);
     };
-    const int64_t t_top = (a.L - 1) / kT * kT;
-    fetch(t_top);
-    for (int64_t t0 = t_top; t0 >= 0; t0 -= kT) {
-        float f[kT][V], keep[kT][V], w[kT][V];      // w = (c_{t-1} - x) f (1 - f)
-        Pack<TT, V> g[kT];
+    fetch((int64_t)slice * T);
+    if (SPLIT) cluster_started(p);
+    int buf = 0;
+    for (int64_t r0 = 0; r0 < a.L; r0 += round, buf ^= 1) {
+        const int64_t t0 = r0 + (int64_t)slice * T;
+        PairLoad<TT> cur[T];
+#pragma unroll
+        for (int i = 0; i < T; ++i) cur[i].p = next[i];
         const unsigned flags = next_flags;
-        {
-            PairLoad<TT, V> cur[kT];
-            Pack<float, V> c = next_c;
+        if (r0 + round < a.L) fetch(t0 + round);
+        float c = carry;
+        if (SPLIT) {
+            float C[T], P[T];
+            float lc = 0.0f, lp = 1.0f;
 #pragma unroll
-            for (int i = 0; i < kT; ++i) { cur[i].p = next_u[i]; g[i] = next_g[i]; }
-            if (t0 > 0) fetch(t0 - kT);
-#pragma unroll
-            for (int i = 0; i < kT; ++i) {
+            for (int i = 0; i < T; ++i) {
                 const bool pad = (flags >> i) & 1u;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const float x = cur[i].x(v);
-                    float fi, ki;
-                    gate(cur[i].g(v), nb[v], &fi, &ki);
-                    w[i][v] = pad ? 0.0f : (c.v[v] - x) * fi * ki;
-                    c.v[v] = pad ? c.v[v] : fmaf(fi, c.v[v], ki * x);
-                    f[i][v] = pad ? 1.0f : fi;
-                    keep[i][v] = pad ? 0.0f : ki;
-                }
+                float f, keep;
+                gate(cur[i].g(), nb, &f, &keep);
+                const float n = fmaf(f, lc, keep * cur[i].x());
+                lc = pad ? lc : n;
+                lp = pad ? lp : lp * f;
+                C[i] = lc;
+                P[i] = lp;
             }
-        }
+            c = exchange(x[0], buf, p, lp, lc, false, &carry);
+            if (a.states && p.on && t0 < a.L) a.states[(t0 / kT) * a.B * a.d + p.col] = c;
+            if (p.on) {
 #pragma unroll
-        for (int i = kT - 1; i >= 0; --i) {
-            const bool pad = (flags >> i) & 1u;
-            Pack<TT, 2 * V> out;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float total = pad ? dc[v] : dc[v] + Cvt<TT>::to_f(g[i].v[v]);
-                const float dg = pad ? 0.0f : w[i][v] * total;
-                out.v[2 * v] = Cvt<TT>::from_f(pad ? 0.0f : keep[i][v] * total);
-                out.v[2 * v + 1] = Cvt<TT>::from_f(dg);
-                db[v] += dg;
-                dc[v] = f[i][v] * total;
+                for (int i = 0; i < T; ++i)
+                    if (t0 + i < a.L) h[(t0 + i) * a.h_t] = Cvt<TT>::from_f((flags >> i) & 1u ? 0.0f : fmaf(P[i], c, C[i]));
             }
-            if (on && t0 + i < a.L) *reinterpret_cast<Pack<TT, 2 * V> *>(gu + 2 * (t0 + i) * a.h_t) = out;
+        } else {
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                if (i % kT == 0 && a.states && p.on && t0 + i < a.L) a.states[((t0 + i) / kT) * a.B * a.d + p.col] = c;
+                const bool pad = (flags >> i) & 1u;
+                float f, keep;
+                gate(cur[i].g(), nb, &f, &keep);
+                const float n = fmaf(f, c, keep * cur[i].x());
+                c = pad ? c : n;
+                if (p.on && t0 + i < a.L) h[(t0 + i) * a.h_t] = Cvt<TT>::from_f(pad ? 0.0f : n);
+            }
+            carry = c;
         }
     }
-    if (on) {
+    if (slice == 0 && p.on && a.last) a.last[p.col] = carry;
+}
+
+template <typename TT, bool SPLIT>
+__global__ void __launch_bounds__(SPLIT ? 256 : 64, SPLIT ? 2 : 8)
+linear_recurrence_bwd_kernel(const LinRecArgs a) {
+    __shared__ Exchange x[1];
+    constexpr int T = kT;
+    Place p;
+    if (!find_place<SPLIT>(a, &p)) return;
+    const TT *u = static_cast<const TT *>(a.u) + p.b * a.u_b + 2 * p.j;
+    const TT *gh = a.grad_h ? static_cast<const TT *>(a.grad_h) + p.b * a.gh_b + p.j : nullptr;
+    TT *gu = static_cast<TT *>(a.h) + 2 * p.col;
+    const uint8_t *mask = a.mask ? a.mask + p.b : nullptr;
+    const float nb = (p.on && a.bias) ? a.bias[p.j] * kNegLog2e : 0.0f;
+    float carry = (p.on && a.first) ? a.first[p.col] : 0.0f, db = 0.0f;
+    const int slices = SPLIT ? p.warps * (int)p.ranks : 1;
+    const int slice = SPLIT ? (int)p.rank * p.warps + p.warp : 0;
+    const int64_t round = (int64_t)slices * T;
+    Pack<TT, 2> next_u[T];
+    Pack<TT, 1> next_g[T];
+    float next_c = 0.0f;
+    unsigned next_flags;
+    auto fetch = [&](int64_t t0) {
+        if (p.on && t0 < a.L) next_c = a.states[(t0 / T) * a.B * a.d + p.col];
+        load_steps<TT, 2, T>(next_u, u + t0 * a.u_t, a.u_t, a.L - t0, p.on);
+        load_steps<TT, 1, T>(next_g, gh + t0 * a.gh_t, a.gh_t, a.L - t0, p.on && gh);
+        next_flags = load_flags<T>(mask ? mask + t0 * a.m_t : nullptr, a.m_t, a.L - t0, p.lane);
+    };
+    const int64_t r_top = (a.L - 1) / round * round;
+    fetch(r_top + (int64_t)slice * T);
+    if (SPLIT) cluster_started(p);
+    int buf = 0;
+    for (int64_t r0 = r_top; r0 >= 0; r0 -= round, buf ^= 1) {
+        const int64_t t0 = r0 + (int64_t)slice * T;
+        float f[T], keep[T], w[T];      // w = (c_{t-1} - x) f (1 - f)
+        Pack<TT, 1> g[T];
+        const unsigned flags = next_flags;
+        {
+            PairLoad<TT> cur[T];
+            float c = next_c;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            if (a.last) a.last[col + v] = dc[v];
-            if (a.bias_part) a.bias_part[b * a.d + j + v] = db[v];
+            for (int i = 0; i < T; ++i) { cur[i].p = next_u[i]; g[i] = next_g[i]; }
+            if (r0 > 0) fetch(t0 - round);
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                const bool pad = (flags >> i) & 1u;
+                const float xi = cur[i].x();
+                float fi, ki;
+                gate(cur[i].g(), nb, &fi, &ki);
+                w[i] = pad ? 0.0f : (c - xi) * fi * ki;
+                c = pad ? c : fmaf(fi, c, ki * xi);
+                f[i] = pad ? 1.0f : fi;
+                keep[i] = pad ? 0.0f : ki;
+            }
         }
+        float dc = carry;
+        if (SPLIT) {
+            float lc = 0.0f, lp = 1.0f;
+#pragma unroll
+            for (int i = T - 1; i >= 0; --i) {
+                lc = f[i] * ((flags >> i) & 1u ? lc : lc + Cvt<TT>::to_f(g[i].v[0]));
+                lp *= f[i];
+            }
+            dc = exchange(x[0], buf, p, lp, lc, true, &carry);
+        }
+#pragma unroll
+        for (int i = T - 1; i >= 0; --i) {
+            const bool pad = (flags >> i) & 1u;
+            const float total = pad ? dc : dc + Cvt<TT>::to_f(g[i].v[0]);
+            const float dg = pad ? 0.0f : w[i] * total;
+            Pack<TT, 2> out;
+            out.v[0] = Cvt<TT>::from_f(pad ? 0.0f : keep[i] * total);
+            out.v[1] = Cvt<TT>::from_f(dg);
+            db += dg;
+            dc = f[i] * total;
+            if (p.on && t0 + i < a.L) *reinterpret_cast<Pack<TT, 2> *>(gu + 2 * (t0 + i) * a.h_t) = out;
+        }
+        if (!SPLIT) carry = dc;
+    }
+    if (p.on) {
+        if (a.last && slice == 0) a.last[p.col] = carry;
+        if (a.bias_part) a.bias_part[(p.b * slices + slice) * a.d + p.j] = db;
     }
 }
 
@@ -269,28 +369,54 @@ void reverse_time(LinRecArgs *a, size_t size, int units) {
     a->u_t = -a->u_t; a->h_t = -a->h_t; a->gh_t = -a->gh_t; a->m_t = -a->m_t;
 }
 
-template <typename TT> int launch(const LinRecArgs &a0, bool backward, cudaStream_t st) {
+Slices choose_slices(int64_t L, int64_t B, int64_t d) {
+    const int64_t columns = (d + 31) / 32 * B;              // warps that one walk over time takes
+    int64_t want = option(OPT_LINREC_SLICES, 0);
+    if (want <= 0) {
+        want = 1;
+        while (want < 64 && columns * want * 2 <= 148 * 24) want *= 2;
+    }
+    want = std::min<int64_t>(std::min<int64_t>(want, 64), (L + kT - 1) / kT);
+    Slices s;
+    s.ranks = (int)((want + kMaxWarps - 1) / kMaxWarps);
+    s.warps = (int)((want + s.ranks - 1) / s.ranks);
+    return s;
+}
+
+template <typename TT> int launch(const LinRecArgs &a0, const Slices &s, bool backward, cudaStream_t st) {
     LinRecArgs a = a0;
-    constexpr int V = 1;
-    a.groups = (a.d + 32 * V - 1) / (32 * V);
-    const int64_t warps = (int64_t)a.groups * a.B;
-    const int64_t blocks = (warps + 1) / 2;
-    if (blocks > 0x7fffffff) return set_error(SRU_ERR_UNSUPPORTED, "linear recurrence: batch * hidden too large");
-    if (backward) linear_recurrence_bwd_kernel<TT, V><<<(unsigned)blocks, 64, 0, st>>>(a);
-    else linear_recurrence_fwd_kernel<TT, V><<<(unsigned)blocks, 64, 0, st>>>(a);
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    a.groups = (a.d + 31) / 32;
+    const int64_t columns = (int64_t)a.groups * a.B;
+    if (columns * s.ranks > 0x7fffffff) return set_error(SRU_ERR_UNSUPPORTED, "linear recurrence: batch * hidden too large");
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)s.ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    if (s.count() > 1) {
+        cfg.gridDim = dim3((unsigned)(columns * s.ranks), 1, 1);
+        cfg.blockDim = dim3(32 * s.warps, 1, 1);
+        cfg.numAttrs = 1;
+        if (backward) SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_recurrence_bwd_kernel<TT, true>, a));
+        else SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_recurrence_fwd_kernel<TT, kT, true>, a));
+    } else {
+        cfg.gridDim = dim3((unsigned)((columns + 1) / 2), 1, 1);
+        cfg.blockDim = dim3(64, 1, 1);
+        if (backward) SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_recurrence_bwd_kernel<TT, false>, a));
+        else SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_recurrence_fwd_kernel<TT, 2 * kT, false>, a));
+    }
     return 0;
 }
 
-int dispatch(const LinRecArgs &a, int dtype, bool backward, cudaStream_t st) {
+int dispatch(const LinRecArgs &a, const Slices &s, int dtype, bool backward, cudaStream_t st) {
     switch (dtype) {
-        case SRU_F16: return launch<__half>(a, backward, st);
-        case SRU_BF16: return launch<__nv_bfloat16>(a, backward, st);
-        default: return launch<float>(a, backward, st);
+        case SRU_F16: return launch<__half>(a, s, backward, st);
+        case SRU_BF16: return launch<__nv_bfloat16>(a, s, backward, st);
+        default: return launch<float>(a, s, backward, st);
     }
 }
-
-int64_t bias_parts(int64_t B) { return B; }
 
 }  // namespace
 
@@ -324,12 +450,12 @@ int sru_b200_linear_recurrence_forward(void *h, float *c_last, void *states, con
     a.u_t = u_stride_t; a.u_b = u_stride_b;
     a.h_t = batch * hidden; a.m_t = batch;
     if (reverse) reverse_time(&a, size, 1);
-    return dispatch(a, dtype, false, static_cast<cudaStream_t>(stream));
+    return dispatch(a, choose_slices(length, batch, hidden), dtype, false, static_cast<cudaStream_t>(stream));
 }
 
 size_t sru_b200_linear_recurrence_backward_workspace_bytes(int64_t length, int64_t batch, int64_t hidden) {
     if (length < 1 || batch < 1 || hidden < 1) return 0;
-    return (size_t)bias_parts(batch) * (size_t)hidden * sizeof(float);
+    return (size_t)batch * choose_slices(length, batch, hidden).count() * (size_t)hidden * sizeof(float);
 }
 
 int sru_b200_linear_recurrence_backward(void *grad_u, float *grad_bias, float *grad_init, const void *u,
@@ -345,8 +471,9 @@ int sru_b200_linear_recurrence_backward(void *grad_u, float *grad_bias, float *g
     const size_t size = dtype_size(dtype);
     if ((reinterpret_cast<uintptr_t>(u) % (2 * size)) || u_stride_t % 2 || u_stride_b % 2)
         return set_error(SRU_ERR_BAD_ARG, "linear recurrence: the pairs of u must be aligned to their size");
+    const Slices s = choose_slices(length, batch, hidden);
     if (grad_bias) {
-        const size_t need = sru_b200_linear_recurrence_backward_workspace_bytes(length, batch, hidden);
+        const size_t need = (size_t)batch * s.count() * (size_t)hidden * sizeof(float);
         if (!workspace || workspace_bytes < need)
             return set_error(SRU_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     }
@@ -360,10 +487,10 @@ int sru_b200_linear_recurrence_backward(void *grad_u, float *grad_bias, float *g
     a.h_t = batch * hidden; a.m_t = batch;
     if (reverse) reverse_time(&a, size, 2);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    rc = dispatch(a, dtype, true, st);
+    rc = dispatch(a, s, dtype, true, st);
     if (rc || !grad_bias) return rc;
     linear_recurrence_bias_kernel<<<(unsigned)((hidden + 31) / 32), 256, 0, st>>>(grad_bias, a.bias_part,
-                                                                                   bias_parts(batch), (int)hidden);
+                                                                                   batch * s.count(), (int)hidden);
     SRUB_CUDA_CHECK(cudaGetLastError());
     return 0;
 }
