@@ -8,9 +8,9 @@
 //   dc_t = grad_h_t + f_{t+1} dc_{t+1},   dx_t = (1 - f_t) dc_t,   dg_t = dc_t (c_{t-1} - x_t) f_t (1 - f_t),
 //   dbias = sum over t, b of dg,          dc_0 = f_first dc_first.
 //
-// HBM-bound: 3 elements per column-step forward, 5 backward.  A lane owns V adjacent columns of one sequence and walks
-// time in chunks of kT steps; the next chunk's loads are issued before the current chunk is worked on.  The forward
-// pass leaves the float32 state in front of every chunk (kT = 16: a quarter of a byte per column-step); the backward
+// HBM-bound: 3 elements per column-step forward, 5 backward.  A lane owns V = 2 adjacent columns of one sequence (1 where
+// sizes or alignment forbid pairs) and walks time in chunks of kT steps; the next chunk's loads are issued before the current chunk is worked on.  The forward
+// pass leaves the float32 state in front of every chunk (kT = 8: half a byte per column-step); the backward
 // pass recomputes the states of a chunk from it, which is cheaper than reading a saved history (2 or 4 bytes) and
 // exact in the 16-bit types, whose rounded h would enter c_{t-1} - x_t.
 //
@@ -19,13 +19,14 @@
 #include <algorithm>
 #include <cstring>
 
-#include "common.cuh"
+#include "f32x2.cuh"
+#include "tcgen05.cuh"
 
 namespace srub {
 
 namespace {
 
-constexpr int kT = 16;          // steps per chunk, and between two saved states
+constexpr int kT = 8;           // steps per chunk, and between two saved states
 
 // Slices of time per column: warps of a CTA, times CTAs of a cluster.
 struct Slices {
@@ -46,7 +47,74 @@ struct LinRecArgs {
     int64_t u_t, u_b, gh_t, gh_b;   // strides in elements (time strides signed: a reversed scan starts at the end)
     int64_t h_t, m_t;               // signed time strides of h / grad_u's column unit and of the mask
     int d, groups;                  // groups: warps' worth of columns per sequence
+    int *err;
 };
+
+// ---- V float32 values, one per column of a lane; pairs go through the two-lane instructions -------------------------
+template <int V> struct Num;
+template <> struct Num<1> {
+    float a;
+    __device__ __forceinline__ float get(int) const { return a; }
+};
+template <> struct Num<2> {
+    F2 a;
+    __device__ __forceinline__ float get(int v) const {
+        float lo, hi;
+        f2_split(a, lo, hi);
+        return v ? hi : lo;
+    }
+};
+__device__ __forceinline__ Num<1> num(const float (&v)[1]) { return Num<1>{v[0]}; }
+__device__ __forceinline__ Num<2> num(const float (&v)[2]) { return Num<2>{f2_make(v[0], v[1])}; }
+template <int V> __device__ __forceinline__ Num<V> all(float x) {
+    float v[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = x;
+    return num(v);
+}
+__device__ __forceinline__ Num<1> fma(Num<1> a, Num<1> b, Num<1> c) { return {fmaf(a.a, b.a, c.a)}; }
+__device__ __forceinline__ Num<1> mul(Num<1> a, Num<1> b) { return {a.a * b.a}; }
+__device__ __forceinline__ Num<1> add(Num<1> a, Num<1> b) { return {a.a + b.a}; }
+__device__ __forceinline__ Num<1> sub(Num<1> a, Num<1> b) { return {a.a - b.a}; }
+__device__ __forceinline__ Num<2> fma(Num<2> a, Num<2> b, Num<2> c) { return {f2_fma(a.a, b.a, c.a)}; }
+__device__ __forceinline__ Num<2> mul(Num<2> a, Num<2> b) { return {f2_mul(a.a, b.a)}; }
+__device__ __forceinline__ Num<2> add(Num<2> a, Num<2> b) { return {f2_add(a.a, b.a)}; }
+__device__ __forceinline__ Num<2> sub(Num<2> a, Num<2> b) { return {f2_sub(a.a, b.a)}; }
+__device__ __forceinline__ Num<1> pick(bool first, Num<1> a, Num<1> b) { return first ? a : b; }
+__device__ __forceinline__ Num<2> pick(bool first, Num<2> a, Num<2> b) { return {f2_select(first, a.a, b.a)}; }
+
+template <typename TT> __device__ __forceinline__ Pack<TT, 2> pack2(float a, float b) {
+    Pack<TT, 2> r;
+    r.v[0] = Cvt<TT>::from_f(a);
+    r.v[1] = Cvt<TT>::from_f(b);
+    return r;
+}
+template <> __device__ __forceinline__ Pack<__half, 2> pack2<__half>(float a, float b) {
+    const __half2 t = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const Pack<__half, 2> *>(&t);
+}
+template <> __device__ __forceinline__ Pack<__nv_bfloat16, 2> pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const Pack<__nv_bfloat16, 2> *>(&t);
+}
+template <typename TT> __device__ __forceinline__ Pack<TT, 1> rounded(Num<1> a) {
+    Pack<TT, 1> r;
+    r.v[0] = Cvt<TT>::from_f(a.a);
+    return r;
+}
+template <typename TT> __device__ __forceinline__ Pack<TT, 2> rounded(Num<2> a) { return pack2<TT>(a.get(0), a.get(1)); }
+template <typename TT> __device__ __forceinline__ Num<1> widened(const Pack<TT, 1> &p) { return {Cvt<TT>::to_f(p.v[0])}; }
+template <typename TT> __device__ __forceinline__ Num<2> widened(const Pack<TT, 2> &p) {
+    return {f2_make(Cvt<TT>::to_f(p.v[0]), Cvt<TT>::to_f(p.v[1]))};
+}
+// the pairs (x, g) of V columns
+template <typename TT, int V> __device__ __forceinline__ void unpair(const Pack<TT, 2 * V> &p, Num<V> *x, Num<V> *g) {
+    float a[V], b[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) { a[v] = Cvt<TT>::to_f(p.v[2 * v]); b[v] = Cvt<TT>::to_f(p.v[2 * v + 1]); }
+    *x = num(a);
+    *g = num(b);
+}
 
 __device__ __forceinline__ float min_nan(float a, float b) {     // NaN if either is
     float r;
@@ -54,58 +122,55 @@ __device__ __forceinline__ float min_nan(float a, float b) {     // NaN if eithe
     return r;
 }
 
-// One step's pair of u, as loaded.
-template <typename TT> struct PairLoad {
-    Pack<TT, 2> p;
-    __device__ __forceinline__ float x() const { return Cvt<TT>::to_f(p.v[0]); }
-    __device__ __forceinline__ float g() const { return Cvt<TT>::to_f(p.v[1]); }
-};
-
-template <typename P> __device__ __forceinline__ P zero_pack() {
-    P p;
-    memset(&p, 0, sizeof(P));
-    return p;
+// f and 1 - f from the gate's logit; nb = -bias * log2(e).  The exponential stays at most 2^126, so that e f is finite.
+template <int V> __device__ __forceinline__ void gate(Num<V> g, Num<V> nb, Num<V> *f, Num<V> *keep) {
+    const Num<V> z = fma(g, all<V>(kNegLog2e), nb);
+    float e[V], r[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) e[v] = ex2_approx(min_nan(z.get(v), 126.0f));
+    const Num<V> en = num(e), den = add(en, all<V>(1.0f));
+#pragma unroll
+    for (int v = 0; v < V; ++v) r[v] = rcp_approx(den.get(v));
+    *f = num(r);
+    *keep = mul(en, *f);
 }
 
-// T steps of a strided stream of N elements per lane and step; steps from `n` on are left zero and not read.
+// T steps of a strided stream of N elements per lane and step; of a chunk that sticks out, steps from `n` on are zero and
+// not read.
 template <typename TT, int N, int T>
-__device__ __forceinline__ void load_steps(Pack<TT, N> (&r)[T], const TT *p, int64_t stride, int64_t n, bool on) {
-    if (on && n >= T) {
+__device__ __forceinline__ void load_steps(Pack<TT, N> (&r)[T], const TT *p, int64_t stride, int64_t n) {
+    if (n >= T) {
 #pragma unroll
-        for (int i = 0; i < T; ++i) r[i] = *reinterpret_cast<const Pack<TT, N> *>(p + i * stride);
+        for (int i = 0; i < T; ++i, p += stride) r[i] = *reinterpret_cast<const Pack<TT, N> *>(p);
     } else {
 #pragma unroll
-        for (int i = 0; i < T; ++i)
-            r[i] = (on && i < n) ? *reinterpret_cast<const Pack<TT, N> *>(p + i * stride) : zero_pack<Pack<TT, N>>();
+        for (int i = 0; i < T; ++i, p += stride) {
+            if (i < n) r[i] = *reinterpret_cast<const Pack<TT, N> *>(p);
+            else memset(&r[i], 0, sizeof(r[i]));
+        }
     }
 }
 
 // Bit i: step i of the chunk is padded or lies behind the end.  The whole warp works on one sequence, so the flags are
-// uniform; lane i fetches step i's byte.
+// uniform; lane i fetches step i's byte.  0 is the common case, and takes the paths without selects.
 template <int T> __device__ __forceinline__ unsigned load_flags(const uint8_t *mask, int64_t stride, int64_t n, int lane) {
-    bool pad = lane >= n;
-    if (mask && lane < T && lane < n) pad = mask[lane * stride] != 0;
+    if (!mask) return n >= T ? 0u : (n <= 0 ? 0xffffffffu : 0xffffffffu << n) & (uint32_t)((1ull << T) - 1);
+    bool pad = lane < T && lane >= n;
+    if (lane < T && lane < n) pad = mask[lane * stride] != 0;
     return __ballot_sync(0xffffffffu, pad);
 }
 
-// f and 1 - f from the gate's logit; nb = -bias * log2(e)
-__device__ __forceinline__ void gate(float g, float nb, float *f, float *keep) {
-    const float e = ex2_approx(min_nan(fmaf(g, kNegLog2e, nb), 126.0f));    // at most 2^126, so that e * f stays finite
-    *f = rcp_approx(1.0f + e);
-    *keep = e * *f;
-}
-
-// Where a warp stands: its sequence and column, and which of the `slices` interleaved parts of time it works on.  Slices are
-// the warps of a CTA and the CTAs of a cluster; chunk k of a column belongs to slice k mod slices.
+// Where a warp stands: its sequence and columns, and which of the interleaved slices of time it works on.  Slices are the
+// warps of a CTA and the CTAs of a cluster; chunk k of a column belongs to slice k mod slices.  Lanes behind the last
+// column repeat it (they load and store the same values), so that no access needs a predicate.
 struct Place {
     int lane, warp, warps;          // of the CTA
     uint32_t rank, ranks;           // of the cluster
     int64_t b, col;
-    int j;
-    bool on;
+    int j, shift;                   // first column; its place behind the first column of lane 0
 };
 
-template <bool SPLIT> __device__ __forceinline__ bool find_place(const LinRecArgs &a, Place *p) {
+template <int V, bool SPLIT> __device__ __forceinline__ bool find_place(const LinRecArgs &a, Place *p) {
     p->lane = threadIdx.x & 31;
     p->warp = threadIdx.x >> 5;
     p->warps = blockDim.x >> 5;
@@ -119,217 +184,456 @@ template <bool SPLIT> __device__ __forceinline__ bool find_place(const LinRecArg
         wid = (int64_t)blockIdx.x * p->warps + p->warp;
     }
     p->b = wid / a.groups;
-    p->j = (int)(wid - p->b * a.groups) * 32 + p->lane;
-    p->on = p->j < a.d;
+    const int j0 = (int)(wid - p->b * a.groups) * 32 * V;
+    p->j = min(j0 + p->lane * V, a.d - V);
+    p->shift = p->j - j0;
     p->col = p->b * a.d + p->j;
     return p->b < a.B;
+}
+
+template <int V> __device__ __forceinline__ Num<V> load_small(const float *p, int64_t at) {
+    float v[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = p ? p[at + k] : 0.0f;
+    return num(v);
+}
+template <int V> __device__ __forceinline__ void store_small(float *p, int64_t at, Num<V> v) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) p[at + k] = v.get(k);
+}
+template <int V> __device__ __forceinline__ Num<V> load_state(const float *p) {
+    return widened<float>(*reinterpret_cast<const Pack<float, V> *>(p));
+}
+template <int V> __device__ __forceinline__ void store_state(float *p, Num<V> v) {
+    *reinterpret_cast<Pack<float, V> *>(p) = rounded<float>(v);
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // The affine maps s -> P s + C of all slices' chunks, exchanged: returns the value in front of this warp's chunk and moves
 // *carry behind the last one.  `back`: the slices follow each other from the last to the first.  One buffer is written while
 // the other may still be read, so one barrier per round is enough.
 constexpr int kMaxWarps = 8, kMaxRanks = 8;
-struct Exchange {
-    float2 warp[2][kMaxWarps][32];
-    float2 cta[2][kMaxRanks][32];
+template <int V> struct Map { Num<V> P, C; };
+template <int V> struct Exchange {
+    Map<V> warp[2][kMaxWarps][32];
+    Map<V> cta[2][kMaxRanks][32];
 };
 
-__device__ __forceinline__ float exchange(Exchange &x, int buf, const Place &p, float P, float C, bool back, float *carry) {
-    x.warp[buf][p.warp][p.lane] = make_float2(P, C);
+template <int V, bool BACK>
+__device__ __forceinline__ Num<V> exchange(Exchange<V> &x, int buf, const Place &p, Map<V> own, Num<V> *carry) {
+    x.warp[buf][p.warp][p.lane] = own;
     __syncthreads();
-    float start = *carry;
+    Num<V> start = *carry;
     if (p.ranks > 1) {
         if (p.warp == 0) {
-            float tp = 1.0f, tc = 0.0f;
+            Map<V> t{all<V>(1.0f), all<V>(0.0f)};
             for (int k = 0; k < p.warps; ++k) {
-                const float2 m = x.warp[buf][back ? p.warps - 1 - k : k][p.lane];
-                tc = fmaf(m.x, tc, m.y);
-                tp *= m.x;
+                const Map<V> m = x.warp[buf][BACK ? p.warps - 1 - k : k][p.lane];
+                t.C = fma(m.P, t.C, m.C);
+                t.P = mul(t.P, m.P);
             }
             const uint32_t here = smem_u32(&x.cta[buf][p.rank][p.lane]);
             for (uint32_t r = 0; r < p.ranks; ++r) {
                 uint32_t there;
                 asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(r));
-                asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(tp), "f"(tc) : "memory");
+                if constexpr (V == 1)
+                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(t.P.a), "f"(t.C.a) : "memory");
+                else
+                    asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(there), "l"(t.P.a.v), "l"(t.C.a.v) : "memory");
             }
         }
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        float s = *carry;
+        cluster_sync();
+        Num<V> s = *carry;
         for (uint32_t k = 0; k < p.ranks; ++k) {
-            const uint32_t r = back ? p.ranks - 1 - k : k;
-            if (r == p.rank) start = s;
-            const float2 m = x.cta[buf][r][p.lane];
-            s = fmaf(m.x, s, m.y);
+            const uint32_t r = BACK ? p.ranks - 1 - k : k;
+            start = pick(r == p.rank, s, start);
+            const Map<V> m = x.cta[buf][r][p.lane];
+            s = fma(m.P, s, m.C);
         }
         *carry = s;
     }
-    float s = start, mine = start;
+    Num<V> s = start, mine = start;
     for (int k = 0; k < p.warps; ++k) {
-        const int w = back ? p.warps - 1 - k : k;
-        if (w == p.warp) mine = s;
-        const float2 m = x.warp[buf][w][p.lane];
-        s = fmaf(m.x, s, m.y);
+        const int w = BACK ? p.warps - 1 - k : k;
+        mine = pick(w == p.warp, s, mine);
+        const Map<V> m = x.warp[buf][w][p.lane];
+        s = fma(m.P, s, m.C);
     }
     if (p.ranks == 1) *carry = s;
     return mine;
 }
 
-// No CTA of a cluster writes to another's shared memory before that one has started.
-__device__ __forceinline__ void cluster_started(const Place &p) {
-    if (p.ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+// ---- how a chunk gets to its lanes ----------------------------------------------------------------------------------
+// Ring: a warp's chunks are boxes of T steps x 32 V columns that the copy engine brings into the warp's own part of
+// shared memory, DEPTH of them in flight; lane 0 asks for the box of the chunk DEPTH rounds ahead when all lanes are done
+// with a stage.  This needs 16-byte aligned rows.  Without a ring (other layouts, and a few steps, where setting it up
+// costs more) the next chunk is loaded to registers while the current one is worked on.
+template <typename TT> struct Cut {
+    static constexpr int kFwdT = sizeof(TT) == 2 ? 16 : 8;      // steps of a slice's chunk, forward, with a ring
+    static constexpr int kFwdDepth = 3;
+    static constexpr int kBwdDepth = sizeof(TT) == 2 ? 4 : 2;
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+template <typename P> __device__ __forceinline__ P load_shared(uint32_t addr) {
+    P p;
+    if constexpr (sizeof(P) == 16) {
+        uint4 v;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+        memcpy(&p, &v, 16);
+    } else if constexpr (sizeof(P) == 8) {
+        uint2 v;
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+        memcpy(&p, &v, 8);
+    } else {
+        uint32_t v;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+        memcpy(&p, &v, 4);
+    }
+    return p;
 }
 
-// SPLIT: the slices' chunks are scanned locally, c_t = C_t + P_t c_in, and finished once c_in is known.
-template <typename TT, int T, bool SPLIT>
-__global__ void __launch_bounds__(SPLIT ? 256 : 64, SPLIT ? 3 : 8)
-linear_recurrence_fwd_kernel(const LinRecArgs a) {
-    __shared__ Exchange x[1];
+// One warp's ring.  A wait that gives up raises the device error flag; from then on the warp neither waits nor asks for
+// copies, but keeps taking part in its CTA's barriers.
+template <int DEPTH> struct Ring {
+    uint32_t data, bars, bytes;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool dead = false;
+    __device__ __forceinline__ void start(uint32_t data_, uint32_t bars_, uint32_t bytes_, int lane) {
+        data = data_; bars = bars_; bytes = bytes_;
+        if (lane == 0) {
+            for (int s = 0; s < DEPTH; ++s) mbar_init(bars + 8 * s, 1);
+            fence_mbar_init();
+            fence_proxy_async();
+        }
+        __syncwarp();
+    }
+    __device__ __forceinline__ uint32_t at() const { return data + stage * bytes; }
+    __device__ __forceinline__ uint32_t bar() const { return bars + 8 * stage; }
+    __device__ __forceinline__ void wait(int *err) {
+        if (dead || mbar_wait_bounded(bar(), phase)) return;
+        dead = true;
+        atomicExch(err, 41);
+        for (int s = 0; s < DEPTH; ++s)             // copies still in flight land before the CTA can leave
+            mbar_wait_bounded(bars + 8 * s, s < stage ? phase ^ 1 : phase);
+    }
+    __device__ __forceinline__ void next() { if (++stage == DEPTH) { stage = 0; phase ^= 1; } }
+};
+
+constexpr int kBarBytes = 256;
+template <int V, int DEPTH> constexpr size_t ring_shared(int warps, size_t stage, bool split) {
+    return (split ? sizeof(Exchange<V>) : 0) + kBarBytes + 128 + (size_t)warps * DEPTH * stage;
+}
+
+// ---- forward --------------------------------------------------------------------------------------------------------
+// A chunk scanned from 0 in registers, with the products of f: the state after step i is C[i] + P[i] c_in, whatever c_in
+// turns out to be.  CLEAN: no step is padded.
+template <typename TT, int V, int T, bool CLEAN, typename In>
+__device__ __forceinline__ void scan_local(In in, Num<V> nb, unsigned flags, Num<V> (&C)[T], Num<V> (&P)[T]) {
+    Num<V> lc = all<V>(0.0f), lp = all<V>(1.0f);
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+        Num<V> x, g, f, keep;
+        unpair<TT, V>(in(i), &x, &g);
+        gate<V>(g, nb, &f, &keep);
+        const bool pad = !CLEAN && ((flags >> i) & 1u);
+        const Num<V> n = fma(f, lc, mul(keep, x));
+        lc = CLEAN ? n : pick(pad, lc, n);
+        lp = CLEAN ? mul(lp, f) : pick(pad, lp, mul(lp, f));
+        C[i] = lc;
+        P[i] = lp;
+    }
+}
+
+template <typename TT, int V, int T, bool SPLIT, bool RING>
+__global__ void __launch_bounds__(SPLIT ? 256 : 64, SPLIT ? 2 : 6)
+linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const LinRecArgs a) {
+    extern __shared__ __align__(128) uint8_t shared[];
+    Exchange<V> *x = reinterpret_cast<Exchange<V> *>(shared);
     Place p;
-    if (!find_place<SPLIT>(a, &p)) return;
-    const TT *u = static_cast<const TT *>(a.u) + p.b * a.u_b + 2 * p.j;
-    TT *h = static_cast<TT *>(a.h) + p.col;
-    const uint8_t *mask = a.mask ? a.mask + p.b : nullptr;
-    const float nb = (p.on && a.bias) ? a.bias[p.j] * kNegLog2e : 0.0f;
-    float carry = (p.on && a.first) ? a.first[p.col] : 0.0f;
+    if (!find_place<V, SPLIT>(a, &p)) return;
+    const Num<V> nb = mul(load_small<V>(a.bias, p.j), all<V>(kNegLog2e));
+    Num<V> carry = load_small<V>(a.first, p.col);
     const int slices = SPLIT ? p.warps * (int)p.ranks : 1;
     const int slice = SPLIT ? (int)p.rank * p.warps + p.warp : 0;
     const int64_t round = (int64_t)slices * T;
-    Pack<TT, 2> next[T];
-    unsigned next_flags;
-    auto fetch = [&](int64_t t0) {
-        load_steps<TT, 2, T>(next, u + t0 * a.u_t, a.u_t, a.L - t0, p.on);
-        next_flags = load_flags<T>(mask ? mask + t0 * a.m_t : nullptr, a.m_t, a.L - t0, p.lane);
+    int64_t left = a.L - (int64_t)slice * T;        // steps from the start of this warp's chunk to the end
+    const TT *u = static_cast<const TT *>(a.u) + p.b * a.u_b + 2 * p.j + (int64_t)slice * T * a.u_t;
+    TT *h = static_cast<TT *>(a.h) + p.col + (int64_t)slice * T * a.h_t;
+    const uint8_t *mask = a.mask ? a.mask + p.b + (int64_t)slice * T * a.m_t : nullptr;
+    const int64_t states_t = a.B * a.d;
+    float *states = a.states ? a.states + (int64_t)slice * (T / kT) * states_t + p.col : nullptr;
+
+    constexpr uint32_t kRow = 32 * V * 2 * sizeof(TT);
+    constexpr int DEPTH = Cut<TT>::kFwdDepth;
+    Ring<DEPTH> ring;
+    const bool back = a.h_t < 0;                    // time runs backwards: the box's rows as well
+    auto ask = [&](int64_t n, uint32_t to, uint32_t bar) {      // the box of the chunk in front of which n steps are left
+        if (p.lane == 0 && n > 0 && !ring.dead) {
+            mbar_arrive_expect_tx(bar, T * kRow);
+            tma_load_3d(to, &map_u, bar, 2 * (p.j - p.shift), (int)p.b, (int)(back ? n - T : a.L - n));
+        }
     };
-    fetch((int64_t)slice * T);
-    if (SPLIT) cluster_started(p);
+    Pack<TT, 2 * V> next[RING ? 1 : T];
+    unsigned next_flags;
+    if constexpr (RING) {
+        const uint32_t base = smem_u32(shared) + (SPLIT ? (uint32_t)sizeof(Exchange<V>) : 0u);
+        ring.start(base + kBarBytes + p.warp * DEPTH * T * kRow, base + p.warp * DEPTH * 8, T * kRow, p.lane);
+        for (int s = 0; s < DEPTH; ++s) ask(left - s * round, ring.data + s * T * kRow, ring.bars + 8 * s);
+    } else {
+        load_steps<TT, 2 * V, T>(next, u, a.u_t, left);
+    }
+    next_flags = load_flags<T>(mask, a.m_t, left, p.lane);
+    if (SPLIT && p.ranks > 1) cluster_sync();       // every CTA has started before another writes to its shared memory
     int buf = 0;
-    for (int64_t r0 = 0; r0 < a.L; r0 += round, buf ^= 1) {
-        const int64_t t0 = r0 + (int64_t)slice * T;
-        PairLoad<TT> cur[T];
-#pragma unroll
-        for (int i = 0; i < T; ++i) cur[i].p = next[i];
+    for (int64_t r0 = 0; r0 < a.L; r0 += round, buf ^= 1, left -= round) {
         const unsigned flags = next_flags;
-        if (r0 + round < a.L) fetch(t0 + round);
-        float c = carry;
-        if (SPLIT) {
-            float C[T], P[T];
-            float lc = 0.0f, lp = 1.0f;
-#pragma unroll
-            for (int i = 0; i < T; ++i) {
-                const bool pad = (flags >> i) & 1u;
-                float f, keep;
-                gate(cur[i].g(), nb, &f, &keep);
-                const float n = fmaf(f, lc, keep * cur[i].x());
-                lc = pad ? lc : n;
-                lp = pad ? lp : lp * f;
-                C[i] = lc;
-                P[i] = lp;
-            }
-            c = exchange(x[0], buf, p, lp, lc, false, &carry);
-            if (a.states && p.on && t0 < a.L) a.states[(t0 / kT) * a.B * a.d + p.col] = c;
-            if (p.on) {
-#pragma unroll
-                for (int i = 0; i < T; ++i)
-                    if (t0 + i < a.L) h[(t0 + i) * a.h_t] = Cvt<TT>::from_f((flags >> i) & 1u ? 0.0f : fmaf(P[i], c, C[i]));
-            }
+        if (r0 + round < a.L) {
+            if (mask) mask += round * a.m_t;
+            next_flags = load_flags<T>(mask, a.m_t, left - round, p.lane);
+        }
+        Pack<TT, 2 * V> cur[RING ? 1 : T];
+        uint32_t row = 0;
+        int32_t row_step = 0;
+        if constexpr (RING) {
+            if (left > 0) ring.wait(a.err);
+            row = ring.at() + p.shift * 2 * sizeof(TT) + (back ? (T - 1) * kRow : 0u);
+            row_step = back ? -(int32_t)kRow : (int32_t)kRow;
         } else {
 #pragma unroll
-            for (int i = 0; i < T; ++i) {
-                if (i % kT == 0 && a.states && p.on && t0 + i < a.L) a.states[((t0 + i) / kT) * a.B * a.d + p.col] = c;
-                const bool pad = (flags >> i) & 1u;
-                float f, keep;
-                gate(cur[i].g(), nb, &f, &keep);
-                const float n = fmaf(f, c, keep * cur[i].x());
-                c = pad ? c : n;
-                if (p.on && t0 + i < a.L) h[(t0 + i) * a.h_t] = Cvt<TT>::from_f(pad ? 0.0f : n);
+            for (int i = 0; i < T; ++i) cur[i] = next[i];
+            if (r0 + round < a.L) {
+                u += round * a.u_t;
+                load_steps<TT, 2 * V, T>(next, u, a.u_t, left - round);
             }
-            carry = c;
         }
+        auto in = [&](int i) -> Pack<TT, 2 * V> {
+            if constexpr (RING) return load_shared<Pack<TT, 2 * V>>(row + i * row_step);
+            else return cur[i];
+        };
+        auto release = [&]() {
+            if constexpr (RING) {
+                __syncwarp();
+                ask(left - DEPTH * round, ring.at(), ring.bar());
+                ring.next();
+            }
+        };
+        if constexpr (SPLIT) {
+            Num<V> C[T], P[T];
+            if (flags == 0) scan_local<TT, V, T, true>(in, nb, flags, C, P);
+            else scan_local<TT, V, T, false>(in, nb, flags, C, P);
+            release();
+            const Num<V> c = exchange<V, false>(*x, buf, p, Map<V>{P[T - 1], C[T - 1]}, &carry);
+            if (states) {
+#pragma unroll
+                for (int i = 0; i < T; i += kT)
+                    if (i < left) store_state<V>(states + (i / kT) * states_t, i ? fma(P[i - 1], c, C[i - 1]) : c);
+            }
+            TT *q = h;
+            if (flags == 0) {
+#pragma unroll
+                for (int i = 0; i < T; ++i, q += a.h_t)
+                    *reinterpret_cast<Pack<TT, V> *>(q) = rounded<TT>(fma(P[i], c, C[i]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < T; ++i, q += a.h_t)
+                    if (i < left)
+                        *reinterpret_cast<Pack<TT, V> *>(q) = rounded<TT>(pick((flags >> i) & 1u, all<V>(0.0f), fma(P[i], c, C[i])));
+            }
+        } else {
+            TT *q = h;
+            auto walk = [&](auto clean) {
+                constexpr bool CLEAN = decltype(clean)::value;
+#pragma unroll
+                for (int i = 0; i < T; ++i, q += a.h_t) {
+                    if (i % kT == 0 && states && (CLEAN || i < left)) store_state<V>(states + (i / kT) * states_t, carry);
+                    Num<V> xi, g, f, keep;
+                    unpair<TT, V>(in(i), &xi, &g);
+                    gate<V>(g, nb, &f, &keep);
+                    const bool pad = !CLEAN && ((flags >> i) & 1u);
+                    const Num<V> n = fma(f, carry, mul(keep, xi));
+                    carry = CLEAN ? n : pick(pad, carry, n);
+                    if (CLEAN || i < left)
+                        *reinterpret_cast<Pack<TT, V> *>(q) = rounded<TT>(CLEAN ? n : pick(pad, all<V>(0.0f), n));
+                }
+            };
+            if (flags == 0) walk(std::true_type());
+            else walk(std::false_type());
+            release();
+        }
+        h += round * a.h_t;
+        if (states) states += (int64_t)slices * (T / kT) * states_t;
     }
-    if (slice == 0 && p.on && a.last) a.last[p.col] = carry;
+    if (slice == 0 && a.last) store_small<V>(a.last, p.col, carry);
 }
 
-template <typename TT, bool SPLIT>
+// ---- backward -------------------------------------------------------------------------------------------------------
+template <typename TT, int V, bool SPLIT, bool RING>
 __global__ void __launch_bounds__(SPLIT ? 256 : 64, SPLIT ? 2 : 8)
-linear_recurrence_bwd_kernel(const LinRecArgs a) {
-    __shared__ Exchange x[1];
+linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_g, const LinRecArgs a) {
+    extern __shared__ __align__(128) uint8_t shared[];
+    Exchange<V> *x = reinterpret_cast<Exchange<V> *>(shared);
     constexpr int T = kT;
     Place p;
-    if (!find_place<SPLIT>(a, &p)) return;
-    const TT *u = static_cast<const TT *>(a.u) + p.b * a.u_b + 2 * p.j;
-    const TT *gh = a.grad_h ? static_cast<const TT *>(a.grad_h) + p.b * a.gh_b + p.j : nullptr;
-    TT *gu = static_cast<TT *>(a.h) + 2 * p.col;
-    const uint8_t *mask = a.mask ? a.mask + p.b : nullptr;
-    const float nb = (p.on && a.bias) ? a.bias[p.j] * kNegLog2e : 0.0f;
-    float carry = (p.on && a.first) ? a.first[p.col] : 0.0f, db = 0.0f;
+    if (!find_place<V, SPLIT>(a, &p)) return;
+    const Num<V> nb = mul(load_small<V>(a.bias, p.j), all<V>(kNegLog2e));
+    Num<V> carry = load_small<V>(a.first, p.col), db = all<V>(0.0f);
     const int slices = SPLIT ? p.warps * (int)p.ranks : 1;
     const int slice = SPLIT ? (int)p.rank * p.warps + p.warp : 0;
     const int64_t round = (int64_t)slices * T;
-    Pack<TT, 2> next_u[T];
-    Pack<TT, 1> next_g[T];
-    float next_c = 0.0f;
-    unsigned next_flags;
-    auto fetch = [&](int64_t t0) {
-        if (p.on && t0 < a.L) next_c = a.states[(t0 / T) * a.B * a.d + p.col];
-        load_steps<TT, 2, T>(next_u, u + t0 * a.u_t, a.u_t, a.L - t0, p.on);
-        load_steps<TT, 1, T>(next_g, gh + t0 * a.gh_t, a.gh_t, a.L - t0, p.on && gh);
-        next_flags = load_flags<T>(mask ? mask + t0 * a.m_t : nullptr, a.m_t, a.L - t0, p.lane);
+    const int64_t r_top = (a.L - 1) / round * round, t_top = r_top + (int64_t)slice * T;
+    int64_t left = a.L - t_top;
+    const TT *u = static_cast<const TT *>(a.u) + p.b * a.u_b + 2 * p.j + t_top * a.u_t;
+    const TT *gh = a.grad_h ? static_cast<const TT *>(a.grad_h) + p.b * a.gh_b + p.j + t_top * a.gh_t : nullptr;
+    TT *gu = static_cast<TT *>(a.h) + 2 * (p.col + t_top * a.h_t);
+    const uint8_t *mask = a.mask ? a.mask + p.b + t_top * a.m_t : nullptr;
+    const int64_t states_t = a.B * a.d;
+    const float *states = a.states + (t_top / T) * states_t + p.col;
+
+    constexpr uint32_t kRowU = 32 * V * 2 * sizeof(TT), kRowG = kRowU / 2, kStage = T * (kRowU + kRowG);
+    constexpr int DEPTH = Cut<TT>::kBwdDepth;
+    Ring<DEPTH> ring;
+    const bool back = a.h_t < 0;
+    auto ask = [&](int64_t n, bool more, uint32_t to, uint32_t bar) {
+        if (p.lane == 0 && more && n <= 0) {
+            mbar_arrive(bar);           // a chunk behind the end (first round only): the stage's turn passes empty
+        } else if (p.lane == 0 && more && !ring.dead) {
+            const int t = (int)(back ? n - T : a.L - n), j0 = p.j - p.shift;
+            mbar_arrive_expect_tx(bar, gh ? kStage : T * kRowU);
+            tma_load_3d(to, &map_u, bar, 2 * j0, (int)p.b, t);
+            if (gh) tma_load_3d(to + T * kRowU, &map_g, bar, j0, (int)p.b, t);
+        }
     };
-    const int64_t r_top = (a.L - 1) / round * round;
-    fetch(r_top + (int64_t)slice * T);
-    if (SPLIT) cluster_started(p);
+    Pack<TT, 2 * V> next_u[RING ? 1 : T];
+    Pack<TT, V> next_g[RING ? 1 : T];
+    Num<V> next_c = all<V>(0.0f);
+    unsigned next_flags;
+    auto fetch = [&](int64_t n) {
+        if (n > 0) next_c = load_state<V>(states);
+        if constexpr (!RING) {
+            load_steps<TT, 2 * V, T>(next_u, u, a.u_t, n);
+            if (gh) load_steps<TT, V, T>(next_g, gh, a.gh_t, n);
+            else memset(&next_g, 0, sizeof(next_g));
+        }
+        next_flags = load_flags<T>(mask, a.m_t, n, p.lane);
+    };
+    if constexpr (RING) {
+        const uint32_t base = smem_u32(shared) + (SPLIT ? (uint32_t)sizeof(Exchange<V>) : 0u);
+        ring.start(base + kBarBytes + p.warp * DEPTH * kStage, base + p.warp * DEPTH * 8, kStage, p.lane);
+        for (int s = 0; s < DEPTH; ++s) ask(left + s * round, r_top >= s * round, ring.data + s * kStage, ring.bars + 8 * s);
+    }
+    fetch(left);
+    if (SPLIT && p.ranks > 1) cluster_sync();
     int buf = 0;
-    for (int64_t r0 = r_top; r0 >= 0; r0 -= round, buf ^= 1) {
-        const int64_t t0 = r0 + (int64_t)slice * T;
-        float f[T], keep[T], w[T];      // w = (c_{t-1} - x) f (1 - f)
-        Pack<TT, 1> g[T];
+    for (int64_t r0 = r_top; r0 >= 0; r0 -= round, buf ^= 1, left += round) {
         const unsigned flags = next_flags;
-        {
-            PairLoad<TT> cur[T];
-            float c = next_c;
+        Num<V> c = next_c;
+        Num<V> f[T], keep[T], w[T];      // w = (c_{t-1} - x) f (1 - f)
+        Pack<TT, V> g[T];
+        Pack<TT, 2 * V> cur[RING ? 1 : T];
+        uint32_t row = 0;
+        int32_t row_step = 0;
+        if constexpr (!RING) {
 #pragma unroll
-            for (int i = 0; i < T; ++i) { cur[i].p = next_u[i]; g[i] = next_g[i]; }
-            if (r0 > 0) fetch(t0 - round);
+            for (int i = 0; i < T; ++i) { cur[i] = next_u[i]; g[i] = next_g[i]; }
+        }
+        if (r0 > 0) {
+            if constexpr (!RING) {
+                u -= round * a.u_t;
+                if (gh) gh -= round * a.gh_t;
+            }
+            if (mask) mask -= round * a.m_t;
+            states -= (int64_t)slices * states_t;
+            fetch(left + round);
+        }
+        if constexpr (RING) {
+            if (left > 0) ring.wait(a.err);
+            row = ring.at() + p.shift * 2 * sizeof(TT) + (back ? (T - 1) * kRowU : 0u);
+            row_step = back ? -(int32_t)kRowU : (int32_t)kRowU;
+            uint32_t grow = ring.at() + T * kRowU + p.shift * sizeof(TT) + (back ? (T - 1) * kRowG : 0u);
+#pragma unroll
+            for (int i = 0; i < T; ++i, grow += row_step / 2) {
+                if (gh) g[i] = load_shared<Pack<TT, V>>(grow);
+                else memset(&g[i], 0, sizeof(g[i]));
+            }
+        }
+        auto in = [&](int i) -> Pack<TT, 2 * V> {
+            if constexpr (RING) return load_shared<Pack<TT, 2 * V>>(row + i * row_step);
+            else return cur[i];
+        };
+        const Num<V> zero = all<V>(0.0f), one = all<V>(1.0f);
+        Map<V> own{one, zero};
+        auto recompute = [&](auto clean) {
+            constexpr bool CLEAN = decltype(clean)::value;
 #pragma unroll
             for (int i = 0; i < T; ++i) {
-                const bool pad = (flags >> i) & 1u;
-                const float xi = cur[i].x();
-                float fi, ki;
-                gate(cur[i].g(), nb, &fi, &ki);
-                w[i] = pad ? 0.0f : (c - xi) * fi * ki;
-                c = pad ? c : fmaf(fi, c, ki * xi);
-                f[i] = pad ? 1.0f : fi;
-                keep[i] = pad ? 0.0f : ki;
+                const bool pad = !CLEAN && ((flags >> i) & 1u);
+                Num<V> xi, gi, fi, ki;
+                unpair<TT, V>(in(i), &xi, &gi);
+                gate<V>(gi, nb, &fi, &ki);
+                const Num<V> wi = mul(mul(sub(c, xi), fi), ki), ci = fma(fi, c, mul(ki, xi));
+                w[i] = CLEAN ? wi : pick(pad, zero, wi);
+                c = CLEAN ? ci : pick(pad, c, ci);
+                f[i] = CLEAN ? fi : pick(pad, one, fi);
+                keep[i] = CLEAN ? ki : pick(pad, zero, ki);
             }
-        }
-        float dc = carry;
-        if (SPLIT) {
-            float lc = 0.0f, lp = 1.0f;
+            if constexpr (SPLIT) {
 #pragma unroll
-            for (int i = T - 1; i >= 0; --i) {
-                lc = f[i] * ((flags >> i) & 1u ? lc : lc + Cvt<TT>::to_f(g[i].v[0]));
-                lp *= f[i];
+                for (int i = T - 1; i >= 0; --i) {
+                    const bool pad = !CLEAN && ((flags >> i) & 1u);
+                    const Num<V> s = add(own.C, widened<TT>(g[i]));
+                    own.C = mul(f[i], CLEAN ? s : pick(pad, own.C, s));
+                    own.P = mul(own.P, f[i]);
+                }
             }
-            dc = exchange(x[0], buf, p, lp, lc, true, &carry);
+        };
+        if (flags == 0) recompute(std::true_type());
+        else recompute(std::false_type());
+        if constexpr (RING) {
+            __syncwarp();
+            ask(left + DEPTH * round, r0 >= DEPTH * round, ring.at(), ring.bar());
+            ring.next();
         }
+        Num<V> dc = carry;
+        if constexpr (SPLIT) dc = exchange<V, true>(*x, buf, p, own, &carry);
+        auto finish = [&](auto clean) {
+            constexpr bool CLEAN = decltype(clean)::value;
+            TT *q = gu + 2 * (T - 1) * a.h_t;
 #pragma unroll
-        for (int i = T - 1; i >= 0; --i) {
-            const bool pad = (flags >> i) & 1u;
-            const float total = pad ? dc : dc + Cvt<TT>::to_f(g[i].v[0]);
-            const float dg = pad ? 0.0f : w[i] * total;
-            Pack<TT, 2> out;
-            out.v[0] = Cvt<TT>::from_f(pad ? 0.0f : keep[i] * total);
-            out.v[1] = Cvt<TT>::from_f(dg);
-            db += dg;
-            dc = f[i] * total;
-            if (p.on && t0 + i < a.L) *reinterpret_cast<Pack<TT, 2> *>(gu + 2 * (t0 + i) * a.h_t) = out;
-        }
+            for (int i = T - 1; i >= 0; --i, q -= 2 * a.h_t) {
+                const bool pad = !CLEAN && ((flags >> i) & 1u);
+                const Num<V> s = add(dc, widened<TT>(g[i]));
+                const Num<V> total = CLEAN ? s : pick(pad, dc, s);
+                Num<V> dx = mul(keep[i], total), dg = mul(w[i], total);
+                if (!CLEAN) { dx = pick(pad, zero, dx); dg = pick(pad, zero, dg); }
+                db = add(db, dg);
+                dc = mul(f[i], total);
+                Pack<TT, 2 * V> out;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const Pack<TT, 2> o = pack2<TT>(dx.get(v), dg.get(v));
+                    out.v[2 * v] = o.v[0];
+                    out.v[2 * v + 1] = o.v[1];
+                }
+                if (CLEAN || i < left) *reinterpret_cast<Pack<TT, 2 * V> *>(q) = out;
+            }
+        };
+        if (flags == 0) finish(std::true_type());
+        else finish(std::false_type());
         if (!SPLIT) carry = dc;
+        gu -= 2 * round * a.h_t;
     }
-    if (p.on) {
-        if (a.last && slice == 0) a.last[p.col] = carry;
-        if (a.bias_part) a.bias_part[(p.b * slices + slice) * a.d + p.j] = db;
-    }
+    if (a.last && slice == 0) store_small<V>(a.last, p.col, carry);
+    if (a.bias_part) store_small<V>(a.bias_part, (p.b * slices + slice) * a.d + p.j, db);
 }
 
 // grad_bias[j] = sum over the parts in a fixed order: 8 slices of the parts per column, then the slices.
@@ -370,7 +674,7 @@ void reverse_time(LinRecArgs *a, size_t size, int units) {
 }
 
 Slices choose_slices(int64_t L, int64_t B, int64_t d) {
-    const int64_t columns = (d + 31) / 32 * B;              // warps that one walk over time takes
+    const int64_t columns = (d + 63) / 64 * B;              // warps that one walk over time takes
     int64_t want = option(OPT_LINREC_SLICES, 0);
     if (want <= 0) {
         want = 1;
@@ -383,38 +687,101 @@ Slices choose_slices(int64_t L, int64_t B, int64_t d) {
     return s;
 }
 
-template <typename TT> int launch(const LinRecArgs &a0, const Slices &s, bool backward, cudaStream_t st) {
-    LinRecArgs a = a0;
-    a.groups = (a.d + 31) / 32;
+// Boxes of `cols` elements, one sequence and `steps` steps; outside reads as zero.
+template <typename TT>
+int make_box(CUtensorMap *map, const void *base, int64_t inner, int64_t B, int64_t L, int64_t s_b, int64_t s_t, int cols, int steps) {
+    auto fn = get_encode_fn();
+    if (!fn) return set_error(SRU_ERR_CUDA, "cuTensorMapEncodeTiled entry point not found");
+    const CUtensorMapDataType type = sizeof(TT) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : std::is_same<TT, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)B, (cuuint64_t)L};
+    cuuint64_t strides[2] = {(cuuint64_t)s_b * sizeof(TT), (cuuint64_t)s_t * sizeof(TT)};
+    cuuint32_t box[3] = {(cuuint32_t)cols, 1, (cuuint32_t)steps}, estr[3] = {1, 1, 1};
+    CUresult r = fn(map, type, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(SRU_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
+    return 0;
+}
+
+struct Maps { CUtensorMap u, g; };
+
+template <typename TT, int V, bool SPLIT, bool RING>
+int launch(LinRecArgs a, const Slices &s, const Maps &maps, bool backward, cudaStream_t st) {
+    // a slice's chunk is the same with and without a ring, and with it the order of all roundings: bits do not depend on layout
+    constexpr int T = SPLIT || RING ? Cut<TT>::kFwdT : 2 * kT;
+    constexpr size_t kRow = 32 * V * 2 * sizeof(TT);
+    auto fwd = linear_recurrence_fwd_kernel<TT, V, T, SPLIT, RING>;
+    auto bwd = linear_recurrence_bwd_kernel<TT, V, SPLIT, RING>;
+    a.groups = (a.d + 32 * V - 1) / (32 * V);
     const int64_t columns = (int64_t)a.groups * a.B;
-    if (columns * s.ranks > 0x7fffffff) return set_error(SRU_ERR_UNSUPPORTED, "linear recurrence: batch * hidden too large");
+    const int warps = SPLIT ? s.warps : 2;
+    const int64_t blocks = SPLIT ? columns * s.ranks : (columns + 1) / 2;
+    if (blocks > 0x7fffffff) return set_error(SRU_ERR_UNSUPPORTED, "linear recurrence: batch * hidden too large");
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.stream = st;
+    cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+    cfg.blockDim = dim3(32 * warps, 1, 1);
+    cfg.dynamicSmemBytes = SPLIT ? sizeof(Exchange<V>) : 0;
+    if (RING) {
+        constexpr size_t f = ring_shared<V, Cut<TT>::kFwdDepth>(SPLIT ? kMaxWarps : 2, T * kRow, SPLIT);
+        constexpr size_t b = ring_shared<V, Cut<TT>::kBwdDepth>(SPLIT ? kMaxWarps : 2, kT * kRow * 3 / 2, SPLIT);
+        static bool attr_set[64] = {false};
+        int dev = 0;
+        SRUB_CUDA_CHECK(cudaGetDevice(&dev));
+        if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+            SRUB_CUDA_CHECK(cudaFuncSetAttribute(fwd, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f));
+            SRUB_CUDA_CHECK(cudaFuncSetAttribute(bwd, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)b));
+            attr_set[dev] = true;
+        }
+        cfg.dynamicSmemBytes = backward ? ring_shared<V, Cut<TT>::kBwdDepth>(warps, kT * kRow * 3 / 2, SPLIT)
+                                        : ring_shared<V, Cut<TT>::kFwdDepth>(warps, T * kRow, SPLIT);
+    }
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)s.ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    if (s.count() > 1) {
-        cfg.gridDim = dim3((unsigned)(columns * s.ranks), 1, 1);
-        cfg.blockDim = dim3(32 * s.warps, 1, 1);
-        cfg.numAttrs = 1;
-        if (backward) SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_recurrence_bwd_kernel<TT, true>, a));
-        else SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_recurrence_fwd_kernel<TT, kT, true>, a));
-    } else {
-        cfg.gridDim = dim3((unsigned)((columns + 1) / 2), 1, 1);
-        cfg.blockDim = dim3(64, 1, 1);
-        if (backward) SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_recurrence_bwd_kernel<TT, false>, a));
-        else SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_recurrence_fwd_kernel<TT, 2 * kT, false>, a));
-    }
+    cfg.numAttrs = SPLIT ? 1 : 0;
+    if (backward) SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, bwd, maps.u, maps.g, a));
+    else SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fwd, maps.u, a));
     return 0;
 }
 
-int dispatch(const LinRecArgs &a, const Slices &s, int dtype, bool backward, cudaStream_t st) {
+// Two columns per lane and a ring where all rows are 16-byte aligned and pairs of columns aligned to their size.
+bool ring_fits(const LinRecArgs &a, int64_t size, bool backward) {
+    auto at = [](const void *p, int64_t unit) { return reinterpret_cast<uintptr_t>(p) % unit == 0; };
+    auto rows = [&](const void *p, int64_t t, int64_t b) {
+        return at(p, 16) && t > 0 && t * size % 16 == 0 && (a.B == 1 || (b > 0 && b * size % 16 == 0));
+    };
+    if (a.L < 2 * kT || a.d % 2 || a.L > 0x7fffffff - 1024 || a.B > 0x7fffffff || !at(a.states, 8)) return false;
+    if (!at(a.h, (backward ? 4 : 2) * size) || !rows(a.u, a.u_t, a.u_b)) return false;
+    return !a.grad_h || rows(a.grad_h, a.gh_t, a.gh_b);
+}
+
+template <typename TT> int launch_typed(LinRecArgs a, const Slices &s, bool reverse, bool backward, cudaStream_t st) {
+    Maps maps;
+    memset(&maps, 0, sizeof(maps));
+    const bool ring = ring_fits(a, sizeof(TT), backward);
+    if (ring) {
+        if (int rc = ensure_context()) return rc;
+        const bool one = a.B == 1;       // the stride of a single sequence is never taken
+        int rc = make_box<TT>(&maps.u, a.u, 2 * a.d, a.B, a.L, one ? a.u_t : a.u_b, a.u_t, 128, backward ? kT : Cut<TT>::kFwdT);
+        if (!rc && a.grad_h) rc = make_box<TT>(&maps.g, a.grad_h, a.d, a.B, a.L, one ? a.gh_t : a.gh_b, a.gh_t, 64, kT);
+        if (rc) return rc;
+    }
+    a.err = device_error_flag();
+    if (!a.err) return set_error(SRU_ERR_CUDA, "device error flag unavailable");
+    if (reverse) reverse_time(&a, sizeof(TT), backward ? 2 : 1);
+    const bool split = s.count() > 1;
+    if (ring) return split ? launch<TT, 2, true, true>(a, s, maps, backward, st) : launch<TT, 2, false, true>(a, s, maps, backward, st);
+    return split ? launch<TT, 1, true, false>(a, s, maps, backward, st) : launch<TT, 1, false, false>(a, s, maps, backward, st);
+}
+
+int dispatch(const LinRecArgs &a, const Slices &s, int dtype, bool reverse, bool backward, cudaStream_t st) {
     switch (dtype) {
-        case SRU_F16: return launch<__half>(a, s, backward, st);
-        case SRU_BF16: return launch<__nv_bfloat16>(a, s, backward, st);
-        default: return launch<float>(a, s, backward, st);
+        case SRU_F16: return launch_typed<__half>(a, s, reverse, backward, st);
+        case SRU_BF16: return launch_typed<__nv_bfloat16>(a, s, reverse, backward, st);
+        default: return launch_typed<float>(a, s, reverse, backward, st);
     }
 }
 
@@ -449,8 +816,7 @@ int sru_b200_linear_recurrence_forward(void *h, float *c_last, void *states, con
     a.L = length; a.B = batch; a.d = (int)hidden;
     a.u_t = u_stride_t; a.u_b = u_stride_b;
     a.h_t = batch * hidden; a.m_t = batch;
-    if (reverse) reverse_time(&a, size, 1);
-    return dispatch(a, choose_slices(length, batch, hidden), dtype, false, static_cast<cudaStream_t>(stream));
+    return dispatch(a, choose_slices(length, batch, hidden), dtype, reverse != 0, false, static_cast<cudaStream_t>(stream));
 }
 
 size_t sru_b200_linear_recurrence_backward_workspace_bytes(int64_t length, int64_t batch, int64_t hidden) {
@@ -485,9 +851,8 @@ int sru_b200_linear_recurrence_backward(void *grad_u, float *grad_bias, float *g
     a.L = length; a.B = batch; a.d = (int)hidden;
     a.u_t = u_stride_t; a.u_b = u_stride_b; a.gh_t = gh_stride_t; a.gh_b = gh_stride_b;
     a.h_t = batch * hidden; a.m_t = batch;
-    if (reverse) reverse_time(&a, size, 2);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    rc = dispatch(a, s, dtype, true, st);
+    rc = dispatch(a, s, dtype, reverse != 0, true, st);
     if (rc || !grad_bias) return rc;
     linear_recurrence_bias_kernel<<<(unsigned)((hidden + 31) / 32), 256, 0, st>>>(grad_bias, a.bias_part,
                                                                                    batch * s.count(), (int)hidden);

@@ -111,6 +111,15 @@ def test_few_and_many_columns(L, B, d):
     check(L, B, d, F32, seed=L + 1, reverse=True)
 
 
+@pytest.mark.parametrize("slices", [1, 2, 3, 7, 8, 9, 16, 24, 33, 64])
+def test_every_cut_of_time(slices):
+    """The number of slices a column's time is cut into (option linrec_slices) changes only the order of roundings."""
+    with _lib.options(linrec_slices=slices):
+        check(700, 3, 70, BF16, seed=slices)
+        check(1025, 2, 33, F32, seed=slices, reverse=True)
+        check(8 * slices + 1, 2, 64, F16, seed=slices, mask=False)
+
+
 def test_empty():
     for L, B in ((0, 3), (4, 0), (0, 0)):
         check(L, B, 8, F32, mask=False)
@@ -204,7 +213,7 @@ def test_strides_and_unused_gradients():
 def test_single_steps_equal_the_sequence():
     """Token by token, the state handed on: the same arithmetic as one pass in a single walk over time."""
     u, c0, b, m, *_ = (None if t is None else t.to(DEV) for t in make(12, 5, 80, BF16, 2))
-    with torch.no_grad():
+    with torch.no_grad(), _lib.options(linrec_slices=1):
         h, c = gated_linear_recurrence(u, c0, b, m)
         state = c0
         for t in range(12):

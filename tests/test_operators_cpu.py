@@ -33,7 +33,7 @@ def test_linear_recurrence_c_arguments():
     g = L.sru_b200_linear_recurrence_backward
     assert g(one, None, None, one, None, None, None, None, None, 4, 2, 8, 32, 16, 16, 8, 0, 0, None, 0, None) == -1
     assert g(one, one, None, one, one, one, None, None, None, 4, 2, 8, 32, 16, 16, 8, 0, 0, None, 0, None) == -3
-    assert L.sru_b200_linear_recurrence_states_bytes(17, 3, 5) == 2 * 3 * 5 * 4
+    assert L.sru_b200_linear_recurrence_states_bytes(17, 3, 5) == 3 * 3 * 5 * 4
     assert L.sru_b200_linear_recurrence_states_bytes(0, 3, 5) == 0
 
 
