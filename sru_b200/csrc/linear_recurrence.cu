@@ -274,7 +274,7 @@ __device__ __forceinline__ Num<V> exchange(Exchange<V> &x, int buf, const Place 
 template <typename TT> struct Cut {
     static constexpr int kFwdT = sizeof(TT) == 2 ? 16 : 8;      // steps of a slice's chunk, forward, with a ring
     static constexpr int kFwdDepth = 3;
-    static constexpr int kBwdDepth = sizeof(TT) == 2 ? 4 : 2;
+    static constexpr int kBwdDepth = sizeof(TT) == 2 ? 3 : 2;
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
@@ -479,7 +479,8 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
 // ---- backward -------------------------------------------------------------------------------------------------------
 template <typename TT, int V, bool SPLIT, bool RING>
 __global__ void __launch_bounds__(SPLIT ? 256 : 64, SPLIT ? 2 : 8)
-linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_g, const LinRecArgs a) {
+linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_g,
+                             const __grid_constant__ CUtensorMap map_s, const LinRecArgs a) {
     extern __shared__ __align__(128) uint8_t shared[];
     Exchange<V> *x = reinterpret_cast<Exchange<V> *>(shared);
     constexpr int T = kT;
@@ -499,7 +500,8 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
     const int64_t states_t = a.B * a.d;
     const float *states = a.states + (t_top / T) * states_t + p.col;
 
-    constexpr uint32_t kRowU = 32 * V * 2 * sizeof(TT), kRowG = kRowU / 2, kStage = T * (kRowU + kRowG);
+    constexpr uint32_t kRowU = 32 * V * 2 * sizeof(TT), kRowG = kRowU / 2, kRowS = 32 * V * 4;
+    constexpr uint32_t kStage = T * (kRowU + kRowG) + kRowS;
     constexpr int DEPTH = Cut<TT>::kBwdDepth;
     Ring<DEPTH> ring;
     const bool back = a.h_t < 0;
@@ -508,8 +510,9 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
             mbar_arrive(bar);           // a chunk behind the end (first round only): the stage's turn passes empty
         } else if (p.lane == 0 && more && !ring.dead) {
             const int t = (int)(back ? n - T : a.L - n), j0 = p.j - p.shift;
-            mbar_arrive_expect_tx(bar, gh ? kStage : T * kRowU);
+            mbar_arrive_expect_tx(bar, gh ? kStage : T * kRowU + kRowS);
             tma_load_3d(to, &map_u, bar, 2 * j0, (int)p.b, t);
+            tma_load_3d(to + T * (kRowU + kRowG), &map_s, bar, j0, (int)p.b, (int)((a.L - n) / T));
             if (gh) tma_load_3d(to + T * kRowU, &map_g, bar, j0, (int)p.b, t);
         }
     };
@@ -518,8 +521,8 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
     Num<V> next_c = all<V>(0.0f);
     unsigned next_flags;
     auto fetch = [&](int64_t n) {
-        if (n > 0) next_c = load_state<V>(states);
         if constexpr (!RING) {
+            if (n > 0) next_c = load_state<V>(states);
             load_steps<TT, 2 * V, T>(next_u, u, a.u_t, n);
             if (gh) load_steps<TT, V, T>(next_g, gh, a.gh_t, n);
             else memset(&next_g, 0, sizeof(next_g));
@@ -559,6 +562,7 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
             if (left > 0) ring.wait(a.err);
             row = ring.at() + p.shift * 2 * sizeof(TT) + (back ? (T - 1) * kRowU : 0u);
             row_step = back ? -(int32_t)kRowU : (int32_t)kRowU;
+            c = widened<float>(load_shared<Pack<float, V>>(ring.at() + T * (kRowU + kRowG) + p.shift * 4));
             uint32_t grow = ring.at() + T * kRowU + p.shift * sizeof(TT) + (back ? (T - 1) * kRowG : 0u);
 #pragma unroll
             for (int i = 0; i < T; ++i, grow += row_step / 2) {
@@ -676,9 +680,14 @@ void reverse_time(LinRecArgs *a, size_t size, int units) {
 Slices choose_slices(int64_t L, int64_t B, int64_t d) {
     const int64_t columns = (d + 63) / 64 * B;              // warps that one walk over time takes
     int64_t want = option(OPT_LINREC_SLICES, 0);
+    // One walk takes about 70 ns a step forward and 130 backward however few columns there are, which is what HBM needs
+    // for some 75 000 columns: with 1024 warps of columns (512 x 32 x 2048) one walk takes 36 / 67 us and two slices
+    // 47 / 88.  With fewer, slices fill the GPU with 14 warps an SM, all it holds at their register count: 384 warps
+    // (1000 x 24 x 1024) 49 / 107 us in one walk, 34 / 62 in four slices; 32 warps (65536 x 2048) 2670 us and 282 in 64.
     if (want <= 0) {
         want = 1;
-        while (want < 64 && columns * want * 2 <= 148 * 24) want *= 2;
+        if (columns < 148 * 6)
+            while (want < 64 && columns * want * 2 <= 148 * 14) want *= 2;
     }
     want = std::min<int64_t>(std::min<int64_t>(want, 64), (L + kT - 1) / kT);
     Slices s;
@@ -703,7 +712,7 @@ int make_box(CUtensorMap *map, const void *base, int64_t inner, int64_t B, int64
     return 0;
 }
 
-struct Maps { CUtensorMap u, g; };
+struct Maps { CUtensorMap u, g, s; };
 
 template <typename TT, int V, bool SPLIT, bool RING>
 int launch(LinRecArgs a, const Slices &s, const Maps &maps, bool backward, cudaStream_t st) {
@@ -725,7 +734,7 @@ int launch(LinRecArgs a, const Slices &s, const Maps &maps, bool backward, cudaS
     cfg.dynamicSmemBytes = SPLIT ? sizeof(Exchange<V>) : 0;
     if (RING) {
         constexpr size_t f = ring_shared<V, Cut<TT>::kFwdDepth>(SPLIT ? kMaxWarps : 2, T * kRow, SPLIT);
-        constexpr size_t b = ring_shared<V, Cut<TT>::kBwdDepth>(SPLIT ? kMaxWarps : 2, kT * kRow * 3 / 2, SPLIT);
+        constexpr size_t b = ring_shared<V, Cut<TT>::kBwdDepth>(SPLIT ? kMaxWarps : 2, kT * kRow * 3 / 2 + 32 * V * 4, SPLIT);
         static bool attr_set[64] = {false};
         int dev = 0;
         SRUB_CUDA_CHECK(cudaGetDevice(&dev));
@@ -734,7 +743,7 @@ int launch(LinRecArgs a, const Slices &s, const Maps &maps, bool backward, cudaS
             SRUB_CUDA_CHECK(cudaFuncSetAttribute(bwd, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)b));
             attr_set[dev] = true;
         }
-        cfg.dynamicSmemBytes = backward ? ring_shared<V, Cut<TT>::kBwdDepth>(warps, kT * kRow * 3 / 2, SPLIT)
+        cfg.dynamicSmemBytes = backward ? ring_shared<V, Cut<TT>::kBwdDepth>(warps, kT * kRow * 3 / 2 + 32 * V * 4, SPLIT)
                                         : ring_shared<V, Cut<TT>::kFwdDepth>(warps, T * kRow, SPLIT);
     }
     cudaLaunchAttribute attr[1];
@@ -742,7 +751,7 @@ int launch(LinRecArgs a, const Slices &s, const Maps &maps, bool backward, cudaS
     attr[0].val.clusterDim.x = (unsigned)s.ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = SPLIT ? 1 : 0;
-    if (backward) SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, bwd, maps.u, maps.g, a));
+    if (backward) SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, bwd, maps.u, maps.g, maps.s, a));
     else SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fwd, maps.u, a));
     return 0;
 }
@@ -753,7 +762,7 @@ bool ring_fits(const LinRecArgs &a, int64_t size, bool backward) {
     auto rows = [&](const void *p, int64_t t, int64_t b) {
         return at(p, 16) && t > 0 && t * size % 16 == 0 && (a.B == 1 || (b > 0 && b * size % 16 == 0));
     };
-    if (a.L < 2 * kT || a.d % 2 || a.L > 0x7fffffff - 1024 || a.B > 0x7fffffff || !at(a.states, 8)) return false;
+    if (a.L < 2 * kT || a.d % 4 || a.L > 0x7fffffff - 1024 || a.B > 0x7fffffff || !at(a.states, 16)) return false;
     if (!at(a.h, (backward ? 4 : 2) * size) || !rows(a.u, a.u_t, a.u_b)) return false;
     return !a.grad_h || rows(a.grad_h, a.gh_t, a.gh_b);
 }
@@ -767,6 +776,8 @@ template <typename TT> int launch_typed(LinRecArgs a, const Slices &s, bool reve
         const bool one = a.B == 1;       // the stride of a single sequence is never taken
         int rc = make_box<TT>(&maps.u, a.u, 2 * a.d, a.B, a.L, one ? a.u_t : a.u_b, a.u_t, 128, backward ? kT : Cut<TT>::kFwdT);
         if (!rc && a.grad_h) rc = make_box<TT>(&maps.g, a.grad_h, a.d, a.B, a.L, one ? a.gh_t : a.gh_b, a.gh_t, 64, kT);
+        if (!rc && backward)
+            rc = make_box<float>(&maps.s, a.states, a.d, a.B, (a.L + kT - 1) / kT, a.d, a.B * a.d, 64, 1);
         if (rc) return rc;
     }
     a.err = device_error_flag();
