@@ -109,6 +109,20 @@ def load_torch_ops():
         _torch_ops_loaded = True
 
 
+def native_op(name):
+    """``torch.ops.sru_b200.<name>`` where a call through it is wanted: not while a KernelTimer or NVTX ranges look at
+    single launches, which the Python form of the operator reports."""
+    if timer is not None or nvtx_ranges:
+        return None
+    op = _native_ops.get(name)
+    if op is None:
+        load_torch_ops()
+        op = _native_ops[name] = getattr(torch.ops.sru_b200, name).default
+    return op
+
+
+_native_ops = {}
+
 SCAN_KERNEL_NAMES = {0: "none", 1: "pipelined", 2: "generic", 3: "split"}
 
 

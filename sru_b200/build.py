@@ -66,11 +66,12 @@ def build_capi(force=False, verbose=False):
 
 
 def build_torch_binding(force=False):
-    src = os.path.join(CSRC, "torch_binding.cpp")
-    if not os.path.exists(src):
+    srcs = [os.path.join(CSRC, f) for f in ("torch_binding.cpp", "torch_layers.cpp")]
+    if not all(os.path.exists(f) for f in srcs):
         return None
     build_capi()
-    if not force and not _stale(TORCH_SO, [src, CAPI_SO, os.path.join(HERE, "..", "include", "sru_b200.h")]):
+    header = os.path.join(HERE, "..", "include", "sru_b200.h")
+    if not force and not _stale(TORCH_SO, srcs + [CAPI_SO, header]):
         return TORCH_SO
     import torch
     from torch.utils import cpp_extension as ce
@@ -79,9 +80,18 @@ def build_torch_binding(force=False):
         incs += ["-isystem", p]
     incs += ["-isystem", os.path.join(CUDA_HOME, "include")]
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)] + incs + [
-           src, "-o", TORCH_SO, "-L" + LIBDIR, "-lsru_b200", "-Wl,-rpath,$ORIGIN",
+    flags = ["-O2", "-std=c++17", "-fPIC", "-w", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+
+    def compile_one(src):
+        obj = os.path.join(OBJDIR, os.path.basename(src)[:-4] + ".o")
+        if force or _stale(obj, [src, header]):
+            subprocess.check_call(["g++"] + flags + incs + ["-c", src, "-o", obj])
+        return obj
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=2) as ex:
+        objs = list(ex.map(compile_one, srcs))
+    cmd = ["g++", "-shared"] + objs + [
+           "-o", TORCH_SO, "-L" + LIBDIR, "-lsru_b200", "-Wl,-rpath,$ORIGIN",
            "-L" + tlib, "-Wl,-rpath," + tlib, "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda",
            "-L" + os.path.join(CUDA_HOME, "lib64"), "-lcudart"]
     subprocess.check_call(cmd)

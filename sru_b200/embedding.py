@@ -85,6 +85,10 @@ def embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding
         if not -vocabulary <= padding_idx < vocabulary:
             raise _lib.SruB200Error("padding_idx %d is outside a table of %d rows" % (padding_idx, vocabulary))
         padding_idx %= vocabulary
+    op = _lib.native_op("embedding_lookup")
+    if op is not None:
+        _lib.launch_count += 1
+        return op(tokens, weight, scale, padding_idx, out_dtype)
     if weight.stride(1) != 1 or weight.stride(0) < weight.size(1):
         weight = weight.contiguous()
     flat = tokens.detach().reshape(-1)

@@ -96,6 +96,15 @@ class _GatedLinearRecurrence(Function):
                 grad_bias.to(bias_dtype) if need_bias else None, None, None)
 
 
+def _check(u: Tensor, t: Tensor, name: str, shape: tuple) -> None:
+    if t.device != u.device:
+        raise _lib.SruB200Error("%s is on %s, u on %s" % (name, t.device, u.device))
+    if t.shape != shape:
+        raise _lib.SruB200Error("%s must have shape %s, got %s" % (name, shape, tuple(t.shape)))
+    if name != "mask_pad" and not t.is_floating_point():
+        raise _lib.SruB200Error("%s must be a floating-point tensor, got %s" % (name, t.dtype))
+
+
 def gated_linear_recurrence(u: Tensor, c0: Optional[Tensor] = None, bias: Optional[Tensor] = None,
                             mask_pad: Optional[Tensor] = None, reverse: bool = False) -> Tuple[Tensor, Tensor]:
     """The recurrence over u (length, batch, 2 * hidden), or (batch, 2 * hidden) for a single step.
@@ -116,22 +125,24 @@ def gated_linear_recurrence(u: Tensor, c0: Optional[Tensor] = None, bias: Option
         raise _lib.SruB200Error("sru_b200 has no CPU path: u must be a CUDA tensor")
     if u.dtype not in _TYPES:
         raise _lib.SruB200Error("gated_linear_recurrence takes float32, float16 or bfloat16, got %s" % u.dtype)
-    if u.dim() not in (2, 3) or u.size(-1) < 2 or u.size(-1) % 2:
+    if u.dim() not in (2, 3) or u.shape[-1] < 2 or u.shape[-1] % 2:
         raise _lib.SruB200Error("u must be (length, batch, 2 * hidden) or (batch, 2 * hidden), got %s" % (tuple(u.shape),))
     single = u.dim() == 2
     if single:
         u = u.unsqueeze(0)
         mask_pad = None if mask_pad is None else mask_pad.unsqueeze(0)
-    length, batch, d = u.size(0), u.size(1), u.size(2) // 2
-    for name, t, shape in (("c0", c0, (batch, d)), ("bias", bias, (d,)), ("mask_pad", mask_pad, (length, batch))):
-        if t is None:
-            continue
-        if t.device != u.device:
-            raise _lib.SruB200Error("%s is on %s, u on %s" % (name, t.device, u.device))
-        if tuple(t.shape) != shape:
-            raise _lib.SruB200Error("%s must have shape %s, got %s" % (name, shape, tuple(t.shape)))
-        if name != "mask_pad" and not t.is_floating_point():
-            raise _lib.SruB200Error("%s must be a floating-point tensor, got %s" % (name, t.dtype))
+    length, batch, width = u.shape
+    if c0 is not None:
+        _check(u, c0, "c0", (batch, width // 2))
+    if bias is not None:
+        _check(u, bias, "bias", (width // 2,))
+    if mask_pad is not None:
+        _check(u, mask_pad, "mask_pad", (length, batch))
+    op = _lib.native_op("gated_linear_recurrence")
+    if op is not None:
+        _lib.launch_count += 1
+        h, c_last = op(u, c0, bias, mask_pad, reverse)
+        return (h.squeeze(0) if single else h), c_last
     mask = None if mask_pad is None else mask_pad.bool().contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (u, c0, bias)):
         h, c_last = _GatedLinearRecurrence.apply(u, c0, bias, mask, bool(reverse))
