@@ -27,18 +27,16 @@ namespace {
 constexpr int kBK = 64;
 constexpr int kABytes = 128 * kBK * 2;          // a CTA's 128 rows of the first operand per stage
 constexpr int kNsThreads = 192;
-constexpr int kMaxParts = 128;                  // partial sums of squares per matrix
+constexpr int kMaxParts = 256;                  // partial sums of squares per matrix
 
 enum { kPlain = 0, kCombine = 1 };
 
 struct NsArgs {
-    __half *c;                      // product; rows ldc apart, matrices c_batch apart
-    const __half *d;                // kCombine: A, laid out as c
-    int64_t ldc, c_batch;
     int M, N, K, batch, tiles_m, tiles_n;
     int symmetric;                  // only tiles that reach the diagonal or lie right of it; the others are mirrored
     int per_matrix;                 // tiles computed per matrix
     float ca, cb, cc;
+    int bf16;                       // the last product's output type is the caller's
     int *err;
 };
 
@@ -47,6 +45,23 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
         ::"r"(dst), "l"(map), "r"(bar & 0xFEFFFFFFu), "r"(x), "r"(y), "r"(z)
         : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z) : "memory");
+}
+// The launches of one call follow each other closely: a kernel may start while the one before it still runs, sets itself
+// up, and touches memory only when that one is complete.
+__device__ __forceinline__ void after_previous_kernel() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Unit -> matrix and tile.  A symmetric product keeps, of 256-row block i, the 128-column tiles from 2 i on.
@@ -67,24 +82,38 @@ __device__ __forceinline__ void ns_unit(const NsArgs &g, int unit, int *z, int *
 template <int BN> struct NsShape {
     static constexpr int kBBytes = BN / 2 * kBK * 2;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kStages = BN == 128 ? 8 : 6;
-    static constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
+    static constexpr int kStages = BN == 128 ? 6 : 5;
+    static constexpr int kOut = 32 * BN * 2;                    // an epilogue warp's 32 rows, boxes of 64 columns
+    static constexpr int kTurned = BN == 128 ? 128 * 32 * 2 : 0;    // the same transposed, for the mirrored tile
+    static constexpr int kBars = 1024;
+    static constexpr int kSmem = kStages * kStageBytes + 4 * (kOut + kTurned) + 1024 + kBars;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-// BMN: the second operand is stored (K, N) (MN-major), else (N, K).
-template <int BN, bool BMN, int MODE>
+// AMN, BMN: the first operand is stored (K, M), the second (K, N) (MN-major), else (M, K) and (N, K).
+//
+// Epilogue.  A thread gets one ROW of the accumulator; written from there to global memory every store instruction would
+// touch 32 rows, and the four warps of a CTA took 0.5 us per 32 columns that way (half of a 128 x 384 update's time).  The
+// warp stages its rows in shared memory in the 128-byte swizzle of the output's tensor map instead and hands boxes of
+// 32 x 64 to the copy engine, which clips what lies outside the matrix.  kCombine's A comes the same way into the same
+// place, asked for before the accumulator is ready.  A tile right of the diagonal of a symmetric product is staged a second
+// time transposed and stored as its mirror image.
+template <int BN, bool AMN, bool BMN, int MODE>
 __global__ void __launch_bounds__(kNsThreads, 1)
-ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const NsArgs g) {
+ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                  const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_t,
+                  const __grid_constant__ CUtensorMap map_d, const NsArgs g) {
     using S = NsShape<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kStages * S::kStageBytes);
+    uint8_t *staging = smem + S::kStages * S::kStageBytes;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + 4 * (S::kOut + S::kTurned));
     const uint32_t bar_full = smem_u32(bars);                 // in the leader: loads of both CTAs
     const uint32_t bar_empty = bar_full + 8 * S::kStages;
     const uint32_t bar_tfull = bar_empty + 8 * S::kStages;    // [2]
     const uint32_t bar_tempty = bar_tfull + 16;               // [2] in the leader
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::kStages + 4);
+    const uint32_t bar_d = bar_tempty + 16;                   // [4] one per epilogue warp
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::kStages + 8);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
@@ -95,6 +124,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) { mbar_init(bar_full + 8 * s, 1); mbar_init(bar_empty + 8 * s, 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(bar_tfull + 8 * i, 1); mbar_init(bar_tempty + 8 * i, 8); }
+        for (int i = 0; i < 4; ++i) mbar_init(bar_d + 8 * i, 1);
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -106,6 +136,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    after_previous_kernel();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -121,7 +152,12 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     const uint32_t full = bar_full + 8 * stage;
                     if (rank == 0) mbar_arrive_expect_tx(full, 2 * S::kStageBytes);
                     const uint32_t sa = smem_u32(smem + stage * S::kStageBytes), sb = sa + kABytes;
-                    tma_load_3d_pair(sa, &map_a, full, kb * kBK, m0, z);
+                    if (!AMN) {
+                        tma_load_3d_pair(sa, &map_a, full, kb * kBK, m0, z);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) tma_load_3d_pair(sa + j * 8192, &map_a, full, m0 + j * 64, kb * kBK, z);
+                    }
                     if (!BMN) {
                         tma_load_3d_pair(sb, &map_b, full, kb * kBK, n0, z);
                     } else {
@@ -134,8 +170,9 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
-            // instruction descriptor: float32 accumulator, fp16 operands, second operand's major, N / 8, M / 16
-            constexpr uint32_t idesc = (1u << 4) | ((BMN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((256u >> 4) << 24);
+            // instruction descriptor: float32 accumulator, fp16 operands, the operands' majors, N / 8, M / 16
+            constexpr uint32_t idesc = (1u << 4) | ((AMN ? 1u : 0u) << 15) | ((BMN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((256u >> 4) << 24);
+            constexpr uint32_t a_step = AMN ? 2048u : 32u, a_lbo = AMN ? 8192u : 16u;
             constexpr uint32_t b_step = BMN ? 2048u : 32u, b_lbo = BMN ? 8192u : 16u;
             int stage = 0, it = 0;
             uint32_t phase = 0;
@@ -150,7 +187,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     const uint32_t sa = smem_u32(smem + stage * S::kStageBytes), sb = sa + kABytes;
 #pragma unroll
                     for (int k16 = 0; k16 < kBK / 16; ++k16)
-                        tc_mma_pair(tmem_base + acc * BN, make_desc(sa + k16 * 32, 16, 1024),
+                        tc_mma_pair(tmem_base + acc * BN, make_desc(sa + k16 * a_step, a_lbo, 1024),
                                     make_desc(sb + k16 * b_step, b_lbo, 1024), idesc, (kb | k16) ? 1u : 0u);
                     tc_commit_pair(bar_empty + 8 * stage);
                     if (++stage == S::kStages) { stage = 0; phase ^= 1; }
@@ -161,17 +198,27 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     } else {
         const int q = warp & 3;                 // TMEM lane quarter: 32 of the CTA's 128 rows
         const uint32_t tempty_leader = map_to_cta(bar_tempty, 0);
+        const uint32_t out = smem_u32(staging + q * (S::kOut + S::kTurned)), turned = out + S::kOut;
         int it = 0;
         for (int unit = pair; unit < nunits; unit += npairs, ++it) {
             int z, mb, nb;
             ns_unit(g, unit, &z, &mb, &nb);
             const int acc = it & 1;
-            if (!mbar_wait_bounded(bar_tfull + 8 * acc, (it >> 1) & 1)) { if (lane == 0) atomicExch(g.err, 34); break; }
+            const int row0 = mb * 256 + (int)rank * 128 + q * 32, row = row0 + lane;
+            const bool mirror = BN == 128 && g.symmetric && 2 * mb < (nb & ~1);   // the transposed tile is computed by nobody
+            if (lane == 0) {
+                bulk_wait_read_all();           // the stores of the tile before have left the staging
+                if (MODE == kCombine) {
+                    mbar_arrive_expect_tx(bar_d + 8 * q, S::kOut);
+#pragma unroll
+                    for (int b = 0; b < BN / 64; ++b) tma_load_3d(out + b * 4096, &map_d, bar_d + 8 * q, nb * BN + b * 64, row0, z);
+                }
+            }
+            __syncwarp();
+            bool ok = mbar_wait_bounded(bar_tfull + 8 * acc, (it >> 1) & 1);
+            if (MODE == kCombine) ok = mbar_wait_bounded(bar_d + 8 * q, it & 1) && ok;
+            if (!ok) { if (lane == 0) atomicExch(g.err, 34); break; }
             tc_fence_after();
-            const int row = mb * 256 + (int)rank * 128 + q * 32 + lane;
-            const bool mirror = g.symmetric && 2 * mb < (nb & ~1);      // the transposed tile is computed by nobody
-            __half *c = g.c + (int64_t)z * g.c_batch;
-            const __half *d = MODE == kCombine ? g.d + (int64_t)z * g.c_batch : nullptr;
 #pragma unroll 1
             for (int cc = 0; cc < BN / 32; ++cc) {
                 const int col0 = nb * BN + cc * 32;
@@ -179,43 +226,63 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 uint32_t r[32];
                 tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + cc * 32, r);
                 tmem_ld_wait();
-                // rows are padded to 8 elements: a group of 8 that starts inside the matrix is inside its row
+                const uint32_t line = out + (cc >> 1) * 4096 + lane * 128;
 #pragma unroll
                 for (int j0 = 0; j0 < 32; j0 += 8) {
-                    const bool in = row < g.M && col0 + j0 < g.N;
+                    const uint32_t at = line + ((((cc & 1) * 4 + j0 / 8) ^ (lane & 7)) << 4);
                     float v[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[j0 + j]);
-                    if (MODE == kCombine && in) {
-                        const Pack<__half, 8> a = *reinterpret_cast<const Pack<__half, 8> *>(d + row * g.ldc + col0 + j0);
+                    if (MODE == kCombine) {
+                        uint4 d;
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(d.x), "=r"(d.y), "=r"(d.z), "=r"(d.w) : "r"(at));
+                        const __half2 *a2 = reinterpret_cast<const __half2 *>(&d);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            v[j] = fmaf(g.cc, v[j], fmaf(g.cb, __half2float(a.v[j]), row == col0 + j0 + j ? g.ca : 0.0f));
+                        for (int j = 0; j < 8; ++j) {
+                            const float a = (j & 1) ? __high2float(a2[j >> 1]) : __low2float(a2[j >> 1]);
+                            v[j] = fmaf(g.cc, v[j], fmaf(g.cb, a, row == col0 + j0 + j ? g.ca : 0.0f));
+                        }
                     }
-                    if (in) store8<__half>(c + row * g.ldc + col0 + j0, v);
-                    if (g.symmetric) {
+                    uint32_t w[4];
+                    if (MODE == kPlain && g.bf16) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) r[j0 + j] = __float_as_uint(v[j]);
+                        for (int j = 0; j < 4; ++j) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+                            w[j] = *reinterpret_cast<const uint32_t *>(&h);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+                            w[j] = *reinterpret_cast<const uint32_t *>(&h);
+                        }
                     }
-                }
-                if (mirror) {
-                    // element (row, col) again at (col, row): lanes hold consecutive rows; two rows to a 4-byte store,
-                    // even lanes store column k, odd lanes column k + 1
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                    if (BN == 128 && mirror) {
+                        // element (row, col) at [col][row]: the 32 lanes of a store fill 64 contiguous bytes
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        const float mine = __uint_as_float(lane & 1 ? r[k + 1] : r[k]);
-                        const float give = __uint_as_float(lane & 1 ? r[k] : r[k + 1]);
-                        const float got = __shfl_xor_sync(0xffffffffu, give, 1);
-                        const int col = col0 + k + (lane & 1);
-                        const __half2 two = lane & 1 ? __floats2half2_rn(got, mine) : __floats2half2_rn(mine, got);
-                        if (col < g.N && (row & ~1) < g.M) *reinterpret_cast<__half2 *>(c + col * g.ldc + (row & ~1)) = two;
+                        for (int j = 0; j < 8; ++j) {
+                            const uint16_t e = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(turned + (cc * 32 + j0 + j) * 64 + lane * 2), "h"(e) : "memory");
+                        }
                     }
                 }
             }
             tc_fence_before();
+            fence_proxy_async();                // the staged values become visible to the copy engine
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * acc);
+            if (lane == 0) {
+                mbar_arrive_cluster(tempty_leader + 8 * acc);
+                if (row0 < g.M) {
+#pragma unroll
+                    for (int b = 0; b < BN / 64; ++b)
+                        if (nb * BN + b * 64 < g.N) tma_store_3d(&map_c, out + b * 4096, nb * BN + b * 64, row0, z);
+                    if (BN == 128 && mirror) tma_store_3d(&map_t, turned, row0, nb * BN, z);
+                }
+                bulk_commit();
+            }
         }
+        if (lane == 0) bulk_wait_all();
     }
 
     tc_fence_before();
@@ -236,69 +303,114 @@ struct NsEdge {
     int m, n;                       // the iterate's sizes (m <= n)
     int64_t s_i, s_j, s_b;          // strides of the caller's matrix along the iterate's rows, columns, and batch
     int64_t ldx, x_batch;           // the iterate's row pitch and matrix pitch
+    int64_t lines, len, pitch;      // the source as lines along its contiguous direction
+    bool wide;                      // lines are 16-byte aligned
     double eps;
 };
 
-// Partial sums of squares in 64 bits (squares of the extremes of bf16 leave float32's range); one warp per line along
-// the contiguous direction.
+// N elements from p + k on, of which those below `len` count (the others are 0); wide: p is 16-byte aligned and N * size a
+// multiple of 16.
+template <typename T, int N> __device__ __forceinline__ void load_line(float (&v)[N], const T *p, int64_t k, int64_t len, bool wide) {
+    if (wide && k + N <= len) {
+        Pack<T, N> t = *reinterpret_cast<const Pack<T, N> *>(p + k);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = Cvt<T>::to_f(t.v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = k + i < len ? Cvt<T>::to_f(p[k + i]) : 0.0f;
+    }
+}
+
+// Partial sums of squares in 64 bits (squares of the extremes of bf16 leave float32's range).  Units of 2048 elements of
+// a line along the contiguous direction, one warp each, in a fixed order.
 template <typename T> __global__ void __launch_bounds__(256) ns_norm_kernel(const NsEdge e) {
     __shared__ double s[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool across = e.s_j != 1;                       // lines run along i
-    const int lines = across ? e.n : e.m, len = across ? e.m : e.n;
-    const int64_t pitch = across ? e.s_j : e.s_i;
     const T *g = static_cast<const T *>(e.src) + blockIdx.y * e.s_b;
-    double sum = 0.0;
-    for (int l = blockIdx.x * 8 + warp; l < lines; l += gridDim.x * 8) {
-        const T *p = g + l * pitch;
-        for (int k = lane; k < len; k += 32) {
-            const double v = (double)Cvt<T>::to_f(p[k]);
-            sum = fma(v, v, sum);
+    const int64_t per = (e.len + 2047) / 2048, units = e.lines * per;
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int64_t u = (int64_t)blockIdx.x * 8 + warp; u < units; u += gridDim.x * 8) {
+        const int64_t l = u / per, k0 = (u - l * per) * 2048 + lane * 8;
+        const T *p = g + l * e.pitch;
+#pragma unroll 4
+        for (int k = 0; k < 2048; k += 256) {
+            if (k0 + k >= e.len) break;
+            float v[8];
+            load_line<T, 8>(v, p, k0 + k, e.len, e.wide);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i & 3] = fma((double)v[i], (double)v[i], sum[i & 3]);
         }
     }
+    double t = (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s[warp] = sum;
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (lane == 0) s[warp] = t;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 8; ++w) sum += s[w];
-        e.part[(int64_t)blockIdx.y * e.parts + blockIdx.x] = sum;
+        for (int w = 1; w < 8; ++w) t += s[w];
+        e.part[(int64_t)blockIdx.y * e.parts + blockIdx.x] = t;
     }
 }
 
-// X_0 in fp16, tiles of 32 x 32 through shared memory: the source is read along its contiguous direction.
-template <typename T> __global__ void __launch_bounds__(256) ns_first_kernel(const NsEdge e) {
-    __shared__ float tile[32][33];
-    __shared__ float scale;
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    if (ty == 0) {
+// 1 / (|G|_F + eps) from the partial sums, by every block for itself.
+__device__ __forceinline__ float ns_scale(const NsEdge &e, int64_t z, float *shared) {
+    if (threadIdx.x < 32) {
         double sum = 0.0;
-        for (int p = tx; p < e.parts; p += 32) sum += e.part[(int64_t)blockIdx.z * e.parts + p];
+        for (int p = threadIdx.x; p < e.parts; p += 32) sum += e.part[z * e.parts + p];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (tx == 0) scale = (float)(1.0 / (sqrt(sum) + e.eps));
+        if (threadIdx.x == 0) *shared = (float)(1.0 / (sqrt(sum) + e.eps));
     }
     __syncthreads();
-    const T *g = static_cast<const T *>(e.src) + blockIdx.z * e.s_b;
-    __half *x = static_cast<__half *>(e.dst) + blockIdx.z * e.x_batch;
-    const int i0 = blockIdx.y * 32, j0 = blockIdx.x * 32;
-    const bool across = e.s_j != 1;
+    return *shared;
+}
+
+// X_0 in fp16 where the iterate's rows are contiguous in the source: 8 columns per thread.
+template <typename T> __global__ void __launch_bounds__(256) ns_first_rows_kernel(const NsEdge e) {
+    __shared__ float shared;
+    const float scale = ns_scale(e, blockIdx.y, &shared);
+    const T *g = static_cast<const T *>(e.src) + blockIdx.y * e.s_b;
+    __half *x = static_cast<__half *>(e.dst) + blockIdx.y * e.x_batch;
+    const int64_t per = e.ldx / 8, groups = per * e.m;
+    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < groups; u += (int64_t)gridDim.x * 256) {
+        const int64_t i = u / per, j = (u - i * per) * 8;
+        float v[8];
+        load_line<T, 8>(v, g + i * e.s_i, j, e.n, e.wide);
+        Pack<__half, 8> h;
 #pragma unroll
-    for (int k = 0; k < 32; k += 8) {
-        const int i = i0 + (across ? tx : ty + k), j = j0 + (across ? ty + k : tx);
-        const float v = (i < e.m && j < e.n) ? Cvt<T>::to_f(g[i * e.s_i + j * e.s_j]) * scale : 0.0f;
-        if (across) tile[tx][ty + k] = v;
-        else tile[ty + k][tx] = v;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 32; k += 8) {
-        const int i = i0 + ty + k, j = j0 + tx;
-        if (i < e.m && j < e.ldx) x[i * e.ldx + j] = __float2half_rn(tile[ty + k][tx]);
+        for (int k = 0; k < 8; ++k) h.v[k] = __float2half_rn(v[k] * scale);
+        *reinterpret_cast<Pack<__half, 8> *>(x + i * e.ldx + j) = h;
     }
 }
 
-// The last iterate into the caller's contiguous matrix and type.
+// X_0 where the iterate's columns are contiguous in the source (tall matrices): tiles of 64 x 64 through shared memory.
+template <typename T> __global__ void __launch_bounds__(256) ns_first_turned_kernel(const NsEdge e) {
+    __shared__ float shared;
+    __shared__ float tile[64][65];
+    const float scale = ns_scale(e, blockIdx.z, &shared);
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const T *g = static_cast<const T *>(e.src) + blockIdx.z * e.s_b;
+    __half *x = static_cast<__half *>(e.dst) + blockIdx.z * e.x_batch;
+    const int64_t i0 = (int64_t)blockIdx.y * 64, j0 = (int64_t)blockIdx.x * 64;
+#pragma unroll
+    for (int k = 0; k < 64; k += 8) {
+        const int64_t j = j0 + ty + k;
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+            const int64_t i = i0 + tx + c;
+            tile[ty + k][tx + c] = (i < e.m && j < e.n) ? Cvt<T>::to_f(g[i + j * e.s_j]) * scale : 0.0f;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 64; k += 8) {
+        const int64_t i = i0 + ty + k, j = j0 + 2 * tx;
+        if (i < e.m && j < e.ldx)           // ldx is a multiple of 8
+            *reinterpret_cast<__half2 *>(x + i * e.ldx + j) = __floats2half2_rn(tile[2 * tx][ty + k], tile[2 * tx + 1][ty + k]);
+    }
+}
+
+// The last iterate into the caller's contiguous matrix and type, where the last product cannot write it.
 template <typename T> __global__ void __launch_bounds__(256) ns_last_kernel(const NsEdge e) {
     __shared__ float tile[32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -340,23 +452,34 @@ NsPlan ns_plan(int64_t batch, int64_t rows, int64_t cols) {
     return p;
 }
 
-// (inner, rows, batch) fp16 matrices; boxes of 64 x box_rows elements, 128-byte swizzle; outside reads as zero.
-int ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t rows, int64_t batch, int64_t ld, int box_rows) {
+// (inner, rows, batch) fp16 matrices; boxes of 64 x box_rows elements in the 128-byte swizzle (of 32 elements: as they
+// are); outside reads as zero and is not written.
+int ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t rows, int64_t batch, int64_t ld, int box_rows, int box_cols = 64) {
     auto fn = get_encode_fn();
     if (!fn) return set_error(SRU_ERR_CUDA, "cuTensorMapEncodeTiled entry point not found");
     cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)batch};
     cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(ld * rows) * 2};
-    cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, estr[3] = {1, 1, 1};
+    cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, estr[3] = {1, 1, 1};
     CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(SRU_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
     return 0;
 }
 
-template <int BN, bool BMN, int MODE>
-int ns_product(const CUtensorMap &map_a, const CUtensorMap &map_b, NsArgs g, int sms, cudaStream_t st) {
-    auto kernel = ns_product_kernel<BN, BMN, MODE>;
+// One matrix (or batch) as the products see it: first operand, second operand, output and its mirror image.
+struct NsMaps { CUtensorMap a, b, c, t; };
+int ns_maps(NsMaps *m, const void *base, int64_t inner, int64_t rows, int64_t batch, int64_t ld) {
+    int rc = ns_map(&m->a, base, inner, rows, batch, ld, 128);
+    if (!rc) rc = ns_map(&m->b, base, inner, rows, batch, ld, 64);
+    if (!rc) rc = ns_map(&m->c, base, inner, rows, batch, ld, 32);
+    if (!rc) rc = ns_map(&m->t, base, inner, rows, batch, ld, 128, 32);
+    return rc;
+}
+
+template <int BN, bool AMN, bool BMN, int MODE>
+int ns_product(const NsMaps &a, const NsMaps &b, const NsMaps &out, const NsMaps &d, NsArgs g, int sms, cudaStream_t st) {
+    auto kernel = ns_product_kernel<BN, AMN, BMN, MODE>;
     static bool attr_set[64] = {false};
     int dev = 0;
     SRUB_CUDA_CHECK(cudaGetDevice(&dev));
@@ -377,12 +500,14 @@ int ns_product(const CUtensorMap &map_a, const CUtensorMap &map_b, NsArgs g, int
     cfg.blockDim = dim3(kNsThreads, 1, 1);
     cfg.dynamicSmemBytes = NsShape<BN>::kSmem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, g));
+    cfg.numAttrs = 2;
+    SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, AMN ? a.b : a.a, b.b, out.c, out.t, d.c, g));
     return 0;
 }
 
@@ -427,8 +552,8 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     char *ws = static_cast<char *>(workspace);
     double *part = reinterpret_cast<double *>(ws);
     __half *x[2] = {reinterpret_cast<__half *>(ws + p.part_bytes), reinterpret_cast<__half *>(ws + p.part_bytes + p.x_bytes)};
-    __half *am = reinterpret_cast<__half *>(ws + p.part_bytes + 2 * p.x_bytes);
-    __half *mm = reinterpret_cast<__half *>(ws + p.part_bytes + 2 * p.x_bytes + p.a_bytes);
+    __half *a_buf = reinterpret_cast<__half *>(ws + p.part_bytes + 2 * p.x_bytes);
+    __half *m_buf = reinterpret_cast<__half *>(ws + p.part_bytes + 2 * p.x_bytes + p.a_bytes);
 
     const bool tall = rows > cols;
     NsEdge e;
@@ -437,46 +562,62 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     e.m = (int)p.m; e.n = (int)p.n;
     e.s_i = tall ? stride_col : stride_row; e.s_j = tall ? stride_row : stride_col; e.s_b = stride_batch;
     e.ldx = p.ldx; e.x_batch = p.m * p.ldx; e.eps = eps;
-    const int64_t lines = e.s_j != 1 ? p.n : p.m;
-    e.parts = (int)std::min<int64_t>((lines + 7) / 8, kMaxParts);
+    const bool turned = e.s_j != 1;
+    e.lines = turned ? p.n : p.m; e.len = turned ? p.m : p.n; e.pitch = turned ? e.s_j : e.s_i;
+    const int64_t size = (int64_t)dtype_size(grad_dtype);
+    e.wide = reinterpret_cast<uintptr_t>(grad) % 16 == 0 && e.pitch * size % 16 == 0 && (batch == 1 || e.s_b * size % 16 == 0);
+    if (e.pitch == e.len || e.lines == 1) { e.len *= e.lines; e.lines = 1; e.pitch = 0; }       // one line
+    e.parts = (int)std::min<int64_t>((e.lines * ((e.len + 2047) / 2048) + 7) / 8, kMaxParts);
     const dim3 norm_grid((unsigned)e.parts, (unsigned)batch);
-    const dim3 tile_grid((unsigned)((p.ldx + 31) / 32), (unsigned)((p.m + 31) / 32), (unsigned)batch);
     auto begin = [&](auto t) {
         using T = decltype(t);
         ns_norm_kernel<T><<<norm_grid, 256, 0, st>>>(e);
-        ns_first_kernel<T><<<tile_grid, 256, 0, st>>>(e);
+        if (turned) {
+            const dim3 grid((unsigned)((p.ldx + 63) / 64), (unsigned)((p.m + 63) / 64), (unsigned)batch);
+            ns_first_turned_kernel<T><<<grid, 256, 0, st>>>(e);
+        } else {
+            const dim3 grid((unsigned)std::min<int64_t>((p.m * p.ldx / 8 + 255) / 256, 148 * 8), (unsigned)batch);
+            ns_first_rows_kernel<T><<<grid, 256, 0, st>>>(e);
+        }
     };
     if (grad_dtype == SRU_F32) begin(float());
     else if (grad_dtype == SRU_F16) begin(__half());
     else begin(__nv_bfloat16());
     SRUB_CUDA_CHECK(cudaGetLastError());
 
-    CUtensorMap xa[2], xb[2], aa, ab, ma;             // as first operand (128-row boxes), as second (64)
-    int rc = 0;
-    for (int i = 0; i < 2 && steps > 0; ++i) {
-        if ((rc = ns_map(&xa[i], x[i], p.n, p.m, batch, p.ldx, 128))) return rc;
-        if ((rc = ns_map(&xb[i], x[i], p.n, p.m, batch, p.ldx, 64))) return rc;
-    }
+    // The last product writes the caller's matrix itself where its rows are 16-byte aligned.
+    const bool direct = steps > 0 && cols % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    NsMaps xm[2], am, mm, om;
+    if (direct)
+        if (int rc = ns_maps(&om, out, cols, rows, batch, cols)) return rc;
     if (steps > 0) {
-        if ((rc = ns_map(&aa, am, p.m, p.m, batch, p.ldm, 128))) return rc;
-        if ((rc = ns_map(&ab, am, p.m, p.m, batch, p.ldm, 64))) return rc;
-        if ((rc = ns_map(&ma, mm, p.m, p.m, batch, p.ldm, 128))) return rc;
+        int rc = ns_maps(&am, a_buf, p.m, p.m, batch, p.ldm);
+        if (!rc) rc = ns_maps(&mm, m_buf, p.m, p.m, batch, p.ldm);
+        for (int i = 0; i < 2 && !rc; ++i) rc = ns_maps(&xm[i], x[i], p.n, p.m, batch, p.ldx);
+        if (rc) return rc;
     }
     for (int s = 0; s < steps; ++s) {
         const int cur = s & 1;
         NsArgs g;
         memset(&g, 0, sizeof(g));
         g.batch = (int)batch; g.err = err;
-        g.c = am; g.ldc = p.ldm; g.c_batch = p.m * p.ldm;
         g.M = (int)p.m; g.N = (int)p.m; g.K = (int)p.n; g.symmetric = 1;
-        if ((rc = ns_product<128, false, kPlain>(xa[cur], xb[cur], g, sms, st))) return rc;
-        g.c = mm; g.d = am; g.K = (int)p.m;
         g.ca = (float)a; g.cb = (float)b; g.cc = (float)c;
-        if ((rc = ns_product<128, false, kCombine>(aa, ab, g, sms, st))) return rc;
-        g.c = x[cur ^ 1]; g.d = nullptr; g.ldc = p.ldx; g.c_batch = p.m * p.ldx;
+        if (int rc = ns_product<128, false, false, kPlain>(xm[cur], xm[cur], am, am, g, sms, st)) return rc;
+        g.K = (int)p.m;
+        if (int rc = ns_product<128, false, false, kCombine>(am, am, mm, am, g, sms, st)) return rc;
         g.N = (int)p.n; g.symmetric = 0;
-        if ((rc = ns_product<256, true, kPlain>(ma, xb[cur], g, sms, st))) return rc;
+        const bool last = s == steps - 1 && direct;
+        g.bf16 = last && out_dtype == SRU_BF16;
+        if (last && tall) {             // X^T = X_before^T M, rows as the caller has them
+            g.M = (int)p.n; g.N = (int)p.m;
+            if (int rc = ns_product<128, true, false, kPlain>(xm[cur], mm, om, am, g, sms, st)) return rc;
+        } else if (int rc = ns_product<256, false, true, kPlain>(mm, xm[cur], last ? om : xm[cur ^ 1], am, g, sms, st)) {
+            return rc;
+        }
     }
+    if (direct) return 0;
+    const dim3 tile_grid((unsigned)((p.ldx + 31) / 32), (unsigned)((p.m + 31) / 32), (unsigned)batch);
     e.src = x[steps & 1]; e.dst = out;
     e.s_i = tall ? 1 : cols; e.s_j = tall ? cols : 1; e.s_b = rows * cols;
     if (out_dtype == SRU_F16) ns_last_kernel<__half><<<tile_grid, 256, 0, st>>>(e);
