@@ -434,6 +434,252 @@ template <typename T> __global__ void __launch_bounds__(256) ns_last_kernel(cons
     }
 }
 
+// ---- small matrices ------------------------------------------------------------------------------------------------
+// One CTA takes a whole matrix through all its steps when the iterate fits in shared memory: X (at most 128 x 768 in fp16)
+// as 64-column tiles of 128 rows in the 128-byte swizzle, which the tensor cores read as the K-major operand of X X^T and as
+// the MN-major operand of M X alike, and one 128 x 128 matrix that holds A and then, in place, M.  Nothing leaves the SM
+// between load and store.  Bound by the latency of the chain (product, accumulator to registers, shared memory, next
+// product; about 3 us a step at 128 x 384), where the general path pays for three launches a step (about 6 us each).
+constexpr int kSmallM = 128, kSmallN = 768, kSmallThreads = 512;
+constexpr int kTileBytes = 128 * 64 * 2;
+
+__device__ __forceinline__ uint32_t tile_at(int row, int col) {     // byte offset of 8 columns' group in the tiles
+    return (uint32_t)(col >> 6) * kTileBytes + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ uint4 shared_16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ void store_halves(uint32_t at, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
+struct NsSmall {
+    NsEdge e;                       // source and sizes; dst is the result
+    int64_t o_i, o_j, o_b;          // strides of the result along the iterate's rows, columns, and batch
+    int steps;
+    float ca, cb, cc;
+    bool out_wide;                  // rows of the result are 16-byte aligned
+    int *err;
+};
+
+template <typename T, typename TO>
+__global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmall a) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ double sums[kSmallThreads / 32];
+    __shared__ uint64_t bars[2];
+    __shared__ uint32_t tmem_slot;
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const NsEdge &e = a.e;
+    const int tiles = (e.n + 63) / 64;
+    const uint32_t am = smem_u32(smem), x = am + 2 * kTileBytes;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int q = warp & 3, part = warp >> 2, row = q * 32 + lane;      // accumulator row and column part of this thread
+    const T *g = static_cast<const T *>(e.src) + blockIdx.x * e.s_b;
+
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&bars[0]), 1);
+        mbar_init(smem_u32(&bars[1]), 1);
+        fence_mbar_init();
+    }
+    if (warp == 0) {
+        tmem_alloc(smem_u32(&tmem_slot), 512);
+        tmem_relinquish();
+    }
+    // the norm, in 64 bits and a fixed order
+    double sum[2] = {0.0, 0.0};
+    {
+        const int64_t groups = (e.len + 7) / 8, units = e.lines * groups;
+#pragma unroll 4
+        for (int64_t u = threadIdx.x; u < units; u += kSmallThreads) {
+            const int64_t l = u / groups, k = (u - l * groups) * 8;
+            float v[8];
+            load_line<T, 8>(v, g + l * e.pitch, k, e.len, e.wide);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i & 1] = fma((double)v[i], (double)v[i], sum[i & 1]);
+        }
+    }
+    double t = sum[0] + sum[1];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (lane == 0) sums[warp] = t;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    t = 0.0;
+    for (int w = 0; w < kSmallThreads / 32; ++w) t += sums[w];
+    const float scale = (float)(1.0 / (sqrt(t) + e.eps));
+    if (e.s_j == 1) {
+#pragma unroll 2
+        for (int u = threadIdx.x; u < kSmallM * tiles * 8; u += kSmallThreads) {
+            const int i = u / (tiles * 8), j = (u - i * tiles * 8) * 8;
+            float v[8];
+            load_line<T, 8>(v, g + i * e.s_i, j, i < e.m ? e.n : 0, e.wide);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= scale;
+            store_halves(x + tile_at(i, j), v);
+        }
+    } else {
+#pragma unroll 4
+        for (int u = threadIdx.x; u < kSmallM * tiles * 64; u += kSmallThreads) {
+            const int i = u & (kSmallM - 1), j = u / kSmallM;
+            const float v = (i < e.m && j < e.n) ? Cvt<T>::to_f(g[i + j * e.s_j]) * scale : 0.0f;
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(x + tile_at(i, j & ~7) + (j & 7) * 2), "h"(__half_as_ushort(__float2half_rn(v))) : "memory");
+        }
+    }
+
+    constexpr uint32_t kDesc = (1u << 4) | ((128u >> 4) << 24);
+    uint32_t phase[2] = {0, 0};
+    bool ok = true;
+    // everyone's shared-memory writes are done and visible to the tensor cores
+    auto settle = [&]() {
+        fence_proxy_async();
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+    };
+    auto arrive = [&](int bar) {
+        const bool here = mbar_wait_bounded(smem_u32(&bars[bar]), phase[bar]);
+        phase[bar] ^= 1;
+        if (!here && lane == 0) atomicExch(a.err, 35);
+        ok = __syncthreads_and(here);
+        tc_fence_after();
+    };
+    const int k_m = (e.m + 15) / 16, k_n = (e.n + 15) / 16, groups = (tiles + 3) / 4;
+    settle();
+    for (int s = 0; s < a.steps && ok; ++s) {
+        // A = X X^T
+        if (threadIdx.x == 0) {
+            for (int k = 0; k < k_n; ++k) {
+                const uint64_t d = make_desc(x + (k >> 2) * kTileBytes + (k & 3) * 32, 16, 1024);
+                tc_mma(tmem, d, d, kDesc | ((128u >> 3) << 17), k ? 1u : 0u);
+            }
+            tc_commit(smem_u32(&bars[0]));
+        }
+        __syncwarp();
+        arrive(0);
+        if (!ok) break;
+        uint32_t r[32];
+        tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + part * 32, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j0 = 0; j0 < 32; j0 += 8) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[j0 + j]);
+            store_halves(am + tile_at(row, part * 32 + j0), v);
+        }
+        settle();
+        // M = a I + b A + c A A, over A
+        if (threadIdx.x == 0) {
+            for (int k = 0; k < k_m; ++k) {
+                const uint64_t d = make_desc(am + (k >> 2) * kTileBytes + (k & 3) * 32, 16, 1024);
+                tc_mma(tmem + 128, d, d, kDesc | ((128u >> 3) << 17), k ? 1u : 0u);
+            }
+            tc_commit(smem_u32(&bars[0]));
+        }
+        __syncwarp();
+        arrive(0);
+        if (!ok) break;
+        tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + 128 + part * 32, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j0 = 0; j0 < 32; j0 += 8) {
+            const int col = part * 32 + j0;
+            const uint32_t at = am + tile_at(row, col);
+            const uint4 w = shared_16(at);
+            const __half2 *a2 = reinterpret_cast<const __half2 *>(&w);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float old = (j & 1) ? __high2float(a2[j >> 1]) : __low2float(a2[j >> 1]);
+                v[j] = fmaf(a.cc, __uint_as_float(r[j0 + j]), fmaf(a.cb, old, row == col + j ? a.ca : 0.0f));
+            }
+            store_halves(at, v);
+        }
+        settle();
+        // X = M X, 256 columns at a time; a column of the product needs that column of X alone, so it is replaced in place
+        auto multiply = [&](int group) {
+            if (threadIdx.x == 0) {
+                const int n = min(4, tiles - 4 * group) * 64;
+                for (int k = 0; k < k_m; ++k)
+                    tc_mma(tmem + (group & 1) * 256, make_desc(am + (k >> 2) * kTileBytes + (k & 3) * 32, 16, 1024),
+                           make_desc(x + group * 4 * kTileBytes + k * 2048, kTileBytes, 1024),
+                           kDesc | (1u << 16) | ((uint32_t)(n >> 3) << 17), k ? 1u : 0u);
+                tc_commit(smem_u32(&bars[group & 1]));
+            }
+            __syncwarp();
+        };
+        multiply(0);
+        if (groups > 1) multiply(1);
+        for (int group = 0; group < groups && ok; ++group) {
+            arrive(group & 1);
+            if (!ok) break;
+            const int col0 = group * 256 + part * 64;
+            if (col0 < tiles * 64) {
+#pragma unroll
+                for (int half = 0; half < 64; half += 32) {
+                    tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (group & 1) * 256 + part * 64 + half, r);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j0 = 0; j0 < 32; j0 += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[j0 + j]);
+                        store_halves(x + tile_at(row, col0 + half + j0), v);
+                    }
+                }
+            }
+            if (group + 2 < groups) {
+                settle();
+                multiply(group + 2);
+            }
+        }
+        settle();
+    }
+    __syncthreads();
+    TO *out = static_cast<TO *>(e.dst) + blockIdx.x * a.o_b;
+    if (a.o_j == 1) {
+        for (int u = threadIdx.x; u < e.m * tiles * 8; u += kSmallThreads) {
+            const int i = u / (tiles * 8), j = (u - i * tiles * 8) * 8;
+            if (j >= e.n) continue;
+            const uint4 w = shared_16(x + tile_at(i, j));
+            const __half *h = reinterpret_cast<const __half *>(&w);
+            Pack<TO, 8> o;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o.v[k] = Cvt<TO>::from_f(__half2float(h[k]));
+            TO *p = out + i * a.o_i + j;
+            if (a.out_wide && j + 8 <= e.n) *reinterpret_cast<Pack<TO, 8> *>(p) = o;
+            else
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (j + k < e.n) p[k] = o.v[k];
+        }
+    } else {
+        for (int u = threadIdx.x; u < kSmallM * e.n; u += kSmallThreads) {
+            const int i = u & (kSmallM - 1), j = u / kSmallM;
+            if (i >= e.m) continue;
+            uint16_t h;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(x + tile_at(i, j & ~7) + (j & 7) * 2));
+            out[i + j * a.o_j] = Cvt<TO>::from_f(__half2float(__ushort_as_half(h)));
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------------
 struct NsPlan {
     int64_t m, n, batch, ldx, ldm;
@@ -511,6 +757,21 @@ int ns_product(const NsMaps &a, const NsMaps &b, const NsMaps &out, const NsMaps
     return 0;
 }
 
+template <typename T, typename TO> int ns_small(const NsSmall &a, int64_t batch, cudaStream_t st) {
+    auto kernel = ns_small_kernel<T, TO>;
+    const int bytes = (2 + (a.e.n + 63) / 64) * kTileBytes + 1024;
+    static bool attr_set[64] = {false};
+    int dev = 0;
+    SRUB_CUDA_CHECK(cudaGetDevice(&dev));
+    if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+        SRUB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 + kSmallN / 64) * kTileBytes + 1024));
+        attr_set[dev] = true;
+    }
+    kernel<<<(unsigned)batch, kSmallThreads, bytes, st>>>(a);
+    SRUB_CUDA_CHECK(cudaGetLastError());
+    return 0;
+}
+
 }  // namespace
 
 }  // namespace srub
@@ -525,7 +786,7 @@ size_t sru_b200_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64
 }
 
 int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t rows, int64_t cols, int64_t stride_batch,
-                           int64_t stride_row, int64_t stride_col, int steps, double a, double b, double c, double eps,
+                           int64_t stride_row, int64_t stride_col, int steps, double ca, double cb, double cc, double eps,
                            int grad_dtype, int out_dtype, void *workspace, size_t workspace_bytes, void *stream) {
     if (batch < 0 || rows < 0 || cols < 0 || batch > 65535 || rows > (1 << 20) || cols > (1 << 20))
         return set_error(SRU_ERR_BAD_ARG, "bad sizes: %lld matrices of %lld x %lld", (long long)batch, (long long)rows, (long long)cols);
@@ -569,6 +830,17 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     if (e.pitch == e.len || e.lines == 1) { e.len *= e.lines; e.lines = 1; e.pitch = 0; }       // one line
     e.parts = (int)std::min<int64_t>((e.lines * ((e.len + 2047) / 2048) + 7) / 8, kMaxParts);
     const dim3 norm_grid((unsigned)e.parts, (unsigned)batch);
+    if (p.m <= kSmallM && p.n <= kSmallN) {
+        NsSmall a;
+        memset(&a, 0, sizeof(a));
+        a.e = e; a.e.dst = out;
+        a.o_i = tall ? 1 : cols; a.o_j = tall ? cols : 1; a.o_b = rows * cols;
+        a.steps = steps; a.ca = (float)ca; a.cb = (float)cb; a.cc = (float)cc; a.err = err;
+        a.out_wide = cols % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+        auto go = [&](auto t, auto to) { return ns_small<decltype(t), decltype(to)>(a, batch, st); };
+        auto go_out = [&](auto t) { return out_dtype == SRU_F16 ? go(t, __half()) : go(t, __nv_bfloat16()); };
+        return grad_dtype == SRU_F32 ? go_out(float()) : grad_dtype == SRU_F16 ? go_out(__half()) : go_out(__nv_bfloat16());
+    }
     auto begin = [&](auto t) {
         using T = decltype(t);
         ns_norm_kernel<T><<<norm_grid, 256, 0, st>>>(e);
@@ -602,7 +874,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         memset(&g, 0, sizeof(g));
         g.batch = (int)batch; g.err = err;
         g.M = (int)p.m; g.N = (int)p.m; g.K = (int)p.n; g.symmetric = 1;
-        g.ca = (float)a; g.cb = (float)b; g.cc = (float)c;
+        g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc;
         if (int rc = ns_product<128, false, false, kPlain>(xm[cur], xm[cur], am, am, g, sms, st)) return rc;
         g.K = (int)p.m;
         if (int rc = ns_product<128, false, false, kCombine>(am, am, mm, am, g, sms, st)) return rc;

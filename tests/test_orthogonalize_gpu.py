@@ -75,6 +75,14 @@ def test_larger(rows, cols):
     assert float(values[0]) < 1.3
 
 
+@pytest.mark.parametrize("rows,cols", [(128, 768), (768, 128), (128, 769), (770, 127), (128, 255), (120, 511), (65, 512),
+                                       (64, 513), (16, 700), (3, 768), (129, 768), (129, 640)])
+def test_where_one_cta_takes_the_matrix(rows, cols):
+    """Both sides of the sizes at which a matrix stays in one SM's shared memory, and of its column groups."""
+    check(gradient(1, rows, cols, F32, rows + cols)[0], F16)
+    check(gradient(4, rows, cols, F16, rows + cols), BF16)
+
+
 def test_singular_values_gather_around_one():
     g = torch.Generator().manual_seed(9)
     got = orthogonalize(torch.randn(300, 900, generator=g).to(DEV)).double().cpu()
