@@ -144,6 +144,20 @@ __device__ __forceinline__ void bulk_copy_g2s(uint32_t dst_smem, const void *src
 }
 
 // ---------------------------------------------------------------------------------------
+// Launches that follow each other closely (programmatic dependent launch): the second kernel starts while the first still
+// runs, sets itself up, and touches memory only after previous_kernel_done(), which waits until the first is complete and
+// its writes are visible.  early_next_kernel() lets the next one start.
+// ---------------------------------------------------------------------------------------
+__device__ __forceinline__ void early_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void previous_kernel_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+static inline cudaLaunchAttribute early_launch() {
+    cudaLaunchAttribute a;
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    return a;
+}
+
+// ---------------------------------------------------------------------------------------
 // Fast sigmoid pieces: sigma(z) = 1 / (1 + 2^(-z*log2(e)))
 // ---------------------------------------------------------------------------------------
 __device__ __forceinline__ float ex2_approx(float x) {

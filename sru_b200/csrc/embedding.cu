@@ -35,6 +35,8 @@ struct EmbArgs {
     int d;
     int passes;
     float scale;
+    int dst_size;                     // bytes of an element of dW
+    bool fill16;                      // rows of dW are 16-byte aligned
     int *err;
 };
 
@@ -43,35 +45,41 @@ template <typename TK> __device__ __forceinline__ int64_t token_at(const void *t
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------
-// One warp per (row, block of 32 * VEC * REP columns): REP loads of VEC elements per lane in flight.
+// y taken as one line of groups of VEC elements, REP groups per thread, neighbouring threads on neighbouring groups: every
+// store instruction fills whole lines whatever the row length (a warp per block of a row left most lanes idle in the last
+// block of a row: 520 floats 18.5 us for 32768 rows, 68 MB).
 template <typename TK, typename TI, typename TO, int VEC, int REP>
-__global__ void __launch_bounds__(256) embedding_fwd_kernel(const EmbArgs a, int blocks_per_row) {
-    const int lane = threadIdx.x & 31;
-    const int64_t units = a.n * blocks_per_row, step = (int64_t)gridDim.x * 8;
-    for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < units; w += step) {
-        const int64_t row = w / blocks_per_row;
-        const int c0 = (int)(w - row * blocks_per_row) * (32 * VEC * REP) + lane * VEC;
-        const int64_t t = token_at<TK>(a.tokens, row);
-        const bool ok = t >= 0 && t < a.v;
-        const TI *src = static_cast<const TI *>(a.src) + (ok ? t : 0) * a.ld;
-        TO *dst = static_cast<TO *>(a.dst) + row * a.d;
-        Pack<TI, VEC> in[REP];
+__global__ void __launch_bounds__(256) embedding_fwd_kernel(const EmbArgs a, uint32_t groups_per_row, uint32_t step_rows, uint32_t step_groups) {
+    const int64_t total = a.n * groups_per_row;
+    const int64_t g0 = (int64_t)blockIdx.x * (256 * REP) + threadIdx.x;
+    // row and group within it, by one division; 256 groups on are step_rows rows and step_groups groups
+    uint32_t row = total <= 0xffffffffll ? (uint32_t)g0 / groups_per_row : (uint32_t)(g0 / groups_per_row);
+    uint32_t col = (uint32_t)(g0 - (int64_t)row * groups_per_row);
+    const uint32_t n = (uint32_t)a.n, ld = (uint32_t)a.ld;      // all below 2^31
+    const uint64_t v = (uint64_t)a.v;
+    Pack<TI, VEC> in[REP];
+    bool bad = false;
 #pragma unroll
-        for (int r = 0; r < REP; ++r) {
-            const int c = c0 + r * 32 * VEC;
-            if (ok && c < a.d) in[r] = *reinterpret_cast<const Pack<TI, VEC> *>(src + c);
-            else memset(&in[r], 0, sizeof(in[r]));
+    for (int r = 0; r < REP; ++r) {
+        memset(&in[r], 0, sizeof(in[r]));
+        if (row < n) {
+            const uint64_t t = (uint64_t)token_at<TK>(a.tokens, row);       // a negative one is a large one
+            if (t < v) in[r] = *reinterpret_cast<const Pack<TI, VEC> *>(static_cast<const TI *>(a.src) + (uint64_t)(uint32_t)t * ld + col * VEC);
+            else bad = true;
         }
-#pragma unroll
-        for (int r = 0; r < REP; ++r) {
-            const int c = c0 + r * 32 * VEC;
-            Pack<TO, VEC> out;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) out.v[k] = Cvt<TO>::from_f(Cvt<TI>::to_f(in[r].v[k]) * a.scale);
-            if (c < a.d) *reinterpret_cast<Pack<TO, VEC> *>(dst + c) = out;
-        }
-        if (!ok && lane == 0) atomicExch(a.err, kSiteToken);
+        row += step_rows;
+        col += step_groups;
+        if (col >= groups_per_row) { col -= groups_per_row; ++row; }
     }
+#pragma unroll
+    for (int r = 0; r < REP; ++r) {
+        const int64_t g = g0 + r * 256;
+        Pack<TO, VEC> out;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) out.v[k] = Cvt<TO>::from_f(Cvt<TI>::to_f(in[r].v[k]) * a.scale);
+        if (g < total) *reinterpret_cast<Pack<TO, VEC> *>(static_cast<TO *>(a.dst) + g * VEC) = out;
+    }
+    if (bad) atomicExch(a.err, kSiteToken);
 }
 
 // ---- sort -------------------------------------------------------------------------------------------------------
@@ -99,13 +107,19 @@ template <typename TK> __device__ __forceinline__ uint32_t key_at(const EmbArgs 
 // Stable radix sort, 8 bits a pass, by ONE cluster: every warp owns a contiguous part of the positions and a histogram of
 // its own; counts become starting offsets by a prefix over (digit, CTA, warp), the CTAs' totals travelling through
 // distributed shared memory; then every warp writes its entries in order.  Counts are integers: no order matters.
-template <typename TK>
-__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortWarps * 32)
-embedding_sort_kernel(const EmbArgs a) {
-    __shared__ uint32_t hist[kSortWarps][kBins];
-    __shared__ uint32_t totals[kSortCtas][kBins];
-    __shared__ uint32_t offs[kBins];
-    __shared__ uint32_t warp_sum[8];
+constexpr int kHeld = 8;              // entries per lane that stay in registers between counting and writing
+struct SortShared {
+    uint32_t hist[kSortWarps][kBins];
+    uint32_t totals[kSortCtas][kBins];
+    uint32_t offs[kBins];
+    uint32_t warp_sum[8];
+};
+
+template <typename TK> __device__ __forceinline__ void sort_tokens(const EmbArgs &a, SortShared &sh) {
+    auto &hist = sh.hist;
+    auto &totals = sh.totals;
+    auto &offs = sh.offs;
+    auto &warp_sum = sh.warp_sum;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int64_t per = ((a.n + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps) + 31) / 32 * 32;
@@ -121,9 +135,24 @@ embedding_sort_kernel(const EmbArgs a) {
             if (pass == 0) return make_uint2(key_at<TK>(a, i), (uint32_t)i);
             return __ldcg(in + i);         // written by other SMs of the cluster: past L1
         };
+        const bool held = per <= 32 * kHeld;        // the same for all warps
+        uint2 mine[kHeld];
+        if (held) {
+#pragma unroll
+            for (int h = 0; h < kHeld; ++h) {
+                const int64_t i = i0 + h * 32 + lane;
+                mine[h] = i < i1 ? entry(i) : make_uint2(0u, 0u);
+            }
+        }
         for (int k = lane; k < kBins; k += 32) hist[warp][k] = 0;
         __syncwarp();
-        for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&hist[warp][(entry(i).x >> shift) & 255u], 1u);
+        if (held) {
+#pragma unroll
+            for (int h = 0; h < kHeld; ++h)
+                if (i0 + h * 32 + lane < i1) atomicAdd(&hist[warp][(mine[h].x >> shift) & 255u], 1u);
+        } else {
+            for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&hist[warp][(entry(i).x >> shift) & 255u], 1u);
+        }
         __syncthreads();
         if (threadIdx.x < kBins) {
             uint32_t s = 0;
@@ -159,9 +188,7 @@ embedding_sort_kernel(const EmbArgs a) {
             offs[threadIdx.x] = base + below;
         }
         __syncthreads();
-        for (int64_t i = i0; i < i1; i += 32) {
-            const bool on = i + lane < i1;
-            const uint2 e = on ? entry(i + lane) : make_uint2(0u, 0u);
+        auto write = [&](bool on, uint2 e) {
             const uint32_t digit = (e.x >> shift) & 255u;
             const unsigned same = __match_any_sync(0xffffffffu, on ? digit : 256u + lane);
             const uint32_t at = on ? hist[warp][digit] : 0u;
@@ -171,9 +198,60 @@ embedding_sort_kernel(const EmbArgs a) {
                 out[offs[digit] + at + __popc(same & ((1u << lane) - 1u))] = e;
             }
             __syncwarp();
+        };
+        if (held) {
+#pragma unroll
+            for (int h = 0; h < kHeld; ++h)
+                if (i0 + h * 32 < i1) write(i0 + h * 32 + lane < i1, mine[h]);
+        } else {
+            for (int64_t i = i0; i < i1; i += 32) {
+                const bool on = i + lane < i1;
+                write(on, on ? entry(i + lane) : make_uint2(0u, 0u));
+            }
         }
         __threadfence();
         cluster_barrier();
+    }
+}
+
+template <typename TK>
+__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortWarps * 32)
+embedding_sort_kernel(const EmbArgs a) {
+    __shared__ SortShared sh;
+    early_next_kernel();
+    sort_tokens<TK>(a, sh);
+}
+
+// Zeros in those of the rows [block * kFillRows, ...) of dW whose token does not occur, which a bisection of the sorted
+// positions tells for every row.  (Zeros everywhere before the sums, in the sort's launch or as a memory set, write the rows
+// that occur twice and leave L2 full of lines that the sums then have to push out: 133 and 121 us for 16384 tokens over
+// 50000 x 2048 floats.)
+constexpr int kFillRows = 64;
+__device__ __forceinline__ void fill_absent(const EmbArgs &a, int64_t block) {
+    __shared__ bool present[kFillRows];
+    const int64_t r0 = block * kFillRows;
+    const int rows = (int)min((int64_t)kFillRows, a.v - r0);
+    if (threadIdx.x < rows) {
+        const uint32_t row = (uint32_t)(r0 + threadIdx.x);
+        int64_t lo = 0, hi = a.n;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi) >> 1;
+            if (a.sorted[mid].x < row) lo = mid + 1;
+            else hi = mid;
+        }
+        present[threadIdx.x] = lo < a.n && a.sorted[lo].x == row;
+    }
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row_bytes = (int64_t)a.d * a.dst_size;
+    for (int k = warp; k < rows; k += blockDim.x >> 5) {
+        if (present[k]) continue;
+        char *p = static_cast<char *>(a.dst) + (r0 + k) * row_bytes;
+        if (a.fill16) {
+            for (int64_t c = lane * 16; c < row_bytes; c += 512) __stcs(reinterpret_cast<uint4 *>(p + c), make_uint4(0, 0, 0, 0));
+        } else {
+            for (int64_t c = lane * 2; c < row_bytes; c += 64) *reinterpret_cast<uint16_t *>(p + c) = 0;
+        }
     }
 }
 
@@ -192,10 +270,17 @@ __device__ __forceinline__ void store_sum(TO *row, int c0, int d, const float (&
     }
 }
 
+// The grid's last CTAs fill the rows of absent tokens meanwhile.
 template <typename TI, typename TO, int VEC, int REP>
-__global__ void __launch_bounds__(128) embedding_sum_kernel(const EmbArgs a, int blocks_per_row) {
+__global__ void __launch_bounds__(128) embedding_sum_kernel(const EmbArgs a, int blocks_per_row, unsigned sum_ctas) {
+    early_next_kernel();
+    previous_kernel_done();
+    if (blockIdx.x >= sum_ctas) {
+        fill_absent(a, blockIdx.x - sum_ctas);
+        return;
+    }
     const int lane = threadIdx.x & 31;
-    const int64_t tiles = (a.n + kTile - 1) / kTile, units = tiles * blocks_per_row, step = (int64_t)gridDim.x * 4;
+    const int64_t tiles = (a.n + kTile - 1) / kTile, units = tiles * blocks_per_row, step = (int64_t)sum_ctas * 4;
     for (int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); w < units; w += step) {
         const int64_t tile = w / blocks_per_row, i0 = tile * kTile;
         const int c0 = (int)(w - tile * blocks_per_row) * (32 * VEC * REP) + lane * VEC;
@@ -203,103 +288,126 @@ __global__ void __launch_bounds__(128) embedding_sum_kernel(const EmbArgs a, int
         const uint2 mine = (i0 + lane < a.n) ? a.sorted[i0 + lane] : make_uint2(none, 0u);
         const uint32_t before = i0 > 0 ? a.sorted[i0 - 1].x : none;
         const uint32_t after = i0 + kTile < a.n ? a.sorted[i0 + kTile].x : none;
-        if (__shfl_sync(0xffffffffu, mine.x, 0) == none) continue;      // sorted: nothing follows
+        // sorted: the positions that count come first, and a bit says where a run ends (the tile's end ends them all)
+        const int count = __popc(__ballot_sync(0xffffffffu, mine.x != none));
+        const uint32_t next_key = __shfl_down_sync(0xffffffffu, mine.x, 1);
+        const unsigned ends = __ballot_sync(0xffffffffu, lane == kTile - 1 || next_key != mine.x);
+        const TI *src = static_cast<const TI *>(a.src) + c0;
         float acc[REP][VEC];
 #pragma unroll
         for (int r = 0; r < REP; ++r)
 #pragma unroll
             for (int k = 0; k < VEC; ++k) acc[r][k] = 0.0f;
         bool whole_head = true;                             // the current run reaches back to the tile's first entry
-        constexpr int G = 4;                                // rows requested together
-        for (int e0 = 0; e0 < kTile; e0 += G) {
+        constexpr int G = 8;                                // rows requested together
+        for (int e0 = 0; e0 < count; e0 += G) {
             Pack<TI, VEC> in[G][REP];
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const uint32_t key = __shfl_sync(0xffffffffu, mine.x, e0 + g), pos = __shfl_sync(0xffffffffu, mine.y, e0 + g);
-                const TI *row = static_cast<const TI *>(a.src) + (int64_t)pos * a.d;
+                const TI *row = src + (int64_t)__shfl_sync(0xffffffffu, mine.y, e0 + g) * a.d;
 #pragma unroll
                 for (int r = 0; r < REP; ++r) {
-                    const int c = c0 + r * 32 * VEC;
-                    if (key != none && c < a.d) in[g][r] = *reinterpret_cast<const Pack<TI, VEC> *>(row + c);
+                    if (e0 + g < count && c0 + r * 32 * VEC < a.d) in[g][r] = *reinterpret_cast<const Pack<TI, VEC> *>(row + r * 32 * VEC);
                     else memset(&in[g][r], 0, sizeof(in[g][r]));
                 }
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const int e = e0 + g;
-                const uint32_t key = __shfl_sync(0xffffffffu, mine.x, e);
-                const uint32_t next = e + 1 < kTile ? __shfl_sync(0xffffffffu, mine.x, e + 1 & 31) : after;
 #pragma unroll
                 for (int r = 0; r < REP; ++r)
 #pragma unroll
                     for (int k = 0; k < VEC; ++k) acc[r][k] += Cvt<TI>::to_f(in[g][r].v[k]);
-                if (key == none) continue;
-                const bool crosses_in = whole_head && key == before;
-                if (next != key || e == kTile - 1) {
-                    if (crosses_in)
-                        store_sum<float, VEC, REP>(a.part + (tile * 2) * a.d, c0, a.d, acc, 1.0f);
-                    else if (next == key)
-                        store_sum<float, VEC, REP>(a.part + (tile * 2 + 1) * a.d, c0, a.d, acc, 1.0f);
-                    else
-                        store_sum<TO, VEC, REP>(static_cast<TO *>(a.dst) + (int64_t)key * a.d, c0, a.d, acc, a.scale);
+                if (!((ends >> e) & 1u) || e >= count) continue;
+                const uint32_t key = __shfl_sync(0xffffffffu, mine.x, e);
+                if (whole_head && key == before)
+                    store_sum<float, VEC, REP>(a.part + (tile * 2) * a.d, c0, a.d, acc, 1.0f);
+                else if (e == kTile - 1 && after == key)
+                    store_sum<float, VEC, REP>(a.part + (tile * 2 + 1) * a.d, c0, a.d, acc, 1.0f);
+                else
+                    store_sum<TO, VEC, REP>(static_cast<TO *>(a.dst) + (int64_t)key * a.d, c0, a.d, acc, a.scale);
 #pragma unroll
-                    for (int r = 0; r < REP; ++r)
+                for (int r = 0; r < REP; ++r)
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) acc[r][k] = 0.0f;
-                    whole_head = false;
-                }
+                    for (int k = 0; k < VEC; ++k) acc[r][k] = 0.0f;
+                whole_head = false;
             }
         }
     }
 }
 
-// Runs that cross tiles: the warp of the tile in which the run starts adds the tiles' partial rows in order.
+// Runs that cross tiles: of the tile in which the run starts, a CTA per block of columns adds the tiles' partial rows, the
+// tiles in four contiguous parts, one warp each, then the parts in order: the order is fixed by the tokens alone.
 template <typename TO, int VEC, int REP>
-__global__ void __launch_bounds__(128) embedding_join_kernel(const EmbArgs a, int blocks_per_row) {
-    const int lane = threadIdx.x & 31;
-    const int64_t tiles = (a.n + kTile - 1) / kTile, units = tiles * blocks_per_row, step = (int64_t)gridDim.x * 4;
-    for (int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); w < units; w += step) {
-        const int64_t tile = w / blocks_per_row, i0 = tile * kTile, i1 = i0 + kTile;
-        if (i1 >= a.n) continue;
-        const uint32_t key = a.sorted[i1 - 1].x;
-        if (key == (uint32_t)a.v || a.sorted[i1].x != key) continue;                       // nothing continues
-        if (i0 > 0 && a.sorted[i0].x == key && a.sorted[i0 - 1].x == key) continue;         // it started earlier
-        const int c0 = (int)(w - tile * blocks_per_row) * (32 * VEC * REP) + lane * VEC;
-        float acc[REP][VEC];
-#pragma unroll
-        for (int r = 0; r < REP; ++r) {
-            const int c = c0 + r * 32 * VEC;
-            Pack<float, VEC> p;
-            memset(&p, 0, sizeof(p));
-            if (c < a.d) p = *reinterpret_cast<const Pack<float, VEC> *>(a.part + (tile * 2 + 1) * a.d + c);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[r][k] = p.v[k];
+__global__ void __launch_bounds__(128) embedding_join_kernel(const EmbArgs a) {
+    __shared__ float parts[3][32 * VEC * REP];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t tiles = (a.n + kTile - 1) / kTile, tile = blockIdx.x, i0 = tile * kTile, i1 = i0 + kTile;
+    previous_kernel_done();
+    if (i1 >= a.n) return;
+    const uint32_t key = a.sorted[i1 - 1].x, next = a.sorted[i1].x, first = a.sorted[i0].x;
+    const uint32_t before = i0 > 0 ? a.sorted[i0 - 1].x : (uint32_t)a.v;
+    if (key == (uint32_t)a.v || next != key || (first == key && before == key)) return;     // no run starts here and goes on
+    // tiles that the run reaches behind this one: the first 32, then by bisection in 32 parts
+    int64_t lo = tile + 1, hi = tiles;          // the run covers the start of every tile below lo, of none from hi on
+    const unsigned m = __ballot_sync(0xffffffffu, lo + lane < hi && a.sorted[(lo + lane) * kTile].x == key);
+    if (m != 0xffffffffu) {
+        lo += __ffs(~m) - 1;
+    } else {
+        for (lo += 32; lo < hi;) {
+            const int64_t step = (hi - lo + 31) / 32, u = lo + lane * step;
+            const unsigned c = __ballot_sync(0xffffffffu, u < hi && a.sorted[u * kTile].x == key);
+            const int covered = c == 0xffffffffu ? 32 : __ffs(~c) - 1;
+            if (covered == 0) break;
+            const int64_t last = lo + (covered - 1) * step;     // the last probed tile inside the run
+            hi = min(hi, last + step);
+            lo = last + 1;
         }
-        for (int64_t u0 = tile + 1;; u0 += 32) {
-            // how many of the next 32 tiles begin inside this run
-            const int64_t u = u0 + lane;
-            const bool in = u < tiles && a.sorted[u * kTile].x == key;
-            const unsigned m = __ballot_sync(0xffffffffu, in);
-            const int count = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
-#pragma unroll 4
-            for (int q = 0; q < count; ++q) {
-#pragma unroll
-                for (int r = 0; r < REP; ++r) {
-                    const int c = c0 + r * 32 * VEC;
-                    if (c >= a.d) continue;
-                    const Pack<float, VEC> p = *reinterpret_cast<const Pack<float, VEC> *>(a.part + (u0 + q) * 2 * a.d + c);
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) acc[r][k] += p.v[k];
-                }
-            }
-            if (count < 32) break;
-        }
-        store_sum<TO, VEC, REP>(static_cast<TO *>(a.dst) + (int64_t)key * a.d, c0, a.d, acc, a.scale);
     }
+    const int64_t count = lo - (tile + 1), per = (count + 3) / 4, q0 = min(count, warp * per), q1 = min(count, q0 + per);
+    const int c0 = blockIdx.y * (32 * VEC * REP) + lane * VEC;
+    float acc[REP][VEC];
+#pragma unroll
+    for (int r = 0; r < REP; ++r)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[r][k] = 0.0f;
+    constexpr int G = 8;                        // rows requested together
+    auto add_rows = [&](int64_t row, int64_t step, int n) {
+        Pack<float, VEC> in[G][REP];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int r = 0; r < REP; ++r) {
+                const int c = c0 + r * 32 * VEC;
+                if (g < n && c < a.d) in[g][r] = *reinterpret_cast<const Pack<float, VEC> *>(a.part + (row + g * step) * a.d + c);
+                else memset(&in[g][r], 0, sizeof(in[g][r]));
+            }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int r = 0; r < REP; ++r)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) acc[r][k] += in[g][r].v[k];
+    };
+    if (warp == 0) add_rows(tile * 2 + 1, 0, 1);
+    for (int64_t q = q0; q < q1; q += G) add_rows((tile + 1 + q) * 2, 2, (int)min((int64_t)G, q1 - q));
+    if (warp > 0)
+#pragma unroll
+        for (int r = 0; r < REP; ++r)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) parts[warp - 1][(r * 32 + lane) * VEC + k] = acc[r][k];
+    __syncthreads();
+    if (warp > 0) return;
+    for (int w = 0; w < 3; ++w)
+#pragma unroll
+        for (int r = 0; r < REP; ++r)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc[r][k] += parts[w][(r * 32 + lane) * VEC + k];
+    store_sum<TO, VEC, REP>(static_cast<TO *>(a.dst) + (int64_t)key * a.d, c0, a.d, acc, a.scale);
 }
 
 int check_embedding(int64_t n, int64_t v, int64_t d, int64_t ld, int token_bytes, int table_dtype, int y_dtype) {
-    if (n < 0 || v < 1 || d < 1 || ld < d || n > 0x7fffffff || v > 0x7fffffff || d > (1 << 24))
+    if (n < 0 || v < 1 || d < 1 || ld < d || ld > 0x7fffffff || n > 0x7fffffff || v > 0x7fffffff || d > (1 << 24))
         return set_error(SRU_ERR_BAD_ARG, "bad sizes: %lld tokens, table (%lld, %lld) with row stride %lld", (long long)n,
                          (long long)v, (long long)d, (long long)ld);
     if (token_bytes != 4 && token_bytes != 8) return set_error(SRU_ERR_BAD_ARG, "tokens must be 4 or 8 bytes wide");
@@ -315,33 +423,43 @@ bool aligned16(const void *p, int64_t row_bytes) { return reinterpret_cast<uintp
 template <typename TK, typename TI, typename TO> int launch_forward(const EmbArgs &a, cudaStream_t st) {
     constexpr int VEC = 16 / sizeof(TO);
     const bool wide = aligned16(a.src, a.ld * sizeof(TI)) && aligned16(a.dst, a.d * sizeof(TO));
-    auto go = [&](auto vec, auto rep) {
+    auto go = [&](auto vec, auto rep) -> int {
         constexpr int V = decltype(vec)::value, R = decltype(rep)::value;
-        const int per_row = (a.d + 32 * V * R - 1) / (32 * V * R);
-        const int64_t blocks = std::min<int64_t>((a.n * per_row + 7) / 8, 148 * 64);
-        embedding_fwd_kernel<TK, TI, TO, V, R><<<(unsigned)blocks, 256, 0, st>>>(a, per_row);
+        const int64_t blocks = (a.n * (a.d / V) + 256 * R - 1) / (256 * R);
+        if (blocks > 0x7fffffff) return set_error(SRU_ERR_UNSUPPORTED, "embedding: n * hidden too large");
+        const uint32_t groups = a.d / V;
+        embedding_fwd_kernel<TK, TI, TO, V, R><<<(unsigned)blocks, 256, 0, st>>>(a, groups, 256 / groups, 256 % groups);
+        SRUB_CUDA_CHECK(cudaGetLastError());
+        return 0;
     };
-    if (wide) go(std::integral_constant<int, VEC>(), std::integral_constant<int, 2>());
-    else go(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
-    SRUB_CUDA_CHECK(cudaGetLastError());
-    return 0;
+    if (!wide) return go(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
+    // a few rows: one group per thread, so that they reach all SMs
+    if (a.n * (a.d / VEC) < 148 * 2048) return go(std::integral_constant<int, VEC>(), std::integral_constant<int, 1>());
+    return go(std::integral_constant<int, VEC>(), std::integral_constant<int, 2>());
 }
 
 template <typename TI, typename TO> int launch_sums(const EmbArgs &a, cudaStream_t st) {
     constexpr int VEC = 16 / sizeof(TI);
     const bool wide = aligned16(a.src, a.d * sizeof(TI)) && aligned16(a.dst, a.d * sizeof(TO));
-    auto go = [&](auto vec, auto rep) {
+    auto go = [&](auto vec, auto rep) -> int {
         constexpr int V = decltype(vec)::value, R = decltype(rep)::value;
         const int per_row = (a.d + 32 * V * R - 1) / (32 * V * R);
+        if (per_row > 65535) return set_error(SRU_ERR_UNSUPPORTED, "embedding: hidden too large");
         const int64_t units = (a.n + kTile - 1) / kTile * per_row;
-        const int64_t blocks = std::min<int64_t>((units + 3) / 4, 148 * 64);
-        embedding_sum_kernel<TI, TO, V, R><<<(unsigned)blocks, 128, 0, st>>>(a, per_row);
-        embedding_join_kernel<TO, V, R><<<(unsigned)blocks, 128, 0, st>>>(a, per_row);
+        const int64_t sums = std::min<int64_t>((units + 3) / 4, 148 * 64), fill = (a.v + kFillRows - 1) / kFillRows;
+        cudaLaunchConfig_t cfg;
+        memset(&cfg, 0, sizeof(cfg));
+        cudaLaunchAttribute early = early_launch();
+        cfg.attrs = &early; cfg.numAttrs = 1; cfg.stream = st;
+        cfg.blockDim = dim3(128);
+        cfg.gridDim = dim3((unsigned)(sums + fill));
+        SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, embedding_sum_kernel<TI, TO, V, R>, a, per_row, (unsigned)sums));
+        cfg.gridDim = dim3((unsigned)((a.n + kTile - 1) / kTile), per_row);
+        SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, embedding_join_kernel<TO, V, R>, a));
+        return 0;
     };
-    if (wide) go(std::integral_constant<int, VEC>(), std::integral_constant<int, 1>());
-    else go(std::integral_constant<int, 1>(), std::integral_constant<int, 4>());
-    SRUB_CUDA_CHECK(cudaGetLastError());
-    return 0;
+    if (wide) return go(std::integral_constant<int, VEC>(), std::integral_constant<int, 1>());
+    return go(std::integral_constant<int, 1>(), std::integral_constant<int, 4>());
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
@@ -396,8 +514,10 @@ int sru_b200_embedding_backward(void *grad_table, const void *tokens, const void
     const size_t need = sru_b200_embedding_backward_workspace_bytes(n, vocabulary, hidden);
     if (n > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
         return set_error(SRU_ERR_WORKSPACE, "16-byte aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
-    SRUB_CUDA_CHECK(cudaMemsetAsync(grad_table, 0, (size_t)vocabulary * hidden * dtype_size(table_dtype), st));
-    if (n == 0) return 0;
+    if (n == 0) {
+        SRUB_CUDA_CHECK(cudaMemsetAsync(grad_table, 0, (size_t)vocabulary * hidden * dtype_size(table_dtype), st));
+        return 0;
+    }
     EmbArgs a;
     memset(&a, 0, sizeof(a));
     char *ws = static_cast<char *>(workspace);
@@ -410,6 +530,8 @@ int sru_b200_embedding_backward(void *grad_table, const void *tokens, const void
     while (a.passes < 4 && (vocabulary >> (8 * a.passes)) != 0) ++a.passes;     // the largest key is `vocabulary`
     a.err = device_error_flag();
     if (!a.err) return set_error(SRU_ERR_CUDA, "device error flag unavailable");
+    a.dst_size = (int)dtype_size(table_dtype);
+    a.fill16 = aligned16(grad_table, hidden * a.dst_size);
     if (token_bytes == 4) embedding_sort_kernel<int32_t><<<kSortCtas, kSortWarps * 32, 0, st>>>(a);
     else embedding_sort_kernel<int64_t><<<kSortCtas, kSortWarps * 32, 0, st>>>(a);
     SRUB_CUDA_CHECK(cudaGetLastError());

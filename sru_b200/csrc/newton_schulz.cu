@@ -57,13 +57,6 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t sr
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
                  ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z) : "memory");
 }
-// The launches of one call follow each other closely: a kernel may start while the one before it still runs, sets itself
-// up, and touches memory only when that one is complete.
-__device__ __forceinline__ void after_previous_kernel() {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 // Unit -> matrix and tile.  A symmetric product keeps, of 256-row block i, the 128-column tiles from 2 i on.
 __device__ __forceinline__ void ns_unit(const NsArgs &g, int unit, int *z, int *mb, int *nb) {
     *z = unit / g.per_matrix;
@@ -136,7 +129,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    after_previous_kernel();
+    early_next_kernel();
+    previous_kernel_done();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -749,8 +743,7 @@ int ns_product(const NsMaps &a, const NsMaps &b, const NsMaps &out, const NsMaps
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    attr[1] = early_launch();
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, AMN ? a.b : a.a, b.b, out.c, out.t, d.c, g));
