@@ -110,15 +110,17 @@ def load_torch_ops():
 
 
 def native_op(name):
-    """``torch.ops.sru_b200.<name>`` where a call through it is wanted: not while a KernelTimer or NVTX ranges look at
-    single launches, which the Python form of the operator reports."""
-    if timer is not None or nvtx_ranges:
-        return None
+    """``torch.ops.sru_b200.<name>``, whose refusals arrive as RuntimeError."""
     op = _native_ops.get(name)
     if op is None:
         load_torch_ops()
         op = _native_ops[name] = getattr(torch.ops.sru_b200, name).default
     return op
+
+
+def refused(error):
+    """A refusal by a native operator as this package's error; anything else (out of memory, for instance) as it is."""
+    return SruB200Error(str(error)) if type(error) is RuntimeError else error
 
 
 _native_ops = {}

@@ -1,7 +1,7 @@
 // Torch operators of the parts around the recurrent layers, with their autograd: one native call per forward and per
 // backward pass instead of a Python function each (a call costs 8 us instead of 25 on the host, a training step of a
 // short layer a third).  Same C-ABI entry points with the same arguments as the Python functions of
-// linear_recurrence.py and embedding.py, which check the arguments and use these unless a timer is installed.
+// linear_recurrence.py and embedding.py, which use these unless a timer is installed.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -61,6 +61,13 @@ Tensor small(const OptTensor &t) {
     return t->detach().to(at::kFloat).contiguous();
 }
 
+void check_like(const Tensor &u, const OptTensor &t, const char *name, at::IntArrayRef shape, bool floating) {
+    if (!t.has_value() || !t->defined()) return;
+    TORCH_CHECK(t->device() == u.device(), name, " is on ", t->device(), ", u on ", u.device());
+    TORCH_CHECK(t->sizes() == shape, name, " must have shape ", shape, ", got ", t->sizes());
+    TORCH_CHECK(!floating || t->is_floating_point(), name, " must be a floating-point tensor, got ", t->scalar_type());
+}
+
 struct Scanned { Tensor h, last, states; };
 
 Scanned scan(const Tensor &u, const Tensor &c0, const Tensor &bias, const Tensor &mask, bool reverse, bool need_states) {
@@ -86,16 +93,19 @@ class GatedLinearRecurrence : public torch::autograd::Function<GatedLinearRecurr
     static variable_list forward(AutogradContext *ctx, const Tensor &u, const OptTensor &c0, const OptTensor &bias,
                                  const OptTensor &mask, bool reverse) {
         ctx->set_materialize_grads(false);
-        const Tensor r = rows(u.detach(), 2), b = small(bias), m = mask.has_value() ? *mask : Tensor();
+        const bool single = u.dim() == 2;
+        const Tensor r = rows(single ? u.detach().unsqueeze(0) : u.detach(), 2), b = small(bias), m = mask.has_value() ? *mask : Tensor();
         Scanned s = scan(r, small(c0), b, m, reverse, true);
         ctx->save_for_backward({r, b, m, s.states});
+        ctx->saved_data["single"] = single;
         ctx->saved_data["reverse"] = reverse;
         ctx->saved_data["u"] = u.requires_grad();
         ctx->saved_data["c0"] = c0.has_value() && c0->requires_grad() ? (int64_t)c0->scalar_type() : (int64_t)-1;
         ctx->saved_data["bias"] = bias.has_value() && bias->requires_grad() ? (int64_t)bias->scalar_type() : (int64_t)-1;
-        return {s.h, s.last};
+        return {single ? s.h.squeeze(0) : s.h, s.last};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const bool single = ctx->saved_data["single"].toBool();
         const auto saved = ctx->get_saved_variables();
         const Tensor &u = saved[0], &bias = saved[1], &mask = saved[2], &states = saved[3];
         const int64_t c0_type = ctx->saved_data["c0"].toInt(), bias_type = ctx->saved_data["bias"].toInt();
@@ -110,7 +120,7 @@ class GatedLinearRecurrence : public torch::autograd::Function<GatedLinearRecurr
             if (gb.defined()) gb.zero_();
             if (gi.defined()) gl.defined() ? gi.copy_(gl) : gi.zero_();
         } else {
-            if (grads[0].defined()) gh = rows(grads[0].detach().to(u.scalar_type()), 1);
+            if (grads[0].defined()) gh = rows((single ? grads[0].detach().unsqueeze(0) : grads[0].detach()).to(u.scalar_type()), 1);
             const size_t bytes = gb.defined() ? sru_b200_linear_recurrence_backward_workspace_bytes(L, B, d) : 0;
             Tensor ws;
             if (bytes) ws = at::empty({(int64_t)bytes}, u.options().dtype(at::kByte));
@@ -123,22 +133,34 @@ class GatedLinearRecurrence : public torch::autograd::Function<GatedLinearRecurr
         if (gi.defined()) gi = gi.to((at::ScalarType)c0_type);
         if (gb.defined()) gb = gb.to((at::ScalarType)bias_type);
         if (!ctx->saved_data["u"].toBool()) gu = Tensor();
+        else if (single) gu = gu.squeeze(0);
         return once({gu, gi, gb, Tensor(), Tensor()}, "gated_linear_recurrence");
     }
 };
 
 std::tuple<Tensor, Tensor> gated_linear_recurrence(const Tensor &u, const OptTensor &c0, const OptTensor &bias,
                                                    const OptTensor &mask_pad, bool reverse) {
+    TORCH_CHECK(u.is_cuda(), "sru_b200 has no CPU path: u must be a CUDA tensor");
+    code_of(u.scalar_type());
+    TORCH_CHECK((u.dim() == 2 || u.dim() == 3) && u.size(-1) >= 2 && u.size(-1) % 2 == 0,
+                "u must be (length, batch, 2 * hidden) or (batch, 2 * hidden), got ", u.sizes());
+    const bool single = u.dim() == 2;
+    const int64_t B = u.size(-2), d = u.size(-1) / 2;
+    check_like(u, c0, "c0", {B, d}, true);
+    check_like(u, bias, "bias", {d}, true);
+    if (single) check_like(u, mask_pad, "mask_pad", {B}, false);
+    else check_like(u, mask_pad, "mask_pad", {u.size(0), B}, false);
     c10::cuda::CUDAGuard guard(u.device());
     OptTensor mask;
-    if (mask_pad.has_value() && mask_pad->defined()) mask = mask_pad->to(at::kBool).contiguous();
+    if (mask_pad.has_value() && mask_pad->defined()) mask = mask_pad->to(at::kBool).contiguous();      // one step: (B) as (1, B)
     auto learns = [](const OptTensor &t) { return t.has_value() && t->requires_grad(); };
     if (at::GradMode::is_enabled() && (u.requires_grad() || learns(c0) || learns(bias))) {
         variable_list out = GatedLinearRecurrence::apply(u, c0, bias, mask, reverse);
         return {out[0], out[1]};
     }
-    Scanned s = scan(rows(u.detach(), 2), small(c0), small(bias), mask.has_value() ? *mask : Tensor(), reverse, false);
-    return {s.h, s.last};
+    const Tensor r = rows(single ? u.detach().unsqueeze(0) : u.detach(), 2);
+    Scanned s = scan(r, small(c0), small(bias), mask.has_value() ? *mask : Tensor(), reverse, false);
+    return {single ? s.h.squeeze(0) : s.h, s.last};
 }
 
 // ---- embedding ------------------------------------------------------------------------------------------------------
@@ -181,7 +203,22 @@ class EmbeddingLookup : public torch::autograd::Function<EmbeddingLookup> {
     }
 };
 
-Tensor embedding_lookup(const Tensor &tokens, const Tensor &weight, double scale, int64_t padding_idx, at::ScalarType out_dtype) {
+Tensor embedding_lookup(const Tensor &tokens, const Tensor &weight, double scale, c10::optional<int64_t> padding,
+                        c10::optional<at::ScalarType> out_type) {
+    TORCH_CHECK(weight.is_cuda() && tokens.is_cuda(), "sru_b200 has no CPU path: tokens and weight must be CUDA tensors");
+    TORCH_CHECK(tokens.device() == weight.device(), "tokens are on ", tokens.device(), ", weight on ", weight.device());
+    TORCH_CHECK(tokens.scalar_type() == at::kInt || tokens.scalar_type() == at::kLong, "tokens must be int32 or int64, got ", tokens.scalar_type());
+    TORCH_CHECK(weight.dim() == 2 && weight.size(0) > 0 && weight.size(1) > 0, "weight must be (vocabulary, hidden), got ", weight.sizes());
+    const at::ScalarType type = weight.scalar_type(), out_dtype = out_type.value_or(type);
+    code_of(type);
+    TORCH_CHECK(out_dtype == type || (type == at::kFloat && (out_dtype == at::kHalf || out_dtype == at::kBFloat16)),
+                "a ", type, " table cannot be read into ", out_dtype);
+    int64_t padding_idx = -1;
+    if (padding.has_value()) {
+        const int64_t v = weight.size(0);
+        TORCH_CHECK(*padding >= -v && *padding < v, "padding_idx ", *padding, " is outside a table of ", v, " rows");
+        padding_idx = *padding < 0 ? *padding + v : *padding;
+    }
     c10::cuda::CUDAGuard guard(weight.device());
     const Tensor table = weight.stride(1) == 1 && weight.stride(0) >= weight.size(1) ? weight : weight.contiguous();
     const Tensor flat = tokens.detach().reshape({-1}).contiguous();
@@ -195,8 +232,9 @@ Tensor embedding_lookup(const Tensor &tokens, const Tensor &weight, double scale
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(sru_b200, m) {
-    m.def("gated_linear_recurrence(Tensor u, Tensor? c0, Tensor? bias, Tensor? mask_pad, bool reverse) -> (Tensor, Tensor)",
+    m.def("gated_linear_recurrence(Tensor u, Tensor? c0=None, Tensor? bias=None, Tensor? mask_pad=None, bool reverse=False) "
+          "-> (Tensor, Tensor)",
           &gated_linear_recurrence);
-    m.def("embedding_lookup(Tensor tokens, Tensor weight, float scale, int padding_idx, ScalarType out_dtype) -> Tensor",
+    m.def("embedding_lookup(Tensor tokens, Tensor weight, float scale=1.0, int? padding_idx=None, ScalarType? out_dtype=None) -> Tensor",
           &embedding_lookup);
 }

@@ -65,6 +65,12 @@ def embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding
     no gradient.  A token outside the table gives a row of zeros and no gradient, and raises the device error
     flag: ``_lib.check_device_error()`` then raises.
     """
+    if _lib.timer is None and not _lib.nvtx_ranges:
+        _lib.launch_count += 1
+        try:
+            return _lib.native_op("embedding_lookup")(tokens, weight, scale, padding_idx, out_dtype)
+        except RuntimeError as e:
+            raise _lib.refused(e) from None
     if not weight.is_cuda or not tokens.is_cuda:
         raise _lib.SruB200Error("sru_b200 has no CPU path: tokens and weight must be CUDA tensors")
     if tokens.device != weight.device:
@@ -85,10 +91,6 @@ def embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding
         if not -vocabulary <= padding_idx < vocabulary:
             raise _lib.SruB200Error("padding_idx %d is outside a table of %d rows" % (padding_idx, vocabulary))
         padding_idx %= vocabulary
-    op = _lib.native_op("embedding_lookup")
-    if op is not None:
-        _lib.launch_count += 1
-        return op(tokens, weight, scale, padding_idx, out_dtype)
     if weight.stride(1) != 1 or weight.stride(0) < weight.size(1):
         weight = weight.contiguous()
     flat = tokens.detach().reshape(-1)

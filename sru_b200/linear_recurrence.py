@@ -121,6 +121,12 @@ def gated_linear_recurrence(u: Tensor, c0: Optional[Tensor] = None, bias: Option
     contiguous pairs (a batch-first tensor transposed, for instance) is read in place.  Differentiable once in u, c0 and
     bias.
     """
+    if _lib.timer is None and not _lib.nvtx_ranges:
+        _lib.launch_count += 1
+        try:
+            return _lib.native_op("gated_linear_recurrence")(u, c0, bias, mask_pad, reverse)
+        except RuntimeError as e:
+            raise _lib.refused(e) from None
     if not u.is_cuda:
         raise _lib.SruB200Error("sru_b200 has no CPU path: u must be a CUDA tensor")
     if u.dtype not in _TYPES:
@@ -138,11 +144,6 @@ def gated_linear_recurrence(u: Tensor, c0: Optional[Tensor] = None, bias: Option
         _check(u, bias, "bias", (width // 2,))
     if mask_pad is not None:
         _check(u, mask_pad, "mask_pad", (length, batch))
-    op = _lib.native_op("gated_linear_recurrence")
-    if op is not None:
-        _lib.launch_count += 1
-        h, c_last = op(u, c0, bias, mask_pad, reverse)
-        return (h.squeeze(0) if single else h), c_last
     mask = None if mask_pad is None else mask_pad.bool().contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (u, c0, bias)):
         h, c_last = _GatedLinearRecurrence.apply(u, c0, bias, mask, bool(reverse))

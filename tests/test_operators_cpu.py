@@ -86,3 +86,17 @@ def test_orthogonalize_c_arguments():
     assert f(one, one, 1, 4, 5, 20, 5, 1, 5, *tail, 0, 2, None, 0, None) == -3
     assert f(one, one, 1, 4, 5, 20, 5, 1, 5, *tail, 0, 2, ctypes.c_void_p(16), big, None) == -3
     assert f(one, one, 0, 4, 5, 20, 5, 1, 5, *tail, 0, 2, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("timed", [False, True])
+def test_refusals_come_as_the_packages_error(timed, monkeypatch):
+    """Through the native operator and through the Python form that a timer sees alike."""
+    from sru_b200 import embedding_lookup, gated_linear_recurrence
+    monkeypatch.setattr(_lib, "timer", object() if timed else None)
+    with pytest.raises(_lib.SruB200Error, match="no CPU path"):
+        gated_linear_recurrence(torch.zeros(2, 1, 8))
+    with pytest.raises(_lib.SruB200Error, match="no CPU path"):
+        embedding_lookup(torch.zeros(3, dtype=torch.long), torch.zeros(5, 8))
+    assert isinstance(_lib.refused(RuntimeError("x")), _lib.SruB200Error)
+    oom = torch.OutOfMemoryError("x")
+    assert _lib.refused(oom) is oom
