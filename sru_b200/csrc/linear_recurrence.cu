@@ -213,50 +213,84 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 // The affine maps s -> P s + C of all slices' chunks, exchanged: returns the value in front of this warp's chunk and moves
-// *carry behind the last one.  `back`: the slices follow each other from the last to the first.  One buffer is written while
+// *carry behind the last one.  `BACK`: the slices follow each other from the last to the first.  One buffer is written while
 // the other may still be read, so one barrier per round is enough.
+//
+// Between the CTAs of a cluster the CTA's map travels as asynchronous stores that count their bytes on an mbarrier of the
+// receiver.  A cluster barrier in their place has to wait until this round's stores of h are performed: 5300 cycles an
+// exchange of eight CTAs against 1200 within one.
 constexpr int kMaxWarps = 8, kMaxRanks = 8;
 template <int V> struct Map { Num<V> P, C; };
 template <int V> struct Exchange {
     Map<V> warp[2][kMaxWarps][32];
     Map<V> cta[2][kMaxRanks][32];
+    uint64_t arrived[2];
+    uint64_t pad[14];
 };
 
+__device__ __forceinline__ void store_async(uint32_t addr, uint32_t bar, Map<1> m) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];"
+                 ::"r"(addr), "r"(__float_as_uint(m.P.a)), "r"(__float_as_uint(m.C.a)), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void store_async(uint32_t addr, uint32_t bar, Map<2> m) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];"
+                 ::"r"(addr), "l"(m.P.a.v), "l"(m.C.a.v), "r"(bar) : "memory");
+}
+
+// Barriers of a cluster's exchange; no CTA writes to another's shared memory before that one is through here.
+template <int V> __device__ __forceinline__ void exchange_start(Exchange<V> &x, const Place &p) {
+    if (p.ranks == 1) return;
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&x.arrived[0]), 1);
+        mbar_init(smem_u32(&x.arrived[1]), 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    cluster_sync();
+}
+
 template <int V, bool BACK>
-__device__ __forceinline__ Num<V> exchange(Exchange<V> &x, int buf, const Place &p, Map<V> own, Num<V> *carry) {
+__device__ __forceinline__ Num<V> exchange(Exchange<V> &x, int64_t round, const Place &p, Map<V> own, Num<V> *carry, int *err) {
+    const int buf = (int)(round & 1);
     x.warp[buf][p.warp][p.lane] = own;
     __syncthreads();
     Num<V> start = *carry;
     if (p.ranks > 1) {
+        const uint32_t bar = smem_u32(&x.arrived[buf]);
         if (p.warp == 0) {
+            if (p.lane == 0) mbar_arrive_expect_tx(bar, p.ranks * 32 * (uint32_t)sizeof(Map<V>));
             Map<V> t{all<V>(1.0f), all<V>(0.0f)};
-            for (int k = 0; k < p.warps; ++k) {
+#pragma unroll
+            for (int k = 0; k < kMaxWarps; ++k) {
+                if (k >= p.warps) break;
                 const Map<V> m = x.warp[buf][BACK ? p.warps - 1 - k : k][p.lane];
                 t.C = fma(m.P, t.C, m.C);
                 t.P = mul(t.P, m.P);
             }
             const uint32_t here = smem_u32(&x.cta[buf][p.rank][p.lane]);
             for (uint32_t r = 0; r < p.ranks; ++r) {
-                uint32_t there;
+                uint32_t there, there_bar;
                 asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(r));
-                if constexpr (V == 1)
-                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(t.P.a), "f"(t.C.a) : "memory");
-                else
-                    asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(there), "l"(t.P.a.v), "l"(t.C.a.v) : "memory");
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there_bar) : "r"(bar), "r"(r));
+                store_async(there, there_bar, t);
             }
         }
-        cluster_sync();
+        if (!mbar_wait_bounded(bar, (uint32_t)(round >> 1) & 1u) && p.lane == 0) atomicExch(err, 42);
         Num<V> s = *carry;
-        for (uint32_t k = 0; k < p.ranks; ++k) {
-            const uint32_t r = BACK ? p.ranks - 1 - k : k;
-            start = pick(r == p.rank, s, start);
+#pragma unroll
+        for (int k = 0; k < kMaxRanks; ++k) {
+            if (k >= (int)p.ranks) break;
+            const int r = BACK ? (int)p.ranks - 1 - k : k;
+            start = pick(r == (int)p.rank, s, start);
             const Map<V> m = x.cta[buf][r][p.lane];
             s = fma(m.P, s, m.C);
         }
         *carry = s;
     }
     Num<V> s = start, mine = start;
-    for (int k = 0; k < p.warps; ++k) {
+#pragma unroll
+    for (int k = 0; k < kMaxWarps; ++k) {
+        if (k >= p.warps) break;
         const int w = BACK ? p.warps - 1 - k : k;
         mine = pick(w == p.warp, s, mine);
         const Map<V> m = x.warp[buf][w][p.lane];
@@ -393,9 +427,9 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
         load_steps<TT, 2 * V, T>(next, u, a.u_t, left);
     }
     next_flags = load_flags<T>(mask, a.m_t, left, p.lane);
-    if (SPLIT && p.ranks > 1) cluster_sync();       // every CTA has started before another writes to its shared memory
-    int buf = 0;
-    for (int64_t r0 = 0; r0 < a.L; r0 += round, buf ^= 1, left -= round) {
+    if (SPLIT) exchange_start(*x, p);
+    int64_t turn = 0;
+    for (int64_t r0 = 0; r0 < a.L; r0 += round, ++turn, left -= round) {
         const unsigned flags = next_flags;
         if (r0 + round < a.L) {
             if (mask) mask += round * a.m_t;
@@ -432,7 +466,7 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
             if (flags == 0) scan_local<TT, V, T, true>(in, nb, flags, C, P);
             else scan_local<TT, V, T, false>(in, nb, flags, C, P);
             release();
-            const Num<V> c = exchange<V, false>(*x, buf, p, Map<V>{P[T - 1], C[T - 1]}, &carry);
+            const Num<V> c = exchange<V, false>(*x, turn, p, Map<V>{P[T - 1], C[T - 1]}, &carry, a.err);
             if (states) {
 #pragma unroll
                 for (int i = 0; i < T; i += kT)
@@ -473,6 +507,7 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
         h += round * a.h_t;
         if (states) states += (int64_t)slices * (T / kT) * states_t;
     }
+    if (SPLIT && p.ranks > 1) cluster_sync();       // a CTA's last message has arrived before its sender or receiver is gone
     if (slice == 0 && a.last) store_small<V>(a.last, p.col, carry);
 }
 
@@ -535,9 +570,9 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
         for (int s = 0; s < DEPTH; ++s) ask(left + s * round, r_top >= s * round, ring.data + s * kStage, ring.bars + 8 * s);
     }
     fetch(left);
-    if (SPLIT && p.ranks > 1) cluster_sync();
-    int buf = 0;
-    for (int64_t r0 = r_top; r0 >= 0; r0 -= round, buf ^= 1, left += round) {
+    if (SPLIT) exchange_start(*x, p);
+    int64_t turn = 0;
+    for (int64_t r0 = r_top; r0 >= 0; r0 -= round, ++turn, left += round) {
         const unsigned flags = next_flags;
         Num<V> c = next_c;
         Num<V> f[T], keep[T], w[T];      // w = (c_{t-1} - x) f (1 - f)
@@ -608,7 +643,7 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
             ring.next();
         }
         Num<V> dc = carry;
-        if constexpr (SPLIT) dc = exchange<V, true>(*x, buf, p, own, &carry);
+        if constexpr (SPLIT) dc = exchange<V, true>(*x, turn, p, own, &carry, a.err);
         auto finish = [&](auto clean) {
             constexpr bool CLEAN = decltype(clean)::value;
             TT *q = gu + 2 * (T - 1) * a.h_t;
@@ -636,6 +671,7 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
         if (!SPLIT) carry = dc;
         gu -= 2 * round * a.h_t;
     }
+    if (SPLIT && p.ranks > 1) cluster_sync();
     if (a.last && slice == 0) store_small<V>(a.last, p.col, carry);
     if (a.bias_part) store_small<V>(a.bias_part, (p.b * slices + slice) * a.d + p.j, db);
 }
