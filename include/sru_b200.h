@@ -333,7 +333,7 @@ int sru_b200_linear_recurrence_forward(
     int64_t u_stride_t, int64_t u_stride_b, int reverse, int dtype, void *stream);
 
 /* Scratch of the backward pass (partial sums of grad_bias); needed only with a grad_bias. */
-size_t sru_b200_linear_recurrence_backward_workspace_bytes(int64_t length, int64_t batch, int64_t hidden);
+size_t sru_b200_linear_recurrence_backward_workspace_bytes(int64_t length, int64_t batch, int64_t hidden, int dtype);
 
 /*
  * Backward of the above.  With dc_t the whole gradient of c_t (dc_t = grad_h_t + f_{t+1} dc_{t+1}, grad_last added at

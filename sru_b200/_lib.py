@@ -79,7 +79,7 @@ def lib():
         l.sru_b200_linear_recurrence_forward.restype = _int
         l.sru_b200_linear_recurrence_forward.argtypes = [_vp] * 7 + [_i64] * 5 + [_int] * 2 + [_vp]
         l.sru_b200_linear_recurrence_backward_workspace_bytes.restype = ctypes.c_size_t
-        l.sru_b200_linear_recurrence_backward_workspace_bytes.argtypes = [_i64] * 3
+        l.sru_b200_linear_recurrence_backward_workspace_bytes.argtypes = [_i64] * 3 + [_int]
         l.sru_b200_linear_recurrence_backward.restype = _int
         l.sru_b200_linear_recurrence_backward.argtypes = [_vp] * 9 + [_i64] * 7 + [_int] * 2 + [_vp, ctypes.c_size_t, _vp]
         l.sru_b200_embedding_forward.restype = _int

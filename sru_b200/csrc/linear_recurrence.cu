@@ -170,21 +170,31 @@ struct Place {
     int j, shift;                   // first column; its place behind the first column of lane 0
 };
 
-template <int V, bool SPLIT> __device__ __forceinline__ bool find_place(const LinRecArgs &a, Place *p) {
+// With a ring and without slices the CTA's warps stand side by side on 64-column groups of one sequence, and its last warp
+// is not one of `warps`: it asks for the copies.
+constexpr int kSide = 2;
+template <int V, bool SPLIT, bool RING> __device__ __forceinline__ bool find_place(const LinRecArgs &a, Place *p) {
     p->lane = threadIdx.x & 31;
     p->warp = threadIdx.x >> 5;
-    p->warps = blockDim.x >> 5;
+    p->warps = (blockDim.x >> 5) - (RING && !SPLIT ? 1 : 0);
     p->rank = 0; p->ranks = 1;
-    int64_t wid;
-    if (SPLIT) {
-        asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(p->rank));
-        asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(p->ranks));
-        wid = blockIdx.x / p->ranks;
+    int j0;
+    if (SPLIT || RING) {
+        if (SPLIT) {
+            asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(p->rank));
+            asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(p->ranks));
+        }
+        const int64_t unit = blockIdx.x / p->ranks;
+        const int units = SPLIT ? a.groups : (a.groups + kSide - 1) / kSide;        // of a sequence
+        p->b = unit / units;
+        j0 = (int)(unit - p->b * units) * (SPLIT ? 1 : kSide) * 32 * V;
+        if (!SPLIT) p->warps = min(p->warps, (a.d - j0 + 32 * V - 1) / (32 * V));
+        if (!SPLIT && p->warp < p->warps) j0 += p->warp * 32 * V;
     } else {
-        wid = (int64_t)blockIdx.x * p->warps + p->warp;
+        const int64_t wid = (int64_t)blockIdx.x * p->warps + p->warp;
+        p->b = wid / a.groups;
+        j0 = (int)(wid - p->b * a.groups) * 32 * V;
     }
-    p->b = wid / a.groups;
-    const int j0 = (int)(wid - p->b * a.groups) * 32 * V;
     p->j = min(j0 + p->lane * V, a.d - V);
     p->shift = p->j - j0;
     p->col = p->b * a.d + p->j;
@@ -249,11 +259,13 @@ template <int V> __device__ __forceinline__ void exchange_start(Exchange<V> &x, 
     cluster_sync();
 }
 
-template <int V, bool BACK>
-__device__ __forceinline__ Num<V> exchange(Exchange<V> &x, int64_t round, const Place &p, Map<V> own, Num<V> *carry, int *err) {
+// refill() is called when all warps of the CTA have read their chunks.
+template <int V, bool BACK, typename Refill>
+__device__ __forceinline__ Num<V> exchange(Exchange<V> &x, int64_t round, const Place &p, Map<V> own, Num<V> *carry, int *err, Refill refill) {
     const int buf = (int)(round & 1);
     x.warp[buf][p.warp][p.lane] = own;
     __syncthreads();
+    refill();
     Num<V> start = *carry;
     if (p.ranks > 1) {
         const uint32_t bar = smem_u32(&x.arrived[buf]);
@@ -301,10 +313,13 @@ __device__ __forceinline__ Num<V> exchange(Exchange<V> &x, int64_t round, const 
 }
 
 // ---- how a chunk gets to its lanes ----------------------------------------------------------------------------------
-// Ring: a warp's chunks are boxes of T steps x 32 V columns that the copy engine brings into the warp's own part of
-// shared memory, DEPTH of them in flight; lane 0 asks for the box of the chunk DEPTH rounds ahead when all lanes are done
-// with a stage.  This needs 16-byte aligned rows.  Without a ring (other layouts, and a few steps, where setting it up
-// costs more) the next chunk is loaded to registers while the current one is worked on.
+// Ring: the chunks that a CTA's warps work on in one round are neighbours (in time with slices, in columns without), so ONE
+// box per tensor brings them all, DEPTH rounds ahead, into a stage of shared memory.  Issued by the scanning warps, each for
+// its own chunk, the requests cost them 340 cycles a round forward and 490 backward, a tenth and a quarter of their time.
+// Without slices a warp of its own asks for the boxes.  With slices the last warp does, behind the exchange's barrier, when
+// all have read the stage; a ninth warp would leave the others 96 registers each.  This needs 16-byte aligned rows.
+// Without a ring (other layouts, and a few steps, where setting it up costs more) a warp loads its next chunk to registers
+// while it works on the current one.
 template <typename TT> struct Cut {
     static constexpr int kFwdT = sizeof(TT) == 2 ? 16 : 8;      // steps of a slice's chunk, forward, with a ring
     static constexpr int kFwdDepth = 3;
@@ -335,37 +350,40 @@ template <typename P> __device__ __forceinline__ P load_shared(uint32_t addr) {
     return p;
 }
 
-// One warp's ring.  A wait that gives up raises the device error flag; from then on the warp neither waits nor asks for
-// copies, but keeps taking part in its CTA's barriers.
+// A wait that gives up raises the device error flag; from then on the warp waits for nothing more, but keeps taking part
+// in its CTA's barriers.  full: the stage's bytes are there; empty: all scanning warps have read it.
 template <int DEPTH> struct Ring {
     uint32_t data, bars, bytes;
     int stage = 0;
     uint32_t phase = 0;
     bool dead = false;
-    __device__ __forceinline__ void start(uint32_t data_, uint32_t bars_, uint32_t bytes_, int lane) {
+    __device__ __forceinline__ void start(uint32_t data_, uint32_t bars_, uint32_t bytes_, int readers) {
         data = data_; bars = bars_; bytes = bytes_;
-        if (lane == 0) {
-            for (int s = 0; s < DEPTH; ++s) mbar_init(bars + 8 * s, 1);
+        if (threadIdx.x == 0) {
+            for (int s = 0; s < DEPTH; ++s) {
+                mbar_init(bars + 8 * s, 1);
+                mbar_init(bars + 8 * (DEPTH + s), readers);
+            }
             fence_mbar_init();
-            fence_proxy_async();
         }
-        __syncwarp();
+        __syncthreads();
     }
     __device__ __forceinline__ uint32_t at() const { return data + stage * bytes; }
-    __device__ __forceinline__ uint32_t bar() const { return bars + 8 * stage; }
-    __device__ __forceinline__ void wait(int *err) {
-        if (dead || mbar_wait_bounded(bar(), phase)) return;
-        dead = true;
-        atomicExch(err, 41);
-        for (int s = 0; s < DEPTH; ++s)             // copies still in flight land before the CTA can leave
-            mbar_wait_bounded(bars + 8 * s, s < stage ? phase ^ 1 : phase);
+    __device__ __forceinline__ uint32_t full() const { return bars + 8 * stage; }
+    __device__ __forceinline__ uint32_t empty() const { return bars + 8 * (DEPTH + stage); }
+    __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, int *err) {
+        if (!dead && !mbar_wait_bounded(bar, parity)) { dead = true; atomicExch(err, 41); }
     }
     __device__ __forceinline__ void next() { if (++stage == DEPTH) { stage = 0; phase ^= 1; } }
+    __device__ __forceinline__ void read(int lane) {       // this warp has read the stage
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty());
+    }
 };
 
-constexpr int kBarBytes = 256;
-template <int V, int DEPTH> constexpr size_t ring_shared(int warps, size_t stage, bool split) {
-    return (split ? sizeof(Exchange<V>) : 0) + kBarBytes + 128 + (size_t)warps * DEPTH * stage;
+constexpr int kBarBytes = 128;
+template <int V> constexpr size_t ring_shared(size_t stage, int depth, bool split) {
+    return (split ? sizeof(Exchange<V>) : 0) + kBarBytes + stage * depth;
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------
@@ -389,12 +407,12 @@ __device__ __forceinline__ void scan_local(In in, Num<V> nb, unsigned flags, Num
 }
 
 template <typename TT, int V, int T, bool SPLIT, bool RING>
-__global__ void __launch_bounds__(SPLIT ? 256 : 64, SPLIT ? 2 : 6)
+__global__ void __launch_bounds__(SPLIT ? 256 : RING ? 96 : 64, SPLIT ? 2 : RING ? 5 : 6)
 linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const LinRecArgs a) {
     extern __shared__ __align__(128) uint8_t shared[];
     Exchange<V> *x = reinterpret_cast<Exchange<V> *>(shared);
     Place p;
-    if (!find_place<V, SPLIT>(a, &p)) return;
+    if (!find_place<V, SPLIT, RING>(a, &p)) return;
     const Num<V> nb = mul(load_small<V>(a.bias, p.j), all<V>(kNegLog2e));
     Num<V> carry = load_small<V>(a.first, p.col);
     const int slices = SPLIT ? p.warps * (int)p.ranks : 1;
@@ -407,25 +425,37 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
     const int64_t states_t = a.B * a.d;
     float *states = a.states ? a.states + (int64_t)slice * (T / kT) * states_t + p.col : nullptr;
 
-    constexpr uint32_t kRow = 32 * V * 2 * sizeof(TT);
     constexpr int DEPTH = Cut<TT>::kFwdDepth;
-    Ring<DEPTH> ring;
+    constexpr uint32_t kRow = (SPLIT ? 1 : kSide) * 32 * V * 2 * sizeof(TT);       // of the box
+    const int steps = SPLIT ? p.warps * T : T;
     const bool back = a.h_t < 0;                    // time runs backwards: the box's rows as well
-    auto ask = [&](int64_t n, uint32_t to, uint32_t bar) {      // the box of the chunk in front of which n steps are left
-        if (p.lane == 0 && n > 0 && !ring.dead) {
-            mbar_arrive_expect_tx(bar, T * kRow);
-            tma_load_3d(to, &map_u, bar, 2 * (p.j - p.shift), (int)p.b, (int)(back ? n - T : a.L - n));
-        }
+    Ring<DEPTH> ring;
+    int64_t box_left = a.L - (int64_t)p.rank * steps;           // steps from the box's first to the end
+    auto ask = [&](int64_t n, uint32_t to, uint32_t bar) {
+        if (n <= 0) return;                         // behind the end: the box's turn never comes
+        mbar_arrive_expect_tx(bar, steps * kRow);
+        tma_load_3d(to, &map_u, bar, 2 * (p.j - p.shift), (int)p.b, (int)(back ? n - steps : a.L - n));
     };
-    Pack<TT, 2 * V> next[RING ? 1 : T];
-    unsigned next_flags;
     if constexpr (RING) {
         const uint32_t base = smem_u32(shared) + (SPLIT ? (uint32_t)sizeof(Exchange<V>) : 0u);
-        ring.start(base + kBarBytes + p.warp * DEPTH * T * kRow, base + p.warp * DEPTH * 8, T * kRow, p.lane);
-        for (int s = 0; s < DEPTH; ++s) ask(left - s * round, ring.data + s * T * kRow, ring.bars + 8 * s);
-    } else {
-        load_steps<TT, 2 * V, T>(next, u, a.u_t, left);
+        ring.start(base + kBarBytes, base, steps * kRow, p.warps);
+        if (!SPLIT && p.warp >= p.warps) {          // the warp that asks (and, beside the last columns, one without any)
+            if (p.lane == 0 && p.warp == kSide) {
+                for (int64_t n = a.L, turn = 0; n > 0; n -= round, ++turn) {
+                    if (turn >= DEPTH) ring.wait(ring.empty(), ring.phase ^ 1, a.err);
+                    if (ring.dead) break;
+                    ask(n, ring.at(), ring.full());
+                    ring.next();
+                }
+            }
+            return;
+        }
+        if (SPLIT && threadIdx.x == 0)
+            for (int s = 0; s < DEPTH; ++s) ask(box_left - s * round, ring.data + s * ring.bytes, ring.bars + 8 * s);
     }
+    Pack<TT, 2 * V> next[RING ? 1 : T];
+    unsigned next_flags;
+    if constexpr (!RING) load_steps<TT, 2 * V, T>(next, u, a.u_t, left);
     next_flags = load_flags<T>(mask, a.m_t, left, p.lane);
     if (SPLIT) exchange_start(*x, p);
     int64_t turn = 0;
@@ -439,8 +469,9 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
         uint32_t row = 0;
         int32_t row_step = 0;
         if constexpr (RING) {
-            if (left > 0) ring.wait(a.err);
-            row = ring.at() + p.shift * 2 * sizeof(TT) + (back ? (T - 1) * kRow : 0u);
+            if (box_left > 0) ring.wait(ring.full(), ring.phase, a.err);
+            const int first = SPLIT ? p.warp * T : 0;
+            row = ring.at() + (p.shift + (SPLIT ? 0 : p.warp * 32 * V)) * 2 * sizeof(TT) + (back ? steps - 1 - first : first) * kRow;
             row_step = back ? -(int32_t)kRow : (int32_t)kRow;
         } else {
 #pragma unroll
@@ -454,19 +485,14 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
             if constexpr (RING) return load_shared<Pack<TT, 2 * V>>(row + i * row_step);
             else return cur[i];
         };
-        auto release = [&]() {
-            if constexpr (RING) {
-                __syncwarp();
-                ask(left - DEPTH * round, ring.at(), ring.bar());
-                ring.next();
-            }
+        auto refill = [&]() {
+            if (RING && threadIdx.x == (p.warps - 1) * 32 && !ring.dead) ask(box_left - DEPTH * round, ring.at(), ring.full());
         };
         if constexpr (SPLIT) {
             Num<V> C[T], P[T];
             if (flags == 0) scan_local<TT, V, T, true>(in, nb, flags, C, P);
             else scan_local<TT, V, T, false>(in, nb, flags, C, P);
-            release();
-            const Num<V> c = exchange<V, false>(*x, turn, p, Map<V>{P[T - 1], C[T - 1]}, &carry, a.err);
+            const Num<V> c = exchange<V, false>(*x, turn, p, Map<V>{P[T - 1], C[T - 1]}, &carry, a.err, refill);
             if (states) {
 #pragma unroll
                 for (int i = 0; i < T; i += kT)
@@ -502,8 +528,10 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
             };
             if (flags == 0) walk(std::true_type());
             else walk(std::false_type());
-            release();
+            if (RING) ring.read(p.lane);
         }
+        if (RING) ring.next();
+        box_left -= round;
         h += round * a.h_t;
         if (states) states += (int64_t)slices * (T / kT) * states_t;
     }
@@ -513,14 +541,14 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
 
 // ---- backward -------------------------------------------------------------------------------------------------------
 template <typename TT, int V, bool SPLIT, bool RING>
-__global__ void __launch_bounds__(SPLIT ? 256 : 64, SPLIT ? 2 : 8)
+__global__ void __launch_bounds__(SPLIT ? 256 : RING ? 96 : 64, SPLIT ? 2 : RING ? 5 : 6)
 linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_g,
                              const __grid_constant__ CUtensorMap map_s, const LinRecArgs a) {
     extern __shared__ __align__(128) uint8_t shared[];
     Exchange<V> *x = reinterpret_cast<Exchange<V> *>(shared);
     constexpr int T = kT;
     Place p;
-    if (!find_place<V, SPLIT>(a, &p)) return;
+    if (!find_place<V, SPLIT, RING>(a, &p)) return;
     const Num<V> nb = mul(load_small<V>(a.bias, p.j), all<V>(kNegLog2e));
     Num<V> carry = load_small<V>(a.first, p.col), db = all<V>(0.0f);
     const int slices = SPLIT ? p.warps * (int)p.ranks : 1;
@@ -535,22 +563,39 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
     const int64_t states_t = a.B * a.d;
     const float *states = a.states + (t_top / T) * states_t + p.col;
 
-    constexpr uint32_t kRowU = 32 * V * 2 * sizeof(TT), kRowG = kRowU / 2, kRowS = 32 * V * 4;
-    constexpr uint32_t kStage = T * (kRowU + kRowG) + kRowS;
     constexpr int DEPTH = Cut<TT>::kBwdDepth;
-    Ring<DEPTH> ring;
+    constexpr uint32_t kCols = (SPLIT ? 1 : kSide) * 32 * V, kRowU = kCols * 2 * sizeof(TT), kRowG = kCols * sizeof(TT), kRowS = kCols * 4;
+    const int chunks = SPLIT ? p.warps : 1, steps = chunks * T;     // of a box
+    const uint32_t g_at = steps * kRowU, s_at = g_at + steps * kRowG, stage_bytes = s_at + chunks * kRowS;
     const bool back = a.h_t < 0;
-    auto ask = [&](int64_t n, bool more, uint32_t to, uint32_t bar) {
-        if (p.lane == 0 && more && n <= 0) {
-            mbar_arrive(bar);           // a chunk behind the end (first round only): the stage's turn passes empty
-        } else if (p.lane == 0 && more && !ring.dead) {
-            const int t = (int)(back ? n - T : a.L - n), j0 = p.j - p.shift;
-            mbar_arrive_expect_tx(bar, gh ? kStage : T * kRowU + kRowS);
-            tma_load_3d(to, &map_u, bar, 2 * j0, (int)p.b, t);
-            tma_load_3d(to + T * (kRowU + kRowG), &map_s, bar, j0, (int)p.b, (int)((a.L - n) / T));
-            if (gh) tma_load_3d(to + T * kRowU, &map_g, bar, j0, (int)p.b, t);
-        }
+    Ring<DEPTH> ring;
+    int64_t box_left = a.L - (r_top + (int64_t)p.rank * steps);      // steps from the box's first to the end
+    auto ask = [&](int64_t n, uint32_t to, uint32_t bar) {
+        if (n > a.L) return;                        // in front of the start
+        if (n <= 0) { mbar_arrive(bar); return; }   // behind the end (first round only): the stage's turn passes empty
+        const int t = (int)(back ? n - steps : a.L - n), j0 = p.j - p.shift;
+        mbar_arrive_expect_tx(bar, gh ? stage_bytes : stage_bytes - steps * kRowG);
+        tma_load_3d(to, &map_u, bar, 2 * j0, (int)p.b, t);
+        if (gh) tma_load_3d(to + g_at, &map_g, bar, j0, (int)p.b, t);
+        tma_load_3d(to + s_at, &map_s, bar, j0, (int)p.b, (int)((a.L - n) / T));
     };
+    if constexpr (RING) {
+        const uint32_t base = smem_u32(shared) + (SPLIT ? (uint32_t)sizeof(Exchange<V>) : 0u);
+        ring.start(base + kBarBytes, base, stage_bytes, p.warps);
+        if (!SPLIT && p.warp >= p.warps) {
+            if (p.lane == 0 && p.warp == kSide) {
+                for (int64_t n = box_left, turn = 0; n <= a.L; n += round, ++turn) {
+                    if (turn >= DEPTH) ring.wait(ring.empty(), ring.phase ^ 1, a.err);
+                    if (ring.dead) break;
+                    ask(n, ring.at(), ring.full());
+                    ring.next();
+                }
+            }
+            return;
+        }
+        if (SPLIT && threadIdx.x == 0)
+            for (int s = 0; s < DEPTH; ++s) ask(box_left + s * round, ring.data + s * ring.bytes, ring.bars + 8 * s);
+    }
     Pack<TT, 2 * V> next_u[RING ? 1 : T];
     Pack<TT, V> next_g[RING ? 1 : T];
     Num<V> next_c = all<V>(0.0f);
@@ -564,11 +609,6 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
         }
         next_flags = load_flags<T>(mask, a.m_t, n, p.lane);
     };
-    if constexpr (RING) {
-        const uint32_t base = smem_u32(shared) + (SPLIT ? (uint32_t)sizeof(Exchange<V>) : 0u);
-        ring.start(base + kBarBytes + p.warp * DEPTH * kStage, base + p.warp * DEPTH * 8, kStage, p.lane);
-        for (int s = 0; s < DEPTH; ++s) ask(left + s * round, r_top >= s * round, ring.data + s * kStage, ring.bars + 8 * s);
-    }
     fetch(left);
     if (SPLIT) exchange_start(*x, p);
     int64_t turn = 0;
@@ -594,11 +634,13 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
             fetch(left + round);
         }
         if constexpr (RING) {
-            if (left > 0) ring.wait(a.err);
-            row = ring.at() + p.shift * 2 * sizeof(TT) + (back ? (T - 1) * kRowU : 0u);
+            ring.wait(ring.full(), ring.phase, a.err);
+            const int first = SPLIT ? p.warp * T : 0, cols = p.shift + (SPLIT ? 0 : p.warp * 32 * V);
+            const int at = back ? steps - 1 - first : first;
+            row = ring.at() + cols * 2 * sizeof(TT) + at * kRowU;
             row_step = back ? -(int32_t)kRowU : (int32_t)kRowU;
-            c = widened<float>(load_shared<Pack<float, V>>(ring.at() + T * (kRowU + kRowG) + p.shift * 4));
-            uint32_t grow = ring.at() + T * kRowU + p.shift * sizeof(TT) + (back ? (T - 1) * kRowG : 0u);
+            c = widened<float>(load_shared<Pack<float, V>>(ring.at() + s_at + (SPLIT ? p.warp : 0) * kRowS + cols * 4));
+            uint32_t grow = ring.at() + g_at + cols * sizeof(TT) + at * kRowG;
 #pragma unroll
             for (int i = 0; i < T; ++i, grow += row_step / 2) {
                 if (gh) g[i] = load_shared<Pack<TT, V>>(grow);
@@ -637,13 +679,16 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
         };
         if (flags == 0) recompute(std::true_type());
         else recompute(std::false_type());
-        if constexpr (RING) {
-            __syncwarp();
-            ask(left + DEPTH * round, r0 >= DEPTH * round, ring.at(), ring.bar());
-            ring.next();
-        }
         Num<V> dc = carry;
-        if constexpr (SPLIT) dc = exchange<V, true>(*x, turn, p, own, &carry, a.err);
+        if constexpr (SPLIT) {
+            dc = exchange<V, true>(*x, turn, p, own, &carry, a.err, [&]() {
+                if (RING && threadIdx.x == (p.warps - 1) * 32 && !ring.dead) ask(box_left + DEPTH * round, ring.at(), ring.full());
+            });
+        } else if constexpr (RING) {
+            ring.read(p.lane);
+        }
+        if (RING) ring.next();
+        box_left += round;
         auto finish = [&](auto clean) {
             constexpr bool CLEAN = decltype(clean)::value;
             TT *q = gu + 2 * (T - 1) * a.h_t;
@@ -713,7 +758,7 @@ void reverse_time(LinRecArgs *a, size_t size, int units) {
     a->u_t = -a->u_t; a->h_t = -a->h_t; a->gh_t = -a->gh_t; a->m_t = -a->m_t;
 }
 
-Slices choose_slices(int64_t L, int64_t B, int64_t d) {
+Slices choose_slices(int64_t L, int64_t B, int64_t d, int dtype, bool backward) {
     const int64_t columns = (d + 63) / 64 * B;              // warps that one walk over time takes
     int64_t want = option(OPT_LINREC_SLICES, 0);
     // One walk takes about 70 ns a step forward and 130 backward however few columns there are, which is what HBM needs
@@ -725,9 +770,12 @@ Slices choose_slices(int64_t L, int64_t B, int64_t d) {
         if (columns < 148 * 6)
             while (want < 64 && columns * want * 2 <= 148 * 14) want *= 2;
     }
-    want = std::min<int64_t>(std::min<int64_t>(want, 64), (L + kT - 1) / kT);
+    // two CTAs an SM: eight warps' float32 stages of the backward pass would leave room for one (4096 x 4 x 512 in 64 slices
+    // 75 us, in 56 of seven warps 49)
+    const int most = dtype == SRU_F32 && backward ? kMaxWarps - 1 : kMaxWarps;
+    want = std::min<int64_t>(std::min<int64_t>(want, most * kMaxRanks), (L + kT - 1) / kT);
     Slices s;
-    s.ranks = (int)((want + kMaxWarps - 1) / kMaxWarps);
+    s.ranks = (int)((want + most - 1) / most);
     s.warps = (int)((want + s.ranks - 1) / s.ranks);
     return s;
 }
@@ -754,33 +802,32 @@ template <typename TT, int V, bool SPLIT, bool RING>
 int launch(LinRecArgs a, const Slices &s, const Maps &maps, bool backward, cudaStream_t st) {
     // a slice's chunk is the same with and without a ring, and with it the order of all roundings: bits do not depend on layout
     constexpr int T = SPLIT || RING ? Cut<TT>::kFwdT : 2 * kT;
-    constexpr size_t kRow = 32 * V * 2 * sizeof(TT);
+    constexpr size_t kRow = (SPLIT ? 1 : kSide) * 32 * V * 2 * sizeof(TT);
     auto fwd = linear_recurrence_fwd_kernel<TT, V, T, SPLIT, RING>;
     auto bwd = linear_recurrence_bwd_kernel<TT, V, SPLIT, RING>;
     a.groups = (a.d + 32 * V - 1) / (32 * V);
     const int64_t columns = (int64_t)a.groups * a.B;
-    const int warps = SPLIT ? s.warps : 2;
-    const int64_t blocks = SPLIT ? columns * s.ranks : (columns + 1) / 2;
+    const int warps = SPLIT ? s.warps : kSide;
+    const int64_t blocks = SPLIT ? columns * s.ranks : RING ? (int64_t)((a.groups + kSide - 1) / kSide) * a.B : (columns + kSide - 1) / kSide;
     if (blocks > 0x7fffffff) return set_error(SRU_ERR_UNSUPPORTED, "linear recurrence: batch * hidden too large");
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.stream = st;
     cfg.gridDim = dim3((unsigned)blocks, 1, 1);
-    cfg.blockDim = dim3(32 * warps, 1, 1);
+    cfg.blockDim = dim3(32 * (warps + (RING && !SPLIT ? 1 : 0)), 1, 1);
     cfg.dynamicSmemBytes = SPLIT ? sizeof(Exchange<V>) : 0;
     if (RING) {
-        constexpr size_t f = ring_shared<V, Cut<TT>::kFwdDepth>(SPLIT ? kMaxWarps : 2, T * kRow, SPLIT);
-        constexpr size_t b = ring_shared<V, Cut<TT>::kBwdDepth>(SPLIT ? kMaxWarps : 2, kT * kRow * 3 / 2 + 32 * V * 4, SPLIT);
+        auto fwd_bytes = [&](int n) { return ring_shared<V>(n * T * kRow, Cut<TT>::kFwdDepth, SPLIT); };
+        auto bwd_bytes = [&](int n) { return ring_shared<V>(n * (kT * kRow * 3 / 2 + kRow / (2 * sizeof(TT)) * 4), Cut<TT>::kBwdDepth, SPLIT); };
         static bool attr_set[64] = {false};
         int dev = 0;
         SRUB_CUDA_CHECK(cudaGetDevice(&dev));
         if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-            SRUB_CUDA_CHECK(cudaFuncSetAttribute(fwd, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f));
-            SRUB_CUDA_CHECK(cudaFuncSetAttribute(bwd, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)b));
+            SRUB_CUDA_CHECK(cudaFuncSetAttribute(fwd, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)fwd_bytes(SPLIT ? kMaxWarps : 1)));
+            SRUB_CUDA_CHECK(cudaFuncSetAttribute(bwd, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bwd_bytes(SPLIT ? kMaxWarps : 1)));
             attr_set[dev] = true;
         }
-        cfg.dynamicSmemBytes = backward ? ring_shared<V, Cut<TT>::kBwdDepth>(warps, kT * kRow * 3 / 2 + 32 * V * 4, SPLIT)
-                                        : ring_shared<V, Cut<TT>::kFwdDepth>(warps, T * kRow, SPLIT);
+        cfg.dynamicSmemBytes = backward ? bwd_bytes(SPLIT ? warps : 1) : fwd_bytes(SPLIT ? warps : 1);
     }
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -806,20 +853,21 @@ bool ring_fits(const LinRecArgs &a, int64_t size, bool backward) {
 template <typename TT> int launch_typed(LinRecArgs a, const Slices &s, bool reverse, bool backward, cudaStream_t st) {
     Maps maps;
     memset(&maps, 0, sizeof(maps));
-    const bool ring = ring_fits(a, sizeof(TT), backward);
+    const bool ring = ring_fits(a, sizeof(TT), backward), split = s.count() > 1;
     if (ring) {
         if (int rc = ensure_context()) return rc;
         const bool one = a.B == 1;       // the stride of a single sequence is never taken
-        int rc = make_box<TT>(&maps.u, a.u, 2 * a.d, a.B, a.L, one ? a.u_t : a.u_b, a.u_t, 128, backward ? kT : Cut<TT>::kFwdT);
-        if (!rc && a.grad_h) rc = make_box<TT>(&maps.g, a.grad_h, a.d, a.B, a.L, one ? a.gh_t : a.gh_b, a.gh_t, 64, kT);
+        const int cols = split ? 64 : 64 * kSide, chunks = split ? s.warps : 1;
+        const int steps = chunks * (backward ? kT : Cut<TT>::kFwdT);
+        int rc = make_box<TT>(&maps.u, a.u, 2 * a.d, a.B, a.L, one ? a.u_t : a.u_b, a.u_t, 2 * cols, steps);
+        if (!rc && a.grad_h) rc = make_box<TT>(&maps.g, a.grad_h, a.d, a.B, a.L, one ? a.gh_t : a.gh_b, a.gh_t, cols, steps);
         if (!rc && backward)
-            rc = make_box<float>(&maps.s, a.states, a.d, a.B, (a.L + kT - 1) / kT, a.d, a.B * a.d, 64, 1);
+            rc = make_box<float>(&maps.s, a.states, a.d, a.B, (a.L + kT - 1) / kT, a.d, a.B * a.d, cols, chunks);
         if (rc) return rc;
     }
     a.err = device_error_flag();
     if (!a.err) return set_error(SRU_ERR_CUDA, "device error flag unavailable");
     if (reverse) reverse_time(&a, sizeof(TT), backward ? 2 : 1);
-    const bool split = s.count() > 1;
     if (ring) return split ? launch<TT, 2, true, true>(a, s, maps, backward, st) : launch<TT, 2, false, true>(a, s, maps, backward, st);
     return split ? launch<TT, 1, true, false>(a, s, maps, backward, st) : launch<TT, 1, false, false>(a, s, maps, backward, st);
 }
@@ -863,12 +911,12 @@ int sru_b200_linear_recurrence_forward(void *h, float *c_last, void *states, con
     a.L = length; a.B = batch; a.d = (int)hidden;
     a.u_t = u_stride_t; a.u_b = u_stride_b;
     a.h_t = batch * hidden; a.m_t = batch;
-    return dispatch(a, choose_slices(length, batch, hidden), dtype, reverse != 0, false, static_cast<cudaStream_t>(stream));
+    return dispatch(a, choose_slices(length, batch, hidden, dtype, false), dtype, reverse != 0, false, static_cast<cudaStream_t>(stream));
 }
 
-size_t sru_b200_linear_recurrence_backward_workspace_bytes(int64_t length, int64_t batch, int64_t hidden) {
+size_t sru_b200_linear_recurrence_backward_workspace_bytes(int64_t length, int64_t batch, int64_t hidden, int dtype) {
     if (length < 1 || batch < 1 || hidden < 1) return 0;
-    return (size_t)batch * choose_slices(length, batch, hidden).count() * (size_t)hidden * sizeof(float);
+    return (size_t)batch * choose_slices(length, batch, hidden, dtype, true).count() * (size_t)hidden * sizeof(float);
 }
 
 int sru_b200_linear_recurrence_backward(void *grad_u, float *grad_bias, float *grad_init, const void *u,
@@ -884,7 +932,7 @@ int sru_b200_linear_recurrence_backward(void *grad_u, float *grad_bias, float *g
     const size_t size = dtype_size(dtype);
     if ((reinterpret_cast<uintptr_t>(u) % (2 * size)) || u_stride_t % 2 || u_stride_b % 2)
         return set_error(SRU_ERR_BAD_ARG, "linear recurrence: the pairs of u must be aligned to their size");
-    const Slices s = choose_slices(length, batch, hidden);
+    const Slices s = choose_slices(length, batch, hidden, dtype, true);
     if (grad_bias) {
         const size_t need = (size_t)batch * s.count() * (size_t)hidden * sizeof(float);
         if (!workspace || workspace_bytes < need)

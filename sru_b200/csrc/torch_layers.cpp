@@ -121,7 +121,7 @@ class GatedLinearRecurrence : public torch::autograd::Function<GatedLinearRecurr
             if (gi.defined()) gl.defined() ? gi.copy_(gl) : gi.zero_();
         } else {
             if (grads[0].defined()) gh = rows((single ? grads[0].detach().unsqueeze(0) : grads[0].detach()).to(u.scalar_type()), 1);
-            const size_t bytes = gb.defined() ? sru_b200_linear_recurrence_backward_workspace_bytes(L, B, d) : 0;
+            const size_t bytes = gb.defined() ? sru_b200_linear_recurrence_backward_workspace_bytes(L, B, d, code_of(u.scalar_type())) : 0;
             Tensor ws;
             if (bytes) ws = at::empty({(int64_t)bytes}, u.options().dtype(at::kByte));
             check(sru_b200_linear_recurrence_backward(

@@ -85,7 +85,7 @@ class _GatedLinearRecurrence(Function):
             gh = None if grad_h is None else _rows(grad_h.to(u.dtype), 1)
             L = _lib.lib()
             with torch.cuda.device(dev):
-                nbytes = int(L.sru_b200_linear_recurrence_backward_workspace_bytes(length, batch, d)) if need_bias else 0
+                nbytes = int(L.sru_b200_linear_recurrence_backward_workspace_bytes(length, batch, d, _lib.DTYPE_CODE[u.dtype])) if need_bias else 0
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
                 _lib.call("linear_recurrence_bwd", 2 if need_bias else 1, L.sru_b200_linear_recurrence_backward,
                           _lib.ptr(grad_u), _lib.ptr(grad_bias), _lib.ptr(grad_first), _lib.ptr(u), _lib.ptr(bias),

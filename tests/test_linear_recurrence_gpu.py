@@ -280,7 +280,7 @@ def test_no_write_outside_the_outputs():
             es = u.element_size()
             sizes = {"h": L * B * d * es, "last": B * d * 4, "states": int(L_.sru_b200_linear_recurrence_states_bytes(L, B, d)),
                      "gu": L * B * 2 * d * es, "gb": d * 4, "gi": B * d * 4,
-                     "ws": int(L_.sru_b200_linear_recurrence_backward_workspace_bytes(L, B, d))}
+                     "ws": int(L_.sru_b200_linear_recurrence_backward_workspace_bytes(L, B, d, _lib.DTYPE_CODE[dtype]))}
             bufs = {k: torch.full((n + 512,), 0xA5, dtype=torch.uint8, device=DEV) for k, n in sizes.items()}
             at = {k: t.data_ptr() + 256 for k, t in bufs.items()}
             st = torch.cuda.current_stream().cuda_stream
