@@ -319,6 +319,7 @@ template <typename T, int N> __device__ __forceinline__ void load_line(float (&v
 // a line along the contiguous direction, one warp each, in a fixed order.
 template <typename T> __global__ void __launch_bounds__(256) ns_norm_kernel(const NsEdge e) {
     __shared__ double s[8];
+    early_next_kernel();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const T *g = static_cast<const T *>(e.src) + blockIdx.y * e.s_b;
     const int64_t per = (e.len + 2047) / 2048, units = e.lines * per;
@@ -348,6 +349,8 @@ template <typename T> __global__ void __launch_bounds__(256) ns_norm_kernel(cons
 
 // 1 / (|G|_F + eps) from the partial sums, by every block for itself.
 __device__ __forceinline__ float ns_scale(const NsEdge &e, int64_t z, float *shared) {
+    early_next_kernel();
+    previous_kernel_done();
     if (threadIdx.x < 32) {
         double sum = 0.0;
         for (int p = threadIdx.x; p < e.parts; p += 32) sum += e.part[z * e.parts + p];
@@ -490,14 +493,19 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
     // the norm, in 64 bits and a fixed order
     double sum[2] = {0.0, 0.0};
     {
-        const int64_t groups = (e.len + 7) / 8, units = e.lines * groups;
-#pragma unroll 4
-        for (int64_t u = threadIdx.x; u < units; u += kSmallThreads) {
-            const int64_t l = u / groups, k = (u - l * groups) * 8;
-            float v[8];
-            load_line<T, 8>(v, g + l * e.pitch, k, e.len, e.wide);
+        constexpr int G = 4;            // groups of 8 elements requested together
+        const int groups = (int)((e.len + 7) / 8), units = (int)e.lines * groups;
+        for (int u0 = threadIdx.x; u0 < units; u0 += G * kSmallThreads) {
+            float v[G][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i & 1] = fma((double)v[i], (double)v[i], sum[i & 1]);
+            for (int k = 0; k < G; ++k) {
+                const int u = u0 + k * kSmallThreads, l = e.lines == 1 ? 0 : u / groups;
+                load_line<T, 8>(v[k], g + l * e.pitch, (int64_t)(u - l * groups) * 8, u < units ? e.len : 0, e.wide && u < units);
+            }
+#pragma unroll
+            for (int k = 0; k < G; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[i & 1] = fma((double)v[k][i], (double)v[k][i], sum[i & 1]);
         }
     }
     double t = sum[0] + sum[1];
@@ -512,14 +520,22 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
     for (int w = 0; w < kSmallThreads / 32; ++w) t += sums[w];
     const float scale = (float)(1.0 / (sqrt(t) + e.eps));
     if (e.s_j == 1) {
-#pragma unroll 2
-        for (int u = threadIdx.x; u < kSmallM * tiles * 8; u += kSmallThreads) {
-            const int i = u / (tiles * 8), j = (u - i * tiles * 8) * 8;
-            float v[8];
-            load_line<T, 8>(v, g + i * e.s_i, j, i < e.m ? e.n : 0, e.wide);
+        constexpr int G = 4;
+        for (int u0 = threadIdx.x; u0 < kSmallM * tiles * 8; u0 += G * kSmallThreads) {      // a multiple of 2 * threads
+            float v[G][8];
+            int at[G];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] *= scale;
-            store_halves(x + tile_at(i, j), v);
+            for (int k = 0; k < G; ++k) {
+                const int u = u0 + k * kSmallThreads, i = u / (tiles * 8), j = (u - i * tiles * 8) * 8;
+                at[k] = i < kSmallM ? (int)tile_at(i, j) : -1;
+                load_line<T, 8>(v[k], g + i * e.s_i, j, i < e.m ? e.n : 0, e.wide && i < e.m);
+            }
+#pragma unroll
+            for (int k = 0; k < G; ++k) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[k][i] *= scale;
+                if (at[k] >= 0) store_halves(x + at[k], v[k]);
+            }
         }
     } else {
 #pragma unroll 4
@@ -750,6 +766,16 @@ int ns_product(const NsMaps &a, const NsMaps &b, const NsMaps &out, const NsMaps
     return 0;
 }
 
+int launch_early(dim3 grid, void (*kernel)(NsEdge), const NsEdge &e, cudaStream_t st) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cudaLaunchAttribute early = early_launch();
+    cfg.gridDim = grid; cfg.blockDim = dim3(256); cfg.stream = st;
+    cfg.attrs = &early; cfg.numAttrs = 1;
+    SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, e));
+    return 0;
+}
+
 template <typename T, typename TO> int ns_small(const NsSmall &a, int64_t batch, cudaStream_t st) {
     auto kernel = ns_small_kernel<T, TO>;
     const int bytes = (2 + (a.e.n + 63) / 64) * kTileBytes + 1024;
@@ -834,21 +860,19 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         auto go_out = [&](auto t) { return out_dtype == SRU_F16 ? go(t, __half()) : go(t, __nv_bfloat16()); };
         return grad_dtype == SRU_F32 ? go_out(float()) : grad_dtype == SRU_F16 ? go_out(__half()) : go_out(__nv_bfloat16());
     }
-    auto begin = [&](auto t) {
+    auto begin = [&](auto t) -> int {
         using T = decltype(t);
         ns_norm_kernel<T><<<norm_grid, 256, 0, st>>>(e);
+        SRUB_CUDA_CHECK(cudaGetLastError());
         if (turned) {
             const dim3 grid((unsigned)((p.ldx + 63) / 64), (unsigned)((p.m + 63) / 64), (unsigned)batch);
-            ns_first_turned_kernel<T><<<grid, 256, 0, st>>>(e);
+            return launch_early(grid, ns_first_turned_kernel<T>, e, st);
         } else {
             const dim3 grid((unsigned)std::min<int64_t>((p.m * p.ldx / 8 + 255) / 256, 148 * 8), (unsigned)batch);
-            ns_first_rows_kernel<T><<<grid, 256, 0, st>>>(e);
+            return launch_early(grid, ns_first_rows_kernel<T>, e, st);
         }
     };
-    if (grad_dtype == SRU_F32) begin(float());
-    else if (grad_dtype == SRU_F16) begin(__half());
-    else begin(__nv_bfloat16());
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    if (int rc = grad_dtype == SRU_F32 ? begin(float()) : grad_dtype == SRU_F16 ? begin(__half()) : begin(__nv_bfloat16())) return rc;
 
     // The last product writes the caller's matrix itself where its rows are 16-byte aligned.
     const bool direct = steps > 0 && cols % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;

@@ -9,6 +9,8 @@
 #include <torch/library.h>
 #include <torch/types.h>
 
+#include <algorithm>
+
 #include "../../include/sru_b200.h"
 
 namespace {
@@ -229,9 +231,32 @@ Tensor embedding_lookup(const Tensor &tokens, const Tensor &weight, double scale
     return y.view(shape);
 }
 
+// ---- orthogonalised update -------------------------------------------------------------------------------------------
+Tensor orthogonalize(const Tensor &grad, int64_t steps, double a, double b, double c, double eps, c10::optional<at::ScalarType> out_type) {
+    TORCH_CHECK(grad.is_cuda(), "sru_b200 has no CPU path: grad must be a CUDA tensor");
+    TORCH_CHECK(grad.dim() == 2 || grad.dim() == 3, "grad must be (rows, cols) or (batch, rows, cols), got ", grad.sizes());
+    const at::ScalarType type = grad.scalar_type(), out_dtype = out_type.value_or(type == at::kFloat ? at::kBFloat16 : type);
+    const int code = code_of(type);
+    TORCH_CHECK(out_dtype == at::kHalf || out_dtype == at::kBFloat16, "the result is float16 or bfloat16, got ", out_dtype);
+    c10::cuda::CUDAGuard guard(grad.device());
+    Tensor out = at::empty(grad.sizes(), grad.options().dtype(out_dtype));
+    Tensor g = grad.detach();
+    if (g.numel() > 0 && g.stride(-1) != 1 && g.stride(-2) != 1) g = g.contiguous();
+    const int64_t batch = g.dim() == 3 ? g.size(0) : 1, rows = g.size(-2), cols = g.size(-1);
+    const size_t bytes = sru_b200_orthogonalize_workspace_bytes(batch, rows, cols);
+    Tensor ws = at::empty({(int64_t)bytes}, g.options().dtype(at::kByte));
+    check(sru_b200_orthogonalize(out.data_ptr(), g.data_ptr(), batch, rows, cols, g.dim() == 3 ? g.stride(0) : 0, g.stride(-2),
+                                 g.stride(-1), (int)std::min<int64_t>(std::max<int64_t>(steps, -1), 1 << 30), a, b, c, eps, code,
+                                 code_of(out_dtype), ws.data_ptr(), bytes, at::cuda::getCurrentCUDAStream().stream()));
+    return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(sru_b200, m) {
+    m.def("orthogonalize(Tensor grad, int steps=5, float a=3.4445, float b=-4.7750, float c=2.0315, float eps=1e-7, "
+          "ScalarType? out_dtype=None) -> Tensor",
+          &orthogonalize);
     m.def("gated_linear_recurrence(Tensor u, Tensor? c0=None, Tensor? bias=None, Tensor? mask_pad=None, bool reverse=False) "
           "-> (Tensor, Tensor)",
           &gated_linear_recurrence);

@@ -91,12 +91,14 @@ def test_orthogonalize_c_arguments():
 @pytest.mark.parametrize("timed", [False, True])
 def test_refusals_come_as_the_packages_error(timed, monkeypatch):
     """Through the native operator and through the Python form that a timer sees alike."""
-    from sru_b200 import embedding_lookup, gated_linear_recurrence
+    from sru_b200 import embedding_lookup, gated_linear_recurrence, orthogonalize
     monkeypatch.setattr(_lib, "timer", object() if timed else None)
     with pytest.raises(_lib.SruB200Error, match="no CPU path"):
         gated_linear_recurrence(torch.zeros(2, 1, 8))
     with pytest.raises(_lib.SruB200Error, match="no CPU path"):
         embedding_lookup(torch.zeros(3, dtype=torch.long), torch.zeros(5, 8))
+    with pytest.raises(_lib.SruB200Error, match="no CPU path"):
+        orthogonalize(torch.zeros(3, 4))
     assert isinstance(_lib.refused(RuntimeError("x")), _lib.SruB200Error)
     oom = torch.OutOfMemoryError("x")
     assert _lib.refused(oom) is oom

@@ -46,6 +46,7 @@ def test_native_and_python_forms_give_the_same_bits(timed):
 
 @pytest.mark.parametrize("python", [False, True])
 def test_differentiable_once(python, timed):
+    """A second derivative is an error, not a wrong number; the orthogonalised update has no derivative at all."""
     if python:
         timed()
     u = torch.randn(9, 2, 8, device=DEV, requires_grad=True)
@@ -58,6 +59,7 @@ def test_differentiable_once(python, timed):
     (grad,) = torch.autograd.grad(y.square().sum(), w, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once|once_differentiable"):
         grad.sum().backward()
+    assert not orthogonalize(w).requires_grad and not orthogonalize(w.square()).requires_grad
 
 
 @pytest.mark.parametrize("python", [False, True])
