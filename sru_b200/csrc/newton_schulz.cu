@@ -13,7 +13,9 @@
 // the start and about 1.2 later, |M| below 10), so fp16's eleven bits are worth more than bf16's range: on
 // gradients with a decaying spectrum the result is 1.2e-3 off the exact steps against 1.0e-2 with bf16 iterates.
 //
-// The products run on pairs of SMs (cta_group::2, 256 x BN tiles) in a persistent grid over (matrix, tile).
+// The products run on pairs of SMs (cta_group::2, 256 x BN tiles) in a persistent grid over (matrix, tile).  A product costs
+// about 6 us beside its multiplications (load latency 1.1, accumulator to memory 2.5, teardown 0.6, next kernel 1.1), which is
+// most of the time up to 1024 x 1024; from there on shared memory and L2 feed the tensor cores at 60 to 75 % of their rate.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -57,27 +59,28 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t sr
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
                  ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z) : "memory");
 }
-// Unit -> matrix and tile.  A symmetric product keeps, of 256-row block i, the 128-column tiles from 2 i on.
-__device__ __forceinline__ void ns_unit(const NsArgs &g, int unit, int *z, int *mb, int *nb) {
+// Unit -> matrix and tile.  A symmetric product keeps, of 256-row block i, the tiles from column 256 i on.
+template <int BN> __device__ __forceinline__ void ns_unit(const NsArgs &g, int unit, int *z, int *mb, int *nb) {
     *z = unit / g.per_matrix;
     int t = unit - *z * g.per_matrix;
     if (g.symmetric) {
         int i = 0, left = g.tiles_n;
-        while (t >= left) { t -= left; left -= 2; ++i; }
+        while (t >= left) { t -= left; left -= 256 / BN; ++i; }
         *mb = i;
-        *nb = 2 * i + t;
+        *nb = 256 / BN * i + t;
     } else {
         *mb = t / g.tiles_n;
         *nb = t - *mb * g.tiles_n;
     }
 }
 
-template <int BN> struct NsShape {
+// TURN: the product may be symmetric.
+template <int BN, bool TURN> struct NsShape {
     static constexpr int kBBytes = BN / 2 * kBK * 2;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kStages = BN == 128 ? 6 : 5;
     static constexpr int kOut = 32 * BN * 2;                    // an epilogue warp's 32 rows, boxes of 64 columns
-    static constexpr int kTurned = BN == 128 ? 128 * 32 * 2 : 0;    // the same transposed, for the mirrored tile
+    static constexpr int kTurned = TURN ? BN * 32 * 2 : 0;      // the same transposed, for the mirrored tile
+    static constexpr int kStages = BN == 128 ? 6 : TURN ? 3 : 5;
     static constexpr int kBars = 1024;
     static constexpr int kSmem = kStages * kStageBytes + 4 * (kOut + kTurned) + 1024 + kBars;
     static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -96,7 +99,8 @@ __global__ void __launch_bounds__(kNsThreads, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_t,
                   const __grid_constant__ CUtensorMap map_d, const NsArgs g) {
-    using S = NsShape<BN>;
+    constexpr bool TURN = !AMN && !BMN;
+    using S = NsShape<BN, TURN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *staging = smem + S::kStages * S::kStageBytes;
@@ -139,7 +143,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             bool ok = true;
             for (int unit = pair; unit < nunits && ok; unit += npairs) {
                 int z, mb, nb;
-                ns_unit(g, unit, &z, &mb, &nb);
+                ns_unit<BN>(g, unit, &z, &mb, &nb);
                 const int m0 = mb * 256 + (int)rank * 128, n0 = nb * BN + (int)rank * (BN / 2);
                 for (int kb = 0; kb < nkb; ++kb) {
                     if (!mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1)) { atomicExch(g.err, 31); ok = false; break; }
@@ -196,10 +200,10 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         int it = 0;
         for (int unit = pair; unit < nunits; unit += npairs, ++it) {
             int z, mb, nb;
-            ns_unit(g, unit, &z, &mb, &nb);
+            ns_unit<BN>(g, unit, &z, &mb, &nb);
             const int acc = it & 1;
             const int row0 = mb * 256 + (int)rank * 128 + q * 32, row = row0 + lane;
-            const bool mirror = BN == 128 && g.symmetric && 2 * mb < (nb & ~1);   // the transposed tile is computed by nobody
+            const bool mirror = TURN && g.symmetric && mb < nb / (256 / BN);   // the transposed tile is computed by nobody
             if (lane == 0) {
                 bulk_wait_read_all();           // the stores of the tile before have left the staging
                 if (MODE == kCombine) {
@@ -252,7 +256,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                         }
                     }
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-                    if (BN == 128 && mirror) {
+                    if (TURN && mirror) {
                         // element (row, col) at [col][row]: the 32 lanes of a store fill 64 contiguous bytes
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
@@ -271,7 +275,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 #pragma unroll
                     for (int b = 0; b < BN / 64; ++b)
                         if (nb * BN + b * 64 < g.N) tma_store_3d(&map_c, out + b * 4096, nb * BN + b * 64, row0, z);
-                    if (BN == 128 && mirror) tma_store_3d(&map_t, turned, row0, nb * BN, z);
+                    if (TURN && mirror) tma_store_3d(&map_t, turned, row0, nb * BN, z);
                 }
                 bulk_commit();
             }
@@ -724,12 +728,13 @@ int ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t rows, int6
 }
 
 // One matrix (or batch) as the products see it: first operand, second operand, output and its mirror image.
-struct NsMaps { CUtensorMap a, b, c, t; };
+struct NsMaps { CUtensorMap a, b, c, t, wide_t; };
 int ns_maps(NsMaps *m, const void *base, int64_t inner, int64_t rows, int64_t batch, int64_t ld) {
     int rc = ns_map(&m->a, base, inner, rows, batch, ld, 128);
     if (!rc) rc = ns_map(&m->b, base, inner, rows, batch, ld, 64);
     if (!rc) rc = ns_map(&m->c, base, inner, rows, batch, ld, 32);
     if (!rc) rc = ns_map(&m->t, base, inner, rows, batch, ld, 128, 32);
+    if (!rc) rc = ns_map(&m->wide_t, base, inner, rows, batch, ld, 256, 32);
     return rc;
 }
 
@@ -740,13 +745,13 @@ int ns_product(const NsMaps &a, const NsMaps &b, const NsMaps &out, const NsMaps
     int dev = 0;
     SRUB_CUDA_CHECK(cudaGetDevice(&dev));
     if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-        SRUB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NsShape<BN>::kSmem));
+        SRUB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NsShape<BN, !AMN && !BMN>::kSmem));
         attr_set[dev] = true;
     }
     g.tiles_m = (g.M + 255) / 256;
     g.tiles_n = (g.N + BN - 1) / BN;
     int64_t per = 0;
-    if (g.symmetric) for (int i = 0; i < g.tiles_m; ++i) per += g.tiles_n - 2 * i;
+    if (g.symmetric) for (int i = 0; i < g.tiles_m; ++i) per += g.tiles_n - 256 / BN * i;
     else per = (int64_t)g.tiles_m * g.tiles_n;
     if (per * g.batch > 0x7fffffff) return set_error(SRU_ERR_UNSUPPORTED, "orthogonalize: too many tiles");
     g.per_matrix = (int)per;
@@ -754,7 +759,7 @@ int ns_product(const NsMaps &a, const NsMaps &b, const NsMaps &out, const NsMaps
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(2u * (unsigned)std::min<int64_t>(per * g.batch, sms / 2), 1, 1);
     cfg.blockDim = dim3(kNsThreads, 1, 1);
-    cfg.dynamicSmemBytes = NsShape<BN>::kSmem;
+    cfg.dynamicSmemBytes = NsShape<BN, !AMN && !BMN>::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -762,8 +767,18 @@ int ns_product(const NsMaps &a, const NsMaps &b, const NsMaps &out, const NsMaps
     attr[1] = early_launch();
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, AMN ? a.b : a.a, b.b, out.c, out.t, d.c, g));
+    SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, AMN ? a.b : a.a, BN == 256 && !BMN ? b.a : b.b, out.c, BN == 256 ? out.wide_t : out.t, d.c, g));
     return 0;
+}
+
+// X X^T and A A.  A 256 x 128 tile takes a pair of SMs about as long as one of 256 x 256 (0.28 us per 64 of the reduction: its
+// operands keep shared memory just as busy), but has the shorter epilogue and room for twice the stages.  It is taken where
+// the tiles all find a pair of their own, and for small matrices.  Five steps with 128 / 256 columns: 4096 x 4096 1276 / 1112
+// us, four 2048 x 2048 761 / 720, six 1024 x 2048 374 / 328, but twelve 700 x 1400 327 / 348.
+template <int MODE> int ns_gram(const NsMaps &a, const NsMaps &out, const NsMaps &d, const NsArgs &g, int sms, cudaStream_t st) {
+    const int64_t rows = (g.M + 255) / 256, narrow = rows * ((g.M + 127) / 128) - rows * (rows - 1);
+    if (narrow * g.batch <= sms / 2 || g.M < 1024) return ns_product<128, false, false, MODE>(a, a, out, d, g, sms, st);
+    return ns_product<256, false, false, MODE>(a, a, out, d, g, sms, st);
 }
 
 int launch_early(dim3 grid, void (*kernel)(NsEdge), const NsEdge &e, cudaStream_t st) {
@@ -892,9 +907,9 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         g.batch = (int)batch; g.err = err;
         g.M = (int)p.m; g.N = (int)p.m; g.K = (int)p.n; g.symmetric = 1;
         g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc;
-        if (int rc = ns_product<128, false, false, kPlain>(xm[cur], xm[cur], am, am, g, sms, st)) return rc;
+        if (int rc = ns_gram<kPlain>(xm[cur], am, am, g, sms, st)) return rc;
         g.K = (int)p.m;
-        if (int rc = ns_product<128, false, false, kCombine>(am, am, mm, am, g, sms, st)) return rc;
+        if (int rc = ns_gram<kCombine>(am, mm, am, g, sms, st)) return rc;
         g.N = (int)p.n; g.symmetric = 0;
         const bool last = s == steps - 1 && direct;
         g.bf16 = last && out_dtype == SRU_BF16;

@@ -83,6 +83,19 @@ def test_where_one_cta_takes_the_matrix(rows, cols):
     check(gradient(4, rows, cols, F16, rows + cols), BF16)
 
 
+@pytest.mark.parametrize("batch,rows,cols", [(6, 1024, 1030), (3, 1500, 1100), (7, 1040, 1024)])
+def test_both_tile_widths(batch, rows, cols):
+    """More tiles than pairs of SMs: the symmetric products run on 256-column tiles."""
+    g = gradient(batch, rows, cols, BF16, 2).to(DEV)
+    many, few = orthogonalize(g), orthogonalize(g[:1])
+    # one matrix alone takes the narrow tiles: the same sums in the same order
+    assert float((many[:1].float() - few.float()).norm()) <= 2.0 ** -9 * float(few.float().norm())
+    one = g[batch - 1].cpu()
+    err, want = many[batch - 1].cpu().double(), steps64(one, 5, False)
+    model = steps64(one, 5, True)
+    assert float((err - want).norm()) <= 1.5 * float((model - want).norm()) + (2.0 ** -8 + 1e-4) * float(want.norm())
+
+
 def test_singular_values_gather_around_one():
     g = torch.Generator().manual_seed(9)
     got = orthogonalize(torch.randn(300, 900, generator=g).to(DEV)).double().cpu()
