@@ -84,6 +84,15 @@ def test_many_tokens():
     check(tokens, 20000, 24, F32, F32)
 
 
+def test_large_vocabulary_and_long_runs():
+    """Keys of three radix digits, rows far apart; 200000 positions, half of them one token (thousands of tiles in a run)."""
+    g = torch.Generator().manual_seed(6)
+    check(torch.randint(0, 17_000_000, (500,), generator=g), 17_000_000, 2, F16, F16)
+    tokens = torch.randint(0, 3000, (200_000,), generator=g)
+    tokens[torch.rand(200_000, generator=g) < 0.5] = 1234
+    check(tokens, 3000, 12, F32, F32)
+
+
 def test_all_padding_and_empty():
     check(torch.full((40,), 3), 9, 16, F32, F32, padding=3)
     check(torch.zeros(0, dtype=torch.long), 9, 16, F32, F32)

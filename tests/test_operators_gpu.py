@@ -1,8 +1,12 @@
 """The operators around the recurrent layers together: a training step through all of them against 64 bits, their native
 and their Python form, refusals of what the documentation does not allow, two calls at once."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
+from conftest import ROOT
 from sru_b200 import _lib, embedding_lookup, gated_linear_recurrence, orthogonalize
 from sru_b200.projection import project
 
@@ -160,6 +164,31 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for a, b in zip(alone, together):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+FIRST_CALL_CAPTURED = """
+import torch
+from sru_b200 import _lib, embedding_lookup, gated_linear_recurrence, orthogonalize
+_lib.load_torch_ops()
+u = torch.randn(300, 2, 64, device="cuda").bfloat16()
+w, t, m = torch.randn(50, 32, device="cuda"), torch.randint(0, 50, (200,), device="cuda"), torch.randn(200, 300, device="cuda")
+small = torch.randn(20, 30, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = [*gated_linear_recurrence(u), embedding_lookup(t, w), orthogonalize(m), orthogonalize(small)]
+graph.replay()
+torch.cuda.synchronize()
+want = [*gated_linear_recurrence(u), embedding_lookup(t, w), orthogonalize(m), orthogonalize(small)]
+assert all(torch.equal(a, b) for a, b in zip(out, want))
+_lib.check_device_error()
+print("same")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_a_captured_one():
+    run = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "same" in run.stdout, run.stderr[-2000:]
 
 
 def test_capture_while_an_eager_graph_lives():

@@ -118,6 +118,23 @@ def test_coefficients():
     assert float((got - want).norm()) <= 1.5 * float((model - want).norm()) + 2.0 ** -10 * float(want.norm())
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 2000), (2000, 1), (3, 900), (900, 5), (7, 4099), (1100, 16)])
+def test_long_and_thin(rows, cols):
+    check(gradient(1, rows, cols, F32, rows + 3 * cols)[0])
+    check(gradient(2, rows, cols, F16, rows + 5 * cols))
+
+
+def test_many_small_matrices():
+    """More matrices than SMs, in one SM's shared memory and beyond."""
+    g = gradient(400, 20, 28, BF16, 7)
+    got = check(g)
+    dev = g.to(DEV)
+    assert torch.equal(orthogonalize(dev[399]).cpu().double(), got[399])
+    g = gradient(150, 140, 20, F32, 8)
+    got = orthogonalize(g.to(DEV))
+    assert torch.equal(orthogonalize(g[149].to(DEV)), got[149])
+
+
 def test_layouts():
     """Transposed views, slices, batches apart, and strides that have to be copied."""
     g = gradient(3, 65, 140, F32, 2)
