@@ -761,13 +761,15 @@ void reverse_time(LinRecArgs *a, size_t size, int units) {
 Slices choose_slices(int64_t L, int64_t B, int64_t d, int dtype, bool backward) {
     const int64_t columns = (d + 63) / 64 * B;              // warps that one walk over time takes
     int64_t want = option(OPT_LINREC_SLICES, 0);
-    // One walk takes about 70 ns a step forward and 130 backward however few columns there are, which is what HBM needs
-    // for some 75 000 columns: with 1024 warps of columns (512 x 32 x 2048) one walk takes 36 / 67 us and two slices
-    // 47 / 88.  With fewer, slices fill the GPU with 14 warps an SM, all it holds at their register count: 384 warps
-    // (1000 x 24 x 1024) 49 / 107 us in one walk, 34 / 62 in four slices; 32 warps (65536 x 2048) 2670 us and 282 in 64.
+    // One walk takes about 70 ns a step forward and 120 backward however few columns there are, which is what HBM needs
+    // for some 70 000 columns: with 1024 warps of columns (512 x 32 x 2048) one walk takes 37 / 63 us, four slices 44 / 68.
+    // With fewer, slices fill the GPU with up to 14 warps an SM, all it holds at their register count, and four at least:
+    // 640 warps (2048 x 40 x 1024) 110 / 216 us in two slices, 99 / 193 in four; 384 (4096 x 24 x 1024) 112 / 219 in four, 121 /
+    // 226 in eight; 256 (8192 x 16 x 1024) 166 / 341 in four, 148 / 281 in eight, 181 / 344 in sixteen; 32 (65536 x 2048) 2410 in
+    // one walk and 193 in 64.
     if (want <= 0) {
-        want = 1;
-        if (columns < 148 * 6)
+        want = columns < 148 * 6 ? 4 : 1;
+        if (want > 1)
             while (want < 64 && columns * want * 2 <= 148 * 14) want *= 2;
     }
     // two CTAs an SM: eight warps' float32 stages of the backward pass would leave room for one (4096 x 4 x 512 in 64 slices
