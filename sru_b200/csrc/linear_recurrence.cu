@@ -151,13 +151,17 @@ __device__ __forceinline__ void load_steps(Pack<TT, N> (&r)[T], const TT *p, int
     }
 }
 
-// Bit i: step i of the chunk is padded or lies behind the end.  The whole warp works on one sequence, so the flags are
-// uniform; lane i fetches step i's byte.  0 is the common case, and takes the paths without selects.
-template <int T> __device__ __forceinline__ unsigned load_flags(const uint8_t *mask, int64_t stride, int64_t n, int lane) {
+// Padding of a chunk.  The whole warp works on one sequence, so the flags are uniform; lane i fetches step i's byte one
+// round ahead, and the flags are formed when the round begins (formed at once, they would wait for the bytes: 34 -> 43 us for
+// 1000 x 24 x 1024).  Bit i: step i is padded or lies behind the end.  0 is the common case, and takes the paths without
+// selects.
+template <int T> __device__ __forceinline__ uint8_t load_pad(const uint8_t *mask, int64_t stride, int64_t n, int lane) {
+    if (mask && lane < T && lane < n) return mask[lane * stride];
+    return lane < T && lane >= n;
+}
+template <int T> __device__ __forceinline__ unsigned pad_flags(const uint8_t *mask, uint8_t pad, int64_t n) {
     if (!mask) return n >= T ? 0u : (n <= 0 ? 0xffffffffu : 0xffffffffu << n) & (uint32_t)((1ull << T) - 1);
-    bool pad = lane < T && lane >= n;
-    if (lane < T && lane < n) pad = mask[lane * stride] != 0;
-    return __ballot_sync(0xffffffffu, pad);
+    return __ballot_sync(0xffffffffu, pad != 0);
 }
 
 // Where a warp stands: its sequence and columns, and which of the interleaved slices of time it works on.  Slices are the
@@ -453,17 +457,18 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
         if (SPLIT && threadIdx.x == 0)
             for (int s = 0; s < DEPTH; ++s) ask(box_left - s * round, ring.data + s * ring.bytes, ring.bars + 8 * s);
     }
+    constexpr unsigned kAll = (unsigned)((1ull << T) - 1);
     Pack<TT, 2 * V> next[RING ? 1 : T];
-    unsigned next_flags;
+    uint8_t next_pad;
     if constexpr (!RING) load_steps<TT, 2 * V, T>(next, u, a.u_t, left);
-    next_flags = load_flags<T>(mask, a.m_t, left, p.lane);
+    next_pad = load_pad<T>(mask, a.m_t, left, p.lane);
     if (SPLIT) exchange_start(*x, p);
     int64_t turn = 0;
     for (int64_t r0 = 0; r0 < a.L; r0 += round, ++turn, left -= round) {
-        const unsigned flags = next_flags;
+        const unsigned flags = pad_flags<T>(mask, next_pad, left);
         if (r0 + round < a.L) {
             if (mask) mask += round * a.m_t;
-            next_flags = load_flags<T>(mask, a.m_t, left - round, p.lane);
+            next_pad = load_pad<T>(mask, a.m_t, left - round, p.lane);
         }
         Pack<TT, 2 * V> cur[RING ? 1 : T];
         uint32_t row = 0;
@@ -490,8 +495,14 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
         };
         if constexpr (SPLIT) {
             Num<V> C[T], P[T];
-            if (flags == 0) scan_local<TT, V, T, true>(in, nb, flags, C, P);
-            else scan_local<TT, V, T, false>(in, nb, flags, C, P);
+            if (flags == 0) {
+                scan_local<TT, V, T, true>(in, nb, flags, C, P);
+            } else if (flags == kAll) {             // nothing but padding
+#pragma unroll
+                for (int i = 0; i < T; ++i) { C[i] = all<V>(0.0f); P[i] = all<V>(1.0f); }
+            } else {
+                scan_local<TT, V, T, false>(in, nb, flags, C, P);
+            }
             const Num<V> c = exchange<V, false>(*x, turn, p, Map<V>{P[T - 1], C[T - 1]}, &carry, a.err, refill);
             if (states) {
 #pragma unroll
@@ -596,10 +607,11 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
         if (SPLIT && threadIdx.x == 0)
             for (int s = 0; s < DEPTH; ++s) ask(box_left + s * round, ring.data + s * ring.bytes, ring.bars + 8 * s);
     }
+    constexpr unsigned kAll = (1u << T) - 1u;
     Pack<TT, 2 * V> next_u[RING ? 1 : T];
     Pack<TT, V> next_g[RING ? 1 : T];
     Num<V> next_c = all<V>(0.0f);
-    unsigned next_flags;
+    uint8_t next_pad;
     auto fetch = [&](int64_t n) {
         if constexpr (!RING) {
             if (n > 0) next_c = load_state<V>(states);
@@ -607,13 +619,13 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
             if (gh) load_steps<TT, V, T>(next_g, gh, a.gh_t, n);
             else memset(&next_g, 0, sizeof(next_g));
         }
-        next_flags = load_flags<T>(mask, a.m_t, n, p.lane);
+        next_pad = load_pad<T>(mask, a.m_t, n, p.lane);
     };
     fetch(left);
     if (SPLIT) exchange_start(*x, p);
     int64_t turn = 0;
     for (int64_t r0 = r_top; r0 >= 0; r0 -= round, ++turn, left += round) {
-        const unsigned flags = next_flags;
+        const unsigned flags = pad_flags<T>(mask, next_pad, left);
         Num<V> c = next_c;
         Num<V> f[T], keep[T], w[T];      // w = (c_{t-1} - x) f (1 - f)
         Pack<TT, V> g[T];
@@ -677,8 +689,14 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
                 }
             }
         };
-        if (flags == 0) recompute(std::true_type());
-        else recompute(std::false_type());
+        if (flags == 0) {
+            recompute(std::true_type());
+        } else if (flags == kAll) {                 // nothing but padding
+#pragma unroll
+            for (int i = 0; i < T; ++i) { f[i] = one; keep[i] = zero; w[i] = zero; }
+        } else {
+            recompute(std::false_type());
+        }
         Num<V> dc = carry;
         if constexpr (SPLIT) {
             dc = exchange<V, true>(*x, turn, p, own, &carry, a.err, [&]() {
