@@ -155,13 +155,13 @@ __device__ __forceinline__ void load_steps(Pack<TT, N> (&r)[T], const TT *p, int
 // round ahead, and the flags are formed when the round begins (formed at once, they would wait for the bytes: 34 -> 43 us for
 // 1000 x 24 x 1024).  Bit i: step i is padded or lies behind the end.  0 is the common case, and takes the paths without
 // selects.
-template <int T> __device__ __forceinline__ uint8_t load_pad(const uint8_t *mask, int64_t stride, int64_t n, int lane) {
-    if (mask && lane < T && lane < n) return mask[lane * stride];
-    return lane < T && lane >= n;
+template <int T> __device__ __forceinline__ uint8_t load_pad(const uint8_t *mask, int64_t stride, int64_t n, int lane, const uint8_t *any) {
+    // an address for every lane, so that nothing but pad_flags depends on the byte
+    return mask ? *(lane < T && lane < n ? mask + lane * stride : any) : (uint8_t)0;
 }
-template <int T> __device__ __forceinline__ unsigned pad_flags(const uint8_t *mask, uint8_t pad, int64_t n) {
+template <int T> __device__ __forceinline__ unsigned pad_flags(const uint8_t *mask, uint8_t pad, int64_t n, int lane) {
     if (!mask) return n >= T ? 0u : (n <= 0 ? 0xffffffffu : 0xffffffffu << n) & (uint32_t)((1ull << T) - 1);
-    return __ballot_sync(0xffffffffu, pad != 0);
+    return __ballot_sync(0xffffffffu, lane < T && (lane >= n || pad != 0));
 }
 
 // Where a warp stands: its sequence and columns, and which of the interleaved slices of time it works on.  Slices are the
@@ -461,14 +461,14 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
     Pack<TT, 2 * V> next[RING ? 1 : T];
     uint8_t next_pad;
     if constexpr (!RING) load_steps<TT, 2 * V, T>(next, u, a.u_t, left);
-    next_pad = load_pad<T>(mask, a.m_t, left, p.lane);
+    next_pad = load_pad<T>(mask, a.m_t, left, p.lane, a.mask + p.b);
     if (SPLIT) exchange_start(*x, p);
     int64_t turn = 0;
     for (int64_t r0 = 0; r0 < a.L; r0 += round, ++turn, left -= round) {
-        const unsigned flags = pad_flags<T>(mask, next_pad, left);
+        const unsigned flags = pad_flags<T>(mask, next_pad, left, p.lane);
         if (r0 + round < a.L) {
             if (mask) mask += round * a.m_t;
-            next_pad = load_pad<T>(mask, a.m_t, left - round, p.lane);
+            next_pad = load_pad<T>(mask, a.m_t, left - round, p.lane, a.mask + p.b);
         }
         Pack<TT, 2 * V> cur[RING ? 1 : T];
         uint32_t row = 0;
@@ -619,13 +619,13 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
             if (gh) load_steps<TT, V, T>(next_g, gh, a.gh_t, n);
             else memset(&next_g, 0, sizeof(next_g));
         }
-        next_pad = load_pad<T>(mask, a.m_t, n, p.lane);
+        next_pad = load_pad<T>(mask, a.m_t, n, p.lane, a.mask + p.b);
     };
     fetch(left);
     if (SPLIT) exchange_start(*x, p);
     int64_t turn = 0;
     for (int64_t r0 = r_top; r0 >= 0; r0 -= round, ++turn, left += round) {
-        const unsigned flags = pad_flags<T>(mask, next_pad, left);
+        const unsigned flags = pad_flags<T>(mask, next_pad, left, p.lane);
         Num<V> c = next_c;
         Num<V> f[T], keep[T], w[T];      // w = (c_{t-1} - x) f (1 - f)
         Pack<TT, V> g[T];
