@@ -48,6 +48,22 @@ def test_native_and_python_forms_give_the_same_bits(timed):
     assert all(a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(native, python))
 
 
+def test_from_a_scripted_program():
+    """TorchScript programs and C++ hosts find the operators by name."""
+    _lib.load_torch_ops()
+
+    @torch.jit.script
+    def program(tokens: torch.Tensor, table: torch.Tensor, u: torch.Tensor):
+        y = torch.ops.sru_b200.embedding_lookup(tokens, table, 2.0)
+        h, c = torch.ops.sru_b200.gated_linear_recurrence(u)
+        return y, h, c, torch.ops.sru_b200.orthogonalize(table)
+    g = torch.Generator().manual_seed(1)
+    tokens, table = torch.randint(0, 30, (5, 7), generator=g).to(DEV), torch.randn(30, 24, generator=g).to(DEV)
+    u = torch.randn(20, 3, 16, generator=g).to(DEV)
+    want = [embedding_lookup(tokens, table, scale=2.0), *gated_linear_recurrence(u), orthogonalize(table)]
+    assert all(torch.equal(a, b) for a, b in zip(program(tokens, table, u), want))
+
+
 @pytest.mark.parametrize("python", [False, True])
 def test_differentiable_once(python, timed):
     """A second derivative is an error, not a wrong number; the orthogonalised update has no derivative at all."""
