@@ -28,7 +28,8 @@ namespace {
 
 constexpr int kBK = 64;
 constexpr int kABytes = 128 * kBK * 2;          // a CTA's 128 rows of the first operand per stage
-constexpr int kNsThreads = 192;
+constexpr int kEpilogueWarps = 8;               // per quarter of the rows, one for each half of the columns
+constexpr int kNsThreads = 64 + 32 * kEpilogueWarps;
 constexpr int kMaxParts = 256;                  // partial sums of squares per matrix
 
 enum { kPlain = 0, kCombine = 1 };
@@ -78,11 +79,12 @@ template <int BN> __device__ __forceinline__ void ns_unit(const NsArgs &g, int u
 template <int BN, bool TURN> struct NsShape {
     static constexpr int kBBytes = BN / 2 * kBK * 2;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kOut = 32 * BN * 2;                    // an epilogue warp's 32 rows, boxes of 64 columns
-    static constexpr int kTurned = TURN ? BN * 32 * 2 : 0;      // the same transposed, for the mirrored tile
+    static constexpr int kCols = BN / 2;                        // columns of an epilogue warp
+    static constexpr int kOut = 32 * kCols * 2;                 // its 32 rows, boxes of 64 columns
+    static constexpr int kTurned = TURN ? kCols * 32 * 2 : 0;      // the same transposed, for the mirrored tile
     static constexpr int kStages = BN == 128 ? 6 : TURN ? 3 : 5;
     static constexpr int kBars = 1024;
-    static constexpr int kSmem = kStages * kStageBytes + 4 * (kOut + kTurned) + 1024 + kBars;
+    static constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * (kOut + kTurned) + 1024 + kBars;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -104,13 +106,13 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *staging = smem + S::kStages * S::kStageBytes;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + 4 * (S::kOut + S::kTurned));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * (S::kOut + S::kTurned));
     const uint32_t bar_full = smem_u32(bars);                 // in the leader: loads of both CTAs
     const uint32_t bar_empty = bar_full + 8 * S::kStages;
     const uint32_t bar_tfull = bar_empty + 8 * S::kStages;    // [2]
     const uint32_t bar_tempty = bar_tfull + 16;               // [2] in the leader
-    const uint32_t bar_d = bar_tempty + 16;                   // [4] one per epilogue warp
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::kStages + 8);
+    const uint32_t bar_d = bar_tempty + 16;                   // one per epilogue warp
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::kStages + 4 + kEpilogueWarps);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
@@ -120,8 +122,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) { mbar_init(bar_full + 8 * s, 1); mbar_init(bar_empty + 8 * s, 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(bar_tfull + 8 * i, 1); mbar_init(bar_tempty + 8 * i, 8); }
-        for (int i = 0; i < 4; ++i) mbar_init(bar_d + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) { mbar_init(bar_tfull + 8 * i, 1); mbar_init(bar_tempty + 8 * i, 2 * kEpilogueWarps); }
+        for (int i = 0; i < kEpilogueWarps; ++i) mbar_init(bar_d + 8 * i, 1);
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -195,8 +197,10 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         }
     } else {
         const int q = warp & 3;                 // TMEM lane quarter: 32 of the CTA's 128 rows
+        const int half = (warp - 2) >> 2, first = half * S::kCols;      // half of the columns
+        const uint32_t bar_mine = bar_d + 8 * (half * 4 + q);
         const uint32_t tempty_leader = map_to_cta(bar_tempty, 0);
-        const uint32_t out = smem_u32(staging + q * (S::kOut + S::kTurned)), turned = out + S::kOut;
+        const uint32_t out = smem_u32(staging + (half * 4 + q) * (S::kOut + S::kTurned)), turned = out + S::kOut;
         int it = 0;
         for (int unit = pair; unit < nunits; unit += npairs, ++it) {
             int z, mb, nb;
@@ -207,22 +211,22 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             if (lane == 0) {
                 bulk_wait_read_all();           // the stores of the tile before have left the staging
                 if (MODE == kCombine) {
-                    mbar_arrive_expect_tx(bar_d + 8 * q, S::kOut);
+                    mbar_arrive_expect_tx(bar_mine, S::kOut);
 #pragma unroll
-                    for (int b = 0; b < BN / 64; ++b) tma_load_3d(out + b * 4096, &map_d, bar_d + 8 * q, nb * BN + b * 64, row0, z);
+                    for (int b = 0; b < S::kCols / 64; ++b) tma_load_3d(out + b * 4096, &map_d, bar_mine, nb * BN + first + b * 64, row0, z);
                 }
             }
             __syncwarp();
             bool ok = mbar_wait_bounded(bar_tfull + 8 * acc, (it >> 1) & 1);
-            if (MODE == kCombine) ok = mbar_wait_bounded(bar_d + 8 * q, it & 1) && ok;
+            if (MODE == kCombine) ok = mbar_wait_bounded(bar_mine, it & 1) && ok;
             if (!ok) { if (lane == 0) atomicExch(g.err, 34); break; }
             tc_fence_after();
 #pragma unroll 1
-            for (int cc = 0; cc < BN / 32; ++cc) {
-                const int col0 = nb * BN + cc * 32;
+            for (int cc = 0; cc < S::kCols / 32; ++cc) {
+                const int col0 = nb * BN + first + cc * 32;
                 if (col0 >= g.N) break;
                 uint32_t r[32];
-                tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + cc * 32, r);
+                tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + first + cc * 32, r);
                 tmem_ld_wait();
                 const uint32_t line = out + (cc >> 1) * 4096 + lane * 128;
 #pragma unroll
@@ -273,14 +277,14 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 mbar_arrive_cluster(tempty_leader + 8 * acc);
                 if (row0 < g.M) {
 #pragma unroll
-                    for (int b = 0; b < BN / 64; ++b)
-                        if (nb * BN + b * 64 < g.N) tma_store_3d(&map_c, out + b * 4096, nb * BN + b * 64, row0, z);
-                    if (TURN && mirror) tma_store_3d(&map_t, turned, row0, nb * BN, z);
+                    for (int b = 0; b < S::kCols / 64; ++b)
+                        if (nb * BN + first + b * 64 < g.N) tma_store_3d(&map_c, out + b * 4096, nb * BN + first + b * 64, row0, z);
+                    if (TURN && mirror && nb * BN + first < g.N) tma_store_3d(&map_t, turned, row0, nb * BN + first, z);
                 }
                 bulk_commit();
             }
         }
-        if (lane == 0) bulk_wait_all();
+        if (lane == 0) bulk_wait_read_all();    // the writes themselves are complete when the grid is
     }
 
     tc_fence_before();
@@ -733,8 +737,8 @@ int ns_maps(NsMaps *m, const void *base, int64_t inner, int64_t rows, int64_t ba
     int rc = ns_map(&m->a, base, inner, rows, batch, ld, 128);
     if (!rc) rc = ns_map(&m->b, base, inner, rows, batch, ld, 64);
     if (!rc) rc = ns_map(&m->c, base, inner, rows, batch, ld, 32);
-    if (!rc) rc = ns_map(&m->t, base, inner, rows, batch, ld, 128, 32);
-    if (!rc) rc = ns_map(&m->wide_t, base, inner, rows, batch, ld, 256, 32);
+    if (!rc) rc = ns_map(&m->t, base, inner, rows, batch, ld, 64, 32);
+    if (!rc) rc = ns_map(&m->wide_t, base, inner, rows, batch, ld, 128, 32);
     return rc;
 }
 
