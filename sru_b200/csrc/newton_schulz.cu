@@ -60,6 +60,21 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t sr
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
                  ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z) : "memory");
 }
+__device__ __forceinline__ uint4 shared_16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ void store_halves(uint32_t at, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
 // Unit -> matrix and tile.  A symmetric product keeps, of 256-row block i, the tiles from column 256 i on.
 template <int BN> __device__ __forceinline__ void ns_unit(const NsArgs &g, int unit, int *z, int *mb, int *nb) {
     *z = unit / g.per_matrix;
@@ -296,6 +311,164 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     }
 }
 
+// A = X X^T of few tiles over a long reduction: S pairs of SMs, one cluster, share a 256 x 128 tile.  Each sums its part of K in
+// its own tensor memory; then pair s gets columns [s, s + 1) * 128 / S of the others' sums through distributed shared
+// memory (into the ring, which nobody reads any more), adds them in a fixed order and stores those columns.
+template <int S> struct SplitShape {
+    static constexpr int kE = 128 / S;                          // columns that a pair finishes
+    static constexpr int kU = kE < 32 ? kE : 32;                // of them, an epilogue warp's
+    static constexpr int kStageBytes = kABytes + 64 * kBK * 2, kStages = 6;
+    static constexpr int kOut = 32 * kU * 2;                    // a warp's 32 rows, and once more transposed
+    static constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * 2 * kOut + 1024 + 1024;
+    static_assert((S - 1) * 128 * kE * 4 <= kStages * kStageBytes && kSmem <= 227 * 1024, "shared memory");
+};
+
+template <int S>
+__global__ void __launch_bounds__(kNsThreads, 1)
+ns_gram_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                     const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_t, const NsArgs g) {
+    using P = SplitShape<S>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *staging = smem + P::kStages * P::kStageBytes;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * 2 * P::kOut);
+    const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * P::kStages, bar_tfull = bar_empty + 8 * P::kStages;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * P::kStages + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank(), side = rank & 1;   // in the cluster, in the pair
+    const int s = (int)(rank >> 1);
+    const uint16_t both = (uint16_t)(3u << (2 * s));
+    int z, mb, nb;
+    ns_unit<128>(g, blockIdx.x / (2 * S), &z, &mb, &nb);
+    const int nkb = (g.K + kBK - 1) / kBK, kb0 = nkb * s / S, kb1 = nkb * (s + 1) / S;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < P::kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
+        mbar_init(bar_tfull, 1);
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc2(smem_u32(tmem_slot), 256);      // 128 columns, and room to read 32 from any column on
+        tmem_relinquish2();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    early_next_kernel();
+    previous_kernel_done();
+
+    const int q = warp & 3, half = (warp - 2) >> 2;             // of an epilogue warp
+    const uint32_t tmem_rows = tmem_base + ((uint32_t)(q * 32) << 16);
+    const int row = q * 32 + lane;                              // of the CTA's 128
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1)) { atomicExch(g.err, 31); break; }
+                const uint32_t full = bar_full + 8 * stage, sa = smem_u32(smem + stage * P::kStageBytes);
+                if (side == 0) mbar_arrive_expect_tx(full, 2 * P::kStageBytes);
+                tma_load_3d_pair(sa, &map_a, full, kb * kBK, mb * 256 + (int)side * 128, z);
+                tma_load_3d_pair(sa + kABytes, &map_b, full, kb * kBK, nb * 128 + (int)side * 64, z);
+                if (++stage == P::kStages) { stage = 0; phase ^= 1; }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && side == 0) {
+            constexpr uint32_t idesc = (1u << 4) | ((128u >> 3) << 17) | ((256u >> 4) << 24);
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait_bounded(bar_full + 8 * stage, phase)) { atomicExch(g.err, 33); ok = false; break; }
+                tc_fence_after();
+                const uint32_t sa = smem_u32(smem + stage * P::kStageBytes), sb = sa + kABytes;
+#pragma unroll
+                for (int k16 = 0; k16 < kBK / 16; ++k16)
+                    tc_mma_pair(tmem_base, make_desc(sa + k16 * 32, 16, 1024), make_desc(sb + k16 * 32, 16, 1024), idesc,
+                                (kb > kb0 || k16) ? 1u : 0u);
+                tc_commit_pair(bar_empty + 8 * stage, both);
+                if (++stage == P::kStages) { stage = 0; phase ^= 1; }
+            }
+            if (ok) tc_commit_pair(bar_tfull, both);
+        }
+    } else {
+        if (!mbar_wait_bounded(bar_tfull, 0) && lane == 0) atomicExch(g.err, 34);
+        tc_fence_after();
+    }
+    __syncwarp();
+    cluster_sync_all();         // every pair has read its operands: the rings are free
+    const uint32_t sums = smem_u32(smem);           // [S - 1][kE / 4][128 rows] groups of four columns
+    if (warp >= 2) {
+#pragma unroll 1
+        for (int c0 = half * 32; c0 < 128; c0 += 64) {
+            if (S <= 4 && c0 / P::kE == s) continue;            // its own
+            uint32_t r[32];
+            tmem_ld32(tmem_rows + c0, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+                const int to = (c0 + j) / P::kE, slot = s < to ? s : s - 1;
+                if (to == s) continue;
+                const uint32_t at = map_to_cta(sums + ((slot * (P::kE / 4) + (c0 + j) % P::kE / 4) * 128 + row) * 16, 2 * to + side);
+                asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};"
+                             ::"r"(at), "r"(r[j]), "r"(r[j + 1]), "r"(r[j + 2]), "r"(r[j + 3]) : "memory");
+            }
+        }
+    }
+    __syncwarp();
+    cluster_sync_all();         // all sums are here
+    if (warp >= 2 && half * P::kU < P::kE) {
+        const int c0 = s * P::kE + half * P::kU, col0 = nb * 128 + c0, row0 = mb * 256 + (int)side * 128 + q * 32;
+        const bool mirror = mb < nb / 2;
+        const uint32_t out = smem_u32(staging + (half * 4 + q) * 2 * P::kOut), turned = out + P::kOut;
+        uint32_t r[32];
+        tmem_ld32(tmem_rows + c0, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j0 = 0; j0 < P::kU; j0 += 8) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[j0 + j]);
+#pragma unroll
+            for (int slot = 0; slot < S - 1; ++slot)
+#pragma unroll
+                for (int j = 0; j < 8; j += 4) {
+                    const uint4 w = shared_16(sums + ((slot * (P::kE / 4) + (half * P::kU + j0 + j) / 4) * 128 + row) * 16);
+                    v[j] += __uint_as_float(w.x);
+                    v[j + 1] += __uint_as_float(w.y);
+                    v[j + 2] += __uint_as_float(w.z);
+                    v[j + 3] += __uint_as_float(w.w);
+                }
+            store_halves(out + lane * (P::kU * 2) + j0 * 2, v);
+            if (mirror) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(turned + (j0 + j) * 64 + lane * 2),
+                                 "h"(__half_as_ushort(__float2half_rn(v[j]))) : "memory");
+            }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0 && row0 < g.M && col0 < g.N) {
+            tma_store_3d(&map_c, out, col0, row0, z);
+            if (mirror) tma_store_3d(&map_t, turned, row0, col0, z);
+            bulk_commit();
+            bulk_wait_read_all();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc2(tmem_base, 256);
+    }
+}
+
 // ---- norm, first iterate, result ------------------------------------------------------------------------------------
 struct NsEdge {
     const void *src;
@@ -451,21 +624,6 @@ constexpr int kTileBytes = 128 * 64 * 2;
 __device__ __forceinline__ uint32_t tile_at(int row, int col) {     // byte offset of 8 columns' group in the tiles
     return (uint32_t)(col >> 6) * kTileBytes + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4);
 }
-__device__ __forceinline__ uint4 shared_16(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-    return v;
-}
-__device__ __forceinline__ void store_halves(uint32_t at, const float (&v)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-        w[j] = *reinterpret_cast<const uint32_t *>(&h);
-    }
-    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-}
-
 struct NsSmall {
     NsEdge e;                       // source and sizes; dst is the result
     int64_t o_i, o_j, o_b;          // strides of the result along the iterate's rows, columns, and batch
@@ -775,6 +933,53 @@ int ns_product(const NsMaps &a, const NsMaps &b, const NsMaps &out, const NsMaps
     return 0;
 }
 
+// The same product split over the reduction: see choose_split.
+template <int S> int ns_gram_split(const NsMaps &a, const void *out, int64_t ldm, NsArgs g, cudaStream_t st) {
+    using P = SplitShape<S>;
+    auto kernel = ns_gram_split_kernel<S>;
+    static bool attr_set[64] = {false};
+    int dev = 0;
+    SRUB_CUDA_CHECK(cudaGetDevice(&dev));
+    if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+        SRUB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmem));
+        SRUB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        attr_set[dev] = true;
+    }
+    CUtensorMap c, t;
+    int rc = ns_map(&c, out, g.M, g.M, g.batch, ldm, 32, P::kU);
+    if (!rc) rc = ns_map(&t, out, g.M, g.M, g.batch, ldm, P::kU, 32);
+    if (rc) return rc;
+    g.tiles_m = (g.M + 255) / 256;
+    g.tiles_n = (g.M + 127) / 128;
+    g.per_matrix = g.tiles_m * g.tiles_n - g.tiles_m * (g.tiles_m - 1);
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)(2 * S * g.per_matrix * g.batch), 1, 1);
+    cfg.blockDim = dim3(kNsThreads, 1, 1);
+    cfg.dynamicSmemBytes = P::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2 * S; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1] = early_launch();
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, a.a, a.b, c, t, g));
+    return 0;
+}
+
+// Pairs that share a tile of X X^T, by the number of tiles and the 64-element blocks of the reduction: as many as the GPU holds
+// clusters for (7, 15 and 33 of 16, 8 and 4 CTAs) while the exchange (1.5 us) is shorter than what it saves.  Five steps with 1 /
+// 2 / 4 / 8 pairs: 64 x 6144 197 / 145 / 118 / 109 us, 64 x 4000 158 / 125 / 118 / 118, 512 x 6144 245 / 192 / 168 / 157, two 500 x
+// 2000 172 / 152 / 145, 500 x 500 149 / 143 / 142, four 300 x 1500 (16 tiles) 145 / 135, 1024 x 4096 (20 tiles) 231 / 194, 700 x 700
+// twice (24 tiles) 151 / 147.
+int choose_split(int64_t tiles, int64_t blocks) {
+    if (tiles <= 7 && blocks >= 64) return 8;
+    if (tiles <= 15 && blocks >= 8) return 4;
+    if (tiles <= 33 && blocks >= 8) return 2;
+    return 1;
+}
+
 // X X^T and A A.  A 256 x 128 tile takes a pair of SMs about as long as one of 256 x 256 (0.28 us per 64 of the reduction: its
 // operands keep shared memory just as busy), but has the shorter epilogue and room for twice the stages.  It is taken where
 // the tiles all find a pair of their own, and for small matrices.  Five steps with 128 / 256 columns: 4096 x 4096 1276 / 1112
@@ -911,7 +1116,11 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         g.batch = (int)batch; g.err = err;
         g.M = (int)p.m; g.N = (int)p.m; g.K = (int)p.n; g.symmetric = 1;
         g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc;
-        if (int rc = ns_gram<kPlain>(xm[cur], am, am, g, sms, st)) return rc;
+        const int64_t tiles = ((p.m + 255) / 256) * ((p.m + 127) / 128 - (p.m + 255) / 256 + 1) * batch;
+        const int split = choose_split(tiles, (p.n + kBK - 1) / kBK);
+        int rc = split == 8 ? ns_gram_split<8>(xm[cur], a_buf, p.ldm, g, st) : split == 4 ? ns_gram_split<4>(xm[cur], a_buf, p.ldm, g, st)
+                 : split == 2 ? ns_gram_split<2>(xm[cur], a_buf, p.ldm, g, st) : ns_gram<kPlain>(xm[cur], am, am, g, sms, st);
+        if (rc) return rc;
         g.K = (int)p.m;
         if (int rc = ns_gram<kCombine>(am, mm, am, g, sms, st)) return rc;
         g.N = (int)p.n; g.symmetric = 0;
