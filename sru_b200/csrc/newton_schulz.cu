@@ -14,8 +14,9 @@
 // gradients with a decaying spectrum the result is 1.2e-3 off the exact steps against 1.0e-2 with bf16 iterates.
 //
 // The products run on pairs of SMs (cta_group::2, 256 x BN tiles) in a persistent grid over (matrix, tile).  A product costs
-// about 6 us beside its multiplications (load latency 1.1, accumulator to memory 2.5, teardown 0.6, next kernel 1.1), which is
-// most of the time up to 1024 x 1024; from there on shared memory and L2 feed the tensor cores at 60 to 75 % of their rate.
+// about 5 us beside its multiplications (load latency 1.1, accumulator to shared memory 0.8, stores and end of the grid 2, next
+// kernel 1.2), which is most of the time up to 1024 x 1024.  Long products take 440 cycles per 64 of K with 128 columns and 521
+// with 256 where the tensor cores need 256 and 512: 24 and 32 KB a SM, close to the 64 bytes a cycle that L2 hands it.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -289,7 +290,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             fence_proxy_async();                // the staged values become visible to the copy engine
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive_cluster(tempty_leader + 8 * acc);
+                mbar_arrive_cluster_relaxed(tempty_leader + 8 * acc);
                 if (row0 < g.M) {
 #pragma unroll
                     for (int b = 0; b < S::kCols / 64; ++b)
@@ -313,14 +314,15 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
 // A = X X^T of few tiles over a long reduction: S pairs of SMs, one cluster, share a 256 x 128 tile.  Each sums its part of K in
 // its own tensor memory; then pair s gets columns [s, s + 1) * 128 / S of the others' sums through distributed shared
-// memory (into the ring, which nobody reads any more), adds them in a fixed order and stores those columns.
+// memory, adds them in a fixed order and stores those columns.
 template <int S> struct SplitShape {
     static constexpr int kE = 128 / S;                          // columns that a pair finishes
     static constexpr int kU = kE < 32 ? kE : 32;                // of them, an epilogue warp's
-    static constexpr int kStageBytes = kABytes + 64 * kBK * 2, kStages = 6;
+    static constexpr int kStageBytes = kABytes + 64 * kBK * 2, kStages = 5;
+    static constexpr int kSums = (S - 1) * 128 * kE * 4;        // the others' sums of its columns
     static constexpr int kOut = 32 * kU * 2;                    // a warp's 32 rows, and once more transposed
-    static constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * 2 * kOut + 1024 + 1024;
-    static_assert((S - 1) * 128 * kE * 4 <= kStages * kStageBytes && kSmem <= 227 * 1024, "shared memory");
+    static constexpr int kSmem = kStages * kStageBytes + kSums + kEpilogueWarps * 2 * kOut + 1024 + 1024;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
 template <int S>
@@ -330,7 +332,8 @@ ns_gram_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     using P = SplitShape<S>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *staging = smem + P::kStages * P::kStageBytes;
+    const uint32_t sums = smem_u32(smem + P::kStages * P::kStageBytes);     // [S - 1][kE / 4][128 rows] groups of four columns
+    uint8_t *staging = smem + P::kStages * P::kStageBytes + P::kSums;
     uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * 2 * P::kOut);
     const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * P::kStages, bar_tfull = bar_empty + 8 * P::kStages;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * P::kStages + 1);
@@ -399,9 +402,6 @@ ns_gram_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         if (!mbar_wait_bounded(bar_tfull, 0) && lane == 0) atomicExch(g.err, 34);
         tc_fence_after();
     }
-    __syncwarp();
-    cluster_sync_all();         // every pair has read its operands: the rings are free
-    const uint32_t sums = smem_u32(smem);           // [S - 1][kE / 4][128 rows] groups of four columns
     if (warp >= 2) {
 #pragma unroll 1
         for (int c0 = half * 32; c0 < 128; c0 += 64) {
@@ -460,6 +460,353 @@ ns_gram_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             bulk_wait_read_all();
         }
     }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc2(tmem_base, 256);
+    }
+}
+
+// ---- one cluster per matrix ---------------------------------------------------------------------------------------
+// Matrices whose products are shorter than what lies between them: one cluster of SM pairs takes a matrix through all its
+// steps, a cluster barrier between the products in place of a launch.  Iterates, A and M stay in L2.  The pairs share the 256 x
+// 128 tiles of each product; where X X^T has fewer tiles than the cluster pairs, several pairs share a tile's reduction, as
+// above.  A product costs 4 us beside its multiplications (in cycles: first operands 1500, accumulator to shared memory 800, to
+// L2 1300, the stores made visible to the copy engine 1000, the barrier 700).
+struct NsCluster {
+    int m, n, steps;
+    float ca, cb, cc;
+    __half *x0, *x1, *a, *mm;       // rows of ldx, ldm elements
+    int64_t ldx, ldm;
+    void *out;                      // the last product's, (m, n) or, turned, (n, m), contiguous; NULL: it goes to x like the others
+    int turned, turned_wide, bf16;  // turned_wide: its rows are 16-byte aligned
+    int *err;
+};
+
+// Pairs that share a tile of X X^T; the exchange takes as long as ten blocks.
+__host__ __device__ inline int pairs_per_tile(int tiles, int pairs, int blocks) {
+    int s = 1;
+    while (s < 8 && tiles * s * 2 <= pairs) s *= 2;
+    return blocks - blocks / s < 10 ? 1 : s;
+}
+
+struct ClusterShape {
+    static constexpr int kStageBytes = kABytes + 64 * kBK * 2, kStages = 6;
+    static constexpr int kOut = 32 * 64 * 2;                    // an epilogue warp's 32 rows and 64 columns; once more transposed
+    static constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * 2 * kOut + 1024 + 1024;
+    static_assert(kSmem <= 227 * 1024 && 7 * 128 * 16 * 4 <= kEpilogueWarps * 2 * kOut, "shared memory");
+};
+
+__global__ void __launch_bounds__(kNsThreads, 1)
+ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_constant__ CUtensorMap map_x0b,
+                  const __grid_constant__ CUtensorMap map_x1a, const __grid_constant__ CUtensorMap map_x1b,
+                  const __grid_constant__ CUtensorMap map_aa, const __grid_constant__ CUtensorMap map_ab,
+                  const __grid_constant__ CUtensorMap map_ac, const __grid_constant__ CUtensorMap map_ma, const NsCluster g) {
+    using P = ClusterShape;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *staging = smem + P::kStages * P::kStageBytes;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * 2 * P::kOut);
+    const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * P::kStages, bar_tfull = bar_empty + 8 * P::kStages;
+    const uint32_t bar_tempty = bar_tfull + 16, bar_d = bar_tempty + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * P::kStages + 4 + kEpilogueWarps);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank(), side = rank & 1;
+    uint32_t ctas;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+    const int pair = (int)(rank >> 1), pairs = (int)(ctas >> 1), z = (int)(blockIdx.x / ctas);
+    const uint16_t both = (uint16_t)(3u << (2 * pair));
+    const int rows = (g.m + 255) / 256, cols = (g.m + 127) / 128;
+    const int nkb_n = (g.n + kBK - 1) / kBK, nkb_m = (g.m + kBK - 1) / kBK;
+    const int square = rows * (cols - rows + 1);                // tiles of a symmetric product
+    const int S = pairs_per_tile(square, pairs, nkb_n);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < P::kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(bar_tfull + 8 * i, 1); mbar_init(bar_tempty + 8 * i, 2 * kEpilogueWarps); }
+        for (int i = 0; i < kEpilogueWarps; ++i) mbar_init(bar_d + 8 * i, 1);
+        fence_mbar_init();
+    }
+    if (threadIdx.x == 32)
+        for (const CUtensorMap *map : {&map_x0a, &map_x0b, &map_x1a, &map_x1b, &map_aa, &map_ab, &map_ac, &map_ma})
+            asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+    __syncwarp();
+    if (warp == 1) {
+        tmem_alloc2(smem_u32(tmem_slot), 256);
+        tmem_relinquish2();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    early_next_kernel();
+    previous_kernel_done();
+
+    // a role's place in the ring and in the accumulators, over all products
+    int stage = 0, it = 0;
+    uint32_t phase = 0, d_phase = 0;
+    bool dead = false;              // a wait gave up: this warp waits for no more mbarriers, but keeps up with the cluster's
+    const int q = warp & 3, half = (warp - 2) >> 2;             // of an epilogue warp
+    const uint32_t tmem_rows = tmem_base + ((uint32_t)(q * 32) << 16), bar_mine = bar_d + 8 * (half * 4 + q);
+    const uint32_t tempty_leader = map_to_cta(bar_tempty, rank & ~1u);
+    const uint32_t out = smem_u32(staging + (half * 4 + q) * 2 * P::kOut), turned = out + P::kOut;
+
+    for (int product = 0; product < 3 * g.steps; ++product) {
+        const int kind = product % 3, cur = (product / 3) & 1;  // 0: A = X X^T, 1: M, 2: X = M X
+        const int split = kind == 0 ? S : 1, mine = pair / split, part = pair % split;
+        const int units = kind == 2 ? rows * ((g.n + 127) / 128) : square;
+        const int nkb = kind == 0 ? nkb_n : nkb_m, kb0 = nkb * part / split, kb1 = nkb * (part + 1) / split;
+        auto tile = [&](int unit, int *mb, int *nb) {
+            if (kind == 2) {
+                *nb = unit / rows;
+                *mb = unit - *nb * rows;
+            } else {
+                int i = 0, left = cols;
+                while (unit >= left) { unit -= left; left -= 2; ++i; }
+                *mb = i;
+                *nb = 2 * i + unit;
+            }
+        };
+        if (warp == 0) {
+            if (lane == 0) {
+                const CUtensorMap *ma = kind == 0 ? (cur ? &map_x1a : &map_x0a) : kind == 1 ? &map_aa : &map_ma;
+                const CUtensorMap *mbp = kind == 1 ? &map_ab : cur ? &map_x1b : &map_x0b;
+                for (int unit = mine; unit < units && !dead; unit += pairs) {
+                    int mb, nb;
+                    tile(unit, &mb, &nb);
+                    const int m0 = mb * 256 + (int)side * 128, n0 = nb * 128 + (int)side * 64;
+                    for (int kb = kb0; kb < kb1; ++kb) {
+                        if (!mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1)) { atomicExch(g.err, 36); dead = true; break; }
+                        const uint32_t full = bar_full + 8 * stage, sa = smem_u32(smem + stage * P::kStageBytes);
+                        if (side == 0) mbar_arrive_expect_tx(full, 2 * P::kStageBytes);
+                        tma_load_3d_pair(sa, ma, full, kb * kBK, m0, z);
+                        if (kind == 2) tma_load_3d_pair(sa + kABytes, mbp, full, n0, kb * kBK, z);
+                        else tma_load_3d_pair(sa + kABytes, mbp, full, kb * kBK, n0, z);
+                        if (++stage == P::kStages) { stage = 0; phase ^= 1; }
+                    }
+                }
+            }
+        } else if (warp == 1) {
+            if (lane == 0 && side == 0) {
+                const uint32_t idesc = (1u << 4) | ((kind == 2 ? 1u : 0u) << 16) | ((128u >> 3) << 17) | ((256u >> 4) << 24);
+                const uint32_t b_step = kind == 2 ? 2048u : 32u, b_lbo = kind == 2 ? 8192u : 16u;
+                for (int unit = mine; unit < units && !dead; unit += pairs, ++it) {
+                    const int acc = it & 1;
+                    if (!mbar_wait_bounded(bar_tempty + 8 * acc, ((it >> 1) & 1) ^ 1)) { atomicExch(g.err, 37); dead = true; break; }
+                    tc_fence_after();
+                    for (int kb = kb0; kb < kb1; ++kb) {
+                        if (!mbar_wait_bounded(bar_full + 8 * stage, phase)) { atomicExch(g.err, 38); dead = true; break; }
+                        tc_fence_after();
+                        const uint32_t sa = smem_u32(smem + stage * P::kStageBytes), sb = sa + kABytes;
+#pragma unroll
+                        for (int k16 = 0; k16 < kBK / 16; ++k16)
+                            tc_mma_pair(tmem_base + acc * 128, make_desc(sa + k16 * 32, 16, 1024),
+                                        make_desc(sb + k16 * b_step, b_lbo, 1024), idesc, (kb > kb0 || k16) ? 1u : 0u);
+                        tc_commit_pair(bar_empty + 8 * stage, both);
+                        if (++stage == P::kStages) { stage = 0; phase ^= 1; }
+                    }
+                    if (!dead) tc_commit_pair(bar_tfull + 8 * acc, both);
+                }
+            }
+        } else if (split == 1) {
+            const bool last = kind == 2 && g.out && product == 3 * g.steps - 1;
+            const int64_t ld = kind == 2 ? (last ? g.n : g.ldx) : g.ldm;
+            __half *dst = kind == 0 ? g.a + z * (g.m * g.ldm) : kind == 1 ? g.mm + z * (g.m * g.ldm)
+                          : last ? static_cast<__half *>(g.out) + z * ((int64_t)g.m * g.n) : (cur ? g.x0 : g.x1) + z * (g.m * g.ldx);
+            const int N = kind == 2 ? g.n : g.m;
+            for (int unit = mine; unit < units; unit += pairs, ++it) {
+                int mb, nb;
+                tile(unit, &mb, &nb);
+                const int acc = it & 1, row0 = mb * 256 + (int)side * 128 + q * 32, row = row0 + lane, first = nb * 128 + half * 64;
+                const bool turn = last && g.turned, across = turn || (kind < 2 && mb < nb / 2);
+                const int64_t ld_across = turn ? g.m : ld;
+                if (kind == 1) {
+                    if (lane == 0) {
+                        if (unit != mine) fence_proxy_async();      // the staging was read with plain loads
+                        mbar_arrive_expect_tx(bar_mine, P::kOut);
+                        tma_load_3d(out, &map_ac, bar_mine, first, row0, z);
+                    }
+                    __syncwarp();
+                }
+                bool ok = dead || mbar_wait_bounded(bar_tfull + 8 * acc, (it >> 1) & 1);
+                if (kind == 1) {
+                    ok = (dead || mbar_wait_bounded(bar_mine, d_phase)) && ok;
+                    d_phase ^= 1;
+                }
+                if (!ok) {
+                    dead = true;
+                    if (lane == 0) atomicExch(g.err, 39);
+                }
+                tc_fence_after();
+                uint32_t both_r[2][32];
+                tmem_ld32(tmem_rows + acc * 128 + half * 64, both_r[0]);
+                tmem_ld32(tmem_rows + acc * 128 + half * 64 + 32, both_r[1]);
+                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster_relaxed(tempty_leader + 8 * acc);
+#pragma unroll
+                for (int cc = 0; cc < 2; ++cc) {
+                    const int col0 = first + cc * 32;
+                    const uint32_t (&r)[32] = both_r[cc];
+#pragma unroll
+                    for (int j0 = 0; j0 < 32; j0 += 8) {
+                        const uint32_t at = out + lane * 128 + (((cc * 4 + j0 / 8) ^ (lane & 7)) << 4);
+                        float v[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[j0 + j]);
+                        if (kind == 1) {
+                            const uint4 d = shared_16(at);
+                            const __half2 *a2 = reinterpret_cast<const __half2 *>(&d);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const float a = (j & 1) ? __high2float(a2[j >> 1]) : __low2float(a2[j >> 1]);
+                                v[j] = fmaf(g.cc, v[j], fmaf(g.cb, a, row == col0 + j0 + j ? g.ca : 0.0f));
+                            }
+                        }
+                        uint32_t w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (last && g.bf16) {
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+                                w[j] = *reinterpret_cast<const uint32_t *>(&h);
+                            } else {
+                                const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+                                w[j] = *reinterpret_cast<const uint32_t *>(&h);
+                            }
+                        }
+                        if (!turn) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                        if (across) {                       // element (row, col) at [col][row]
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                asm volatile("st.shared.u16 [%0], %1;" ::"r"(turned + (cc * 32 + j0 + j) * 64 + lane * 2),
+                                             "h"((unsigned short)(w[j >> 1] >> (16 * (j & 1)))) : "memory");
+                        }
+                    }
+                }
+                __syncwarp();
+                if (!turn) {
+                    uint4 w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {           // 4 rows of 128 bytes
+                        const int rr = i * 4 + (lane >> 3);
+                        w[i] = shared_16(out + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+                    }
+                    const int rr = lane >> 3, col = first + (lane & 7) * 8;
+                    __half *to = dst + (row0 + rr) * ld + col;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i, to += 4 * ld)
+                        if (row0 + rr + i * 4 < g.m && col < N) *reinterpret_cast<uint4 *>(to) = w[i];
+                }
+                if (across) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {           // 8 rows of 64 bytes
+                        const int rr = i * 8 + (lane >> 2), col = row0 + (lane & 3) * 8;
+                        const uint4 w = shared_16(turned + rr * 64 + (lane & 3) * 16);
+                        if (first + rr < N && col < g.m) {
+                            __half *to = dst + (first + rr) * ld_across + col;
+                            if (!turn || g.turned_wide) {
+                                *reinterpret_cast<uint4 *>(to) = w;
+                            } else {
+                                const __half *e = reinterpret_cast<const __half *>(&w);
+#pragma unroll
+                                for (int k = 0; k < 8; ++k)
+                                    if (col + k < g.m) to[k] = e[k];
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        if (split > 1) {
+            // the pairs' sums of a tile, joined: pair `part` of the tile finishes columns [part, part + 1) * E
+            const int E = 128 / split, acc = it & 1;
+            const bool on = warp >= 2 && mine < units;
+            int mb, nb;
+            tile(min(mine, units - 1), &mb, &nb);
+            const int row = q * 32 + lane;
+            const uint32_t sums = smem_u32(staging);        // [split - 1][E / 4][128 rows] groups of four columns
+            if (on) {
+                if (!dead && !mbar_wait_bounded(bar_tfull + 8 * acc, (it >> 1) & 1)) {
+                    dead = true;
+                    if (lane == 0) atomicExch(g.err, 39);
+                }
+                tc_fence_after();
+            }
+            if (on) {
+#pragma unroll 1
+                for (int c0 = half * 16; c0 < 128; c0 += 32) {
+                    const int to = c0 / E, slot = part < to ? part : part - 1;
+                    if (to == part) continue;
+                    uint32_t r[16];
+                    tmem_ld16(tmem_rows + acc * 128 + c0, r);
+                    tmem_ld_wait();
+                    const uint32_t at = map_to_cta(sums + ((slot * (E / 4) + c0 % E / 4) * 128 + row) * 16, 2 * (mine * split + to) + side);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4)
+                        asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};"
+                                     ::"r"(at + j / 4 * 2048), "r"(r[j]), "r"(r[j + 1]), "r"(r[j + 2]), "r"(r[j + 3]) : "memory");
+                }
+            }
+            __syncwarp();
+            cluster_sync_all();         // all sums are here
+            if (on) {
+#pragma unroll 1
+                for (int e0 = half * 16; e0 < E; e0 += 32) {
+                    uint32_t r[16];
+                    tmem_ld16(tmem_rows + acc * 128 + part * E + e0, r);
+                    tmem_ld_wait();
+                    float v[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+                    for (int slot = 0; slot < split - 1; ++slot)
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4) {
+                            const uint4 w = shared_16(sums + ((slot * (E / 4) + (e0 + j) / 4) * 128 + row) * 16);
+                            v[j] += __uint_as_float(w.x);
+                            v[j + 1] += __uint_as_float(w.y);
+                            v[j + 2] += __uint_as_float(w.z);
+                            v[j + 3] += __uint_as_float(w.w);
+                        }
+                    const int i = mb * 256 + (int)side * 128 + row, col0 = nb * 128 + part * E + e0;
+                    __half *dst = g.a + z * (g.m * g.ldm);
+                    __half h[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) h[j] = __float2half_rn(v[j]);
+                    if (i < g.m) {
+#pragma unroll
+                        for (int j = 0; j < 16; j += 8) {
+                            Pack<__half, 8> o;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) o.v[k] = h[j + k];
+                            if (col0 + j < g.m) *reinterpret_cast<Pack<__half, 8> *>(dst + i * g.ldm + col0 + j) = o;
+                        }
+                        if (mb < nb / 2) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                if (col0 + j < g.m) dst[(col0 + j) * g.ldm + i] = h[j];
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster_relaxed(tempty_leader + 8 * acc);
+            }
+            if (on) ++it;
+        }
+        // this product's stores, before the next one's copies
+        if (warp >= 2) {
+            fence_proxy_async_all();
+        }
+        __syncwarp();
+        cluster_sync_all();
+    }
+
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();
@@ -617,7 +964,7 @@ template <typename T> __global__ void __launch_bounds__(256) ns_last_kernel(cons
 // as 64-column tiles of 128 rows in the 128-byte swizzle, which the tensor cores read as the K-major operand of X X^T and as
 // the MN-major operand of M X alike, and one 128 x 128 matrix that holds A and then, in place, M.  Nothing leaves the SM
 // between load and store.  Bound by the latency of the chain (product, accumulator to registers, shared memory, next
-// product; 5 us a step at 128 x 384 and 37 in all, 103 on the general path, which pays for three launches a step).
+// product; 5 us a step at 128 x 384 and 37 in all, 92 in a cluster).
 constexpr int kSmallM = 128, kSmallN = 768, kSmallThreads = 512;
 constexpr int kTileBytes = 128 * 64 * 2;
 
@@ -968,11 +1315,52 @@ template <int S> int ns_gram_split(const NsMaps &a, const void *out, int64_t ldm
     return 0;
 }
 
+int ns_cluster(const NsMaps &x0, const NsMaps &x1, const NsMaps &a, const NsMaps &m, const NsCluster &g, int64_t batch, int ctas, cudaStream_t st) {
+    static bool attr_set[64] = {false};
+    int dev = 0;
+    SRUB_CUDA_CHECK(cudaGetDevice(&dev));
+    if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+        SRUB_CUDA_CHECK(cudaFuncSetAttribute(ns_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ClusterShape::kSmem));
+        SRUB_CUDA_CHECK(cudaFuncSetAttribute(ns_cluster_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        attr_set[dev] = true;
+    }
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)(ctas * batch), 1, 1);
+    cfg.blockDim = dim3(kNsThreads, 1, 1);
+    cfg.dynamicSmemBytes = ClusterShape::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1] = early_launch();
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ns_cluster_kernel, x0.a, x0.b, x1.a, x1.b, a.a, a.b, a.c, m.a, g));
+    return 0;
+}
+
+// CTAs of a cluster that takes a matrix through all its steps, or 0: a launch per product.  A cluster where a pair's share of a
+// step is at most 34 blocks (of 64 of a tile's reduction, 0.23 us each; a tile's epilogue takes as long as six, the exchange
+// between pairs as eight), and the GPU holds clusters for the batch (7 of 16 CTAs, 15 of 8).  With launches / in a cluster:
+// 130 x 200 (18 blocks) 124 / 84 us, 256 x 512 (20) 117 / 84, 500 x 500 (24) 134 / 119, seven 256 x 1024 (26) 111 / 96, twelve 128 x
+// 1000 106 / 96, 400 x 700 (32) 120 / 118, 384 x 1024 (34) 115 / 117, two 512 x 1024 (40) 125 / 128, 700 x 700 (77) 135 / 180.
+int choose_cluster(int64_t m, int64_t n, int64_t batch) {
+    const int64_t ctas = batch <= 7 ? 16 : 8, pairs = ctas / 2, rows = (m + 255) / 256, square = rows * ((m + 127) / 128 - rows + 1);
+    if (batch > 15) return 0;
+    const int split = pairs_per_tile((int)square, (int)pairs, (int)((n + kBK - 1) / kBK));
+    auto tiles = [&](int64_t count, int64_t blocks) { return (count + pairs - 1) / pairs * std::max<int64_t>(blocks, 6); };
+    const int64_t blocks_m = (m + kBK - 1) / kBK, blocks_n = (n + kBK - 1) / kBK;
+    const int64_t share = tiles(square * split, blocks_n / split) + (split > 1 ? 8 : 0) + tiles(square, blocks_m) +
+                          tiles(rows * ((n + 127) / 128), blocks_m);
+    return share <= 34 ? (int)ctas : 0;
+}
+
 // Pairs that share a tile of X X^T, by the number of tiles and the 64-element blocks of the reduction: as many as the GPU holds
-// clusters for (7, 15 and 33 of 16, 8 and 4 CTAs) while the exchange (1.5 us) is shorter than what it saves.  Five steps with 1 /
-// 2 / 4 / 8 pairs: 64 x 6144 197 / 145 / 118 / 109 us, 64 x 4000 158 / 125 / 118 / 118, 512 x 6144 245 / 192 / 168 / 157, two 500 x
-// 2000 172 / 152 / 145, 500 x 500 149 / 143 / 142, four 300 x 1500 (16 tiles) 145 / 135, 1024 x 4096 (20 tiles) 231 / 194, 700 x 700
-// twice (24 tiles) 151 / 147.
+// clusters for (7, 15 and 33 of 16, 8 and 4 CTAs) while the exchange (1 us) is shorter than what it saves.  Five steps with 1 /
+// 2 / 4 / 8 pairs: 64 x 6144 194 / 142 / 118 / 104 us, 64 x 4000 154 / 132 / 124 / 124, 512 x 6144 235 / 181 / 154 / 143; with 1 / 2 /
+// 4: two 500 x 2000 164 / 147 / 139, 500 x 500 141 / 137 / 135; with 1 / 2: four 300 x 1500 (16 tiles) 138 / 129, 1024 x 4096 (20
+// tiles) 222 / 188, two 700 x 700 (24 tiles) 144 / 140.
 int choose_split(int64_t tiles, int64_t blocks) {
     if (tiles <= 7 && blocks >= 64) return 8;
     if (tiles <= 15 && blocks >= 8) return 4;
@@ -982,8 +1370,8 @@ int choose_split(int64_t tiles, int64_t blocks) {
 
 // X X^T and A A.  A 256 x 128 tile takes a pair of SMs about as long as one of 256 x 256 (0.28 us per 64 of the reduction: its
 // operands keep shared memory just as busy), but has the shorter epilogue and room for twice the stages.  It is taken where
-// the tiles all find a pair of their own, and for small matrices.  Five steps with 128 / 256 columns: 4096 x 4096 1276 / 1112
-// us, four 2048 x 2048 761 / 720, six 1024 x 2048 374 / 328, but twelve 700 x 1400 327 / 348.
+// the tiles all find a pair of their own, and for small matrices.  Five steps with 128 / 256 columns: 4096 x 4096 1268 / 1120
+// us, four 2048 x 2048 745 / 660, six 1024 x 2048 378 / 310, but twelve 700 x 1400 322 / 330.
 template <int MODE> int ns_gram(const NsMaps &a, const NsMaps &out, const NsMaps &d, const NsArgs &g, int sms, cudaStream_t st) {
     const int64_t rows = (g.M + 255) / 256, narrow = rows * ((g.M + 127) / 128) - rows * (rows - 1);
     if (narrow * g.batch <= sms / 2 || g.M < 1024) return ns_product<128, false, false, MODE>(a, a, out, d, g, sms, st);
@@ -1098,10 +1486,11 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     };
     if (int rc = grad_dtype == SRU_F32 ? begin(float()) : grad_dtype == SRU_F16 ? begin(__half()) : begin(__nv_bfloat16())) return rc;
 
-    // The last product writes the caller's matrix itself where its rows are 16-byte aligned.
-    const bool direct = steps > 0 && cols % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    // The last product writes the caller's matrix itself where its rows are 16-byte aligned (a cluster's turned one, always).
+    const int ctas = steps > 0 ? choose_cluster(p.m, p.n, batch) : 0;
+    const bool aligned = steps > 0 && cols % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0, direct = aligned || (ctas && tall);
     NsMaps xm[2], am, mm, om;
-    if (direct)
+    if (aligned)
         if (int rc = ns_maps(&om, out, cols, rows, batch, cols)) return rc;
     if (steps > 0) {
         int rc = ns_maps(&am, a_buf, p.m, p.m, batch, p.ldm);
@@ -1109,7 +1498,16 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         for (int i = 0; i < 2 && !rc; ++i) rc = ns_maps(&xm[i], x[i], p.n, p.m, batch, p.ldx);
         if (rc) return rc;
     }
-    for (int s = 0; s < steps; ++s) {
+    if (ctas) {
+        NsCluster g;
+        memset(&g, 0, sizeof(g));
+        g.m = (int)p.m; g.n = (int)p.n; g.steps = steps;
+        g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc;
+        g.x0 = x[0]; g.x1 = x[1]; g.a = a_buf; g.mm = m_buf; g.ldx = p.ldx; g.ldm = p.ldm;
+        g.out = direct ? out : nullptr; g.turned = tall; g.turned_wide = aligned; g.bf16 = out_dtype == SRU_BF16; g.err = err;
+        if (int rc = ns_cluster(xm[0], xm[1], am, mm, g, batch, ctas, st)) return rc;
+    }
+    for (int s = 0; s < steps && !ctas; ++s) {
         const int cur = s & 1;
         NsArgs g;
         memset(&g, 0, sizeof(g));

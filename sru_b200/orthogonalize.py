@@ -57,8 +57,8 @@ def orthogonalize(grad: Tensor, steps: int = 5, coefficients: Tuple[float, float
     with torch.cuda.device(grad.device):
         nbytes = int(L.sru_b200_orthogonalize_workspace_bytes(batch, rows, cols))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)
-        _lib.call("orthogonalize", 1 if max(rows, cols) <= 768 and min(rows, cols) <= 128 else 3 + 3 * int(steps), L.sru_b200_orthogonalize, _lib.ptr(out), _lib.ptr(grad), batch, rows,
-                  cols, grad.stride(0) if grad.dim() == 3 else 0, grad.stride(-2), grad.stride(-1), int(steps), a, b, c,
+        _lib.call("orthogonalize", 1, L.sru_b200_orthogonalize, _lib.ptr(out), _lib.ptr(grad), batch, rows, cols,
+                  grad.stride(0) if grad.dim() == 3 else 0, grad.stride(-2), grad.stride(-1), int(steps), a, b, c,
                   float(eps), _lib.DTYPE_CODE[grad.dtype], _lib.DTYPE_CODE[out_dtype], _lib.ptr(ws), nbytes,
                   _lib.current_stream_ptr(grad.device))
     return out

@@ -96,6 +96,30 @@ def test_both_tile_widths(batch, rows, cols):
     assert float((err - want).norm()) <= 1.5 * float((model - want).norm()) + (2.0 ** -8 + 1e-4) * float(want.norm())
 
 
+@pytest.mark.parametrize("batch,rows,cols", [(1, 130, 200), (7, 201, 333), (8, 140, 260), (15, 200, 136), (16, 130, 200),
+                                             (1, 130, 1700), (1, 1700, 129), (2, 60, 1000), (9, 1000, 100), (1, 385, 390),
+                                             (3, 500, 505), (1, 384, 1024), (1, 384, 1100)])
+def test_where_one_cluster_takes_the_matrix(batch, rows, cols):
+    """Both sides of the sizes and batches at which a cluster takes a matrix through all steps; with and without several
+    pairs to a tile, wide and tall, rows of the result aligned and not."""
+    check(gradient(batch, rows, cols, F32, rows + cols), BF16)
+    for steps in (1, 2):
+        check(gradient(batch, rows, cols, F16, rows + cols), F16, steps=steps)
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 64, 4100), (7, 33, 4160), (1, 500, 4133), (2, 500, 1700), (15, 100, 4000),
+                                             (1, 900, 1200), (16, 129, 2000), (33, 128, 900), (1, 4200, 257)])
+def test_reductions_split_between_pairs(batch, rows, cols):
+    """X X^T of few tiles over a long reduction: two, four and eight pairs of SMs to a tile."""
+    g = gradient(batch, rows, cols, BF16, rows + cols)
+    got = orthogonalize(g.to(DEV))
+    for z in (0, batch - 1):
+        want, model = steps64(g[z], 5, False), steps64(g[z], 5, True)
+        err = float((got[z].cpu().double() - want).norm())
+        assert err <= 1.5 * float((model - want).norm()) + (2.0 ** -8 / 2 + 1e-4) * float(want.norm()), (z, err)
+    _lib.check_device_error()
+
+
 def test_singular_values_gather_around_one():
     g = torch.Generator().manual_seed(9)
     got = orthogonalize(torch.randn(300, 900, generator=g).to(DEV)).double().cpu()
@@ -190,7 +214,7 @@ def test_same_bits_again_other_stream_and_captured():
 def test_no_write_outside_the_outputs():
     L_ = _lib.lib()
     st = torch.cuda.current_stream().cuda_stream
-    for batch, rows, cols in ((1, 130, 67), (3, 65, 300), (2, 257, 301)):
+    for batch, rows, cols in ((1, 130, 67), (3, 65, 300), (2, 257, 301), (2, 333, 140), (1, 500, 2011), (2, 900, 30), (20, 140, 150)):
         g = gradient(batch, rows, cols, F32, rows).to(DEV)
         sizes = {"out": batch * rows * cols * 2, "ws": int(L_.sru_b200_orthogonalize_workspace_bytes(batch, rows, cols))}
         bufs = {k: torch.full((n + 512,), 0xA5, dtype=torch.uint8, device=DEV) for k, n in sizes.items()}
