@@ -21,6 +21,7 @@
 #include <cmath>
 #include <cstring>
 
+#include "f32x2.cuh"
 #include "tcgen05.cuh"
 
 namespace srub {
@@ -843,6 +844,24 @@ template <typename T, int N> __device__ __forceinline__ void load_line(float (&v
     }
 }
 
+// The sum of eight squares in 64 bits.  The largest value's exponent scales them all into [2, 4) and below, where float32
+// holds the sum of their squares whatever the range of v (an infinity or a NaN stays one); one conversion to 64 bits for
+// eight values, which are slow (a 128 x 384 float32 norm took 6900 cycles of one SM with one per value).
+__device__ __forceinline__ double squares(const float (&v)[8]) {
+    float top = fabsf(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+    const int ex = min(max((int)(__float_as_uint(top) >> 23), 1), 254);
+    const float by = __uint_as_float((uint32_t)(255 - ex) << 23);        // 2^(128 - ex)
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float x = v[i] * by;
+        t = fmaf(x, x, t);
+    }
+    return (double)t * __hiloint2double((1023 + 2 * (ex - 128)) << 20, 0);
+}
+
 // Partial sums of squares in 64 bits (squares of the extremes of bf16 leave float32's range).  Units of 2048 elements of
 // a line along the contiguous direction, one warp each, in a fixed order.
 template <typename T> __global__ void __launch_bounds__(256) ns_norm_kernel(const NsEdge e) {
@@ -851,7 +870,7 @@ template <typename T> __global__ void __launch_bounds__(256) ns_norm_kernel(cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const T *g = static_cast<const T *>(e.src) + blockIdx.y * e.s_b;
     const int64_t per = (e.len + 2047) / 2048, units = e.lines * per;
-    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    double t = 0.0;
     for (int64_t u = (int64_t)blockIdx.x * 8 + warp; u < units; u += gridDim.x * 8) {
         const int64_t l = u / per, k0 = (u - l * per) * 2048 + lane * 8;
         const T *p = g + l * e.pitch;
@@ -860,11 +879,9 @@ template <typename T> __global__ void __launch_bounds__(256) ns_norm_kernel(cons
             if (k0 + k >= e.len) break;
             float v[8];
             load_line<T, 8>(v, p, k0 + k, e.len, e.wide);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i & 3] = fma((double)v[i], (double)v[i], sum[i & 3]);
+            t += squares(v);
         }
     }
-    double t = (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     if (lane == 0) s[warp] = t;
@@ -964,7 +981,7 @@ template <typename T> __global__ void __launch_bounds__(256) ns_last_kernel(cons
 // as 64-column tiles of 128 rows in the 128-byte swizzle, which the tensor cores read as the K-major operand of X X^T and as
 // the MN-major operand of M X alike, and one 128 x 128 matrix that holds A and then, in place, M.  Nothing leaves the SM
 // between load and store.  Bound by the latency of the chain (product, accumulator to registers, shared memory, next
-// product; 5 us a step at 128 x 384 and 37 in all, 92 in a cluster).
+// product; 4.5 us a step at 128 x 384 and 35 in all, 92 in a cluster).
 constexpr int kSmallM = 128, kSmallN = 768, kSmallThreads = 512;
 constexpr int kTileBytes = 128 * 64 * 2;
 
@@ -1004,7 +1021,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
         tmem_relinquish();
     }
     // the norm, in 64 bits and a fixed order
-    double sum[2] = {0.0, 0.0};
+    double t = 0.0;
     {
         constexpr int G = 4;            // groups of 8 elements requested together
         const int groups = (int)((e.len + 7) / 8), units = (int)e.lines * groups;
@@ -1017,11 +1034,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
             }
 #pragma unroll
             for (int k = 0; k < G; ++k)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum[i & 1] = fma((double)v[k][i], (double)v[k][i], sum[i & 1]);
+                t += squares(v[k]);
         }
     }
-    double t = sum[0] + sum[1];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     if (lane == 0) sums[warp] = t;
@@ -1032,16 +1047,23 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
     t = 0.0;
     for (int w = 0; w < kSmallThreads / 32; ++w) t += sums[w];
     const float scale = (float)(1.0 / (sqrt(t) + e.eps));
+    // groups of 8 columns, row by row: this thread's first one, and its next from the one before
+    const int first_row = (int)threadIdx.x / (tiles * 8), first_col = (int)threadIdx.x - first_row * tiles * 8;
+    const int step_rows = kSmallThreads / (tiles * 8), step_cols = kSmallThreads - step_rows * tiles * 8;
     if (e.s_j == 1) {
         constexpr int G = 4;
-        for (int u0 = threadIdx.x; u0 < kSmallM * tiles * 8; u0 += G * kSmallThreads) {      // a multiple of 2 * threads
+        // from the last row to the first: what the norm read last is still in L1
+        for (int i = kSmallM - 1 - first_row, c = first_col; i >= 0;) {
             float v[G][8];
             int at[G];
 #pragma unroll
             for (int k = 0; k < G; ++k) {
-                const int u = u0 + k * kSmallThreads, i = u / (tiles * 8), j = (u - i * tiles * 8) * 8;
-                at[k] = i < kSmallM ? (int)tile_at(i, j) : -1;
-                load_line<T, 8>(v[k], g + i * e.s_i, j, i < e.m ? e.n : 0, e.wide && i < e.m);
+                at[k] = i >= 0 ? (int)tile_at(i, c * 8) : -1;
+                const bool in = i >= 0 && i < e.m;
+                load_line<T, 8>(v[k], g + max(i, 0) * e.s_i, c * 8, in ? e.n : 0, e.wide && in);
+                i -= step_rows;
+                c += step_cols;
+                if (c >= tiles * 8) { c -= tiles * 8; --i; }
             }
 #pragma unroll
             for (int k = 0; k < G; ++k) {
@@ -1076,6 +1098,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
         ok = __syncthreads_and(here);
         tc_fence_after();
     };
+    const F2 cb2 = f2_make(a.cb, a.cb), cc2 = f2_make(a.cc, a.cc);
     const int k_m = (e.m + 15) / 16, k_n = (e.n + 15) / 16, groups = (tiles + 3) / 4;
     settle();
     for (int s = 0; s < a.steps && ok; ++s) {
@@ -1122,9 +1145,14 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
             const __half2 *a2 = reinterpret_cast<const __half2 *>(&w);
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float old = (j & 1) ? __high2float(a2[j >> 1]) : __low2float(a2[j >> 1]);
-                v[j] = fmaf(a.cc, __uint_as_float(r[j0 + j]), fmaf(a.cb, old, row == col + j ? a.ca : 0.0f));
+            for (int j = 0; j < 8; j += 2) {
+                const float2 old = __half22float2(a2[j >> 1]);
+                const F2 m = f2_fma(cc2, f2_make(__uint_as_float(r[j0 + j]), __uint_as_float(r[j0 + j + 1])), f2_mul(cb2, f2_make(old.x, old.y)));
+                f2_split(m, v[j], v[j + 1]);
+            }
+            if (part == q) {                        // the diagonal's block
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] += lane == j0 + j ? a.ca : 0.0f;
             }
             store_halves(at, v);
         }
@@ -1171,9 +1199,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
     __syncthreads();
     TO *out = static_cast<TO *>(e.dst) + blockIdx.x * a.o_b;
     if (a.o_j == 1) {
-        for (int u = threadIdx.x; u < e.m * tiles * 8; u += kSmallThreads) {
-            const int i = u / (tiles * 8), j = (u - i * tiles * 8) * 8;
-            if (j >= e.n) continue;
+#pragma unroll 4
+        for (int i = first_row, c = first_col; i < e.m;) {
+            const int j = c * 8;
             const uint4 w = shared_16(x + tile_at(i, j));
             const __half *h = reinterpret_cast<const __half *>(&w);
             Pack<TO, 8> o;
@@ -1185,6 +1213,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     if (j + k < e.n) p[k] = o.v[k];
+            i += step_rows;
+            c += step_cols;
+            if (c >= tiles * 8) { c -= tiles * 8; ++i; }
         }
     } else {
         for (int u = threadIdx.x; u < kSmallM * e.n; u += kSmallThreads) {
