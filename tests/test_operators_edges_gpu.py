@@ -226,3 +226,29 @@ def test_orthogonalize_repeated_rows():
     g = torch.randn(4, 60, 90, device=DEV)
     for v in (g[:1].expand(4, 60, 90), g[:, :1].expand(4, 60, 90), g[..., :1].expand(4, 60, 90), torch.randn(300, 1, device=DEV).expand(300, 200)):
         assert torch.equal(orthogonalize(v), orthogonalize(v.contiguous()))
+
+
+def test_orthogonalize_on_two_streams():
+    """Matrices in one SM, in clusters, split between clusters' pairs and with a launch per product, on two streams at once
+    and in one captured graph: the bits of calls of their own."""
+    g = torch.Generator().manual_seed(4)
+    sizes = [(1, 100, 300), (3, 200, 300), (1, 64, 4200), (2, 700, 900), (1, 500, 2000)]
+    mats = [torch.randn(*s, generator=g).to(DEV) for s in sizes]
+    want = [orthogonalize(m) for m in mats]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = []
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got += [orthogonalize(m) for m in (mats if k else mats[::-1])]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[::-1] + want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [orthogonalize(m) for m in mats]
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    _lib.check_device_error()
