@@ -493,8 +493,12 @@ __host__ __device__ inline int pairs_per_tile(int tiles, int pairs, int blocks) 
     return blocks - blocks / s < 10 ? 1 : s;
 }
 
+// M X on 256 columns a tile where pairs have more than one tile of 128: what L2 hands an SM then keeps the tensor cores busy (521
+// cycles a block for twice the columns instead of 440), but the epilogue is twice as long.  Six 512 x 2048 182 -> 166 us.
+__host__ __device__ inline bool wide_tiles(int narrow, int pairs, int blocks) { return blocks >= 6 && narrow > pairs; }
+
 struct ClusterShape {
-    static constexpr int kStageBytes = kABytes + 64 * kBK * 2, kStages = 6;
+    static constexpr int kStageBytes = kABytes + 128 * kBK * 2, kStages = 5;
     static constexpr int kOut = 32 * 64 * 2;                    // an epilogue warp's 32 rows and 64 columns; once more transposed
     static constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * 2 * kOut + 1024 + 1024;
     static_assert(kSmem <= 227 * 1024 && 7 * 128 * 16 * 4 <= kEpilogueWarps * 2 * kOut, "shared memory");
@@ -536,7 +540,7 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
             asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     __syncwarp();
     if (warp == 1) {
-        tmem_alloc2(smem_u32(tmem_slot), 256);
+        tmem_alloc2(smem_u32(tmem_slot), 512);
         tmem_relinquish2();
     }
     tc_fence_before();
@@ -559,7 +563,9 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
     for (int product = 0; product < 3 * g.steps; ++product) {
         const int kind = product % 3, cur = (product / 3) & 1;  // 0: A = X X^T, 1: M, 2: X = M X
         const int split = kind == 0 ? S : 1, mine = pair / split, part = pair % split;
-        const int units = kind == 2 ? rows * ((g.n + 127) / 128) : square;
+        const bool wide = kind == 2 && wide_tiles(rows * ((g.n + 127) / 128), pairs, nkb_m);
+        const int BN = wide ? 256 : 128;
+        const int units = kind == 2 ? rows * ((g.n + BN - 1) / BN) : square;
         const int nkb = kind == 0 ? nkb_n : nkb_m, kb0 = nkb * part / split, kb1 = nkb * (part + 1) / split;
         auto tile = [&](int unit, int *mb, int *nb) {
             if (kind == 2) {
@@ -579,21 +585,23 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
                 for (int unit = mine; unit < units && !dead; unit += pairs) {
                     int mb, nb;
                     tile(unit, &mb, &nb);
-                    const int m0 = mb * 256 + (int)side * 128, n0 = nb * 128 + (int)side * 64;
+                    const int m0 = mb * 256 + (int)side * 128, n0 = nb * BN + (int)side * (BN / 2);
                     for (int kb = kb0; kb < kb1; ++kb) {
                         if (!mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1)) { atomicExch(g.err, 36); dead = true; break; }
                         const uint32_t full = bar_full + 8 * stage, sa = smem_u32(smem + stage * P::kStageBytes);
-                        if (side == 0) mbar_arrive_expect_tx(full, 2 * P::kStageBytes);
+                        if (side == 0) mbar_arrive_expect_tx(full, 2 * (kABytes + BN / 2 * kBK * 2));
                         tma_load_3d_pair(sa, ma, full, kb * kBK, m0, z);
-                        if (kind == 2) tma_load_3d_pair(sa + kABytes, mbp, full, n0, kb * kBK, z);
-                        else tma_load_3d_pair(sa + kABytes, mbp, full, kb * kBK, n0, z);
+                        if (kind == 2) {
+                            tma_load_3d_pair(sa + kABytes, mbp, full, n0, kb * kBK, z);
+                            if (wide) tma_load_3d_pair(sa + kABytes + 8192, mbp, full, n0 + 64, kb * kBK, z);
+                        } else tma_load_3d_pair(sa + kABytes, mbp, full, kb * kBK, n0, z);
                         if (++stage == P::kStages) { stage = 0; phase ^= 1; }
                     }
                 }
             }
         } else if (warp == 1) {
             if (lane == 0 && side == 0) {
-                const uint32_t idesc = (1u << 4) | ((kind == 2 ? 1u : 0u) << 16) | ((128u >> 3) << 17) | ((256u >> 4) << 24);
+                const uint32_t idesc = (1u << 4) | ((kind == 2 ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((256u >> 4) << 24);
                 const uint32_t b_step = kind == 2 ? 2048u : 32u, b_lbo = kind == 2 ? 8192u : 16u;
                 for (int unit = mine; unit < units && !dead; unit += pairs, ++it) {
                     const int acc = it & 1;
@@ -605,7 +613,7 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
                         const uint32_t sa = smem_u32(smem + stage * P::kStageBytes), sb = sa + kABytes;
 #pragma unroll
                         for (int k16 = 0; k16 < kBK / 16; ++k16)
-                            tc_mma_pair(tmem_base + acc * 128, make_desc(sa + k16 * 32, 16, 1024),
+                            tc_mma_pair(tmem_base + acc * 256, make_desc(sa + k16 * 32, 16, 1024),
                                         make_desc(sb + k16 * b_step, b_lbo, 1024), idesc, (kb > kb0 || k16) ? 1u : 0u);
                         tc_commit_pair(bar_empty + 8 * stage, both);
                         if (++stage == P::kStages) { stage = 0; phase ^= 1; }
@@ -622,14 +630,14 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
             for (int unit = mine; unit < units; unit += pairs, ++it) {
                 int mb, nb;
                 tile(unit, &mb, &nb);
-                const int acc = it & 1, row0 = mb * 256 + (int)side * 128 + q * 32, row = row0 + lane, first = nb * 128 + half * 64;
+                const int acc = it & 1, row0 = mb * 256 + (int)side * 128 + q * 32, row = row0 + lane;
                 const bool turn = last && g.turned, across = turn || (kind < 2 && mb < nb / 2);
                 const int64_t ld_across = turn ? g.m : ld;
                 if (kind == 1) {
                     if (lane == 0) {
                         if (unit != mine) fence_proxy_async();      // the staging was read with plain loads
                         mbar_arrive_expect_tx(bar_mine, P::kOut);
-                        tma_load_3d(out, &map_ac, bar_mine, first, row0, z);
+                        tma_load_3d(out, &map_ac, bar_mine, nb * 128 + half * 64, row0, z);
                     }
                     __syncwarp();
                 }
@@ -643,85 +651,90 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
                     if (lane == 0) atomicExch(g.err, 39);
                 }
                 tc_fence_after();
-                uint32_t both_r[2][32];
-                tmem_ld32(tmem_rows + acc * 128 + half * 64, both_r[0]);
-                tmem_ld32(tmem_rows + acc * 128 + half * 64 + 32, both_r[1]);
-                tmem_ld_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster_relaxed(tempty_leader + 8 * acc);
-#pragma unroll
-                for (int cc = 0; cc < 2; ++cc) {
-                    const int col0 = first + cc * 32;
-                    const uint32_t (&r)[32] = both_r[cc];
-#pragma unroll
-                    for (int j0 = 0; j0 < 32; j0 += 8) {
-                        const uint32_t at = out + lane * 128 + (((cc * 4 + j0 / 8) ^ (lane & 7)) << 4);
-                        float v[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[j0 + j]);
-                        if (kind == 1) {
-                            const uint4 d = shared_16(at);
-                            const __half2 *a2 = reinterpret_cast<const __half2 *>(&d);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const float a = (j & 1) ? __high2float(a2[j >> 1]) : __low2float(a2[j >> 1]);
-                                v[j] = fmaf(g.cc, v[j], fmaf(g.cb, a, row == col0 + j0 + j ? g.ca : 0.0f));
-                            }
-                        }
-                        uint32_t w[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if (last && g.bf16) {
-                                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-                                w[j] = *reinterpret_cast<const uint32_t *>(&h);
-                            } else {
-                                const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-                                w[j] = *reinterpret_cast<const uint32_t *>(&h);
-                            }
-                        }
-                        if (!turn) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-                        if (across) {                       // element (row, col) at [col][row]
-#pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                asm volatile("st.shared.u16 [%0], %1;" ::"r"(turned + (cc * 32 + j0 + j) * 64 + lane * 2),
-                                             "h"((unsigned short)(w[j >> 1] >> (16 * (j & 1)))) : "memory");
-                        }
+                for (int c64 = 0; c64 < BN / 2; c64 += 64) {
+                    const int first = nb * BN + half * (BN / 2) + c64;
+                    uint32_t both_r[2][32];
+                    tmem_ld32(tmem_rows + acc * 256 + half * (BN / 2) + c64, both_r[0]);
+                    tmem_ld32(tmem_rows + acc * 256 + half * (BN / 2) + c64 + 32, both_r[1]);
+                    tmem_ld_wait();
+                    if (c64 + 64 == BN / 2) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster_relaxed(tempty_leader + 8 * acc);
                     }
-                }
-                __syncwarp();
-                if (!turn) {
-                    uint4 w[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {           // 4 rows of 128 bytes
-                        const int rr = i * 4 + (lane >> 3);
-                        w[i] = shared_16(out + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-                    }
-                    const int rr = lane >> 3, col = first + (lane & 7) * 8;
-                    __half *to = dst + (row0 + rr) * ld + col;
+                    for (int cc = 0; cc < 2; ++cc) {
+                        const int col0 = first + cc * 32;
+                        const uint32_t (&r)[32] = both_r[cc];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i, to += 4 * ld)
-                        if (row0 + rr + i * 4 < g.m && col < N) *reinterpret_cast<uint4 *>(to) = w[i];
-                }
-                if (across) {
+                        for (int j0 = 0; j0 < 32; j0 += 8) {
+                            const uint32_t at = out + lane * 128 + (((cc * 4 + j0 / 8) ^ (lane & 7)) << 4);
+                            float v[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {           // 8 rows of 64 bytes
-                        const int rr = i * 8 + (lane >> 2), col = row0 + (lane & 3) * 8;
-                        const uint4 w = shared_16(turned + rr * 64 + (lane & 3) * 16);
-                        if (first + rr < N && col < g.m) {
-                            __half *to = dst + (first + rr) * ld_across + col;
-                            if (!turn || g.turned_wide) {
-                                *reinterpret_cast<uint4 *>(to) = w;
-                            } else {
-                                const __half *e = reinterpret_cast<const __half *>(&w);
+                            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[j0 + j]);
+                            if (kind == 1) {
+                                const uint4 d = shared_16(at);
+                                const __half2 *a2 = reinterpret_cast<const __half2 *>(&d);
 #pragma unroll
-                                for (int k = 0; k < 8; ++k)
-                                    if (col + k < g.m) to[k] = e[k];
+                                for (int j = 0; j < 8; ++j) {
+                                    const float a = (j & 1) ? __high2float(a2[j >> 1]) : __low2float(a2[j >> 1]);
+                                    v[j] = fmaf(g.cc, v[j], fmaf(g.cb, a, row == col0 + j0 + j ? g.ca : 0.0f));
+                                }
+                            }
+                            uint32_t w[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                if (last && g.bf16) {
+                                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+                                    w[j] = *reinterpret_cast<const uint32_t *>(&h);
+                                } else {
+                                    const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+                                    w[j] = *reinterpret_cast<const uint32_t *>(&h);
+                                }
+                            }
+                            if (!turn) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                            if (across) {                       // element (row, col) at [col][row]
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+                                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(turned + (cc * 32 + j0 + j) * 64 + lane * 2),
+                                                 "h"((unsigned short)(w[j >> 1] >> (16 * (j & 1)))) : "memory");
                             }
                         }
                     }
+                    __syncwarp();
+                    if (!turn) {
+                        uint4 w[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {           // 4 rows of 128 bytes
+                            const int rr = i * 4 + (lane >> 3);
+                            w[i] = shared_16(out + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+                        }
+                        const int rr = lane >> 3, col = first + (lane & 7) * 8;
+                        __half *to = dst + (row0 + rr) * ld + col;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i, to += 4 * ld)
+                            if (row0 + rr + i * 4 < g.m && col < N) *reinterpret_cast<uint4 *>(to) = w[i];
+                    }
+                    if (across) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {           // 8 rows of 64 bytes
+                            const int rr = i * 8 + (lane >> 2), col = row0 + (lane & 3) * 8;
+                            const uint4 w = shared_16(turned + rr * 64 + (lane & 3) * 16);
+                            if (first + rr < N && col < g.m) {
+                                __half *to = dst + (first + rr) * ld_across + col;
+                                if (!turn || g.turned_wide) {
+                                    *reinterpret_cast<uint4 *>(to) = w;
+                                } else {
+                                    const __half *e = reinterpret_cast<const __half *>(&w);
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k)
+                                        if (col + k < g.m) to[k] = e[k];
+                                }
+                            }
+                        }
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
         }
         if (split > 1) {
@@ -745,7 +758,7 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
                     const int to = c0 / E, slot = part < to ? part : part - 1;
                     if (to == part) continue;
                     uint32_t r[16];
-                    tmem_ld16(tmem_rows + acc * 128 + c0, r);
+                    tmem_ld16(tmem_rows + acc * 256 + c0, r);
                     tmem_ld_wait();
                     const uint32_t at = map_to_cta(sums + ((slot * (E / 4) + c0 % E / 4) * 128 + row) * 16, 2 * (mine * split + to) + side);
 #pragma unroll
@@ -760,7 +773,7 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
 #pragma unroll 1
                 for (int e0 = half * 16; e0 < E; e0 += 32) {
                     uint32_t r[16];
-                    tmem_ld16(tmem_rows + acc * 128 + part * E + e0, r);
+                    tmem_ld16(tmem_rows + acc * 256 + part * E + e0, r);
                     tmem_ld_wait();
                     float v[16];
 #pragma unroll
@@ -813,7 +826,7 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
     cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc2(tmem_base, 256);
+        tmem_dealloc2(tmem_base, 512);
     }
 }
 
@@ -1372,22 +1385,6 @@ int ns_cluster(const NsMaps &x0, const NsMaps &x1, const NsMaps &a, const NsMaps
     return 0;
 }
 
-// CTAs of a cluster that takes a matrix through all its steps, or 0: a launch per product.  A cluster where a pair's share of a
-// step is at most 34 blocks (of 64 of a tile's reduction, 0.23 us each; a tile's epilogue takes as long as six, the exchange
-// between pairs as eight), and the GPU holds clusters for the batch (7 of 16 CTAs, 15 of 8).  With launches / in a cluster:
-// 130 x 200 (18 blocks) 124 / 84 us, 256 x 512 (20) 117 / 84, 500 x 500 (24) 134 / 119, seven 256 x 1024 (26) 111 / 96, twelve 128 x
-// 1000 106 / 96, 400 x 700 (32) 120 / 118, 384 x 1024 (34) 115 / 117, two 512 x 1024 (40) 125 / 128, 700 x 700 (77) 135 / 180.
-int choose_cluster(int64_t m, int64_t n, int64_t batch) {
-    const int64_t ctas = batch <= 7 ? 16 : 8, pairs = ctas / 2, rows = (m + 255) / 256, square = rows * ((m + 127) / 128 - rows + 1);
-    if (batch > 15) return 0;
-    const int split = pairs_per_tile((int)square, (int)pairs, (int)((n + kBK - 1) / kBK));
-    auto tiles = [&](int64_t count, int64_t blocks) { return (count + pairs - 1) / pairs * std::max<int64_t>(blocks, 6); };
-    const int64_t blocks_m = (m + kBK - 1) / kBK, blocks_n = (n + kBK - 1) / kBK;
-    const int64_t share = tiles(square * split, blocks_n / split) + (split > 1 ? 8 : 0) + tiles(square, blocks_m) +
-                          tiles(rows * ((n + 127) / 128), blocks_m);
-    return share <= 34 ? (int)ctas : 0;
-}
-
 // Pairs that share a tile of X X^T, by the number of tiles and the 64-element blocks of the reduction: as many as the GPU holds
 // clusters for (7, 15 and 33 of 16, 8 and 4 CTAs) while the exchange (1 us) is shorter than what it saves.  Five steps with 1 /
 // 2 / 4 / 8 pairs: 64 x 6144 194 / 142 / 118 / 104 us, 64 x 4000 154 / 132 / 124 / 124, 512 x 6144 235 / 181 / 154 / 143; with 1 / 2 /
@@ -1398,6 +1395,30 @@ int choose_split(int64_t tiles, int64_t blocks) {
     if (tiles <= 15 && blocks >= 8) return 4;
     if (tiles <= 33 && blocks >= 8) return 2;
     return 1;
+}
+
+// CTAs of a cluster that takes a matrix through all its steps, or 0: a launch per product.  Both are counted in blocks (64 of the
+// reduction of a 256 x 128 tile, 0.23 us) that a pair of SMs works through in a step; a tile's epilogue takes as long as six, a
+// wide one's twelve, an exchange between pairs eight.  A cluster where it has at most four more, which its cheaper change from
+// product to product makes up for, and the GPU holds clusters for the batch (7 of 16 CTAs, 15 of 8).  Launches / cluster, us, and
+// what the cluster has more: 500 x 500 132 / 118 (-10), 130 x 200 96 / 81 (-6), 256 x 1024 101 / 91 (0), six 512 x 2048 179 / 166 (0),
+// seven 512 x 1536 169 / 155 (0), fifteen 384 x 384 118 / 106 (0), 384 x 1024 115 / 117 (2), seven 300 x 1500 139 / 135 (6), five 512 x
+// 2048 157 / 161 (8), three 300 x 1500 119 / 129 (12), ten 512 x 512 133 / 136 (16), six 600 x 600 146 / 180 (32).
+int choose_cluster(int64_t m, int64_t n, int64_t batch, int sms) {
+    if (batch > 15) return 0;
+    const int64_t ctas = batch <= 7 ? 16 : 8, pairs = ctas / 2, rows = (m + 255) / 256, square = rows * ((m + 127) / 128 - rows + 1);
+    const int64_t blocks_m = (m + kBK - 1) / kBK, blocks_n = (n + kBK - 1) / kBK;
+    const int64_t narrow = rows * ((n + 127) / 128), wide = rows * ((n + 255) / 256), wide_cost = std::max<int64_t>(blocks_m * 6 / 5, 12);
+    auto tiles = [](int64_t count, int64_t pairs, int64_t cost) { return (count + pairs - 1) / pairs * cost; };
+    auto gram = [&](int64_t count, int64_t pairs, int split) {
+        return tiles(count * split, pairs, std::max<int64_t>(blocks_n / split, 6)) + (split > 1 ? 8 : 0) +
+               tiles(count, pairs, std::max<int64_t>(blocks_m, 6));
+    };
+    const int64_t here = gram(square, pairs, pairs_per_tile((int)square, (int)pairs, (int)blocks_n)) +
+                         (wide_tiles((int)narrow, (int)pairs, (int)blocks_m) ? tiles(wide, pairs, wide_cost)
+                                                                             : tiles(narrow, pairs, std::max<int64_t>(blocks_m, 6)));
+    const int64_t launches = gram(square * batch, sms / 2, choose_split(square * batch, blocks_n)) + tiles(wide * batch, sms / 2, wide_cost);
+    return here <= launches + 4 ? (int)ctas : 0;
 }
 
 // X X^T and A A.  A 256 x 128 tile takes a pair of SMs about as long as one of 256 x 256 (0.28 us per 64 of the reduction: its
@@ -1521,7 +1542,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     if (int rc = grad_dtype == SRU_F32 ? begin(float()) : grad_dtype == SRU_F16 ? begin(__half()) : begin(__nv_bfloat16())) return rc;
 
     // The last product writes the caller's matrix itself where its rows are 16-byte aligned (a cluster's turned one, always).
-    const int ctas = steps > 0 ? choose_cluster(p.m, p.n, batch) : 0;
+    const int ctas = steps > 0 ? choose_cluster(p.m, p.n, batch, sms) : 0;
     const bool aligned = steps > 0 && cols % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0, direct = aligned || (ctas && tall);
     NsMaps xm[2], am, mm, om;
     if (aligned)

@@ -98,7 +98,7 @@ def test_both_tile_widths(batch, rows, cols):
 
 @pytest.mark.parametrize("batch,rows,cols", [(1, 130, 200), (7, 201, 333), (8, 140, 260), (15, 200, 136), (16, 130, 200),
                                              (1, 130, 1700), (1, 1700, 129), (2, 60, 1000), (9, 1000, 100), (1, 385, 390),
-                                             (3, 500, 505), (1, 384, 1024), (1, 384, 1100)])
+                                             (3, 500, 505), (1, 384, 1024), (1, 384, 1100), (7, 400, 1300), (6, 1101, 450)])
 def test_where_one_cluster_takes_the_matrix(batch, rows, cols):
     """Both sides of the sizes and batches at which a cluster takes a matrix through all steps; with and without several
     pairs to a tile, wide and tall, rows of the result aligned and not."""
