@@ -229,6 +229,14 @@ embedding_sort_kernel(const EmbArgs a) {
 // that occur twice and leave L2 full of lines that the sums then have to push out: 133 and 121 us for 16384 tokens over
 // 50000 x 2048 floats.)
 constexpr int kFillRows = 64;
+__device__ __forceinline__ void fill_row(const EmbArgs &a, int64_t row, int64_t row_bytes, int lane) {
+    char *p = static_cast<char *>(a.dst) + row * row_bytes;
+    if (a.fill16) {
+        for (int64_t c = lane * 16; c < row_bytes; c += 512) __stcs(reinterpret_cast<uint4 *>(p + c), make_uint4(0, 0, 0, 0));
+    } else {
+        for (int64_t c = lane * 2; c < row_bytes; c += 64) *reinterpret_cast<uint16_t *>(p + c) = 0;
+    }
+}
 __device__ __forceinline__ void fill_absent(const EmbArgs &a, int64_t block) {
     __shared__ bool present[kFillRows];
     const int64_t r0 = block * kFillRows;
@@ -247,13 +255,7 @@ __device__ __forceinline__ void fill_absent(const EmbArgs &a, int64_t block) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t row_bytes = (int64_t)a.d * a.dst_size;
     for (int k = warp; k < rows; k += blockDim.x >> 5) {
-        if (present[k]) continue;
-        char *p = static_cast<char *>(a.dst) + (r0 + k) * row_bytes;
-        if (a.fill16) {
-            for (int64_t c = lane * 16; c < row_bytes; c += 512) __stcs(reinterpret_cast<uint4 *>(p + c), make_uint4(0, 0, 0, 0));
-        } else {
-            for (int64_t c = lane * 2; c < row_bytes; c += 64) *reinterpret_cast<uint16_t *>(p + c) = 0;
-        }
+        if (!present[k]) fill_row(a, r0 + k, row_bytes, lane);
     }
 }
 
@@ -272,6 +274,63 @@ __device__ __forceinline__ void store_sum(TO *row, int c0, int d, const float (&
     }
 }
 
+// Unit w: a tile of positions, a block of columns.  (Sorted positions past L1: the kernel that sorted them may be this one.)
+template <typename TI, typename TO, int VEC, int REP>
+__device__ __forceinline__ void sum_unit(const EmbArgs &a, int64_t w, int blocks_per_row) {
+    const int lane = threadIdx.x & 31;
+    const int64_t tile = w / blocks_per_row, i0 = tile * kTile;
+    const int c0 = (int)(w - tile * blocks_per_row) * (32 * VEC * REP) + lane * VEC;
+    const uint32_t none = (uint32_t)a.v;                // key of positions that add nothing
+    const uint2 mine = (i0 + lane < a.n) ? __ldcg(a.sorted + i0 + lane) : make_uint2(none, 0u);
+    const uint32_t before = i0 > 0 ? __ldcg(&a.sorted[i0 - 1].x) : none;
+    const uint32_t after = i0 + kTile < a.n ? __ldcg(&a.sorted[i0 + kTile].x) : none;
+    // sorted: the positions that count come first, and a bit says where a run ends (the tile's end ends them all)
+    const int count = __popc(__ballot_sync(0xffffffffu, mine.x != none));
+    const uint32_t next_key = __shfl_down_sync(0xffffffffu, mine.x, 1);
+    const unsigned ends = __ballot_sync(0xffffffffu, lane == kTile - 1 || next_key != mine.x);
+    const TI *src = static_cast<const TI *>(a.src) + c0;
+    float acc[REP][VEC];
+#pragma unroll
+    for (int r = 0; r < REP; ++r)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[r][k] = 0.0f;
+    bool whole_head = true;                             // the current run reaches back to the tile's first entry
+    constexpr int G = 8;                                // rows requested together
+    for (int e0 = 0; e0 < count; e0 += G) {
+        Pack<TI, VEC> in[G][REP];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const TI *row = src + (int64_t)__shfl_sync(0xffffffffu, mine.y, e0 + g) * a.d;
+#pragma unroll
+            for (int r = 0; r < REP; ++r) {
+                if (e0 + g < count && c0 + r * 32 * VEC < a.d) in[g][r] = *reinterpret_cast<const Pack<TI, VEC> *>(row + r * 32 * VEC);
+                else memset(&in[g][r], 0, sizeof(in[g][r]));
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int e = e0 + g;
+#pragma unroll
+            for (int r = 0; r < REP; ++r)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) acc[r][k] += Cvt<TI>::to_f(in[g][r].v[k]);
+            if (!((ends >> e) & 1u) || e >= count) continue;
+            const uint32_t key = __shfl_sync(0xffffffffu, mine.x, e);
+            if (whole_head && key == before)
+                store_sum<float, VEC, REP>(a.part + (tile * 2) * a.d, c0, a.d, acc, 1.0f);
+            else if (e == kTile - 1 && after == key)
+                store_sum<float, VEC, REP>(a.part + (tile * 2 + 1) * a.d, c0, a.d, acc, 1.0f);
+            else
+                store_sum<TO, VEC, REP>(static_cast<TO *>(a.dst) + (int64_t)key * a.d, c0, a.d, acc, a.scale);
+#pragma unroll
+            for (int r = 0; r < REP; ++r)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) acc[r][k] = 0.0f;
+            whole_head = false;
+        }
+    }
+}
+
 // The grid's first CTAs fill the rows of absent tokens: they search, then write, while the others wait for their rows.
 template <typename TI, typename TO, int VEC, int REP>
 __global__ void __launch_bounds__(128) embedding_sum_kernel(const EmbArgs a, int blocks_per_row, unsigned fill_ctas) {
@@ -281,61 +340,40 @@ __global__ void __launch_bounds__(128) embedding_sum_kernel(const EmbArgs a, int
         fill_absent(a, blockIdx.x);
         return;
     }
-    const int lane = threadIdx.x & 31;
     const int64_t tiles = (a.n + kTile - 1) / kTile, units = tiles * blocks_per_row, step = (int64_t)(gridDim.x - fill_ctas) * 4;
-    for (int64_t w = (int64_t)(blockIdx.x - fill_ctas) * 4 + (threadIdx.x >> 5); w < units; w += step) {
-        const int64_t tile = w / blocks_per_row, i0 = tile * kTile;
-        const int c0 = (int)(w - tile * blocks_per_row) * (32 * VEC * REP) + lane * VEC;
-        const uint32_t none = (uint32_t)a.v;                // key of positions that add nothing
-        const uint2 mine = (i0 + lane < a.n) ? a.sorted[i0 + lane] : make_uint2(none, 0u);
-        const uint32_t before = i0 > 0 ? a.sorted[i0 - 1].x : none;
-        const uint32_t after = i0 + kTile < a.n ? a.sorted[i0 + kTile].x : none;
-        // sorted: the positions that count come first, and a bit says where a run ends (the tile's end ends them all)
-        const int count = __popc(__ballot_sync(0xffffffffu, mine.x != none));
-        const uint32_t next_key = __shfl_down_sync(0xffffffffu, mine.x, 1);
-        const unsigned ends = __ballot_sync(0xffffffffu, lane == kTile - 1 || next_key != mine.x);
-        const TI *src = static_cast<const TI *>(a.src) + c0;
-        float acc[REP][VEC];
-#pragma unroll
-        for (int r = 0; r < REP; ++r)
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[r][k] = 0.0f;
-        bool whole_head = true;                             // the current run reaches back to the tile's first entry
-        constexpr int G = 8;                                // rows requested together
-        for (int e0 = 0; e0 < count; e0 += G) {
-            Pack<TI, VEC> in[G][REP];
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const TI *row = src + (int64_t)__shfl_sync(0xffffffffu, mine.y, e0 + g) * a.d;
-#pragma unroll
-                for (int r = 0; r < REP; ++r) {
-                    if (e0 + g < count && c0 + r * 32 * VEC < a.d) in[g][r] = *reinterpret_cast<const Pack<TI, VEC> *>(row + r * 32 * VEC);
-                    else memset(&in[g][r], 0, sizeof(in[g][r]));
-                }
-            }
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const int e = e0 + g;
-#pragma unroll
-                for (int r = 0; r < REP; ++r)
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) acc[r][k] += Cvt<TI>::to_f(in[g][r].v[k]);
-                if (!((ends >> e) & 1u) || e >= count) continue;
-                const uint32_t key = __shfl_sync(0xffffffffu, mine.x, e);
-                if (whole_head && key == before)
-                    store_sum<float, VEC, REP>(a.part + (tile * 2) * a.d, c0, a.d, acc, 1.0f);
-                else if (e == kTile - 1 && after == key)
-                    store_sum<float, VEC, REP>(a.part + (tile * 2 + 1) * a.d, c0, a.d, acc, 1.0f);
-                else
-                    store_sum<TO, VEC, REP>(static_cast<TO *>(a.dst) + (int64_t)key * a.d, c0, a.d, acc, a.scale);
-#pragma unroll
-                for (int r = 0; r < REP; ++r)
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) acc[r][k] = 0.0f;
-                whole_head = false;
-            }
+    for (int64_t w = (int64_t)(blockIdx.x - fill_ctas) * 4 + (threadIdx.x >> 5); w < units; w += step) sum_unit<TI, TO, VEC, REP>(a, w, blocks_per_row);
+}
+
+// Key of the run that starts in this tile and goes on behind it; v: there is none.
+__device__ __forceinline__ uint32_t run_from(const EmbArgs &a, int64_t tile) {
+    const int64_t i0 = tile * kTile, i1 = i0 + kTile;
+    const uint32_t none = (uint32_t)a.v;
+    if (i1 >= a.n) return none;
+    const uint32_t key = __ldcg(&a.sorted[i1 - 1].x), next = __ldcg(&a.sorted[i1].x), first = __ldcg(&a.sorted[i0].x);
+    const uint32_t before = i0 > 0 ? __ldcg(&a.sorted[i0 - 1].x) : none;
+    return next != key || (first == key && before == key) ? none : key;
+}
+// The first tile behind `tile` that its last run does not reach; by a whole warp.
+__device__ __forceinline__ int64_t run_end(const EmbArgs &a, int64_t tile, uint32_t key) {
+    const int lane = threadIdx.x & 31;
+    const int64_t tiles = (a.n + kTile - 1) / kTile;
+    // tiles that the run reaches behind this one: the first 32, then by bisection in 32 parts
+    int64_t lo = tile + 1, hi = tiles;          // the run covers the start of every tile below lo, of none from hi on
+    const unsigned m = __ballot_sync(0xffffffffu, lo + lane < hi && __ldcg(&a.sorted[(lo + lane) * kTile].x) == key);
+    if (m != 0xffffffffu) {
+        lo += __ffs(~m) - 1;
+    } else {
+        for (lo += 32; lo < hi;) {
+            const int64_t step = (hi - lo + 31) / 32, u = lo + lane * step;
+            const unsigned c = __ballot_sync(0xffffffffu, u < hi && __ldcg(&a.sorted[u * kTile].x) == key);
+            const int covered = c == 0xffffffffu ? 32 : __ffs(~c) - 1;
+            if (covered == 0) break;
+            const int64_t last = lo + (covered - 1) * step;     // the last probed tile inside the run
+            hi = min(hi, last + step);
+            lo = last + 1;
         }
     }
+    return lo;
 }
 
 // Runs that cross tiles: of the tile in which the run starts, a CTA per block of columns adds the tiles' partial rows, the
@@ -344,28 +382,11 @@ template <typename TO, int VEC, int REP>
 __global__ void __launch_bounds__(128) embedding_join_kernel(const EmbArgs a) {
     __shared__ float parts[3][32 * VEC * REP];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t tiles = (a.n + kTile - 1) / kTile, tile = blockIdx.x, i0 = tile * kTile, i1 = i0 + kTile;
+    const int64_t tile = blockIdx.x;
     previous_kernel_done();
-    if (i1 >= a.n) return;
-    const uint32_t key = a.sorted[i1 - 1].x, next = a.sorted[i1].x, first = a.sorted[i0].x;
-    const uint32_t before = i0 > 0 ? a.sorted[i0 - 1].x : (uint32_t)a.v;
-    if (key == (uint32_t)a.v || next != key || (first == key && before == key)) return;     // no run starts here and goes on
-    // tiles that the run reaches behind this one: the first 32, then by bisection in 32 parts
-    int64_t lo = tile + 1, hi = tiles;          // the run covers the start of every tile below lo, of none from hi on
-    const unsigned m = __ballot_sync(0xffffffffu, lo + lane < hi && a.sorted[(lo + lane) * kTile].x == key);
-    if (m != 0xffffffffu) {
-        lo += __ffs(~m) - 1;
-    } else {
-        for (lo += 32; lo < hi;) {
-            const int64_t step = (hi - lo + 31) / 32, u = lo + lane * step;
-            const unsigned c = __ballot_sync(0xffffffffu, u < hi && a.sorted[u * kTile].x == key);
-            const int covered = c == 0xffffffffu ? 32 : __ffs(~c) - 1;
-            if (covered == 0) break;
-            const int64_t last = lo + (covered - 1) * step;     // the last probed tile inside the run
-            hi = min(hi, last + step);
-            lo = last + 1;
-        }
-    }
+    const uint32_t key = run_from(a, tile);
+    if (key == (uint32_t)a.v) return;
+    const int64_t lo = run_end(a, tile, key);
     const int64_t count = lo - (tile + 1), per = (count + 3) / 4, q0 = min(count, warp * per), q1 = min(count, q0 + per);
     const int c0 = blockIdx.y * (32 * VEC * REP) + lane * VEC;
     float acc[REP][VEC];
@@ -406,6 +427,56 @@ __global__ void __launch_bounds__(128) embedding_join_kernel(const EmbArgs a) {
 #pragma unroll
             for (int k = 0; k < VEC; ++k) acc[r][k] += parts[w][(r * 32 + lane) * VEC + k];
     store_sum<TO, VEC, REP>(static_cast<TO *>(a.dst) + (int64_t)key * a.d, c0, a.d, acc, a.scale);
+}
+
+// A small gradient in one launch: the cluster that sorts also sums, fills the absent rows and joins the runs, a warp for each of
+// their units.
+template <typename TK, typename TI, typename TO, int VEC, int REP>
+__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortWarps * 32)
+embedding_small_kernel(const EmbArgs a, int blocks_per_row) {
+    __shared__ SortShared sh;
+    sort_tokens<TK>(a, sh);
+    const int lane = threadIdx.x & 31;
+    const int64_t me = (int64_t)cluster_rank() * kSortWarps + (threadIdx.x >> 5), warps = kSortCtas * kSortWarps;
+    const int64_t tiles = (a.n + kTile - 1) / kTile, units = tiles * blocks_per_row, row_bytes = (int64_t)a.d * a.dst_size;
+    for (int64_t w = me; w < units; w += warps) sum_unit<TI, TO, VEC, REP>(a, w, blocks_per_row);
+    for (int64_t r0 = (warps - 1 - me) * 32; r0 < a.v; r0 += warps * 32) {     // from the other end: the last warps have fewer units
+        const int64_t row = r0 + lane;
+        int64_t lo = 0, hi = a.n;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi) >> 1;
+            if (__ldcg(&a.sorted[mid].x) < (uint32_t)row) lo = mid + 1;
+            else hi = mid;
+        }
+        const bool here = lo < a.n && __ldcg(&a.sorted[lo].x) == (uint32_t)row;
+        for (unsigned absent = __ballot_sync(0xffffffffu, row < a.v && !here); absent; absent &= absent - 1)
+            fill_row(a, r0 + __ffs(absent) - 1, row_bytes, lane);
+    }
+    __threadfence();
+    cluster_barrier();
+    for (int64_t w = me; w < units; w += warps) {
+        const int64_t tile = w / blocks_per_row;
+        const uint32_t key = run_from(a, tile);
+        if (key == (uint32_t)a.v) continue;
+        const int c0 = (int)(w - tile * blocks_per_row) * (32 * VEC * REP) + lane * VEC;
+        const int64_t end = run_end(a, tile, key);
+        float acc[REP][VEC];
+#pragma unroll
+        for (int r = 0; r < REP; ++r)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc[r][k] = 0.0f;
+        for (int64_t q = tile; q < end; ++q) {
+            const float *row = a.part + (q == tile ? q * 2 + 1 : q * 2) * a.d;
+#pragma unroll
+            for (int r = 0; r < REP; ++r) {
+                const int c = c0 + r * 32 * VEC;
+                if (c >= a.d) continue;
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) acc[r][k] += __ldcg(row + c + k);
+            }
+        }
+        store_sum<TO, VEC, REP>(static_cast<TO *>(a.dst) + (int64_t)key * a.d, c0, a.d, acc, a.scale);
+    }
 }
 
 int check_embedding(int64_t n, int64_t v, int64_t d, int64_t ld, int token_bytes, int table_dtype, int y_dtype) {
@@ -453,13 +524,32 @@ template <typename TK> int launch_sort(const EmbArgs &a, cudaStream_t st) {
     return 0;
 }
 
-template <typename TI, typename TO> int launch_sums(const EmbArgs &a, cudaStream_t st) {
+// One launch for a gradient of at most 1 MB, which sixteen SMs move about as fast as all: three launches / one, us with the host's
+// share and of the GPU alone: 64 tokens over 100 x 64 20 / 12 and 8.8 / 9.3, 500 over 200 x 64 (0.2 MB) 20 / 12 and 11.0 / 11.3, 500
+// over 1000 x 256 (1.5 MB) 19 / 19 and 14.6 / 17.7, 4000 over 4000 x 256 (8 MB) 19 / 25 and 16.5 / 22.2.
+bool is_small(const EmbArgs &a, int64_t src_size) { return (a.n * src_size + a.v * a.dst_size) * a.d <= (1 << 20); }
+
+template <typename TK, typename TI, typename TO> int launch_backward(const EmbArgs &a, cudaStream_t st) {
     constexpr int VEC = 16 / sizeof(TI);
     const bool wide = aligned16(a.src, a.d * sizeof(TI)) && aligned16(a.dst, a.d * sizeof(TO));
     auto go = [&](auto vec, auto rep) -> int {
         constexpr int V = decltype(vec)::value, R = decltype(rep)::value;
         const int per_row = (a.d + 32 * V * R - 1) / (32 * V * R);
         if (per_row > 65535) return set_error(SRU_ERR_UNSUPPORTED, "embedding: hidden too large");
+        if (is_small(a, sizeof(TI))) {
+            auto kernel = embedding_small_kernel<TK, TI, TO, V, R>;
+            static bool attr_set[64] = {false};
+            int dev = 0;
+            SRUB_CUDA_CHECK(cudaGetDevice(&dev));
+            if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+                SRUB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+                attr_set[dev] = true;
+            }
+            kernel<<<kSortCtas, kSortWarps * 32, 0, st>>>(a, per_row);
+            SRUB_CUDA_CHECK(cudaGetLastError());
+            return 0;
+        }
+        if (int rc = launch_sort<TK>(a, st)) return rc;
         const int64_t units = (a.n + kTile - 1) / kTile * per_row;
         const int64_t sums = std::min<int64_t>((units + 3) / 4, 148 * 64), fill = (a.v + kFillRows - 1) / kFillRows;
         cudaLaunchConfig_t cfg;
@@ -547,14 +637,15 @@ int sru_b200_embedding_backward(void *grad_table, const void *tokens, const void
     if (!a.err) return set_error(SRU_ERR_CUDA, "device error flag unavailable");
     a.dst_size = (int)dtype_size(table_dtype);
     a.fill16 = aligned16(grad_table, hidden * a.dst_size);
-    if (token_bytes == 4) rc = launch_sort<int32_t>(a, st);
-    else rc = launch_sort<int64_t>(a, st);
-    if (rc) return rc;
-    if (table_dtype == SRU_F32 && y_dtype == SRU_F32) return launch_sums<float, float>(a, st);
-    if (table_dtype == SRU_F32 && y_dtype == SRU_F16) return launch_sums<__half, float>(a, st);
-    if (table_dtype == SRU_F32) return launch_sums<__nv_bfloat16, float>(a, st);
-    if (table_dtype == SRU_F16) return launch_sums<__half, __half>(a, st);
-    return launch_sums<__nv_bfloat16, __nv_bfloat16>(a, st);
+    auto go = [&](auto tk) -> int {
+        using TK = decltype(tk);
+        if (table_dtype == SRU_F32 && y_dtype == SRU_F32) return launch_backward<TK, float, float>(a, st);
+        if (table_dtype == SRU_F32 && y_dtype == SRU_F16) return launch_backward<TK, __half, float>(a, st);
+        if (table_dtype == SRU_F32) return launch_backward<TK, __nv_bfloat16, float>(a, st);
+        if (table_dtype == SRU_F16) return launch_backward<TK, __half, __half>(a, st);
+        return launch_backward<TK, __nv_bfloat16, __nv_bfloat16>(a, st);
+    };
+    return token_bytes == 4 ? go(int32_t()) : go(int64_t());
 }
 
 }  // extern "C"

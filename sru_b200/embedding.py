@@ -48,7 +48,7 @@ class _EmbeddingLookup(Function):
         nbytes = int(L.sru_b200_embedding_backward_workspace_bytes(n, vocabulary, hidden))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
-            _lib.call("embedding_bwd", 3, L.sru_b200_embedding_backward, _lib.ptr(out), _lib.ptr(tokens), _lib.ptr(grad),
+            _lib.call("embedding_bwd", 1, L.sru_b200_embedding_backward, _lib.ptr(out), _lib.ptr(tokens), _lib.ptr(grad),
                       n, vocabulary, hidden, padding_idx, scale, tokens.element_size(), _lib.DTYPE_CODE[dtype],
                       _lib.DTYPE_CODE[grad.dtype], _lib.ptr(ws), nbytes, _lib.current_stream_ptr(dev))
         return None, out, None, None, None

@@ -69,6 +69,17 @@ def test_one_token_everywhere(n):
             check(tokens, 6, hidden, BF16, BF16)
 
 
+@pytest.mark.parametrize("n", [1, 31, 32, 33, 63, 64, 65, 96, 1025])
+def test_one_token_in_a_large_table(n):
+    """The same runs where the gradient takes three launches instead of one."""
+    for hidden in (64, 65):
+        tokens = torch.full((n,), 5000)
+        check(tokens, 6000, hidden, F32, F32)
+        tokens[n // 2] = 2
+        check(tokens, 6000, hidden, BF16, BF16, padding=5999)
+        check(tokens, 6000, hidden, F32, F16, padding=2)
+
+
 def test_uneven_frequencies():
     """Runs of every length at every offset against the tiles: token k occurs k times, shuffled."""
     tokens = torch.repeat_interleave(torch.arange(120), torch.arange(120))
