@@ -465,15 +465,25 @@ embedding_small_kernel(const EmbArgs a, int blocks_per_row) {
         for (int r = 0; r < REP; ++r)
 #pragma unroll
             for (int k = 0; k < VEC; ++k) acc[r][k] = 0.0f;
-        for (int64_t q = tile; q < end; ++q) {
-            const float *row = a.part + (q == tile ? q * 2 + 1 : q * 2) * a.d;
+        constexpr int G = 8;                    // rows requested together
+        for (int64_t q0 = tile; q0 < end; q0 += G) {
+            float in[G][REP][VEC];
 #pragma unroll
-            for (int r = 0; r < REP; ++r) {
-                const int c = c0 + r * 32 * VEC;
-                if (c >= a.d) continue;
+            for (int g = 0; g < G; ++g)
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) acc[r][k] += __ldcg(row + c + k);
-            }
+                for (int r = 0; r < REP; ++r) {
+                    const int64_t q = q0 + g;
+                    const int c = c0 + r * 32 * VEC;
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k)
+                        in[g][r][k] = q < end && c < a.d ? __ldcg(a.part + (q == tile ? q * 2 + 1 : q * 2) * a.d + c + k) : 0.0f;
+                }
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int r = 0; r < REP; ++r)
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) acc[r][k] += in[g][r][k];
         }
         store_sum<TO, VEC, REP>(static_cast<TO *>(a.dst) + (int64_t)key * a.d, c0, a.d, acc, a.scale);
     }
@@ -524,10 +534,11 @@ template <typename TK> int launch_sort(const EmbArgs &a, cudaStream_t st) {
     return 0;
 }
 
-// One launch for a gradient of at most 1 MB, which sixteen SMs move about as fast as all: three launches / one, us with the host's
+// One launch for a gradient of at most 1 MB and 2048 tokens, which sixteen SMs move about as fast as all: three launches / one, us with the host's
 // share and of the GPU alone: 64 tokens over 100 x 64 20 / 12 and 8.8 / 9.3, 500 over 200 x 64 (0.2 MB) 20 / 12 and 11.0 / 11.3, 500
 // over 1000 x 256 (1.5 MB) 19 / 19 and 14.6 / 17.7, 4000 over 4000 x 256 (8 MB) 19 / 25 and 16.5 / 22.2.
-bool is_small(const EmbArgs &a, int64_t src_size) { return (a.n * src_size + a.v * a.dst_size) * a.d <= (1 << 20); }
+// A run is joined by one warp there, so that few tiles are wanted.
+bool is_small(const EmbArgs &a, int64_t src_size) { return a.n <= 64 * kTile && (a.n * src_size + a.v * a.dst_size) * a.d <= (1 << 20); }
 
 template <typename TK, typename TI, typename TO> int launch_backward(const EmbArgs &a, cudaStream_t st) {
     constexpr int VEC = 16 / sizeof(TI);
