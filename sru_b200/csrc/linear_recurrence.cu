@@ -263,11 +263,34 @@ template <int V> __device__ __forceinline__ void exchange_start(Exchange<V> &x, 
     cluster_sync();
 }
 
+// The gates of some ten closed steps multiply to less than the smallest float32, although no gate is 0 (gate() keeps f at
+// 2^-126 and above), and 0 * inf would make NaN of an infinite state that a walk step by step keeps.  So a map's P stays at
+// the smallest float32, which is as far off as rounding it to 0.
+template <int V> __device__ __forceinline__ Num<V> not_zero(Num<V> P) {
+    float r[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) r[v] = fmaxf(P.get(v), __int_as_float(1));
+    return num(r);
+}
+// The smallest float32 in the columns where s is infinite, 0 in the others; false: there are none in the warp.
+template <int V> __device__ __forceinline__ bool at_inf(Num<V> s, Num<V> *tiny) {
+    float r[V];
+    bool any = false;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const bool inf = fabsf(s.get(v)) == __int_as_float(0x7f800000);
+        r[v] = inf ? __int_as_float(1) : 0.0f;
+        any |= inf;
+    }
+    *tiny = num(r);
+    return __any_sync(0xffffffffu, any);
+}
+
 // refill() is called when all warps of the CTA have read their chunks.
 template <int V, bool BACK, typename Refill>
 __device__ __forceinline__ Num<V> exchange(Exchange<V> &x, int64_t round, const Place &p, Map<V> own, Num<V> *carry, int *err, Refill refill) {
     const int buf = (int)(round & 1);
-    x.warp[buf][p.warp][p.lane] = own;
+    x.warp[buf][p.warp][p.lane] = {not_zero(own.P), own.C};
     __syncthreads();
     refill();
     Num<V> start = *carry;
@@ -281,7 +304,7 @@ __device__ __forceinline__ Num<V> exchange(Exchange<V> &x, int64_t round, const 
                 if (k >= p.warps) break;
                 const Map<V> m = x.warp[buf][BACK ? p.warps - 1 - k : k][p.lane];
                 t.C = fma(m.P, t.C, m.C);
-                t.P = mul(t.P, m.P);
+                t.P = not_zero(mul(t.P, m.P));
             }
             const uint32_t here = smem_u32(&x.cta[buf][p.rank][p.lane]);
             for (uint32_t r = 0; r < p.ranks; ++r) {
@@ -504,6 +527,11 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
                 scan_local<TT, V, T, false>(in, nb, flags, C, P);
             }
             const Num<V> c = exchange<V, false>(*x, turn, p, Map<V>{P[T - 1], C[T - 1]}, &carry, a.err, refill);
+            Num<V> tiny;
+            if (at_inf(c, &tiny)) {
+#pragma unroll
+                for (int i = 0; i < T; ++i) P[i] = add(P[i], tiny);     // the other columns keep their bits
+            }
             if (states) {
 #pragma unroll
                 for (int i = 0; i < T; i += kT)
