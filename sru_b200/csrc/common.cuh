@@ -136,6 +136,16 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity)
         if (global_timer_ns() - t0 > 2000000000ull) return false;
     }
 }
+// A thread's waits in a loop: after one that gave up the others return at once, so that a lost message costs one limit
+// and not one per round.  give_up() is called once.
+struct Patience {
+    bool gone = false;
+    template <typename Wait, typename GiveUp> __host__ __device__ __forceinline__ void wait(Wait wait_, GiveUp give_up) {
+        if (gone || wait_()) return;
+        gone = true;
+        give_up();
+    }
+};
 // global -> this CTA's shared memory, completion counted in bytes on an mbarrier.
 // Both addresses 16-byte aligned, size a multiple of 16 bytes.
 __device__ __forceinline__ void bulk_copy_g2s(uint32_t dst_smem, const void *src, uint32_t bytes,

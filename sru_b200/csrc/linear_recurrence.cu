@@ -239,8 +239,10 @@ template <int V> struct Exchange {
     Map<V> warp[2][kMaxWarps][32];
     Map<V> cta[2][kMaxRanks][32];
     uint64_t arrived[2];
-    uint64_t pad[14];
+    Patience patience;              // of the whole CTA, here and not in registers, which are short in the float32 backward pass
+    uint8_t pad[111];
 };
+static_assert(sizeof(Exchange<1>) % 128 == 0 && sizeof(Exchange<2>) % 128 == 0, "the ring's boxes lie behind it");
 
 __device__ __forceinline__ void store_async(uint32_t addr, uint32_t bar, Map<1> m) {
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];"
@@ -257,6 +259,7 @@ template <int V> __device__ __forceinline__ void exchange_start(Exchange<V> &x, 
     if (threadIdx.x == 0) {
         mbar_init(smem_u32(&x.arrived[0]), 1);
         mbar_init(smem_u32(&x.arrived[1]), 1);
+        x.patience.gone = false;
         fence_mbar_init();
     }
     __syncthreads();
@@ -284,6 +287,12 @@ template <int V> __device__ __forceinline__ bool at_inf(Num<V> s, Num<V> *tiny) 
     }
     *tiny = num(r);
     return __any_sync(0xffffffffu, any);
+}
+
+// A wait that gives up raises the device error flag; from then on a warp waits for no more stages of its ring, and a CTA for no
+// more messages of its cluster, but both keep taking part in the barriers.
+__device__ __forceinline__ void wait_for(uint32_t bar, uint32_t parity, Patience &patience, int *err, int site) {
+    patience.wait([&]() { return mbar_wait_bounded(bar, parity); }, [&]() { atomicExch(err, site); });
 }
 
 // refill() is called when all warps of the CTA have read their chunks.
@@ -314,7 +323,7 @@ __device__ __forceinline__ Num<V> exchange(Exchange<V> &x, int64_t round, const 
                 store_async(there, there_bar, t);
             }
         }
-        if (!mbar_wait_bounded(bar, (uint32_t)(round >> 1) & 1u) && p.lane == 0) atomicExch(err, 42);
+        wait_for(bar, (uint32_t)(round >> 1) & 1u, x.patience, err, 42);
         Num<V> s = *carry;
 #pragma unroll
         for (int k = 0; k < kMaxRanks; ++k) {
@@ -377,13 +386,12 @@ template <typename P> __device__ __forceinline__ P load_shared(uint32_t addr) {
     return p;
 }
 
-// A wait that gives up raises the device error flag; from then on the warp waits for nothing more, but keeps taking part
-// in its CTA's barriers.  full: the stage's bytes are there; empty: all scanning warps have read it.
+// full: the stage's bytes are there; empty: all scanning warps have read it.
 template <int DEPTH> struct Ring {
     uint32_t data, bars, bytes;
     int stage = 0;
     uint32_t phase = 0;
-    bool dead = false;
+    Patience patience;
     __device__ __forceinline__ void start(uint32_t data_, uint32_t bars_, uint32_t bytes_, int readers) {
         data = data_; bars = bars_; bytes = bytes_;
         if (threadIdx.x == 0) {
@@ -398,9 +406,6 @@ template <int DEPTH> struct Ring {
     __device__ __forceinline__ uint32_t at() const { return data + stage * bytes; }
     __device__ __forceinline__ uint32_t full() const { return bars + 8 * stage; }
     __device__ __forceinline__ uint32_t empty() const { return bars + 8 * (DEPTH + stage); }
-    __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, int *err) {
-        if (!dead && !mbar_wait_bounded(bar, parity)) { dead = true; atomicExch(err, 41); }
-    }
     __device__ __forceinline__ void next() { if (++stage == DEPTH) { stage = 0; phase ^= 1; } }
     __device__ __forceinline__ void read(int lane) {       // this warp has read the stage
         __syncwarp();
@@ -469,8 +474,8 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
         if (!SPLIT && p.warp >= p.warps) {          // the warp that asks (and, beside the last columns, one without any)
             if (p.lane == 0 && p.warp == kSide) {
                 for (int64_t n = a.L, turn = 0; n > 0; n -= round, ++turn) {
-                    if (turn >= DEPTH) ring.wait(ring.empty(), ring.phase ^ 1, a.err);
-                    if (ring.dead) break;
+                    if (turn >= DEPTH) wait_for(ring.empty(), ring.phase ^ 1, ring.patience, a.err, 41);
+                    if (ring.patience.gone) break;
                     ask(n, ring.at(), ring.full());
                     ring.next();
                 }
@@ -497,7 +502,7 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
         uint32_t row = 0;
         int32_t row_step = 0;
         if constexpr (RING) {
-            if (box_left > 0) ring.wait(ring.full(), ring.phase, a.err);
+            if (box_left > 0) wait_for(ring.full(), ring.phase, ring.patience, a.err, 41);
             const int first = SPLIT ? p.warp * T : 0;
             row = ring.at() + (p.shift + (SPLIT ? 0 : p.warp * 32 * V)) * 2 * sizeof(TT) + (back ? steps - 1 - first : first) * kRow;
             row_step = back ? -(int32_t)kRow : (int32_t)kRow;
@@ -514,7 +519,7 @@ linear_recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_u, const Li
             else return cur[i];
         };
         auto refill = [&]() {
-            if (RING && threadIdx.x == (p.warps - 1) * 32 && !ring.dead) ask(box_left - DEPTH * round, ring.at(), ring.full());
+            if (RING && threadIdx.x == (p.warps - 1) * 32 && !ring.patience.gone) ask(box_left - DEPTH * round, ring.at(), ring.full());
         };
         if constexpr (SPLIT) {
             Num<V> C[T], P[T];
@@ -624,8 +629,8 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
         if (!SPLIT && p.warp >= p.warps) {
             if (p.lane == 0 && p.warp == kSide) {
                 for (int64_t n = box_left, turn = 0; n <= a.L; n += round, ++turn) {
-                    if (turn >= DEPTH) ring.wait(ring.empty(), ring.phase ^ 1, a.err);
-                    if (ring.dead) break;
+                    if (turn >= DEPTH) wait_for(ring.empty(), ring.phase ^ 1, ring.patience, a.err, 41);
+                    if (ring.patience.gone) break;
                     ask(n, ring.at(), ring.full());
                     ring.next();
                 }
@@ -674,7 +679,7 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
             fetch(left + round);
         }
         if constexpr (RING) {
-            ring.wait(ring.full(), ring.phase, a.err);
+            wait_for(ring.full(), ring.phase, ring.patience, a.err, 41);
             const int first = SPLIT ? p.warp * T : 0, cols = p.shift + (SPLIT ? 0 : p.warp * 32 * V);
             const int at = back ? steps - 1 - first : first;
             row = ring.at() + cols * 2 * sizeof(TT) + at * kRowU;
@@ -728,7 +733,7 @@ linear_recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_u, const __
         Num<V> dc = carry;
         if constexpr (SPLIT) {
             dc = exchange<V, true>(*x, turn, p, own, &carry, a.err, [&]() {
-                if (RING && threadIdx.x == (p.warps - 1) * 32 && !ring.dead) ask(box_left + DEPTH * round, ring.at(), ring.full());
+                if (RING && threadIdx.x == (p.warps - 1) * 32 && !ring.patience.gone) ask(box_left + DEPTH * round, ring.at(), ring.full());
             });
         } else if constexpr (RING) {
             ring.read(p.lane);
