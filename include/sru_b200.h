@@ -320,7 +320,7 @@ int sru_b200_layer_norm_backward(
  *            Strides of L and B are given in elements (even; the pairs themselves contiguous and aligned to their size)
  *   h        out (L, B, d) contiguous, u's type; 0 at padded positions
  *   c_last   out float (B, d), may be NULL;  c_init  float (B, d) or NULL (zeros);  bias  float[d] or NULL
- *   states   out, ..._states_bytes() bytes, for the backward pass; may be NULL (inference)
+ *   states   out, ..._states_bytes() bytes (floats), for the backward pass; may be NULL (inference)
  *   mask_pad (L, B) bytes or NULL, non-zero = padded: the state passes through, u is not looked at there
  *   reverse  non-zero: time runs from L-1 down to 0
  * The reference has no such operator; with SRU_F64 the call gives SRU_ERR_UNSUPPORTED.
@@ -332,14 +332,14 @@ int sru_b200_linear_recurrence_forward(
     const uint8_t *mask_pad, int64_t length, int64_t batch, int64_t hidden,
     int64_t u_stride_t, int64_t u_stride_b, int reverse, int dtype, void *stream);
 
-/* Scratch of the backward pass (partial sums of grad_bias); needed only with a grad_bias. */
+/* Scratch of the backward pass (partial sums of grad_bias, floats); needed only with a grad_bias. */
 size_t sru_b200_linear_recurrence_backward_workspace_bytes(int64_t length, int64_t batch, int64_t hidden, int dtype);
 
 /*
  * Backward of the above.  With dc_t the whole gradient of c_t (dc_t = grad_h_t + f_{t+1} dc_{t+1}, grad_last added at
  * the last step):  dx_t = (1 - f_t) dc_t,  dg_t = dc_t (c_{t-1} - x_t) f_t (1 - f_t);  both 0 at padded positions.
  *
- *   grad_u     out (L, B, d, 2) contiguous, u's type
+ *   grad_u     out (L, B, d, 2) contiguous, u's type, the pairs aligned to their size
  *   grad_bias  out float[d] or NULL: dg summed over L and B in a fixed order (no atomics)
  *   grad_init  out float (B, d) or NULL
  *   u, bias, mask_pad, sizes, strides, reverse   as in the forward call;  states   what it left

@@ -957,6 +957,8 @@ int sru_b200_linear_recurrence_forward(void *h, float *c_last, void *states, con
     const size_t size = dtype_size(dtype);
     if ((reinterpret_cast<uintptr_t>(u) % (2 * size)) || u_stride_t % 2 || u_stride_b % 2)
         return set_error(SRU_ERR_BAD_ARG, "linear recurrence: the pairs of u must be aligned to their size");
+    if (reinterpret_cast<uintptr_t>(states) % sizeof(float))
+        return set_error(SRU_ERR_BAD_ARG, "linear recurrence: states must be aligned to 4 bytes");
     LinRecArgs a;
     memset(&a, 0, sizeof(a));
     a.h = h; a.last = c_last; a.states = static_cast<float *>(states);
@@ -985,11 +987,15 @@ int sru_b200_linear_recurrence_backward(void *grad_u, float *grad_bias, float *g
     const size_t size = dtype_size(dtype);
     if ((reinterpret_cast<uintptr_t>(u) % (2 * size)) || u_stride_t % 2 || u_stride_b % 2)
         return set_error(SRU_ERR_BAD_ARG, "linear recurrence: the pairs of u must be aligned to their size");
+    if (reinterpret_cast<uintptr_t>(grad_u) % (2 * size))
+        return set_error(SRU_ERR_BAD_ARG, "linear recurrence: the pairs of grad_u must be aligned to their size");
+    if (reinterpret_cast<uintptr_t>(states) % sizeof(float))
+        return set_error(SRU_ERR_BAD_ARG, "linear recurrence: states must be aligned to 4 bytes");
     const Slices s = choose_slices(length, batch, hidden, dtype, true);
     if (grad_bias) {
         const size_t need = (size_t)batch * s.count() * (size_t)hidden * sizeof(float);
-        if (!workspace || workspace_bytes < need)
-            return set_error(SRU_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+        if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % sizeof(float))
+            return set_error(SRU_ERR_WORKSPACE, "4-byte aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     }
     LinRecArgs a;
     memset(&a, 0, sizeof(a));
