@@ -95,6 +95,12 @@ int sru_b200_get_option(const char *name);
 int sru_b200_last_scan_kernel(void);
 
 /*
+ * Kernels that this library has launched in this process so far, over all threads and devices (a kernel that a stream
+ * capture records counts once, its replays do not).  No counterpart in the reference.
+ */
+int64_t sru_b200_launch_count(void);
+
+/*
  * Forward scan.  Replaces the four forward launchers of the reference,
  * sru_cuda_forward_simple / sru_cuda_bi_forward_simple / sru_cuda_forward /
  * sru_cuda_bi_forward (sru/csrc/sru_cuda_kernel.cu:827-860, :911-944, :995-1036,

@@ -46,6 +46,8 @@ def lib():
         l.sru_b200_get_option.argtypes = [ctypes.c_char_p]
         l.sru_b200_last_scan_kernel.restype = _int
         l.sru_b200_last_scan_kernel.argtypes = []
+        l.sru_b200_launch_count.restype = _i64
+        l.sru_b200_launch_count.argtypes = []
         l.sru_b200_scan_forward.restype = _int
         l.sru_b200_scan_forward.argtypes = [_vp] * 10 + [_i64, _i64, _i64, _int, _int, _int, _int, _int,
                                                          ctypes.c_double, _int, _int, _vp]
@@ -197,7 +199,6 @@ class KernelTimer:
 
 
 timer = None          # a KernelTimer, or None
-launch_count = 0      # kernels of this library launched so far (bench.py reports the per-step figure)
 nvtx_ranges = os.environ.get("SRU_B200_NVTX", "0") not in ("", "0")   # see set_nvtx_ranges
 
 
@@ -209,10 +210,16 @@ def set_nvtx_ranges(enabled: bool) -> None:
     nvtx_ranges = bool(enabled)
 
 
-def call(name, n_kernels, fn, *args):
-    """Invoke a C-ABI entry point, count its kernel launches, time it if a timer is installed."""
-    global launch_count
-    launch_count += n_kernels
+def __getattr__(name):
+    """``launch_count``: kernels of this library launched so far, whoever called for them (bench.py reports the per-step
+    figure); counted in the native library, where the launches are."""
+    if name == "launch_count":
+        return int(lib().sru_b200_launch_count())
+    raise AttributeError("module %r has no attribute %r" % (__name__, name))
+
+
+def call(name, fn, *args):
+    """Invoke a C-ABI entry point, time it if a timer is installed."""
     if nvtx_ranges:
         torch.cuda.nvtx.range_push(name)
         try:

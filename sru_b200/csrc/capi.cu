@@ -55,6 +55,9 @@ static int find_option(const char *name) {
 static thread_local int tl_scan_kernel = SCAN_KERNEL_NONE;
 void note_scan_kernel(int which) { tl_scan_kernel = which; }
 
+static std::atomic<int64_t> g_launches{0};
+void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+
 __device__ int g_device_error = 0;
 
 int *device_error_flag() {
@@ -130,6 +133,8 @@ int sru_b200_get_option(const char *name) {
 }
 
 int sru_b200_last_scan_kernel(void) { return tl_scan_kernel; }
+
+int64_t sru_b200_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
 
 const char *sru_b200_last_error(void) { return tl_error; }
 

@@ -42,6 +42,19 @@ void note_scan_kernel(int which);
                                      cudaGetErrorString(err__));                           \
     } while (0)
 
+// Every kernel launch of the library goes through one of these: it is counted (sru_b200_launch_count).
+void count_launch();
+#define SRUB_LAUNCHED() /* behind kernel<<<...>>>(...) */                                  \
+    do {                                                                                   \
+        SRUB_CUDA_CHECK(cudaGetLastError());                                               \
+        ::srub::count_launch();                                                            \
+    } while (0)
+#define SRUB_LAUNCH(...) /* (&config, kernel, arguments...) */                             \
+    do {                                                                                   \
+        SRUB_CUDA_CHECK(cudaLaunchKernelEx(__VA_ARGS__));                                  \
+        ::srub::count_launch();                                                            \
+    } while (0)
+
 static inline size_t dtype_size(int dt) {
     switch (dt) {
         case SRU_F32: return 4;

@@ -49,9 +49,12 @@ static int launch_convert(void *dst, const void *src, int64_t n, cudaStream_t st
         const int64_t want = (n8 + 256 * 4 - 1) / (256 * 4);
         const unsigned blocks = (unsigned)std::min<int64_t>(want, 148 * 16);     // grid-stride: a few resident waves of a B200
         convert_kernel<TI, TO><<<blocks, 256, 0, st>>>(static_cast<TO *>(dst), static_cast<const TI *>(src), n8);
+        SRUB_LAUNCHED();
     }
-    if (n8 * 8 < n) convert_tail_kernel<TI, TO><<<1, 8, 0, st>>>(static_cast<TO *>(dst), static_cast<const TI *>(src), n8 * 8, n);
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    if (n8 * 8 < n) {
+        convert_tail_kernel<TI, TO><<<1, 8, 0, st>>>(static_cast<TO *>(dst), static_cast<const TI *>(src), n8 * 8, n);
+        SRUB_LAUNCHED();
+    }
     return 0;
 }
 

@@ -512,7 +512,7 @@ template <typename TK, typename TI, typename TO> int launch_forward(const EmbArg
         if (blocks > 0x7fffffff) return set_error(SRU_ERR_UNSUPPORTED, "embedding: n * hidden too large");
         const uint32_t groups = a.d / V;
         embedding_fwd_kernel<TK, TI, TO, V, R><<<(unsigned)blocks, 256, 0, st>>>(a, groups, 256 / groups, 256 % groups);
-        SRUB_CUDA_CHECK(cudaGetLastError());
+        SRUB_LAUNCHED();
         return 0;
     };
     if (!wide) return go(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
@@ -530,7 +530,7 @@ template <typename TK> int launch_sort(const EmbArgs &a, cudaStream_t st) {
         attr_set[dev] = true;
     }
     embedding_sort_kernel<TK><<<kSortCtas, kSortWarps * 32, 0, st>>>(a);
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    SRUB_LAUNCHED();
     return 0;
 }
 
@@ -557,7 +557,7 @@ template <typename TK, typename TI, typename TO> int launch_backward(const EmbAr
                 attr_set[dev] = true;
             }
             kernel<<<kSortCtas, kSortWarps * 32, 0, st>>>(a, per_row);
-            SRUB_CUDA_CHECK(cudaGetLastError());
+            SRUB_LAUNCHED();
             return 0;
         }
         if (int rc = launch_sort<TK>(a, st)) return rc;
@@ -569,9 +569,9 @@ template <typename TK, typename TI, typename TO> int launch_backward(const EmbAr
         cfg.attrs = &early; cfg.numAttrs = 1; cfg.stream = st;
         cfg.blockDim = dim3(128);
         cfg.gridDim = dim3((unsigned)(sums + fill));
-        SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, embedding_sum_kernel<TI, TO, V, R>, a, per_row, (unsigned)fill));
+        SRUB_LAUNCH(&cfg, embedding_sum_kernel<TI, TO, V, R>, a, per_row, (unsigned)fill);
         cfg.gridDim = dim3((unsigned)((a.n + kTile - 1) / kTile), per_row);
-        SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, embedding_join_kernel<TO, V, R>, a));
+        SRUB_LAUNCH(&cfg, embedding_join_kernel<TO, V, R>, a);
         return 0;
     };
     if (wide) return go(std::integral_constant<int, VEC>(), std::integral_constant<int, 1>());

@@ -84,14 +84,14 @@ extern "C" int sru_b200_gemm_f32(float *c, const float *a, const float *b, const
         const int64_t rows = trans_a ? k_dim : m, cols = trans_a ? m : k_dim;
         const unsigned blocks = (unsigned)std::min<int64_t>((rows * cols + 255) / 256, 148 * 16);
         split_stack_kernel<<<blocks, 256, 0, st>>>(a, a6, rows, cols, lda, trans_a ? 0 : 1, 0);
-        SRUB_CUDA_CHECK(cudaGetLastError());
+        SRUB_LAUNCHED();
     }
     // op(B) is K x N: stored (K, N) -> stack along its rows; stored (N, K) (trans_b) -> stack along its columns
     {
         const int64_t rows = trans_b ? n : k_dim, cols = trans_b ? k_dim : n;
         const unsigned blocks = (unsigned)std::min<int64_t>((rows * cols + 255) / 256, 148 * 16);
         split_stack_kernel<<<blocks, 256, 0, st>>>(b, b6, rows, cols, ldb, trans_b ? 1 : 0, 1);
-        SRUB_CUDA_CHECK(cudaGetLastError());
+        SRUB_LAUNCHED();
     }
     const int64_t lda6 = trans_a ? m : 6 * k_dim, ldb6 = trans_b ? 6 * k_dim : n;
     return sru_b200_gemm_ws(c, a6, b6, col_bias, m, n, 6 * k_dim, lda6, ldb6, ldc, trans_a, trans_b, SRU_BF16, SRU_F32,

@@ -967,7 +967,7 @@ static int gemm_impl(void *c, const void *a, const void *b, const float *col_bia
         const unsigned grid = (unsigned)std::min<int64_t>(ntiles, plan.workers);
         gemm_tcgen05_kernel<<<grid, kThreads, kSmemBytes, static_cast<cudaStream_t>(stream)>>>(map_a, map_b, g);
     }
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    SRUB_LAUNCHED();
     if (ksplit > 1) {
         const int64_t items = m * (n / 4);
         const unsigned blocks = (unsigned)std::min<int64_t>((items + 255) / 256, (int64_t)plan.workers * 16);
@@ -979,7 +979,7 @@ static int gemm_impl(void *c, const void *a, const void *b, const float *col_bia
             splitk_reduce<__half><<<blocks, 256, 0, st>>>(ws, ksplit, m, n, (__half *)final_c, ldc, final_acc);
         else
             splitk_reduce<float><<<blocks, 256, 0, st>>>(ws, ksplit, m, n, (float *)final_c, ldc, final_acc);
-        SRUB_CUDA_CHECK(cudaGetLastError());
+        SRUB_LAUNCHED();
     }
     return 0;
 }
@@ -1001,7 +1001,7 @@ extern "C" int sru_b200_gate_bias_columns(float *col_bias, const float *bias, in
     const int64_t n = width * k;
     const unsigned blocks = (unsigned)std::min<int64_t>((n + 255) / 256, 1024);
     gate_bias_columns_kernel<<<blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(col_bias, bias, width, k);
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    SRUB_LAUNCHED();
     return 0;
 }
 

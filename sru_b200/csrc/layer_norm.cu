@@ -429,7 +429,7 @@ int ln_forward_w(void *y, float *mean, float *rstd, const void *x, const float *
     // one resident wave that walks the rows: gamma and beta are staged in shared memory once per CTA
     const int blocks = (int)std::min<int64_t>((rows + rpc - 1) / rpc, (int64_t)sm_count() * occ);
     kernel<<<blocks, kLnThreads, smem, st>>>((TO *)y, mean, rstd, (const TI *)x, gamma, beta, rows, n, eps);
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    SRUB_LAUNCHED();
     return 0;
 }
 
@@ -456,7 +456,7 @@ int ln_backward_w(void *dx, void *workspace, size_t workspace_bytes, const void 
         return set_error(SRU_ERR_WORKSPACE, "layer-norm backward needs %zu bytes of workspace, got %zu", need, workspace_bytes);
     kernel<<<blocks, kLnThreads, smem, st>>>((TI *)dx, (float *)workspace, (const TO *)dy,
                                                                      (const TI *)x, mean, rstd, gamma, rows, n);
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    SRUB_LAUNCHED();
     *nparts = blocks;
     return 0;
 }
@@ -543,7 +543,7 @@ int sru_b200_layer_norm_backward(void *dx, float *dgamma, float *dbeta, const vo
     if (rc) return rc;
     if (dgamma || dbeta) {
         ln_reduce_kernel<<<(2 * ni + 31) / 32, 256, 0, st>>>(static_cast<const float *>(workspace), nparts, ni, dgamma, dbeta);
-        SRUB_CUDA_CHECK(cudaGetLastError());
+        SRUB_LAUNCHED();
     }
     return 0;
 }

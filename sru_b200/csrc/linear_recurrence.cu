@@ -887,8 +887,8 @@ int launch(LinRecArgs a, const Slices &s, const Maps &maps, bool backward, cudaS
     attr[0].val.clusterDim.x = (unsigned)s.ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = SPLIT ? 1 : 0;
-    if (backward) SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, bwd, maps.u, maps.g, maps.s, a));
-    else SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fwd, maps.u, a));
+    if (backward) SRUB_LAUNCH(&cfg, bwd, maps.u, maps.g, maps.s, a);
+    else SRUB_LAUNCH(&cfg, fwd, maps.u, a);
     return 0;
 }
 
@@ -1010,7 +1010,7 @@ int sru_b200_linear_recurrence_backward(void *grad_u, float *grad_bias, float *g
     if (rc || !grad_bias) return rc;
     linear_recurrence_bias_kernel<<<(unsigned)((hidden + 31) / 32), 256, 0, st>>>(grad_bias, a.bias_part,
                                                                                    batch * s.count(), (int)hidden);
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    SRUB_LAUNCHED();
     return 0;
 }
 

@@ -1321,7 +1321,7 @@ int ns_product(const NsMaps &a, const NsMaps &b, const NsMaps &out, const NsMaps
     attr[1] = early_launch();
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, AMN ? a.b : a.a, BN == 256 && !BMN ? b.a : b.b, out.c, BN == 256 ? out.wide_t : out.t, d.c, g));
+    SRUB_LAUNCH(&cfg, kernel, AMN ? a.b : a.a, BN == 256 && !BMN ? b.a : b.b, out.c, BN == 256 ? out.wide_t : out.t, d.c, g);
     return 0;
 }
 
@@ -1356,7 +1356,7 @@ template <int S> int ns_gram_split(const NsMaps &a, const void *out, int64_t ldm
     attr[1] = early_launch();
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, a.a, a.b, c, t, g));
+    SRUB_LAUNCH(&cfg, kernel, a.a, a.b, c, t, g);
     return 0;
 }
 
@@ -1381,7 +1381,7 @@ int ns_cluster(const NsMaps &x0, const NsMaps &x1, const NsMaps &a, const NsMaps
     attr[1] = early_launch();
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ns_cluster_kernel, x0.a, x0.b, x1.a, x1.b, a.a, a.b, a.c, m.a, g));
+    SRUB_LAUNCH(&cfg, ns_cluster_kernel, x0.a, x0.b, x1.a, x1.b, a.a, a.b, a.c, m.a, g);
     return 0;
 }
 
@@ -1437,7 +1437,7 @@ int launch_early(dim3 grid, void (*kernel)(NsEdge), const NsEdge &e, cudaStream_
     cudaLaunchAttribute early = early_launch();
     cfg.gridDim = grid; cfg.blockDim = dim3(256); cfg.stream = st;
     cfg.attrs = &early; cfg.numAttrs = 1;
-    SRUB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, e));
+    SRUB_LAUNCH(&cfg, kernel, e);
     return 0;
 }
 
@@ -1452,7 +1452,7 @@ template <typename T, typename TO> int ns_small(const NsSmall &a, int64_t batch,
         attr_set[dev] = true;
     }
     kernel<<<(unsigned)batch, kSmallThreads, bytes, st>>>(a);
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    SRUB_LAUNCHED();
     return 0;
 }
 
@@ -1530,7 +1530,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         using T = decltype(t);
         if (unit == 512) ns_norm_kernel<T, 512><<<norm_grid, 256, 0, st>>>(e);
         else ns_norm_kernel<T, 2048><<<norm_grid, 256, 0, st>>>(e);
-        SRUB_CUDA_CHECK(cudaGetLastError());
+        SRUB_LAUNCHED();
         if (turned) {
             const dim3 grid((unsigned)((p.ldx + 63) / 64), (unsigned)((p.m + 63) / 64), (unsigned)batch);
             return launch_early(grid, ns_first_turned_kernel<T>, e, st);
@@ -1592,7 +1592,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     e.s_i = tall ? 1 : cols; e.s_j = tall ? cols : 1; e.s_b = rows * cols;
     if (out_dtype == SRU_F16) ns_last_kernel<__half><<<tile_grid, 256, 0, st>>>(e);
     else ns_last_kernel<__nv_bfloat16><<<tile_grid, 256, 0, st>>>(e);
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    SRUB_LAUNCHED();
     return 0;
 }
 

@@ -203,7 +203,7 @@ int launch_reduce_partials(const void *part, void *grad_wc, void *grad_bias, int
     const int64_t blocks = (4 * D + 31) / 32;
     reduce_partials<CT><<<(unsigned)blocks, 256, 0, st>>>((const CT *)part, (CT *)grad_wc,
                                                          (CT *)grad_bias, ntiles, D, write_wc);
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    SRUB_LAUNCHED();
     return 0;
 }
 template int launch_reduce_partials<float>(const void *, void *, void *, int64_t, int64_t, int, cudaStream_t);
@@ -220,7 +220,7 @@ static int launch_generic_t(const ScanArgs &a, bool backward, cudaStream_t st) {
     } else {
         scan_bwd_generic<T, TC, CT><<<(unsigned)blocks, threads, 0, st>>>(a);
     }
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    SRUB_LAUNCHED();
     if (backward)
         return launch_reduce_partials<CT>(a.workspace, a.grad_wc, a.grad_bias, a.B,
                                           (int64_t)a.d * a.dirs, a.is_custom ? 0 : 1, st);

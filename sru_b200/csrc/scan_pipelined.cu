@@ -750,7 +750,7 @@ static int launch_t(const ScanMaps &maps, const PipeArgs &p, bool backward, cuda
     const unsigned grid = (unsigned)((int64_t)p.c.nht * p.c.nrt);
     if (backward) bwd<<<grid, p.c.threads, p.c.smem, st>>>(maps, p);
     else fwd<<<grid, p.c.threads, p.c.smem, st>>>(maps, p);
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    SRUB_LAUNCHED();
     return 1;
 }
 

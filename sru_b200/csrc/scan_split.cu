@@ -382,7 +382,7 @@ static int launch_split_t(const ScanMaps &maps, const PipeArgs &p, cudaStream_t 
     }
     const unsigned grid = (unsigned)((int64_t)p.c.nht * p.c.nrt);
     fn<<<grid, p.c.threads, p.c.smem, st>>>(maps, p);
-    SRUB_CUDA_CHECK(cudaGetLastError());
+    SRUB_LAUNCHED();
     return 1;
 }
 

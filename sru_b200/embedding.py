@@ -22,7 +22,7 @@ def _forward(tokens, weight, scale, out_dtype):
     y = torch.empty(n, hidden, dtype=out_dtype, device=weight.device)
     if n:
         with torch.cuda.device(weight.device):
-            _lib.call("embedding_fwd", 1, _lib.lib().sru_b200_embedding_forward, _lib.ptr(y), _lib.ptr(tokens),
+            _lib.call("embedding_fwd", _lib.lib().sru_b200_embedding_forward, _lib.ptr(y), _lib.ptr(tokens),
                       _lib.ptr(weight), n, vocabulary, hidden, weight.stride(0), scale, tokens.element_size(),
                       _lib.DTYPE_CODE[weight.dtype], _lib.DTYPE_CODE[out_dtype], _lib.current_stream_ptr(weight.device))
     return y
@@ -48,7 +48,7 @@ class _EmbeddingLookup(Function):
         nbytes = int(L.sru_b200_embedding_backward_workspace_bytes(n, vocabulary, hidden))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
-            _lib.call("embedding_bwd", 1, L.sru_b200_embedding_backward, _lib.ptr(out), _lib.ptr(tokens), _lib.ptr(grad),
+            _lib.call("embedding_bwd", L.sru_b200_embedding_backward, _lib.ptr(out), _lib.ptr(tokens), _lib.ptr(grad),
                       n, vocabulary, hidden, padding_idx, scale, tokens.element_size(), _lib.DTYPE_CODE[dtype],
                       _lib.DTYPE_CODE[grad.dtype], _lib.ptr(ws), nbytes, _lib.current_stream_ptr(dev))
         return None, out, None, None, None
@@ -66,7 +66,6 @@ def embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding
     flag: ``_lib.check_device_error()`` then raises.
     """
     if _lib.timer is None and not _lib.nvtx_ranges:
-        _lib.launch_count += 1
         try:
             return _lib.native_op("embedding_lookup")(tokens, weight, scale, padding_idx, out_dtype)
         except RuntimeError as e:

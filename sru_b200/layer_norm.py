@@ -51,7 +51,7 @@ def forward_raw(x2d: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], e
     b = None if bias is None else bias.detach().float().contiguous()
     L = _lib.lib()
     with torch.cuda.device(x2d.device):
-        _lib.call("layer_norm_fwd", 1, L.sru_b200_layer_norm_forward,
+        _lib.call("layer_norm_fwd", L.sru_b200_layer_norm_forward,
                   _lib.ptr(y), _lib.ptr(mean), _lib.ptr(rstd), _lib.ptr(x2d), _lib.ptr(w), _lib.ptr(b),
                   rows, n, float(eps), _lib.DTYPE_CODE[x2d.dtype], _lib.DTYPE_CODE[out_dtype],
                   _lib.current_stream_ptr(x2d.device))
@@ -70,7 +70,7 @@ def backward_raw(dy2d: Tensor, x2d: Tensor, mean: Tensor, rstd: Tensor, weight: 
     with torch.cuda.device(x2d.device):
         ws_bytes = int(L.sru_b200_layer_norm_backward_workspace_bytes(rows, n))
         ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=x2d.device)
-        _lib.call("layer_norm_bwd", 2 if need_wb else 1, L.sru_b200_layer_norm_backward,
+        _lib.call("layer_norm_bwd", L.sru_b200_layer_norm_backward,
                   _lib.ptr(dx), _lib.ptr(dg), _lib.ptr(db), _lib.ptr(dy2d), _lib.ptr(x2d), _lib.ptr(mean),
                   _lib.ptr(rstd), _lib.ptr(w), rows, n, _lib.DTYPE_CODE[x2d.dtype],
                   _lib.DTYPE_CODE[dy2d.dtype], _lib.ptr(ws), ws_bytes, _lib.current_stream_ptr(x2d.device))

@@ -44,7 +44,7 @@ def _forward(u, c0, bias, mask, reverse, need_states):
         nbytes = int(L.sru_b200_linear_recurrence_states_bytes(length, batch, d))
         states = torch.empty(nbytes // 4, dtype=torch.float32, device=u.device)
     with torch.cuda.device(u.device):
-        _lib.call("linear_recurrence_fwd", 1, L.sru_b200_linear_recurrence_forward,
+        _lib.call("linear_recurrence_fwd", L.sru_b200_linear_recurrence_forward,
                   _lib.ptr(h), _lib.ptr(c_last), _lib.ptr(states), _lib.ptr(u), _lib.ptr(bias), _lib.ptr(c0), _lib.ptr(mask),
                   length, batch, d, u.stride(0), u.stride(1), int(reverse), _lib.DTYPE_CODE[u.dtype],
                   _lib.current_stream_ptr(u.device))
@@ -87,7 +87,7 @@ class _GatedLinearRecurrence(Function):
             with torch.cuda.device(dev):
                 nbytes = int(L.sru_b200_linear_recurrence_backward_workspace_bytes(length, batch, d, _lib.DTYPE_CODE[u.dtype])) if need_bias else 0
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-                _lib.call("linear_recurrence_bwd", 2 if need_bias else 1, L.sru_b200_linear_recurrence_backward,
+                _lib.call("linear_recurrence_bwd", L.sru_b200_linear_recurrence_backward,
                           _lib.ptr(grad_u), _lib.ptr(grad_bias), _lib.ptr(grad_first), _lib.ptr(u), _lib.ptr(bias),
                           _lib.ptr(states), _lib.ptr(mask), _lib.ptr(gh), _lib.ptr(gl), length, batch, d, u.stride(0),
                           u.stride(1), 0 if gh is None else gh.stride(0), 0 if gh is None else gh.stride(1),
@@ -122,7 +122,6 @@ def gated_linear_recurrence(u: Tensor, c0: Optional[Tensor] = None, bias: Option
     bias.
     """
     if _lib.timer is None and not _lib.nvtx_ranges:
-        _lib.launch_count += 1
         try:
             return _lib.native_op("gated_linear_recurrence")(u, c0, bias, mask_pad, reverse)
         except RuntimeError as e:

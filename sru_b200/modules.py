@@ -627,7 +627,6 @@ class SRU(nn.Module):
             x, w_list, [c.weight_c for c in self.rnn_lst], [c.bias for c in self.rnn_lst],
             scales, c0, mask_pad, self.hidden_size, self.bidirectional, ks, skips, dt == torch.float16,
             has_norm, ln_w, ln_b, ln_eps, normalize_after, cb_list)
-        _lib.launch_count += 2 * len(ks) + sum(has_norm)      # per layer: product, scan (+ layer norm)
         return [out[0], out[1]]
 
     @torch.jit.unused

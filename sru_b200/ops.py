@@ -111,7 +111,7 @@ def scan_forward(u: Tensor, x: Optional[Tensor], weight_c: Tensor, bias: Optiona
         return h, c_hist, c_last
     with torch.cuda.device(u.device):
         _lib.call(
-            "scan_fwd" if need_c_hist else "scan_fwd_infer", 1, _lib.lib().sru_b200_scan_forward,
+            "scan_fwd" if need_c_hist else "scan_fwd_infer", _lib.lib().sru_b200_scan_forward,
             _lib.ptr(h), _lib.ptr(c_hist), _lib.ptr(c_last), _lib.ptr(u), _lib.ptr(x),
             _lib.ptr(weight_c), _lib.ptr(bias), _lib.ptr(c_init), _lib.ptr(mask_c), _lib.ptr(mask_pad),
             length, batch, d, dirs, k, activation_type, skip_type, is_custom, float(scale_x),
@@ -147,7 +147,7 @@ def scan_backward(u, x, weight_c, bias, c_init, mask_c, mask_pad, c_hist, grad_h
     workspace = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=dev)
     with torch.cuda.device(dev):
         _lib.call(
-            "scan_bwd", 2, L.sru_b200_scan_backward,
+            "scan_bwd", L.sru_b200_scan_backward,
             _lib.ptr(grad_u), _lib.ptr(grad_x), _lib.ptr(grad_wc), _lib.ptr(grad_bias), _lib.ptr(grad_init),
             _lib.ptr(u), _lib.ptr(x), _lib.ptr(weight_c), _lib.ptr(bias), _lib.ptr(c_init),
             _lib.ptr(mask_c), _lib.ptr(mask_pad), _lib.ptr(c_hist), _lib.ptr(grad_h), _lib.ptr(grad_last),
@@ -189,7 +189,7 @@ def _convert(t: Tensor, dtype: torch.dtype) -> Tensor:
     out = torch.empty(t.shape, dtype=dtype, device=t.device)
     if t.numel():
         with torch.cuda.device(t.device):
-            _lib.call("convert", 1 if t.numel() % 8 == 0 else 2, _lib.lib().sru_b200_convert, _lib.ptr(out), _lib.ptr(t),
+            _lib.call("convert", _lib.lib().sru_b200_convert, _lib.ptr(out), _lib.ptr(t),
                       t.numel(), _lib.DTYPE_CODE[t.dtype], _lib.DTYPE_CODE[dtype], _lib.current_stream_ptr(t.device))
     return out
 

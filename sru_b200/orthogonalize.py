@@ -29,7 +29,6 @@ def orthogonalize(grad: Tensor, steps: int = 5, coefficients: Tuple[float, float
     if len(coefficients) != 3:
         raise _lib.SruB200Error("coefficients must be (a, b, c), got %r" % (coefficients,))
     if _lib.timer is None and not _lib.nvtx_ranges:
-        _lib.launch_count += 1
         try:
             return _lib.native_op("orthogonalize")(grad, steps, *coefficients, eps, out_dtype)
         except RuntimeError as e:
@@ -57,7 +56,7 @@ def orthogonalize(grad: Tensor, steps: int = 5, coefficients: Tuple[float, float
     with torch.cuda.device(grad.device):
         nbytes = int(L.sru_b200_orthogonalize_workspace_bytes(batch, rows, cols))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)
-        _lib.call("orthogonalize", 1, L.sru_b200_orthogonalize, _lib.ptr(out), _lib.ptr(grad), batch, rows, cols,
+        _lib.call("orthogonalize", L.sru_b200_orthogonalize, _lib.ptr(out), _lib.ptr(grad), batch, rows, cols,
                   grad.stride(0) if grad.dim() == 3 else 0, grad.stride(-2), grad.stride(-1), int(steps), a, b, c,
                   float(eps), _lib.DTYPE_CODE[grad.dtype], _lib.DTYPE_CODE[out_dtype], _lib.ptr(ws), nbytes,
                   _lib.current_stream_ptr(grad.device))

@@ -66,7 +66,7 @@ def gemm(a: Tensor, b: Tensor, trans_a: bool = False, trans_b: bool = False,
         ws_bytes = int(L.sru_b200_gemm_workspace_bytes(m, n, kd, 0 if bias is None else 1))
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=a.device) if ws_bytes else None
         _lib.call(
-            name, 2 if ws_bytes > 32768 else 1, L.sru_b200_gemm_ws,   # K slabs add a reduction kernel
+            name, L.sru_b200_gemm_ws,
             _lib.ptr(out), _lib.ptr(a), _lib.ptr(b), _lib.ptr(bias), m, n, kd,
             a.stride(0), b.stride(0), out.stride(0), int(trans_a), int(trans_b),
             _lib.DTYPE_CODE[a.dtype], _lib.DTYPE_CODE[out.dtype], int(accumulate),
@@ -96,7 +96,7 @@ def gemm_f32(a: Tensor, b: Tensor, trans_a: bool = False, trans_b: bool = False,
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=a.device)
         if name is None:
             name = "gemm_wgrad" if trans_a else ("gemm_dgrad" if trans_b else "gemm_fwd")
-        _lib.call(name, 3, L.sru_b200_gemm_f32, _lib.ptr(out), _lib.ptr(a), _lib.ptr(b), _lib.ptr(bias), m, n, kd,
+        _lib.call(name, L.sru_b200_gemm_f32, _lib.ptr(out), _lib.ptr(a), _lib.ptr(b), _lib.ptr(bias), m, n, kd,
                   a.stride(0), b.stride(0), out.stride(0), int(trans_a), int(trans_b), 0, _lib.ptr(ws), ws_bytes,
                   _lib.current_stream_ptr(a.device))
     return out
@@ -234,7 +234,7 @@ def gate_bias_columns(bias: Tensor, width: int, k: int) -> Tensor:
         b = b.float().contiguous()
     out = torch.empty(width * k, dtype=torch.float32, device=b.device)
     with torch.cuda.device(b.device):
-        _lib.call("gate_bias", 1, _lib.lib().sru_b200_gate_bias_columns, _lib.ptr(out), _lib.ptr(b), width, k,
+        _lib.call("gate_bias", _lib.lib().sru_b200_gate_bias_columns, _lib.ptr(out), _lib.ptr(b), width, k,
                   _lib.current_stream_ptr(b.device))
     return out
 
