@@ -120,6 +120,22 @@ def native_op(name):
     return op
 
 
+def call_native(op, name, backward_name, *args):
+    """A native torch operator with autograd of its own.  With a timer or NVTX ranges installed its launches are bracketed
+    like those of ``call``: the forward pass here, the backward pass by hooks on the operator's node of the graph."""
+    fn = _native_ops.get(op) or native_op(op)
+    try:
+        if (timer is None and not nvtx_ranges) or not args[0].is_cuda:
+            return fn(*args)
+        with torch.cuda.device(args[0].device):
+            out = _watched(name, fn, *args)
+    except RuntimeError as e:
+        raise refused(e) from None
+    if backward_name is not None:
+        _watch_backward(backward_name, out)
+    return out
+
+
 def refused(error):
     """A refusal by a native operator as this package's error; anything else (out of memory, for instance) as it is."""
     return SruB200Error(str(error)) if type(error) is RuntimeError else error
@@ -220,22 +236,53 @@ def __getattr__(name):
 
 def call(name, fn, *args):
     """Invoke a C-ABI entry point, time it if a timer is installed."""
+    return check(_watched(name, fn, *args))
+
+
+def _watched(name, fn, *args):
+    """fn(*args), in an NVTX range and between a pair of events where those are asked for."""
     if nvtx_ranges:
         torch.cuda.nvtx.range_push(name)
-        try:
-            return _call(name, fn, *args)
-        finally:
+    try:
+        if timer is None:
+            return fn(*args)
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        out = fn(*args)
+        end.record()
+        timer.add(name, start, end)
+        return out
+    finally:
+        if nvtx_ranges:
             torch.cuda.nvtx.range_pop()
-    return _call(name, fn, *args)
 
 
-def _call(name, fn, *args):
-    if timer is None:
-        return check(fn(*args))
-    start = torch.cuda.Event(enable_timing=True)
-    end = torch.cuda.Event(enable_timing=True)
-    start.record()
-    rc = fn(*args)
-    end.record()
-    timer.add(name, start, end)
-    return check(rc)
+def _watch_backward(name, out):
+    """The same around the backward pass of the operator that made ``out`` (a tensor or a tuple of them): its node is the
+    first one of C++ behind the views."""
+    node = (out if isinstance(out, torch.Tensor) else out[0]).grad_fn
+    while node is not None and "CppNode" not in node.name():
+        node = node.next_functions[0][0] if node.next_functions else None
+    if node is None:
+        return
+    spans = []      # open ranges, innermost last: a node runs once per backward pass
+
+    def before(grads):
+        if nvtx_ranges:
+            torch.cuda.nvtx.range_push(name)
+        start = None
+        if timer is not None:
+            start = torch.cuda.Event(enable_timing=True)
+            start.record()
+        spans.append((start, nvtx_ranges))
+
+    def after(grads_in, grads_out):
+        start, ranged = spans.pop()
+        if start is not None and timer is not None:
+            end = torch.cuda.Event(enable_timing=True)
+            end.record()
+            timer.add(name, start, end)
+        if ranged:
+            torch.cuda.nvtx.range_pop()
+    node.register_prehook(before)
+    node.register_hook(after)

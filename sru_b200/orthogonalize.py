@@ -11,8 +11,6 @@ from torch import Tensor
 
 from . import _lib
 
-_SIXTEEN = (torch.float16, torch.bfloat16)
-
 
 def orthogonalize(grad: Tensor, steps: int = 5, coefficients: Tuple[float, float, float] = (3.4445, -4.7750, 2.0315),
                   eps: float = 1e-7, out_dtype: Optional[torch.dtype] = None) -> Tensor:
@@ -28,36 +26,4 @@ def orthogonalize(grad: Tensor, steps: int = 5, coefficients: Tuple[float, float
     """
     if len(coefficients) != 3:
         raise _lib.SruB200Error("coefficients must be (a, b, c), got %r" % (coefficients,))
-    if _lib.timer is None and not _lib.nvtx_ranges:
-        try:
-            return _lib.native_op("orthogonalize")(grad, steps, *coefficients, eps, out_dtype)
-        except RuntimeError as e:
-            raise _lib.refused(e) from None
-    if not grad.is_cuda:
-        raise _lib.SruB200Error("sru_b200 has no CPU path: grad must be a CUDA tensor")
-    if grad.dim() not in (2, 3):
-        raise _lib.SruB200Error("grad must be (rows, cols) or (batch, rows, cols), got %s" % (tuple(grad.shape),))
-    if grad.dtype not in (torch.float32,) + _SIXTEEN:
-        raise _lib.SruB200Error("grad must be float32, float16 or bfloat16, got %s" % grad.dtype)
-    if out_dtype is None:
-        out_dtype = torch.bfloat16 if grad.dtype == torch.float32 else grad.dtype
-    if out_dtype not in _SIXTEEN:
-        raise _lib.SruB200Error("the result is float16 or bfloat16, got %s" % out_dtype)
-    out = torch.empty(grad.shape, dtype=out_dtype, device=grad.device)
-    if grad.numel() == 0:
-        return out
-    if grad.stride(-1) != 1 and grad.stride(-2) != 1:
-        grad = grad.contiguous()
-    grad = grad.detach()
-    batch = grad.size(0) if grad.dim() == 3 else 1
-    rows, cols = grad.shape[-2:]
-    L = _lib.lib()
-    a, b, c = (float(v) for v in coefficients)
-    with torch.cuda.device(grad.device):
-        nbytes = int(L.sru_b200_orthogonalize_workspace_bytes(batch, rows, cols))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)
-        _lib.call("orthogonalize", L.sru_b200_orthogonalize, _lib.ptr(out), _lib.ptr(grad), batch, rows, cols,
-                  grad.stride(0) if grad.dim() == 3 else 0, grad.stride(-2), grad.stride(-1), int(steps), a, b, c,
-                  float(eps), _lib.DTYPE_CODE[grad.dtype], _lib.DTYPE_CODE[out_dtype], _lib.ptr(ws), nbytes,
-                  _lib.current_stream_ptr(grad.device))
-    return out
+    return _lib.call_native("orthogonalize", "orthogonalize", None, grad, steps, *coefficients, eps, out_dtype)
