@@ -34,6 +34,12 @@ void check(int rc) { TORCH_CHECK(rc == 0, "sru_b200 call failed (", rc, "): ", s
 void *pointer(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 float *floats(const Tensor &t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 
+// A dual tensor need not require grad, and its tangent would be dropped without a word.
+void refuse_tangent(const OptTensor &t, const char *name, const char *op) {
+    TORCH_CHECK(!t.has_value() || !t->defined() || !t->_fw_grad(0).defined(), op, " has no forward-mode derivative, and ", name,
+                " carries a tangent");
+}
+
 // What a backward pass returns under create_graph: the gradients, with an error where they are differentiated again.
 variable_list once(variable_list grads, const char *name) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -151,6 +157,9 @@ std::tuple<Tensor, Tensor> gated_linear_recurrence(const Tensor &u, const OptTen
     check_like(u, bias, "bias", {d}, true);
     if (single) check_like(u, mask_pad, "mask_pad", {B}, false);
     else check_like(u, mask_pad, "mask_pad", {u.size(0), B}, false);
+    refuse_tangent(u, "u", "gated_linear_recurrence");
+    refuse_tangent(c0, "c0", "gated_linear_recurrence");
+    refuse_tangent(bias, "bias", "gated_linear_recurrence");
     c10::cuda::CUDAGuard guard(u.device());
     OptTensor mask;
     if (mask_pad.has_value() && mask_pad->defined()) mask = mask_pad->to(at::kBool).contiguous();      // one step: (B) as (1, B)
@@ -220,6 +229,7 @@ Tensor embedding_lookup(const Tensor &tokens, const Tensor &weight, double scale
         TORCH_CHECK(*padding >= -v && *padding < v, "padding_idx ", *padding, " is outside a table of ", v, " rows");
         padding_idx = *padding < 0 ? *padding + v : *padding;
     }
+    refuse_tangent(weight, "weight", "embedding_lookup");
     c10::cuda::CUDAGuard guard(weight.device());
     const Tensor table = weight.stride(1) == 1 && weight.stride(0) >= weight.size(1) ? weight : weight.contiguous();
     const Tensor flat = tokens.detach().reshape({-1}).contiguous();

@@ -22,6 +22,7 @@ def embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding
     float32 in the order of their positions, without atomics, so that repeated calls give identical bits.  The row of
     ``padding_idx`` (negative values count from the end, as in ``nn.Embedding``) is read like any other and gets
     no gradient.  A token outside the table gives a row of zeros and no gradient, and raises the device error
-    flag: ``_lib.check_device_error()`` then raises.
+    flag: ``_lib.check_device_error()`` then raises.  Differentiable once, in reverse mode; a table that carries a
+    forward-mode tangent is refused.
     """
     return _lib.call_native("embedding_lookup", "embedding_fwd", "embedding_bwd", tokens, weight, scale, padding_idx, out_dtype)

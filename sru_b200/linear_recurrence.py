@@ -28,6 +28,6 @@ def gated_linear_recurrence(u: Tensor, c0: Optional[Tensor] = None, bias: Option
     first.  Returns ``h`` (length, batch, hidden) in u's type and the state after the last step (batch, hidden), always in
     float32: a sequence processed in chunks, the state handed on, loses nothing to the storage type.  Strided u with
     contiguous pairs (a batch-first tensor transposed, for instance) is read in place.  Differentiable once in u, c0 and
-    bias.
+    bias, in reverse mode; a tensor that carries a forward-mode tangent is refused.
     """
     return _lib.call_native("gated_linear_recurrence", "linear_recurrence_fwd", "linear_recurrence_bwd", u, c0, bias, mask_pad, reverse)

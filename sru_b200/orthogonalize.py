@@ -22,7 +22,8 @@ def orthogonalize(grad: Tensor, steps: int = 5, coefficients: Tuple[float, float
     with X transposed where it is taller than wide.  float32, float16 or bfloat16 in; ``out_dtype`` (float16 or
     bfloat16, by default grad's type, bfloat16 for a float32 grad) out.  The iterates are fp16 with float32 accumulation:
     the result is about 1e-3 (relative, Frobenius) off exact steps, before its rounding to ``out_dtype``.  Repeated calls
-    give identical bits.  Matrices whose rows or columns are contiguous are read in place.  No gradient flows through it.
+    give identical bits.  Matrices whose rows or columns are contiguous are read in place.  No derivative flows
+    through it, in either mode: the result is a constant to autograd.
     """
     if len(coefficients) != 3:
         raise _lib.SruB200Error("coefficients must be (a, b, c), got %r" % (coefficients,))
