@@ -906,8 +906,21 @@ template <typename T, int UNIT> __global__ void __launch_bounds__(256) ns_norm_k
     }
 }
 
-// 1 / (|G|_F + eps) from the partial sums, by every block for itself.
-__device__ __forceinline__ float ns_scale(const NsEdge &e, int64_t z, float *shared) {
+// 1 / (|G|_F + eps) as two factors that are applied one after the other.  The norm of float32 or bf16 values spans 2^-149 to 2^140
+// and more, and its reciprocal leaves float32's range at both ends; a takes half of the exponent, b the rest of it and
+// the fraction.  a is a power of two, so that there is one rounding.
+struct NsScale {
+    float a, b;
+    __device__ __forceinline__ float operator()(float v) const { return v * a * b; }
+};
+__device__ __forceinline__ NsScale ns_factors(double norm) {
+    const int h = min(max(((__double2hiint(norm) >> 20) & 0x7ff) - 1023, -160), 160) >> 1;
+    const float b = (float)(1.0 / norm * __hiloint2double((1023 + h) << 20, 0));
+    // a norm of 0 leaves an infinity, and 0 * inf is the definition's 0 / 0; the smallest eps are not 0, and zeros stay zeros
+    return {__uint_as_float((uint32_t)(127 - h) << 23), norm > 0.0 ? fminf(b, 3.402823466e38f) : b};
+}
+// From the partial sums, by every block for itself.
+__device__ __forceinline__ NsScale ns_scale(const NsEdge &e, int64_t z, NsScale *shared) {
     early_next_kernel();
     previous_kernel_done();
     if (threadIdx.x < 32) {
@@ -915,7 +928,7 @@ __device__ __forceinline__ float ns_scale(const NsEdge &e, int64_t z, float *sha
         for (int p = threadIdx.x; p < e.parts; p += 32) sum += e.part[z * e.parts + p];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (threadIdx.x == 0) *shared = (float)(1.0 / (sqrt(sum) + e.eps));
+        if (threadIdx.x == 0) *shared = ns_factors(sqrt(sum) + e.eps);
     }
     __syncthreads();
     return *shared;
@@ -923,8 +936,8 @@ __device__ __forceinline__ float ns_scale(const NsEdge &e, int64_t z, float *sha
 
 // X_0 in fp16 where the iterate's rows are contiguous in the source: 8 columns per thread.
 template <typename T> __global__ void __launch_bounds__(256) ns_first_rows_kernel(const NsEdge e) {
-    __shared__ float shared;
-    const float scale = ns_scale(e, blockIdx.y, &shared);
+    __shared__ NsScale shared;
+    const NsScale scale = ns_scale(e, blockIdx.y, &shared);
     const T *g = static_cast<const T *>(e.src) + blockIdx.y * e.s_b;
     __half *x = static_cast<__half *>(e.dst) + blockIdx.y * e.x_batch;
     const int64_t per = e.ldx / 8, groups = per * e.m;
@@ -934,16 +947,16 @@ template <typename T> __global__ void __launch_bounds__(256) ns_first_rows_kerne
         load_line<T, 8>(v, g + i * e.s_i, j, e.n, e.wide);
         Pack<__half, 8> h;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) h.v[k] = __float2half_rn(v[k] * scale);
+        for (int k = 0; k < 8; ++k) h.v[k] = __float2half_rn(scale(v[k]));
         *reinterpret_cast<Pack<__half, 8> *>(x + i * e.ldx + j) = h;
     }
 }
 
 // X_0 where the iterate's columns are contiguous in the source (tall matrices): tiles of 64 x 64 through shared memory.
 template <typename T> __global__ void __launch_bounds__(256) ns_first_turned_kernel(const NsEdge e) {
-    __shared__ float shared;
+    __shared__ NsScale shared;
     __shared__ float tile[64][65];
-    const float scale = ns_scale(e, blockIdx.z, &shared);
+    const NsScale scale = ns_scale(e, blockIdx.z, &shared);
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const T *g = static_cast<const T *>(e.src) + blockIdx.z * e.s_b;
     __half *x = static_cast<__half *>(e.dst) + blockIdx.z * e.x_batch;
@@ -954,7 +967,7 @@ template <typename T> __global__ void __launch_bounds__(256) ns_first_turned_ker
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
             const int64_t i = i0 + tx + c;
-            tile[ty + k][tx + c] = (i < e.m && j < e.n) ? Cvt<T>::to_f(g[i + j * e.s_j]) * scale : 0.0f;
+            tile[ty + k][tx + c] = (i < e.m && j < e.n) ? scale(Cvt<T>::to_f(g[i + j * e.s_j])) : 0.0f;
         }
     }
     __syncthreads();
@@ -1060,7 +1073,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
     const uint32_t tmem = tmem_slot;
     t = 0.0;
     for (int w = 0; w < kSmallThreads / 32; ++w) t += sums[w];
-    const float scale = (float)(1.0 / (sqrt(t) + e.eps));
+    const NsScale scale = ns_factors(sqrt(t) + e.eps);
     // groups of 8 columns, row by row: this thread's first one, and its next from the one before
     const int first_row = (int)threadIdx.x / (tiles * 8), first_col = (int)threadIdx.x - first_row * tiles * 8;
     const int step_rows = kSmallThreads / (tiles * 8), step_cols = kSmallThreads - step_rows * tiles * 8;
@@ -1082,7 +1095,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
 #pragma unroll
             for (int k = 0; k < G; ++k) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[k][i] *= scale;
+                for (int i = 0; i < 8; ++i) v[k][i] = scale(v[k][i]);
                 if (at[k] >= 0) store_halves(x + at[k], v[k]);
             }
         }
@@ -1090,7 +1103,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
 #pragma unroll 4
         for (int u = threadIdx.x; u < kSmallM * tiles * 64; u += kSmallThreads) {
             const int i = u & (kSmallM - 1), j = u / kSmallM;
-            const float v = (i < e.m && j < e.n) ? Cvt<T>::to_f(g[i + j * e.s_j]) * scale : 0.0f;
+            const float v = (i < e.m && j < e.n) ? scale(Cvt<T>::to_f(g[i + j * e.s_j])) : 0.0f;
             asm volatile("st.shared.u16 [%0], %1;" ::"r"(x + tile_at(i, j & ~7) + (j & 7) * 2), "h"(__half_as_ushort(__float2half_rn(v))) : "memory");
         }
     }
