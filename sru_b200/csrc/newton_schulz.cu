@@ -10,8 +10,10 @@
 //   X = M X              m x n over m     X is the MN-major operand
 //
 // Iterates, A and M are held in fp16 and accumulated in float32 in tensor memory.  Everything is bounded (|X|_2 <= 1 at
-// the start and about 1.2 later, |M| below 10), so fp16's eleven bits are worth more than bf16's range: on
-// gradients with a decaying spectrum the result is 1.2e-3 off the exact steps against 1.0e-2 with bf16 iterates.
+// the start and about 1.2 later, |M| below 10), so fp16's eleven bits are worth more than bf16's range.  But X has small
+// elements (1 / sqrt(mn) at the start, 2.8e-4 at 2048 x 6144, and far less beside a few large rows), and fp16 is subnormal
+// below 6.1e-5: what is held is 2^k X, k = 12 with the usual coefficients (iterate_exponent).  The powers of two come in with
+// the norm and go out where A and the result are rounded, so they cost no rounding.
 //
 // The products run on pairs of SMs (cta_group::2, 256 x BN tiles) in a persistent grid over (matrix, tile).  A product costs
 // about 5 us beside its multiplications (load latency 1.1, accumulator to shared memory 0.8, stores and end of the grid 2, next
@@ -41,6 +43,7 @@ struct NsArgs {
     int symmetric;                  // only tiles that reach the diagonal or lie right of it; the others are mirrored
     int per_matrix;                 // tiles computed per matrix
     float ca, cb, cc;
+    float by;                       // a plain product's factor: 2^-2k for A, 2^-k for the result
     int bf16;                       // the last product's output type is the caller's
     int *err;
 };
@@ -75,6 +78,13 @@ __device__ __forceinline__ void store_halves(uint32_t at, const float (&v)[8]) {
         w[j] = *reinterpret_cast<const uint32_t *>(&h);
     }
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
+// Eight values times a power of two, two at a time.
+__device__ __forceinline__ void times(float (&v)[8], float by) {
+    const F2 by2 = f2_splat(by);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) f2_split(f2_mul(f2_make(v[j], v[j + 1]), by2), v[j], v[j + 1]);
 }
 
 // Unit -> matrix and tile.  A symmetric product keeps, of 256-row block i, the tiles from column 256 i on.
@@ -261,6 +271,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                             const float a = (j & 1) ? __high2float(a2[j >> 1]) : __low2float(a2[j >> 1]);
                             v[j] = fmaf(g.cc, v[j], fmaf(g.cb, a, row == col0 + j0 + j ? g.ca : 0.0f));
                         }
+                    } else if (g.by != 1.0f) {
+                        times(v, g.by);
                     }
                     uint32_t w[4];
                     if (MODE == kPlain && g.bf16) {
@@ -444,6 +456,7 @@ ns_gram_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     v[j + 2] += __uint_as_float(w.z);
                     v[j + 3] += __uint_as_float(w.w);
                 }
+            times(v, g.by);
             store_halves(out + lane * (P::kU * 2) + j0 * 2, v);
             if (mirror) {
 #pragma unroll
@@ -483,6 +496,7 @@ struct NsCluster {
     int64_t ldx, ldm;
     void *out;                      // the last product's, (m, n) or, turned, (n, m), contiguous; NULL: it goes to x like the others
     int turned, turned_wide, bf16;  // turned_wide: its rows are 16-byte aligned
+    float gram_by, out_by;          // 2^-2k, 2^-k
     int *err;
 };
 
@@ -624,6 +638,7 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
         } else if (split == 1) {
             const bool last = kind == 2 && g.out && product == 3 * g.steps - 1;
             const int64_t ld = kind == 2 ? (last ? g.n : g.ldx) : g.ldm;
+            const float by = kind == 0 ? g.gram_by : last ? g.out_by : 1.0f;
             __half *dst = kind == 0 ? g.a + z * (g.m * g.ldm) : kind == 1 ? g.mm + z * (g.m * g.ldm)
                           : last ? static_cast<__half *>(g.out) + z * ((int64_t)g.m * g.n) : (cur ? g.x0 : g.x1) + z * (g.m * g.ldx);
             const int N = kind == 2 ? g.n : g.m;
@@ -680,6 +695,9 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
                                     const float a = (j & 1) ? __high2float(a2[j >> 1]) : __low2float(a2[j >> 1]);
                                     v[j] = fmaf(g.cc, v[j], fmaf(g.cb, a, row == col0 + j0 + j ? g.ca : 0.0f));
                                 }
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) v[j] *= by;
                             }
                             uint32_t w[4];
 #pragma unroll
@@ -791,7 +809,7 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
                     __half *dst = g.a + z * (g.m * g.ldm);
                     __half h[16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) h[j] = __float2half_rn(v[j]);
+                    for (int j = 0; j < 16; ++j) h[j] = __float2half_rn(v[j] * g.gram_by);
                     if (i < g.m) {
 #pragma unroll
                         for (int j = 0; j < 16; j += 8) {
@@ -842,6 +860,7 @@ struct NsEdge {
     int64_t lines, len, pitch;      // the source as lines along its contiguous direction
     bool wide;                      // lines are 16-byte aligned
     double eps;
+    float up, down;                 // 2^k, 2^-k
 };
 
 // N elements from p + k on, of which those below `len` count (the others are 0); wide: p is 16-byte aligned and N * size a
@@ -906,16 +925,16 @@ template <typename T, int UNIT> __global__ void __launch_bounds__(256) ns_norm_k
     }
 }
 
-// 1 / (|G|_F + eps) as two factors that are applied one after the other.  The norm of float32 or bf16 values spans 2^-149 to 2^140
+// 2^k / (|G|_F + eps) as two factors that are applied one after the other.  The norm of float32 or bf16 values spans 2^-149 to 2^140
 // and more, and its reciprocal leaves float32's range at both ends; a takes half of the exponent, b the rest of it and
 // the fraction.  a is a power of two, so that there is one rounding.
 struct NsScale {
     float a, b;
     __device__ __forceinline__ float operator()(float v) const { return v * a * b; }
 };
-__device__ __forceinline__ NsScale ns_factors(double norm) {
+__device__ __forceinline__ NsScale ns_factors(double norm, float up) {
     const int h = min(max(((__double2hiint(norm) >> 20) & 0x7ff) - 1023, -160), 160) >> 1;
-    const float b = (float)(1.0 / norm * __hiloint2double((1023 + h) << 20, 0));
+    const float b = (float)(up / norm * __hiloint2double((1023 + h) << 20, 0));
     // a norm of 0 leaves an infinity, and 0 * inf is the definition's 0 / 0; the smallest eps are not 0, and zeros stay zeros
     return {__uint_as_float((uint32_t)(127 - h) << 23), norm > 0.0 ? fminf(b, 3.402823466e38f) : b};
 }
@@ -928,13 +947,13 @@ __device__ __forceinline__ NsScale ns_scale(const NsEdge &e, int64_t z, NsScale 
         for (int p = threadIdx.x; p < e.parts; p += 32) sum += e.part[z * e.parts + p];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (threadIdx.x == 0) *shared = ns_factors(sqrt(sum) + e.eps);
+        if (threadIdx.x == 0) *shared = ns_factors(sqrt(sum) + e.eps, e.up);
     }
     __syncthreads();
     return *shared;
 }
 
-// X_0 in fp16 where the iterate's rows are contiguous in the source: 8 columns per thread.
+// 2^k X_0 in fp16 where the iterate's rows are contiguous in the source: 8 columns per thread.
 template <typename T> __global__ void __launch_bounds__(256) ns_first_rows_kernel(const NsEdge e) {
     __shared__ NsScale shared;
     const NsScale scale = ns_scale(e, blockIdx.y, &shared);
@@ -952,7 +971,7 @@ template <typename T> __global__ void __launch_bounds__(256) ns_first_rows_kerne
     }
 }
 
-// X_0 where the iterate's columns are contiguous in the source (tall matrices): tiles of 64 x 64 through shared memory.
+// 2^k X_0 where the iterate's columns are contiguous in the source (tall matrices): tiles of 64 x 64 through shared memory.
 template <typename T> __global__ void __launch_bounds__(256) ns_first_turned_kernel(const NsEdge e) {
     __shared__ NsScale shared;
     __shared__ float tile[64][65];
@@ -990,7 +1009,7 @@ template <typename T> __global__ void __launch_bounds__(256) ns_last_kernel(cons
 #pragma unroll
     for (int k = 0; k < 32; k += 8) {
         const int i = i0 + ty + k, j = j0 + tx;
-        const float v = (i < e.m && j < e.n) ? __half2float(x[i * e.ldx + j]) : 0.0f;
+        const float v = (i < e.m && j < e.n) ? __half2float(x[i * e.ldx + j]) * e.down : 0.0f;
         if (across) tile[ty + k][tx] = v;
         else if (i < e.m && j < e.n) out[i * e.s_i + j] = Cvt<T>::from_f(v);
     }
@@ -1015,11 +1034,21 @@ constexpr int kTileBytes = 128 * 64 * 2;
 __device__ __forceinline__ uint32_t tile_at(int row, int col) {     // byte offset of 8 columns' group in the tiles
     return (uint32_t)(col >> 6) * kTileBytes + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4);
 }
+// 2^-k times two halves in the result's type: one rounding, since bf16 has room for the factor and fp16 rounds where it has not.
+__device__ __forceinline__ void put_down(uint32_t &to, __half2 h, float down, __half) {
+    const __half2 v = __hmul2(h, __float2half2_rn(down));
+    to = *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ void put_down(uint32_t &to, __half2 h, float down, __nv_bfloat16) {
+    const float2 f = __half22float2(h);
+    const __nv_bfloat162 v = __hmul2(__floats2bfloat162_rn(f.x, f.y), __float2bfloat162_rn(down));
+    to = *reinterpret_cast<const uint32_t *>(&v);
+}
 struct NsSmall {
     NsEdge e;                       // source and sizes; dst is the result
     int64_t o_i, o_j, o_b;          // strides of the result along the iterate's rows, columns, and batch
     int steps;
-    float ca, cb, cc;
+    float ca, cb, cc, gram_by;      // gram_by: 2^-2k
     bool out_wide;                  // rows of the result are 16-byte aligned
     int *err;
 };
@@ -1073,7 +1102,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
     const uint32_t tmem = tmem_slot;
     t = 0.0;
     for (int w = 0; w < kSmallThreads / 32; ++w) t += sums[w];
-    const NsScale scale = ns_factors(sqrt(t) + e.eps);
+    const NsScale scale = ns_factors(sqrt(t) + e.eps, e.up);
     // groups of 8 columns, row by row: this thread's first one, and its next from the one before
     const int first_row = (int)threadIdx.x / (tiles * 8), first_col = (int)threadIdx.x - first_row * tiles * 8;
     const int step_rows = kSmallThreads / (tiles * 8), step_cols = kSmallThreads - step_rows * tiles * 8;
@@ -1148,6 +1177,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[j0 + j]);
+            times(v, a.gram_by);
             store_halves(am + tile_at(row, part * 32 + j0), v);
         }
         settle();
@@ -1230,10 +1260,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
         for (int i = first_row, c = first_col; i < e.m;) {
             const int j = c * 8;
             const uint4 w = shared_16(x + tile_at(i, j));
-            const __half *h = reinterpret_cast<const __half *>(&w);
+            const __half2 *h = reinterpret_cast<const __half2 *>(&w);
             Pack<TO, 8> o;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) o.v[k] = Cvt<TO>::from_f(__half2float(h[k]));
+            for (int k = 0; k < 4; ++k) put_down(reinterpret_cast<uint32_t *>(&o)[k], h[k], e.down, TO());
             TO *p = out + i * a.o_i + j;
             if (a.out_wide && j + 8 <= e.n) *reinterpret_cast<Pack<TO, 8> *>(p) = o;
             else
@@ -1250,7 +1280,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
             if (i >= e.m) continue;
             uint16_t h;
             asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(x + tile_at(i, j & ~7) + (j & 7) * 2));
-            out[i + j * a.o_j] = Cvt<TO>::from_f(__half2float(__ushort_as_half(h)));
+            out[i + j * a.o_j] = Cvt<TO>::from_f(__half2float(__ushort_as_half(h)) * e.down);
         }
     }
     tc_fence_before();
@@ -1277,6 +1307,26 @@ NsPlan ns_plan(int64_t batch, int64_t rows, int64_t cols) {
     p.x_bytes = round((size_t)batch * p.m * p.ldx * 2);
     p.a_bytes = round((size_t)batch * p.m * p.ldm * 2);
     return p;
+}
+
+// k of the held iterates 2^k X: as large as elements up to 2^14 allow, a quarter of fp16's range, and 12 at most, which brings
+// the elements of 2048 x 6144 far above its subnormal end.  |x_ij| <= |X|_2 <= r, the largest value that the singular values' map
+// p(s) = a s + b s^3 + c s^5 takes step by step from [0, 1] on: its ends and its turning points.
+int iterate_exponent(int steps, double a, double b, double c) {
+    double r = 1.0;
+    auto value = [&](double s) { return std::fabs(s * (a + s * s * (b + s * s * c))); };
+    for (int i = 0; i < steps; ++i) {
+        double top = value(r);
+        auto turn = [&](double square) { if (square > 0.0 && square < r * r) top = std::max(top, value(std::sqrt(square))); };
+        // p' = a + 3 b s^2 + 5 c s^4; a root that is no number, or none, is not below r^2
+        const double q = -0.5 * (3.0 * b + std::copysign(std::sqrt(9.0 * b * b - 20.0 * a * c), b));
+        turn(q / (5.0 * c));
+        turn(a / q);
+        if (!(top < 16384.0)) return 0;                     // not a number, too
+        if (top <= r) break;
+        r = top;
+    }
+    return std::min(12, std::ilogb(16384.0 / r));
 }
 
 // (inner, rows, batch) fp16 matrices; boxes of 64 x box_rows elements in the 128-byte swizzle (of 32 elements: as they
@@ -1520,6 +1570,9 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     e.m = (int)p.m; e.n = (int)p.n;
     e.s_i = tall ? stride_col : stride_row; e.s_j = tall ? stride_row : stride_col; e.s_b = stride_batch;
     e.ldx = p.ldx; e.x_batch = p.m * p.ldx; e.eps = eps;
+    const int k = iterate_exponent(steps, ca, cb, cc);
+    e.up = std::ldexp(1.0f, k); e.down = std::ldexp(1.0f, -k);
+    const float gram_by = e.down * e.down;
     const bool turned = e.s_j != 1;
     e.lines = turned ? p.n : p.m; e.len = turned ? p.m : p.n; e.pitch = turned ? e.s_j : e.s_i;
     const int64_t size = (int64_t)dtype_size(grad_dtype);
@@ -1533,7 +1586,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         memset(&a, 0, sizeof(a));
         a.e = e; a.e.dst = out;
         a.o_i = tall ? 1 : cols; a.o_j = tall ? cols : 1; a.o_b = rows * cols;
-        a.steps = steps; a.ca = (float)ca; a.cb = (float)cb; a.cc = (float)cc; a.err = err;
+        a.steps = steps; a.ca = (float)ca; a.cb = (float)cb; a.cc = (float)cc; a.gram_by = gram_by; a.err = err;
         a.out_wide = cols % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
         auto go = [&](auto t, auto to) { return ns_small<decltype(t), decltype(to)>(a, batch, st); };
         auto go_out = [&](auto t) { return out_dtype == SRU_F16 ? go(t, __half()) : go(t, __nv_bfloat16()); };
@@ -1573,6 +1626,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc;
         g.x0 = x[0]; g.x1 = x[1]; g.a = a_buf; g.mm = m_buf; g.ldx = p.ldx; g.ldm = p.ldm;
         g.out = direct ? out : nullptr; g.turned = tall; g.turned_wide = aligned; g.bf16 = out_dtype == SRU_BF16; g.err = err;
+        g.gram_by = gram_by; g.out_by = e.down;
         if (int rc = ns_cluster(xm[0], xm[1], am, mm, g, batch, ctas, st)) return rc;
     }
     for (int s = 0; s < steps && !ctas; ++s) {
@@ -1581,7 +1635,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         memset(&g, 0, sizeof(g));
         g.batch = (int)batch; g.err = err;
         g.M = (int)p.m; g.N = (int)p.m; g.K = (int)p.n; g.symmetric = 1;
-        g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc;
+        g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc; g.by = gram_by;
         const int64_t tiles = ((p.m + 255) / 256) * ((p.m + 127) / 128 - (p.m + 255) / 256 + 1) * batch;
         const int split = choose_split(tiles, (p.n + kBK - 1) / kBK);
         int rc = split == 8 ? ns_gram_split<8>(xm[cur], a_buf, p.ldm, g, st) : split == 4 ? ns_gram_split<4>(xm[cur], a_buf, p.ldm, g, st)
@@ -1592,6 +1646,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         g.N = (int)p.n; g.symmetric = 0;
         const bool last = s == steps - 1 && direct;
         g.bf16 = last && out_dtype == SRU_BF16;
+        g.by = last ? e.down : 1.0f;
         if (last && tall) {             // X^T = X_before^T M, rows as the caller has them
             g.M = (int)p.n; g.N = (int)p.m;
             if (int rc = ns_product<128, true, false, kPlain>(xm[cur], mm, om, am, g, sms, st)) return rc;

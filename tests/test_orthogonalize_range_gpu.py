@@ -36,3 +36,57 @@ def test_zeros(rows, cols):
             assert not orthogonalize(zeros, eps=eps).any(), eps
         assert orthogonalize(zeros, eps=0.0).isnan().all()
         assert not orthogonalize(torch.ones_like(zeros), eps=1e300).any()
+
+
+def steps64(g, rounded, abc=(3.4445, -4.7750, 2.0315), steps=5):
+    """The steps in 64 bits; rounded: with A and M rounded to fp16 and X to fp16's eleven bits, not to its range."""
+    half = (lambda t: t.half().double()) if rounded else (lambda t: t)
+    held = (lambda t: (t * 4096).half().double() / 4096) if rounded else (lambda t: t)
+    x = g.double()
+    x = x.mT if x.size(0) > x.size(1) else x
+    x = held(x / (x.norm() + 1e-7))
+    eye = torch.eye(x.size(0), dtype=torch.float64)
+    for _ in range(steps):
+        a = half(x @ x.mT)
+        x = held(half(abc[0] * eye + abc[1] * a + abc[2] * (a @ a)) @ x)
+    return x.mT if g.size(0) > g.size(1) else x
+
+
+@pytest.mark.parametrize("rows,cols", [(128, 384), (384, 128), (256, 1024), (500, 500), (900, 700), (64, 4200), (1024, 1536)])
+@pytest.mark.parametrize("large", [1e4, 1e5])
+def test_one_row_far_above_the_others(rows, cols, large):
+    """The elements of the other rows lie where fp16 is subnormal and has a few bits left; 2^12 X keeps all eleven.  Allowed: 1.5
+    times what the roundings do to 64-bit steps without a range (0.8e-3 to 2.2e-3 of the norm), and half a step of fp16."""
+    g = torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows + cols))
+    g[3] *= large
+    want, model = steps64(g, False), steps64(g, True)
+    norm = float(want.norm())
+    got = orthogonalize(g.to(DEV), out_dtype=F16).cpu().double()
+    assert float((got - want).norm()) <= 1.5 * float((model - want).norm()) + 2.0 ** -11 * norm
+    assert float((model - want).norm()) <= 2.3e-3 * norm
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("a", [3.0, -2.0, 8.0, 12.0])
+def test_coefficients_that_let_the_iterates_grow(rows, cols, a):
+    """X <- a X three times: |a|^3 X_0 whatever power of two is held (9, 11, 5 and 3 of the usual 12).  X_0, each of
+    three steps and the result round to eleven bits (relative 2^-11; where fp16 is subnormal, half of its smallest step, which
+    later steps multiply), and nothing overflows (A = X X^T is at most 12^4)."""
+    g = torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows))
+    got = orthogonalize(g.to(DEV), steps=3, coefficients=(a, 0.0, 0.0), out_dtype=F16).cpu().double()
+    want = a ** 3 * g.double() / (g.double().norm() + 1e-7)
+    assert got.isfinite().all()
+    tiny = 2.0 ** -25 * (abs(a) ** 3 + a ** 2 + abs(a) + 2)
+    assert bool(((got - want).abs() <= 5.05 * 2.0 ** -11 * want.abs() + tiny).all())
+    _lib.check_device_error()
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_no_steps(rows, cols):
+    """G / |G| alone, rounded to eleven bits and to the result's type."""
+    g = torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows))
+    want = g.double() / (g.double().norm() + 1e-7)
+    for out in (F16, BF16):
+        got = orthogonalize(g.to(DEV), steps=0, out_dtype=out).cpu().double()
+        bound = (2.0 ** -11 + torch.finfo(out).eps / 2) * 1.01 * want.abs() + (2.0 ** -25 if out == F16 else 2.0 ** -37)
+        assert bool(((got - want).abs() <= bound).all())
