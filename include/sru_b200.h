@@ -390,8 +390,11 @@ int sru_b200_embedding_backward(
  *
  *   X_0 = G / (|G|_F + eps),   `steps` times  X <- a X + (b A + c A A) X,  A = X X^T     (X the smaller side first)
  *
- * on the tensor cores, with fp16 iterates and float32 accumulation (about 1e-3 off the exact steps with the usual
- * a, b, c = 3.4445, -4.7750, 2.0315; coefficients that let the iterates leave fp16's range give infinities).
+ * on the tensor cores, with iterates held to eleven bits (fp16, scaled by a power of two) and float32 accumulation.  Off the
+ * exact steps (relative, Frobenius; five steps with the usual a, b, c = 3.4445, -4.7750, 2.0315; before the rounding to out's
+ * type): below 2.5e-3 for matrices that are mostly noise, 6e-3 for singular values that fall off as 1 / i, 3e-2 as 1 / i^2, 6e-2 for
+ * four strong directions over noise of a hundredth of their size; the steps multiply small singular values, and the roundings
+ * beside them, by up to a^steps.  Coefficients that let X or X X^T leave fp16's range give infinities.
  *   grad   `batch` matrices (rows, cols), SRU_F32, SRU_F16 or SRU_BF16, element (z, i, j) at
  *          z * stride_batch + i * stride_row + j * stride_col, one of stride_row, stride_col being 1
  *   out    (batch, rows, cols) contiguous, SRU_F16 or SRU_BF16
