@@ -55,6 +55,8 @@ void count_launch();
         ::srub::count_launch();                                                            \
     } while (0)
 
+constexpr int kSms = 148;           // a B200's, for rules of work per SM that were measured on it; no kernel depends on it
+
 static inline size_t dtype_size(int dt) {
     switch (dt) {
         case SRU_F32: return 4;

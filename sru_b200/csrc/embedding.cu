@@ -517,7 +517,7 @@ template <typename TK, typename TI, typename TO> int launch_forward(const EmbArg
     };
     if (!wide) return go(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
     // a few rows: one group per thread, so that they reach all SMs
-    if (a.n * (a.d / VEC) < 148 * 2048) return go(std::integral_constant<int, VEC>(), std::integral_constant<int, 1>());
+    if (a.n * (a.d / VEC) < kSms * 2048) return go(std::integral_constant<int, VEC>(), std::integral_constant<int, 1>());
     return go(std::integral_constant<int, VEC>(), std::integral_constant<int, 2>());
 }
 
@@ -562,7 +562,7 @@ template <typename TK, typename TI, typename TO> int launch_backward(const EmbAr
         }
         if (int rc = launch_sort<TK>(a, st)) return rc;
         const int64_t units = (a.n + kTile - 1) / kTile * per_row;
-        const int64_t sums = std::min<int64_t>((units + 3) / 4, 148 * 64), fill = (a.v + kFillRows - 1) / kFillRows;
+        const int64_t sums = std::min<int64_t>((units + 3) / 4, kSms * 64), fill = (a.v + kFillRows - 1) / kFillRows;
         cudaLaunchConfig_t cfg;
         memset(&cfg, 0, sizeof(cfg));
         cudaLaunchAttribute early = early_launch();

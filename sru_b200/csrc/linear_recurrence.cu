@@ -819,9 +819,9 @@ Slices choose_slices(int64_t L, int64_t B, int64_t d, int dtype, bool backward) 
     // 226 in eight; 256 (8192 x 16 x 1024) 166 / 341 in four, 148 / 281 in eight, 181 / 344 in sixteen; 32 (65536 x 2048) 2410 in
     // one walk and 193 in 64.
     if (want <= 0) {
-        want = columns < 148 * 6 ? 4 : 1;
+        want = columns < kSms * 6 ? 4 : 1;
         if (want > 1)
-            while (want < 64 && columns * want * 2 <= 148 * 14) want *= 2;
+            while (want < 64 && columns * want * 2 <= kSms * 14) want *= 2;
     }
     // two CTAs an SM: eight warps' float32 stages of the backward pass would leave room for one (4096 x 4 x 512 in 64 slices
     // 75 us, in 56 of seven warps 49)

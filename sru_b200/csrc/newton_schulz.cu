@@ -502,11 +502,17 @@ struct NsCluster {
     int *err;
 };
 
-// Pairs that share a tile of X X^T; the exchange takes as long as ten blocks.
+// What joining the sums of a tile costs beside the sums themselves, in blocks of 64 of the reduction of a 256 x 128 tile (0.26 us),
+// from the times with and without it over reductions of 256 to 4096: between the pairs of a cluster that takes a matrix through
+// all steps 7 (two pairs) to 13 (four), in the launch of its own 3 (two), 4 to 6 (four) and 5 to 10 (eight).
+constexpr int kClusterJoin = 10, kSplitJoin = 4;
+
+// Pairs that share a tile of X X^T.  Five steps with one / two / four pairs, us: 200 x 256 72 / 78 / 83, 200 x 768 83 / 84 / 85, 200 x 1024
+// 88 / 87 / 87, 200 x 4096 166 / 137 / 125, 384 x 1152 116 / 120, 384 x 1536 125 / 125.
 __host__ __device__ inline int pairs_per_tile(int tiles, int pairs, int blocks) {
     int s = 1;
     while (s < 8 && tiles * s * 2 <= pairs) s *= 2;
-    return blocks - blocks / s < 10 ? 1 : s;
+    return blocks - blocks / s < kClusterJoin ? 1 : s;
 }
 
 // M X on 256 columns a tile where pairs have more than one tile of 128: what L2 hands an SM then keeps the tensor cores busy (521
@@ -1451,10 +1457,10 @@ int ns_cluster(const NsMaps &x0, const NsMaps &x1, const NsMaps &a, const NsMaps
 }
 
 // Pairs that share a tile of X X^T, by the number of tiles and the 64-element blocks of the reduction: as many as the GPU holds
-// clusters for (7, 15 and 33 of 16, 8 and 4 CTAs) while the exchange (1 us) is shorter than what it saves.  Five steps with 1 /
-// 2 / 4 / 8 pairs: 64 x 6144 194 / 142 / 118 / 104 us, 64 x 4000 154 / 132 / 124 / 124, 512 x 6144 235 / 181 / 154 / 143; with 1 / 2 /
-// 4: two 500 x 2000 164 / 147 / 139, 500 x 500 141 / 137 / 135; with 1 / 2: four 300 x 1500 (16 tiles) 138 / 129, 1024 x 4096 (20
-// tiles) 222 / 188, two 700 x 700 (24 tiles) 144 / 140.
+// clusters for (7, 15 and 33 of 16, 8 and 4 CTAs) while joining the sums is shorter than what that saves.  Five steps in a captured
+// graph with 1 / 2 / 4 / 8 pairs: 100 x 4096 144 / 111 / 93 / 87 us, 100 x 2048 104 / 89 / 82 / 82, 200 x 512 82 / 81 / 80 / 85, 200 x 4096
+// 153 / 118 / 101 / 95, 512 x 512 99 / 96 / 95 / 99, 512 x 4096 170 / 135 / 117 / 115; with 1 / 2: 1024 x 1024 133 / 126, 1024 x 4096 201 / 168,
+// four 300 x 512 (16 tiles) 87 / 88, four 300 x 1536 108 / 101.
 int choose_split(int64_t tiles, int64_t blocks) {
     if (tiles <= 7 && blocks >= 64) return 8;
     if (tiles <= 15 && blocks >= 8) return 4;
@@ -1462,27 +1468,29 @@ int choose_split(int64_t tiles, int64_t blocks) {
     return 1;
 }
 
-// CTAs of a cluster that takes a matrix through all its steps, or 0: a launch per product.  Both are counted in blocks (64 of the
-// reduction of a 256 x 128 tile, 0.23 us) that a pair of SMs works through in a step; a tile's epilogue takes as long as six, a
-// wide one's twelve, an exchange between pairs eight.  A cluster where it has at most four more, which its cheaper change from
-// product to product makes up for, and the GPU holds clusters for the batch (7 of 16 CTAs, 15 of 8).  Launches / cluster, us, and
-// what the cluster has more: 500 x 500 132 / 118 (-10), 130 x 200 96 / 81 (-6), 256 x 1024 101 / 91 (0), six 512 x 2048 179 / 166 (0),
-// seven 512 x 1536 169 / 155 (0), fifteen 384 x 384 118 / 106 (0), 384 x 1024 115 / 117 (2), seven 300 x 1500 139 / 135 (6), five 512 x
-// 2048 157 / 161 (8), three 300 x 1500 119 / 129 (12), ten 512 x 512 133 / 136 (16), six 600 x 600 146 / 180 (32).
+// CTAs of a cluster that takes a matrix through all its steps, or 0: a launch per product.  Both are counted in blocks (as above)
+// that a pair of SMs works through in a step; a tile's epilogue takes as long as six, a wide one's twelve, joined sums what stands
+// above.  A cluster where it has at most four more, which its cheaper change from product to product makes up for (2 us a step
+// between launches of a stream), and the GPU holds clusters for the batch (7 of 16 CTAs, 15 of 8).  Launches / cluster on a stream,
+// us, and what the cluster has more: seven 256 x 512 98 / 81 (-8), 500 x 500 128 / 116 (-6), 130 x 200 91 / 77 (-6), 200 x 768 98 / 89 (-4),
+// 256 x 1024 96 / 87 (0), seven 300 x 1500 136 / 132 (0), six 512 x 2048 174 / 160 (0), fifteen 384 x 384 115 / 103 (0); 200 x 2048 106 / 105
+// (6), 384 x 1024 109 / 111 (6), 512 x 1024 114 / 118 (6), five 512 x 2048 153 / 159 (12), ten 512 x 512 125 / 130 (16), three 300 x 1500
+// 115 / 127 (18), six 600 x 600 143 / 175 (32).  In a captured graph launches follow each other faster, and a cluster is up to 4 us slower
+// where the count is 0.
 int choose_cluster(int64_t m, int64_t n, int64_t batch, int sms) {
     if (batch > 15) return 0;
     const int64_t ctas = batch <= 7 ? 16 : 8, pairs = ctas / 2, rows = (m + 255) / 256, square = rows * ((m + 127) / 128 - rows + 1);
     const int64_t blocks_m = (m + kBK - 1) / kBK, blocks_n = (n + kBK - 1) / kBK;
     const int64_t narrow = rows * ((n + 127) / 128), wide = rows * ((n + 255) / 256), wide_cost = std::max<int64_t>(blocks_m * 6 / 5, 12);
     auto tiles = [](int64_t count, int64_t pairs, int64_t cost) { return (count + pairs - 1) / pairs * cost; };
-    auto gram = [&](int64_t count, int64_t pairs, int split) {
-        return tiles(count * split, pairs, std::max<int64_t>(blocks_n / split, 6)) + (split > 1 ? 8 : 0) +
+    auto gram = [&](int64_t count, int64_t pairs, int split, int join) {
+        return tiles(count * split, pairs, std::max<int64_t>(blocks_n / split, 6)) + (split > 1 ? join : 0) +
                tiles(count, pairs, std::max<int64_t>(blocks_m, 6));
     };
-    const int64_t here = gram(square, pairs, pairs_per_tile((int)square, (int)pairs, (int)blocks_n)) +
+    const int64_t here = gram(square, pairs, pairs_per_tile((int)square, (int)pairs, (int)blocks_n), kClusterJoin) +
                          (wide_tiles((int)narrow, (int)pairs, (int)blocks_m) ? tiles(wide, pairs, wide_cost)
                                                                              : tiles(narrow, pairs, std::max<int64_t>(blocks_m, 6)));
-    const int64_t launches = gram(square * batch, sms / 2, choose_split(square * batch, blocks_n)) + tiles(wide * batch, sms / 2, wide_cost);
+    const int64_t launches = gram(square * batch, sms / 2, choose_split(square * batch, blocks_n), kSplitJoin) + tiles(wide * batch, sms / 2, wide_cost);
     return here <= launches + 4 ? (int)ctas : 0;
 }
 
@@ -1552,7 +1560,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     if (!workspace || workspace_bytes < p.total() || reinterpret_cast<uintptr_t>(workspace) % 256)
         return set_error(SRU_ERR_WORKSPACE, "256-byte aligned workspace of %zu bytes needed, %zu given", p.total(), workspace_bytes);
     if (int rc = ensure_context()) return rc;
-    int dev = 0, sms = 148;
+    int dev = 0, sms = 0;
     SRUB_CUDA_CHECK(cudaGetDevice(&dev));
     SRUB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     int *err = device_error_flag();
@@ -1580,7 +1588,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     const int64_t size = (int64_t)dtype_size(grad_dtype);
     e.wide = reinterpret_cast<uintptr_t>(grad) % 16 == 0 && e.pitch * size % 16 == 0 && (batch == 1 || e.s_b * size % 16 == 0);
     if (e.pitch == e.len || e.lines == 1) { e.len *= e.lines; e.lines = 1; e.pitch = 0; }       // one line
-    const int unit = e.lines * ((e.len + 2047) / 2048) * batch < 148 * 8 ? 512 : 2048;
+    const int unit = e.lines * ((e.len + 2047) / 2048) * batch < sms * 8 ? 512 : 2048;
     e.parts = (int)std::min<int64_t>((e.lines * ((e.len + unit - 1) / unit) + 7) / 8, kMaxParts);
     const dim3 norm_grid((unsigned)e.parts, (unsigned)batch);
     if (p.m <= kSmallM && p.n <= kSmallN) {
@@ -1603,7 +1611,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
             const dim3 grid((unsigned)((p.ldx + 63) / 64), (unsigned)((p.m + 63) / 64), (unsigned)batch);
             return launch_early(grid, ns_first_turned_kernel<T>, e, st);
         } else {
-            const dim3 grid((unsigned)std::min<int64_t>((p.m * p.ldx / 8 + 255) / 256, 148 * 8), (unsigned)batch);
+            const dim3 grid((unsigned)std::min<int64_t>((p.m * p.ldx / 8 + 255) / 256, sms * 8), (unsigned)batch);
             return launch_early(grid, ns_first_rows_kernel<T>, e, st);
         }
     };

@@ -64,7 +64,7 @@ def test_embedding(n, vocabulary, launches):
     assert counted(lambda: torch.autograd.grad(embedding_lookup(t, w), w, dy)) == launches
 
 
-@pytest.mark.parametrize("shape,launches", [((100, 300), 1), ((256, 1024), 3), ((256, 1025), 4), ((2048, 2048), 17), ((700, 900), None),
+@pytest.mark.parametrize("shape,launches", [((100, 300), 1), ((256, 1024), 3), ((256, 1025), 18), ((2048, 2048), 17), ((700, 900), None),
                                             ((64, 4200), None)])
 def test_orthogonalize(shape, launches):
     g = torch.randn(shape, device=DEV)
