@@ -390,19 +390,24 @@ int sru_b200_embedding_backward(
  *
  *   X_0 = G / (|G|_F + eps),   `steps` times  X <- a X + (b A + c A A) X,  A = X X^T     (X the smaller side first)
  *
- * on the tensor cores, with iterates held to eleven bits (fp16, scaled by a power of two) and float32 accumulation.  Off the
- * exact steps (relative, Frobenius; five steps with the usual a, b, c = 3.4445, -4.7750, 2.0315; before the rounding to out's
- * type): below 2.5e-3 for matrices that are mostly noise, 6e-3 for singular values that fall off as 1 / i, 3e-2 as 1 / i^2, 6e-2 for
- * four strong directions over noise of a hundredth of their size; the steps multiply small singular values, and the roundings
- * beside them, by up to a^steps.  Coefficients that let X or X X^T leave fp16's range give infinities.
+ * on the tensor cores, with float32 accumulation.  The iterates have the bits that the result's type needs.
+ *   out SRU_BF16 (eight bits): iterates of eleven bits, fp16 scaled by a power of two.  Off the exact steps (relative, Frobenius;
+ *     five steps with the usual a, b, c = 3.4445, -4.7750, 2.0315; before the rounding to bf16): below 2.5e-3 for matrices that are
+ *     mostly noise, 6e-3 for singular values that fall off as 1 / i, 3e-2 as 1 / i^2, 6e-2 for four strong directions over noise
+ *     of a hundredth of their size; the steps multiply small singular values, and the roundings beside them, by up to a^steps
+ *   out SRU_F16 (eleven bits): pairs of fp16, 22 bits, and three products for each, at 1.5 to 4 times the time.  The exact steps
+ *     rounded once: 2.1e-4 (at most 3e-4, and 7e-4 for the four directions)
+ * Coefficients that let X or X X^T leave fp16's range give infinities or NaN.
  *   grad   `batch` matrices (rows, cols), SRU_F32, SRU_F16 or SRU_BF16, element (z, i, j) at
  *          z * stride_batch + i * stride_row + j * stride_col, one of stride_row, stride_col being 1
  *   out    (batch, rows, cols) contiguous, SRU_F16 or SRU_BF16
- *   workspace   256-byte aligned, ..._workspace_bytes(); calls that share one must be stream-ordered
+ *   workspace   256-byte aligned, ..._workspace_bytes_for() (..._workspace_bytes() is enough for either type of the result);
+ *          calls that share one must be stream-ordered
  * The norm is summed in 64 bits in a fixed order: repeated calls give identical bits.  The reference has no such
  * operator; its applications step plain SGD and Adam (language_model/train_enwik8.py).
  */
 size_t sru_b200_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
+size_t sru_b200_orthogonalize_workspace_bytes_for(int64_t batch, int64_t rows, int64_t cols, int out_dtype);
 
 int sru_b200_orthogonalize(
     void *out, const void *grad, int64_t batch, int64_t rows, int64_t cols,

@@ -92,6 +92,8 @@ def lib():
         l.sru_b200_embedding_backward.argtypes = [_vp] * 3 + [_i64] * 4 + [ctypes.c_double] + [_int] * 3 + [_vp, ctypes.c_size_t, _vp]
         l.sru_b200_orthogonalize_workspace_bytes.restype = ctypes.c_size_t
         l.sru_b200_orthogonalize_workspace_bytes.argtypes = [_i64] * 3
+        l.sru_b200_orthogonalize_workspace_bytes_for.restype = ctypes.c_size_t
+        l.sru_b200_orthogonalize_workspace_bytes_for.argtypes = [_i64] * 3 + [_int]
         l.sru_b200_orthogonalize.restype = _int
         l.sru_b200_orthogonalize.argtypes = ([_vp] * 2 + [_i64] * 6 + [_int] + [ctypes.c_double] * 4 + [_int] * 2
                                              + [_vp, ctypes.c_size_t, _vp])

@@ -17,6 +17,12 @@
 // roundings; with bf16 iterates; 768 x 2304): normal 1.1e-3; 9.0e-3, singular values as 1 / i 4.0e-3; 3.2e-2, as 1 / i^2 2.1e-2;
 // 1.7e-1.  Most of it is X_0's rounding, which the steps multiply by up to a^steps along the smallest singular directions.
 //
+// That is enough for a result in bf16, not for one in fp16, which has as many bits as such iterates.  There X, A and M are pairs of
+// fp16 (PAIR: the value rounded, and the rest rounded), 22 bits; each product is three, lower times lower left out, in one
+// accumulator, and an epilogue stores both parts.  The result is the exact steps rounded once: 2.1e-4 off where eleven bits
+// gave 1.0e-3 (2.1e-4 and 2e-2 for 1 / i^2).  2048 x 6144 1366 us instead of 495, 256 x 1024 145 instead of 87.  Pairs take a launch
+// per product: the one-SM and the one-cluster form below have neither the shared memory nor the bits for them.
+//
 // The products run on pairs of SMs (cta_group::2, 256 x BN tiles) in a persistent grid over (matrix, tile).  A product costs
 // about 5 us beside its multiplications (load latency 1.1, accumulator to shared memory 0.8, stores and end of the grid 2, next
 // kernel 1.2), which is most of the time up to 1024 x 1024.  Long products take 440 cycles per 64 of K with 128 columns and 521
@@ -46,7 +52,7 @@ struct NsArgs {
     int per_matrix;                 // tiles computed per matrix
     float ca, cb, cc;
     float by;                       // a plain product's factor: 2^-2k for A, 2^-k for the result
-    int bf16;                       // the last product's output type is the caller's
+    int last;                       // it writes the caller's matrix
     int *err;
 };
 
@@ -89,6 +95,44 @@ __device__ __forceinline__ void times(float (&v)[8], float by) {
     for (int j = 0; j < 8; j += 2) f2_split(f2_mul(f2_make(v[j], v[j + 1]), by2), v[j], v[j + 1]);
 }
 
+__device__ __forceinline__ void pack_halves(uint32_t (&w)[4], const float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+// What rounding v to w has left out, rounded in turn: v = w + lo to 22 bits, or to the last bit of fp16's smallest step.
+__device__ __forceinline__ void pack_rest(uint32_t (&lo)[4], const uint32_t (&w)[4], const float (&v)[8]) {
+    float rest[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+        rest[2 * j] = v[2 * j] - h.x;
+        rest[2 * j + 1] = v[2 * j + 1] - h.y;
+    }
+    pack_halves(lo, rest);
+}
+__device__ __forceinline__ void shared_store(uint32_t at, const uint32_t (&w)[4]) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+// Eight values of a row, columns j0 on, at [column][row]: the 32 lanes of a store fill 64 contiguous bytes.
+__device__ __forceinline__ void shared_turn(uint32_t turned, int j0, int lane, const uint32_t (&w)[4]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(turned + (j0 + j) * 64 + lane * 2), "h"((uint16_t)(w[j >> 1] >> (16 * (j & 1)))) : "memory");
+}
+
+// Pairs: a product of sums of two is three products, the small ones first, while the accumulator is small and its own
+// rounding with it.  Block kb of 3 * blocks -> block of the reduction; *za, *zb: the operands' matrices (upper parts first,
+// `batch` of them, then the lower ones).
+__device__ __forceinline__ int pair_block(int kb, int blocks, int batch, int *za, int *zb) {
+    const int part = kb / blocks;
+    *zb += part == 0 ? batch : 0;
+    *za += part == 1 ? batch : 0;
+    return kb - part * blocks;
+}
+
 // Unit -> matrix and tile.  A symmetric product keeps, of 256-row block i, the tiles from column 256 i on.
 template <int BN> __device__ __forceinline__ void ns_unit(const NsArgs &g, int unit, int *z, int *mb, int *nb) {
     *z = unit / g.per_matrix;
@@ -104,16 +148,18 @@ template <int BN> __device__ __forceinline__ void ns_unit(const NsArgs &g, int u
     }
 }
 
-// TURN: the product may be symmetric.
-template <int BN, bool TURN> struct NsShape {
+// TURN: the product may be symmetric.  PAIR: operands and output are pairs.
+template <int BN, bool TURN, bool PAIR> struct NsShape {
+    static constexpr int kParts = PAIR ? 2 : 1;
     static constexpr int kBBytes = BN / 2 * kBK * 2;
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kCols = BN / 2;                        // columns of an epilogue warp
     static constexpr int kOut = 32 * kCols * 2;                 // its 32 rows, boxes of 64 columns
     static constexpr int kTurned = TURN ? kCols * 32 * 2 : 0;      // the same transposed, for the mirrored tile
-    static constexpr int kStages = BN == 128 ? 6 : TURN ? 3 : 5;
+    static constexpr int kStages = PAIR ? (BN == 128 ? 4 : 3) : BN == 128 ? 6 : TURN ? 3 : 5;
     static constexpr int kBars = 1024;
-    static constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * (kOut + kTurned) + 1024 + kBars;
+    static constexpr int kStaging = kParts * (kOut + kTurned);  // of a warp: the parts, the parts transposed
+    static constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kStaging + 1024 + kBars;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -125,17 +171,17 @@ template <int BN, bool TURN> struct NsShape {
 // 32 x 64 to the copy engine, which clips what lies outside the matrix.  kCombine's A comes the same way into the same
 // place, asked for before the accumulator is ready.  A tile right of the diagonal of a symmetric product is staged a second
 // time transposed and stored as its mirror image.
-template <int BN, bool AMN, bool BMN, int MODE>
+template <int BN, bool AMN, bool BMN, int MODE, bool PAIR>
 __global__ void __launch_bounds__(kNsThreads, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_t,
                   const __grid_constant__ CUtensorMap map_d, const NsArgs g) {
     constexpr bool TURN = !AMN && !BMN;
-    using S = NsShape<BN, TURN>;
+    using S = NsShape<BN, TURN, PAIR>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *staging = smem + S::kStages * S::kStageBytes;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * (S::kOut + S::kTurned));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * S::kStaging);
     const uint32_t bar_full = smem_u32(bars);                 // in the leader: loads of both CTAs
     const uint32_t bar_empty = bar_full + 8 * S::kStages;
     const uint32_t bar_tfull = bar_empty + 8 * S::kStages;    // [2]
@@ -147,7 +193,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     const uint32_t rank = cluster_ctarank();
     const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
     const int nunits = g.per_matrix * g.batch;
-    const int nkb = (g.K + kBK - 1) / kBK;
+    const int blocks = (g.K + kBK - 1) / kBK, nkb = PAIR ? 3 * blocks : blocks;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) { mbar_init(bar_full + 8 * s, 1); mbar_init(bar_empty + 8 * s, 1); }
@@ -181,17 +227,19 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     const uint32_t full = bar_full + 8 * stage;
                     if (rank == 0) mbar_arrive_expect_tx(full, 2 * S::kStageBytes);
                     const uint32_t sa = smem_u32(smem + stage * S::kStageBytes), sb = sa + kABytes;
+                    int za = z, zb = z;
+                    const int k0 = (PAIR ? pair_block(kb, blocks, g.batch, &za, &zb) : kb) * kBK;
                     if (!AMN) {
-                        tma_load_3d_pair(sa, &map_a, full, kb * kBK, m0, z);
+                        tma_load_3d_pair(sa, &map_a, full, k0, m0, za);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) tma_load_3d_pair(sa + j * 8192, &map_a, full, m0 + j * 64, kb * kBK, z);
+                        for (int j = 0; j < 2; ++j) tma_load_3d_pair(sa + j * 8192, &map_a, full, m0 + j * 64, k0, za);
                     }
                     if (!BMN) {
-                        tma_load_3d_pair(sb, &map_b, full, kb * kBK, n0, z);
+                        tma_load_3d_pair(sb, &map_b, full, k0, n0, zb);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < BN / 128; ++j) tma_load_3d_pair(sb + j * 8192, &map_b, full, n0 + j * 64, kb * kBK, z);
+                        for (int j = 0; j < BN / 128; ++j) tma_load_3d_pair(sb + j * 8192, &map_b, full, n0 + j * 64, k0, zb);
                     }
                     if (++stage == S::kStages) { stage = 0; phase ^= 1; }
                 }
@@ -229,7 +277,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         const int half = (warp - 2) >> 2, first = half * S::kCols;      // half of the columns
         const uint32_t bar_mine = bar_d + 8 * (half * 4 + q);
         const uint32_t tempty_leader = map_to_cta(bar_tempty, 0);
-        const uint32_t out = smem_u32(staging + (half * 4 + q) * (S::kOut + S::kTurned)), turned = out + S::kOut;
+        const uint32_t out = smem_u32(staging + (half * 4 + q) * S::kStaging), turned = out + S::kParts * S::kOut;
+        const int parts = PAIR && !g.last ? 2 : 1;          // of the output
         int it = 0;
         for (int unit = pair; unit < nunits; unit += npairs, ++it) {
             int z, mb, nb;
@@ -240,9 +289,11 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             if (lane == 0) {
                 bulk_wait_read_all();           // the stores of the tile before have left the staging
                 if (MODE == kCombine) {
-                    mbar_arrive_expect_tx(bar_mine, S::kOut);
+                    mbar_arrive_expect_tx(bar_mine, S::kParts * S::kOut);
 #pragma unroll
-                    for (int b = 0; b < S::kCols / 64; ++b) tma_load_3d(out + b * 4096, &map_d, bar_mine, nb * BN + first + b * 64, row0, z);
+                    for (int b = 0; b < S::kParts * S::kCols / 64; ++b)
+                        tma_load_3d(out + b * 4096, &map_d, bar_mine, nb * BN + first + b % (S::kCols / 64) * 64, row0,
+                                    z + b / (S::kCols / 64) * g.batch);
                 }
             }
             __syncwarp();
@@ -265,39 +316,37 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[j0 + j]);
                     if (MODE == kCombine) {
-                        uint4 d;
-                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(d.x), "=r"(d.y), "=r"(d.z), "=r"(d.w) : "r"(at));
+                        const uint4 d = shared_16(at);
                         const __half2 *a2 = reinterpret_cast<const __half2 *>(&d);
+                        uint4 d_lo = make_uint4(0, 0, 0, 0);
+                        if (PAIR) d_lo = shared_16(at + S::kOut);
+                        const __half2 *lo2 = reinterpret_cast<const __half2 *>(&d_lo);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const float a = (j & 1) ? __high2float(a2[j >> 1]) : __low2float(a2[j >> 1]);
+                            float a = (j & 1) ? __high2float(a2[j >> 1]) : __low2float(a2[j >> 1]);
+                            if (PAIR) a += (j & 1) ? __high2float(lo2[j >> 1]) : __low2float(lo2[j >> 1]);
                             v[j] = fmaf(g.cc, v[j], fmaf(g.cb, a, row == col0 + j0 + j ? g.ca : 0.0f));
                         }
                     } else if (g.by != 1.0f) {
                         times(v, g.by);
                     }
                     uint32_t w[4];
-                    if (MODE == kPlain && g.bf16) {
+                    if (MODE == kPlain && !PAIR && g.last) {    // bf16; of pairs the result is fp16, like all before it
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
                             w[j] = *reinterpret_cast<const uint32_t *>(&h);
                         }
                     } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-                            w[j] = *reinterpret_cast<const uint32_t *>(&h);
-                        }
+                        pack_halves(w, v);
                     }
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-                    if (TURN && mirror) {
-                        // element (row, col) at [col][row]: the 32 lanes of a store fill 64 contiguous bytes
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const uint16_t e = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
-                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(turned + (cc * 32 + j0 + j) * 64 + lane * 2), "h"(e) : "memory");
-                        }
+                    shared_store(at, w);
+                    if (TURN && mirror) shared_turn(turned, cc * 32 + j0, lane, w);
+                    if (PAIR && parts == 2) {
+                        uint32_t lo[4];
+                        pack_rest(lo, w, v);
+                        shared_store(at + S::kOut, lo);
+                        if (TURN && mirror) shared_turn(turned + S::kTurned, cc * 32 + j0, lane, lo);
                     }
                 }
             }
@@ -307,10 +356,15 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             if (lane == 0) {
                 mbar_arrive_cluster_relaxed(tempty_leader + 8 * acc);
                 if (row0 < g.M) {
+                    for (int part = 0; part < parts; ++part) {
+                        const int to = z + part * g.batch;
 #pragma unroll
-                    for (int b = 0; b < S::kCols / 64; ++b)
-                        if (nb * BN + first + b * 64 < g.N) tma_store_3d(&map_c, out + b * 4096, nb * BN + first + b * 64, row0, z);
-                    if (TURN && mirror && nb * BN + first < g.N) tma_store_3d(&map_t, turned, row0, nb * BN + first, z);
+                        for (int b = 0; b < S::kCols / 64; ++b)
+                            if (nb * BN + first + b * 64 < g.N)
+                                tma_store_3d(&map_c, out + part * S::kOut + b * 4096, nb * BN + first + b * 64, row0, to);
+                        if (TURN && mirror && nb * BN + first < g.N)
+                            tma_store_3d(&map_t, turned + part * S::kTurned, row0, nb * BN + first, to);
+                    }
                 }
                 bulk_commit();
             }
@@ -330,26 +384,26 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 // A = X X^T of few tiles over a long reduction: S pairs of SMs, one cluster, share a 256 x 128 tile.  Each sums its part of K in
 // its own tensor memory; then pair s gets columns [s, s + 1) * 128 / S of the others' sums through distributed shared
 // memory, adds them in a fixed order and stores those columns.
-template <int S> struct SplitShape {
+template <int S, bool PAIR> struct SplitShape {
     static constexpr int kE = 128 / S;                          // columns that a pair finishes
     static constexpr int kU = kE < 32 ? kE : 32;                // of them, an epilogue warp's
-    static constexpr int kStageBytes = kABytes + 64 * kBK * 2, kStages = 5;
+    static constexpr int kStageBytes = kABytes + 64 * kBK * 2, kStages = PAIR ? 4 : 5, kParts = PAIR ? 2 : 1;
     static constexpr int kSums = (S - 1) * 128 * kE * 4;        // the others' sums of its columns
     static constexpr int kOut = 32 * kU * 2;                    // a warp's 32 rows, and once more transposed
-    static constexpr int kSmem = kStages * kStageBytes + kSums + kEpilogueWarps * 2 * kOut + 1024 + 1024;
+    static constexpr int kSmem = kStages * kStageBytes + kSums + kEpilogueWarps * kParts * 2 * kOut + 1024 + 1024;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-template <int S>
+template <int S, bool PAIR>
 __global__ void __launch_bounds__(kNsThreads, 1)
 ns_gram_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                      const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_t, const NsArgs g) {
-    using P = SplitShape<S>;
+    using P = SplitShape<S, PAIR>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sums = smem_u32(smem + P::kStages * P::kStageBytes);     // [S - 1][kE / 4][128 rows] groups of four columns
     uint8_t *staging = smem + P::kStages * P::kStageBytes + P::kSums;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * 2 * P::kOut);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * P::kParts * 2 * P::kOut);
     const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * P::kStages, bar_tfull = bar_empty + 8 * P::kStages;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * P::kStages + 1);
 
@@ -359,7 +413,7 @@ ns_gram_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const uint16_t both = (uint16_t)(3u << (2 * s));
     int z, mb, nb;
     ns_unit<128>(g, blockIdx.x / (2 * S), &z, &mb, &nb);
-    const int nkb = (g.K + kBK - 1) / kBK, kb0 = nkb * s / S, kb1 = nkb * (s + 1) / S;
+    const int blocks = (g.K + kBK - 1) / kBK, nkb = PAIR ? 3 * blocks : blocks, kb0 = nkb * s / S, kb1 = nkb * (s + 1) / S;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < P::kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
@@ -389,8 +443,10 @@ ns_gram_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 if (!mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1)) { atomicExch(g.err, 31); break; }
                 const uint32_t full = bar_full + 8 * stage, sa = smem_u32(smem + stage * P::kStageBytes);
                 if (side == 0) mbar_arrive_expect_tx(full, 2 * P::kStageBytes);
-                tma_load_3d_pair(sa, &map_a, full, kb * kBK, mb * 256 + (int)side * 128, z);
-                tma_load_3d_pair(sa + kABytes, &map_b, full, kb * kBK, nb * 128 + (int)side * 64, z);
+                int za = z, zb = z;
+                const int k0 = (PAIR ? pair_block(kb, blocks, g.batch, &za, &zb) : kb) * kBK;
+                tma_load_3d_pair(sa, &map_a, full, k0, mb * 256 + (int)side * 128, za);
+                tma_load_3d_pair(sa + kABytes, &map_b, full, k0, nb * 128 + (int)side * 64, zb);
                 if (++stage == P::kStages) { stage = 0; phase ^= 1; }
             }
         }
@@ -439,7 +495,7 @@ ns_gram_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     if (warp >= 2 && half * P::kU < P::kE) {
         const int c0 = s * P::kE + half * P::kU, col0 = nb * 128 + c0, row0 = mb * 256 + (int)side * 128 + q * 32;
         const bool mirror = mb < nb / 2;
-        const uint32_t out = smem_u32(staging + (half * 4 + q) * 2 * P::kOut), turned = out + P::kOut;
+        const uint32_t out = smem_u32(staging + (half * 4 + q) * P::kParts * 2 * P::kOut), turned = out + P::kParts * P::kOut;
         uint32_t r[32];
         tmem_ld32(tmem_rows + c0, r);
         tmem_ld_wait();
@@ -459,19 +515,24 @@ ns_gram_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     v[j + 3] += __uint_as_float(w.w);
                 }
             times(v, g.by);
-            store_halves(out + lane * (P::kU * 2) + j0 * 2, v);
-            if (mirror) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(turned + (j0 + j) * 64 + lane * 2),
-                                 "h"(__half_as_ushort(__float2half_rn(v[j]))) : "memory");
+            uint32_t w[4];
+            pack_halves(w, v);
+            shared_store(out + lane * (P::kU * 2) + j0 * 2, w);
+            if (mirror) shared_turn(turned, j0, lane, w);
+            if (PAIR) {
+                uint32_t lo[4];
+                pack_rest(lo, w, v);
+                shared_store(out + P::kOut + lane * (P::kU * 2) + j0 * 2, lo);
+                if (mirror) shared_turn(turned + P::kOut, j0, lane, lo);
             }
         }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0 && row0 < g.M && col0 < g.N) {
-            tma_store_3d(&map_c, out, col0, row0, z);
-            if (mirror) tma_store_3d(&map_t, turned, row0, col0, z);
+            for (int part = 0; part < P::kParts; ++part) {
+                tma_store_3d(&map_c, out + part * P::kOut, col0, row0, z + part * g.batch);
+                if (mirror) tma_store_3d(&map_t, turned + part * P::kOut, row0, col0, z + part * g.batch);
+            }
             bulk_commit();
             bulk_wait_read_all();
         }
@@ -497,7 +558,7 @@ struct NsCluster {
     __half *x0, *x1, *a, *mm;       // rows of ldx, ldm elements
     int64_t ldx, ldm;
     void *out;                      // the last product's, (m, n) or, turned, (n, m), contiguous; NULL: it goes to x like the others
-    int turned, turned_wide, bf16;  // turned_wide: its rows are 16-byte aligned
+    int turned, turned_wide;        // turned_wide: its rows are 16-byte aligned
     float gram_by, out_by;          // 2^-2k, 2^-k
     int *err;
 };
@@ -710,7 +771,7 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
                             uint32_t w[4];
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                if (last && g.bf16) {
+                                if (last) {                     // the result is bf16
                                     const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
                                     w[j] = *reinterpret_cast<const uint32_t *>(&h);
                                 } else {
@@ -865,6 +926,7 @@ struct NsEdge {
     int m, n;                       // the iterate's sizes (m <= n)
     int64_t s_i, s_j, s_b;          // strides of the caller's matrix along the iterate's rows, columns, and batch
     int64_t ldx, x_batch;           // the iterate's row pitch and matrix pitch
+    int64_t x_lo;                   // pairs: from an upper part to its lower part; 0: there are none
     int64_t lines, len, pitch;      // the source as lines along its contiguous direction
     bool wide;                      // lines are 16-byte aligned
     double eps;
@@ -972,10 +1034,15 @@ template <typename T> __global__ void __launch_bounds__(256) ns_first_rows_kerne
         const int64_t i = u / per, j = (u - i * per) * 8;
         float v[8];
         load_line<T, 8>(v, g + i * e.s_i, j, e.n, e.wide);
-        Pack<__half, 8> h;
+        Pack<__half, 8> h, lo;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) h.v[k] = __float2half_rn(scale(v[k]));
+        for (int k = 0; k < 8; ++k) {
+            const float t = scale(v[k]);
+            h.v[k] = __float2half_rn(t);
+            lo.v[k] = __float2half_rn(t - __half2float(h.v[k]));
+        }
         *reinterpret_cast<Pack<__half, 8> *>(x + i * e.ldx + j) = h;
+        if (e.x_lo) *reinterpret_cast<Pack<__half, 8> *>(x + e.x_lo + i * e.ldx + j) = lo;
     }
 }
 
@@ -1001,8 +1068,12 @@ template <typename T> __global__ void __launch_bounds__(256) ns_first_turned_ker
 #pragma unroll
     for (int k = 0; k < 64; k += 8) {
         const int64_t i = i0 + ty + k, j = j0 + 2 * tx;
-        if (i < e.m && j < e.ldx)           // ldx is a multiple of 8
-            *reinterpret_cast<__half2 *>(x + i * e.ldx + j) = __floats2half2_rn(tile[2 * tx][ty + k], tile[2 * tx + 1][ty + k]);
+        if (i < e.m && j < e.ldx) {         // ldx is a multiple of 8
+            const float a = tile[2 * tx][ty + k], b = tile[2 * tx + 1][ty + k];
+            const __half2 h = __floats2half2_rn(a, b);
+            *reinterpret_cast<__half2 *>(x + i * e.ldx + j) = h;
+            if (e.x_lo) *reinterpret_cast<__half2 *>(x + e.x_lo + i * e.ldx + j) = __floats2half2_rn(a - __low2float(h), b - __high2float(h));
+        }
     }
 }
 
@@ -1017,7 +1088,12 @@ template <typename T> __global__ void __launch_bounds__(256) ns_last_kernel(cons
 #pragma unroll
     for (int k = 0; k < 32; k += 8) {
         const int i = i0 + ty + k, j = j0 + tx;
-        const float v = (i < e.m && j < e.n) ? __half2float(x[i * e.ldx + j]) * e.down : 0.0f;
+        float v = 0.0f;
+        if (i < e.m && j < e.n) {
+            v = __half2float(x[i * e.ldx + j]);
+            if (e.x_lo) v += __half2float(x[e.x_lo + i * e.ldx + j]);
+            v *= e.down;
+        }
         if (across) tile[ty + k][tx] = v;
         else if (i < e.m && j < e.n) out[i * e.s_i + j] = Cvt<T>::from_f(v);
     }
@@ -1042,16 +1118,6 @@ constexpr int kTileBytes = 128 * 64 * 2;
 __device__ __forceinline__ uint32_t tile_at(int row, int col) {     // byte offset of 8 columns' group in the tiles
     return (uint32_t)(col >> 6) * kTileBytes + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4);
 }
-// 2^-k times two halves in the result's type: one rounding, since bf16 has room for the factor and fp16 rounds where it has not.
-__device__ __forceinline__ void put_down(uint32_t &to, __half2 h, float down, __half) {
-    const __half2 v = __hmul2(h, __float2half2_rn(down));
-    to = *reinterpret_cast<const uint32_t *>(&v);
-}
-__device__ __forceinline__ void put_down(uint32_t &to, __half2 h, float down, __nv_bfloat16) {
-    const float2 f = __half22float2(h);
-    const __nv_bfloat162 v = __hmul2(__floats2bfloat162_rn(f.x, f.y), __float2bfloat162_rn(down));
-    to = *reinterpret_cast<const uint32_t *>(&v);
-}
 struct NsSmall {
     NsEdge e;                       // source and sizes; dst is the result
     int64_t o_i, o_j, o_b;          // strides of the result along the iterate's rows, columns, and batch
@@ -1061,7 +1127,7 @@ struct NsSmall {
     int *err;
 };
 
-template <typename T, typename TO>
+template <typename T>
 __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmall a) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ double sums[kSmallThreads / 32];
@@ -1262,8 +1328,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
         settle();
     }
     __syncthreads();
+    using TO = __nv_bfloat16;
     TO *out = static_cast<TO *>(e.dst) + blockIdx.x * a.o_b;
     if (a.o_j == 1) {
+        const __nv_bfloat162 down = __float2bfloat162_rn(e.down);       // exact behind the rounding, too
 #pragma unroll 4
         for (int i = first_row, c = first_col; i < e.m;) {
             const int j = c * 8;
@@ -1271,7 +1339,12 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
             const __half2 *h = reinterpret_cast<const __half2 *>(&w);
             Pack<TO, 8> o;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) put_down(reinterpret_cast<uint32_t *>(&o)[k], h[k], e.down, TO());
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = __half22float2(h[k]);
+                const __nv_bfloat162 b = __hmul2(__floats2bfloat162_rn(f.x, f.y), down);
+                o.v[2 * k] = __low2bfloat16(b);
+                o.v[2 * k + 1] = __high2bfloat16(b);
+            }
             TO *p = out + i * a.o_i + j;
             if (a.out_wide && j + 8 <= e.n) *reinterpret_cast<Pack<TO, 8> *>(p) = o;
             else
@@ -1302,18 +1375,20 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
 // ---- host side ------------------------------------------------------------------------------------------------------
 struct NsPlan {
     int64_t m, n, batch, ldx, ldm;
+    int parts;                                // of an iterate, A and M: 2 for pairs
     size_t part_bytes, x_bytes, a_bytes;      // each rounded to 256
     size_t total() const { return part_bytes + 2 * x_bytes + 2 * a_bytes; }
 };
 
-NsPlan ns_plan(int64_t batch, int64_t rows, int64_t cols) {
+NsPlan ns_plan(int64_t batch, int64_t rows, int64_t cols, bool pairs) {
     auto round = [](size_t v) { return (v + 255) / 256 * 256; };
     NsPlan p;
     p.m = std::min(rows, cols); p.n = std::max(rows, cols); p.batch = batch;
     p.ldx = (p.n + 7) / 8 * 8; p.ldm = (p.m + 7) / 8 * 8;
     p.part_bytes = round((size_t)batch * kMaxParts * sizeof(double));
-    p.x_bytes = round((size_t)batch * p.m * p.ldx * 2);
-    p.a_bytes = round((size_t)batch * p.m * p.ldm * 2);
+    p.parts = pairs ? 2 : 1;
+    p.x_bytes = round((size_t)p.parts * batch * p.m * p.ldx * 2);
+    p.a_bytes = round((size_t)p.parts * batch * p.m * p.ldm * 2);
     return p;
 }
 
@@ -1363,14 +1438,15 @@ int ns_maps(NsMaps *m, const void *base, int64_t inner, int64_t rows, int64_t ba
     return rc;
 }
 
-template <int BN, bool AMN, bool BMN, int MODE>
+template <int BN, bool AMN, bool BMN, int MODE, bool PAIR>
 int ns_product(const NsMaps &a, const NsMaps &b, const NsMaps &out, const NsMaps &d, NsArgs g, int sms, cudaStream_t st) {
-    auto kernel = ns_product_kernel<BN, AMN, BMN, MODE>;
+    using S = NsShape<BN, !AMN && !BMN, PAIR>;
+    auto kernel = ns_product_kernel<BN, AMN, BMN, MODE, PAIR>;
     static bool attr_set[64] = {false};
     int dev = 0;
     SRUB_CUDA_CHECK(cudaGetDevice(&dev));
     if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-        SRUB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NsShape<BN, !AMN && !BMN>::kSmem));
+        SRUB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
         attr_set[dev] = true;
     }
     g.tiles_m = (g.M + 255) / 256;
@@ -1384,7 +1460,7 @@ int ns_product(const NsMaps &a, const NsMaps &b, const NsMaps &out, const NsMaps
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(2u * (unsigned)std::min<int64_t>(per * g.batch, sms / 2), 1, 1);
     cfg.blockDim = dim3(kNsThreads, 1, 1);
-    cfg.dynamicSmemBytes = NsShape<BN, !AMN && !BMN>::kSmem;
+    cfg.dynamicSmemBytes = S::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1397,9 +1473,9 @@ int ns_product(const NsMaps &a, const NsMaps &b, const NsMaps &out, const NsMaps
 }
 
 // The same product split over the reduction: see choose_split.
-template <int S> int ns_gram_split(const NsMaps &a, const void *out, int64_t ldm, NsArgs g, cudaStream_t st) {
-    using P = SplitShape<S>;
-    auto kernel = ns_gram_split_kernel<S>;
+template <int S, bool PAIR> int ns_gram_split(const NsMaps &a, const void *out, int64_t ldm, NsArgs g, cudaStream_t st) {
+    using P = SplitShape<S, PAIR>;
+    auto kernel = ns_gram_split_kernel<S, PAIR>;
     static bool attr_set[64] = {false};
     int dev = 0;
     SRUB_CUDA_CHECK(cudaGetDevice(&dev));
@@ -1409,8 +1485,8 @@ template <int S> int ns_gram_split(const NsMaps &a, const void *out, int64_t ldm
         attr_set[dev] = true;
     }
     CUtensorMap c, t;
-    int rc = ns_map(&c, out, g.M, g.M, g.batch, ldm, 32, P::kU);
-    if (!rc) rc = ns_map(&t, out, g.M, g.M, g.batch, ldm, P::kU, 32);
+    int rc = ns_map(&c, out, g.M, g.M, P::kParts * g.batch, ldm, 32, P::kU);
+    if (!rc) rc = ns_map(&t, out, g.M, g.M, P::kParts * g.batch, ldm, P::kU, 32);
     if (rc) return rc;
     g.tiles_m = (g.M + 255) / 256;
     g.tiles_n = (g.M + 127) / 128;
@@ -1498,10 +1574,30 @@ int choose_cluster(int64_t m, int64_t n, int64_t batch, int sms) {
 // operands keep shared memory just as busy), but has the shorter epilogue and room for twice the stages.  It is taken where
 // the tiles all find a pair of their own, and for small matrices.  Five steps with 128 / 256 columns: 4096 x 4096 1268 / 1120
 // us, four 2048 x 2048 745 / 660, six 1024 x 2048 378 / 310, but twelve 700 x 1400 322 / 330.
-template <int MODE> int ns_gram(const NsMaps &a, const NsMaps &out, const NsMaps &d, const NsArgs &g, int sms, cudaStream_t st) {
+// Pairs have no room to stage the wider tile's parts and their mirror images.
+template <int MODE, bool PAIR> int ns_gram(const NsMaps &a, const NsMaps &out, const NsMaps &d, const NsArgs &g, int sms, cudaStream_t st) {
     const int64_t rows = (g.M + 255) / 256, narrow = rows * ((g.M + 127) / 128) - rows * (rows - 1);
-    if (narrow * g.batch <= sms / 2 || g.M < 1024) return ns_product<128, false, false, MODE>(a, a, out, d, g, sms, st);
-    return ns_product<256, false, false, MODE>(a, a, out, d, g, sms, st);
+    if (PAIR || narrow * g.batch <= sms / 2 || g.M < 1024) return ns_product<128, false, false, MODE, PAIR>(a, a, out, d, g, sms, st);
+    if constexpr (!PAIR) return ns_product<256, false, false, MODE, PAIR>(a, a, out, d, g, sms, st);
+    return 0;
+}
+
+// One step by a launch per product: X -> next, the last of all to the caller's matrix if `to` is not null.
+template <bool PAIR>
+int ns_step(const NsMaps &x, const NsMaps &next, const NsMaps &am, const NsMaps &mm, const NsMaps *to, const void *a_buf, const NsPlan &p,
+            NsArgs g, float gram_by, float down, bool tall, int sms, cudaStream_t st) {
+    g.M = (int)p.m; g.N = (int)p.m; g.K = (int)p.n; g.symmetric = 1; g.by = gram_by;
+    const int64_t tiles = ((p.m + 255) / 256) * ((p.m + 127) / 128 - (p.m + 255) / 256 + 1) * p.batch;
+    const int split = choose_split(tiles, (PAIR ? 3 : 1) * ((p.n + kBK - 1) / kBK));
+    int rc = split == 8 ? ns_gram_split<8, PAIR>(x, a_buf, p.ldm, g, st) : split == 4 ? ns_gram_split<4, PAIR>(x, a_buf, p.ldm, g, st)
+             : split == 2 ? ns_gram_split<2, PAIR>(x, a_buf, p.ldm, g, st) : ns_gram<kPlain, PAIR>(x, am, am, g, sms, st);
+    g.K = (int)p.m;
+    if (!rc) rc = ns_gram<kCombine, PAIR>(am, mm, am, g, sms, st);
+    if (rc) return rc;
+    g.N = (int)p.n; g.symmetric = 0; g.last = to != nullptr; g.by = to ? down : 1.0f;
+    if (!to || !tall) return ns_product<256, false, true, kPlain, PAIR>(mm, x, to ? *to : next, am, g, sms, st);
+    g.M = (int)p.n; g.N = (int)p.m;         // X^T = X_before^T M, rows as the caller has them
+    return ns_product<128, true, false, kPlain, PAIR>(x, mm, *to, am, g, sms, st);
 }
 
 int launch_early(dim3 grid, void (*kernel)(NsEdge), const NsEdge &e, cudaStream_t st) {
@@ -1514,8 +1610,8 @@ int launch_early(dim3 grid, void (*kernel)(NsEdge), const NsEdge &e, cudaStream_
     return 0;
 }
 
-template <typename T, typename TO> int ns_small(const NsSmall &a, int64_t batch, cudaStream_t st) {
-    auto kernel = ns_small_kernel<T, TO>;
+template <typename T> int ns_small(const NsSmall &a, int64_t batch, cudaStream_t st) {
+    auto kernel = ns_small_kernel<T>;
     const int bytes = (2 + (a.e.n + 63) / 64) * kTileBytes + 1024;
     static bool attr_set[64] = {false};
     int dev = 0;
@@ -1537,9 +1633,13 @@ using namespace srub;
 
 extern "C" {
 
-size_t sru_b200_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols) {
+size_t sru_b200_orthogonalize_workspace_bytes_for(int64_t batch, int64_t rows, int64_t cols, int out_dtype) {
     if (batch < 1 || rows < 1 || cols < 1) return 0;
-    return ns_plan(batch, rows, cols).total();
+    return ns_plan(batch, rows, cols, out_dtype != SRU_BF16).total();
+}
+
+size_t sru_b200_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols) {
+    return sru_b200_orthogonalize_workspace_bytes_for(batch, rows, cols, SRU_F16);
 }
 
 int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t rows, int64_t cols, int64_t stride_batch,
@@ -1556,7 +1656,8 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     if (batch == 0 || rows == 0 || cols == 0) return 0;
     if (!out || !grad) return set_error(SRU_ERR_BAD_ARG, "orthogonalize: a required pointer is null");
     if (stride_col != 1 && stride_row != 1) return set_error(SRU_ERR_BAD_ARG, "orthogonalize: rows or columns must be contiguous");
-    const NsPlan p = ns_plan(batch, rows, cols);
+    const bool pairs = out_dtype == SRU_F16;
+    const NsPlan p = ns_plan(batch, rows, cols, pairs);
     if (!workspace || workspace_bytes < p.total() || reinterpret_cast<uintptr_t>(workspace) % 256)
         return set_error(SRU_ERR_WORKSPACE, "256-byte aligned workspace of %zu bytes needed, %zu given", p.total(), workspace_bytes);
     if (int rc = ensure_context()) return rc;
@@ -1579,7 +1680,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     e.src = grad; e.dst = x[0]; e.part = part;
     e.m = (int)p.m; e.n = (int)p.n;
     e.s_i = tall ? stride_col : stride_row; e.s_j = tall ? stride_row : stride_col; e.s_b = stride_batch;
-    e.ldx = p.ldx; e.x_batch = p.m * p.ldx; e.eps = eps;
+    e.ldx = p.ldx; e.x_batch = p.m * p.ldx; e.x_lo = pairs ? batch * p.m * p.ldx : 0; e.eps = eps;
     const int k = iterate_exponent(steps, ca, cb, cc);
     e.up = std::ldexp(1.0f, k); e.down = std::ldexp(1.0f, -k);
     const float gram_by = e.down * e.down;
@@ -1591,16 +1692,15 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     const int unit = e.lines * ((e.len + 2047) / 2048) * batch < sms * 8 ? 512 : 2048;
     e.parts = (int)std::min<int64_t>((e.lines * ((e.len + unit - 1) / unit) + 7) / 8, kMaxParts);
     const dim3 norm_grid((unsigned)e.parts, (unsigned)batch);
-    if (p.m <= kSmallM && p.n <= kSmallN) {
+    if (!pairs && p.m <= kSmallM && p.n <= kSmallN) {
         NsSmall a;
         memset(&a, 0, sizeof(a));
         a.e = e; a.e.dst = out;
         a.o_i = tall ? 1 : cols; a.o_j = tall ? cols : 1; a.o_b = rows * cols;
         a.steps = steps; a.ca = (float)ca; a.cb = (float)cb; a.cc = (float)cc; a.gram_by = gram_by; a.err = err;
         a.out_wide = cols % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-        auto go = [&](auto t, auto to) { return ns_small<decltype(t), decltype(to)>(a, batch, st); };
-        auto go_out = [&](auto t) { return out_dtype == SRU_F16 ? go(t, __half()) : go(t, __nv_bfloat16()); };
-        return grad_dtype == SRU_F32 ? go_out(float()) : grad_dtype == SRU_F16 ? go_out(__half()) : go_out(__nv_bfloat16());
+        return grad_dtype == SRU_F32 ? ns_small<float>(a, batch, st) : grad_dtype == SRU_F16 ? ns_small<__half>(a, batch, st)
+                                                                                          : ns_small<__nv_bfloat16>(a, batch, st);
     }
     auto begin = [&](auto t) -> int {
         using T = decltype(t);
@@ -1618,15 +1718,15 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     if (int rc = grad_dtype == SRU_F32 ? begin(float()) : grad_dtype == SRU_F16 ? begin(__half()) : begin(__nv_bfloat16())) return rc;
 
     // The last product writes the caller's matrix itself where its rows are 16-byte aligned (a cluster's turned one, always).
-    const int ctas = steps > 0 ? choose_cluster(p.m, p.n, batch, sms) : 0;
+    const int ctas = steps > 0 && !pairs ? choose_cluster(p.m, p.n, batch, sms) : 0;
     const bool aligned = steps > 0 && cols % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0, direct = aligned || (ctas && tall);
     NsMaps xm[2], am, mm, om;
     if (aligned)
         if (int rc = ns_maps(&om, out, cols, rows, batch, cols)) return rc;
     if (steps > 0) {
-        int rc = ns_maps(&am, a_buf, p.m, p.m, batch, p.ldm);
-        if (!rc) rc = ns_maps(&mm, m_buf, p.m, p.m, batch, p.ldm);
-        for (int i = 0; i < 2 && !rc; ++i) rc = ns_maps(&xm[i], x[i], p.n, p.m, batch, p.ldx);
+        int rc = ns_maps(&am, a_buf, p.m, p.m, p.parts * batch, p.ldm);
+        if (!rc) rc = ns_maps(&mm, m_buf, p.m, p.m, p.parts * batch, p.ldm);
+        for (int i = 0; i < 2 && !rc; ++i) rc = ns_maps(&xm[i], x[i], p.n, p.m, p.parts * batch, p.ldx);
         if (rc) return rc;
     }
     if (ctas) {
@@ -1635,7 +1735,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         g.m = (int)p.m; g.n = (int)p.n; g.steps = steps;
         g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc;
         g.x0 = x[0]; g.x1 = x[1]; g.a = a_buf; g.mm = m_buf; g.ldx = p.ldx; g.ldm = p.ldm;
-        g.out = direct ? out : nullptr; g.turned = tall; g.turned_wide = aligned; g.bf16 = out_dtype == SRU_BF16; g.err = err;
+        g.out = direct ? out : nullptr; g.turned = tall; g.turned_wide = aligned; g.err = err;
         g.gram_by = gram_by; g.out_by = e.down;
         if (int rc = ns_cluster(xm[0], xm[1], am, mm, g, batch, ctas, st)) return rc;
     }
@@ -1644,25 +1744,11 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         NsArgs g;
         memset(&g, 0, sizeof(g));
         g.batch = (int)batch; g.err = err;
-        g.M = (int)p.m; g.N = (int)p.m; g.K = (int)p.n; g.symmetric = 1;
-        g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc; g.by = gram_by;
-        const int64_t tiles = ((p.m + 255) / 256) * ((p.m + 127) / 128 - (p.m + 255) / 256 + 1) * batch;
-        const int split = choose_split(tiles, (p.n + kBK - 1) / kBK);
-        int rc = split == 8 ? ns_gram_split<8>(xm[cur], a_buf, p.ldm, g, st) : split == 4 ? ns_gram_split<4>(xm[cur], a_buf, p.ldm, g, st)
-                 : split == 2 ? ns_gram_split<2>(xm[cur], a_buf, p.ldm, g, st) : ns_gram<kPlain>(xm[cur], am, am, g, sms, st);
+        g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc;
+        const NsMaps *to = s == steps - 1 && direct ? &om : nullptr;
+        const int rc = pairs ? ns_step<true>(xm[cur], xm[cur ^ 1], am, mm, to, a_buf, p, g, gram_by, e.down, tall, sms, st)
+                             : ns_step<false>(xm[cur], xm[cur ^ 1], am, mm, to, a_buf, p, g, gram_by, e.down, tall, sms, st);
         if (rc) return rc;
-        g.K = (int)p.m;
-        if (int rc = ns_gram<kCombine>(am, mm, am, g, sms, st)) return rc;
-        g.N = (int)p.n; g.symmetric = 0;
-        const bool last = s == steps - 1 && direct;
-        g.bf16 = last && out_dtype == SRU_BF16;
-        g.by = last ? e.down : 1.0f;
-        if (last && tall) {             // X^T = X_before^T M, rows as the caller has them
-            g.M = (int)p.n; g.N = (int)p.m;
-            if (int rc = ns_product<128, true, false, kPlain>(xm[cur], mm, om, am, g, sms, st)) return rc;
-        } else if (int rc = ns_product<256, false, true, kPlain>(mm, xm[cur], last ? om : xm[cur ^ 1], am, g, sms, st)) {
-            return rc;
-        }
     }
     if (direct) return 0;
     const dim3 tile_grid((unsigned)((p.ldx + 31) / 32), (unsigned)((p.m + 31) / 32), (unsigned)batch);

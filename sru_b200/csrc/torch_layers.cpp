@@ -252,7 +252,7 @@ Tensor orthogonalize(const Tensor &grad, int64_t steps, double a, double b, doub
     Tensor g = grad.detach();
     if (g.numel() > 0 && g.stride(-1) != 1 && g.stride(-2) != 1) g = g.contiguous();
     const int64_t batch = g.dim() == 3 ? g.size(0) : 1, rows = g.size(-2), cols = g.size(-1);
-    const size_t bytes = sru_b200_orthogonalize_workspace_bytes(batch, rows, cols);
+    const size_t bytes = sru_b200_orthogonalize_workspace_bytes_for(batch, rows, cols, code_of(out_dtype));
     Tensor ws = at::empty({(int64_t)bytes}, g.options().dtype(at::kByte));
     check(sru_b200_orthogonalize(out.data_ptr(), g.data_ptr(), batch, rows, cols, g.dim() == 3 ? g.stride(0) : 0, g.stride(-2),
                                  g.stride(-1), (int)std::min<int64_t>(std::max<int64_t>(steps, -1), 1 << 30), a, b, c, eps, code,

@@ -24,13 +24,14 @@ def orthogonalize(grad: Tensor, steps: int = 5, coefficients: Tuple[float, float
     give identical bits.  Matrices whose rows or columns are contiguous are read in place.  No derivative flows
     through it, in either mode: the result is a constant to autograd.
 
-    Accuracy.  The norm is summed in 64 bits and products in float32, but the iterates are held to eleven bits (fp16, scaled
-    clear of its subnormals); there is no float32 form.  How far the result is off exact steps depends on grad, because the steps
-    multiply its smallest singular values, and the rounding of its largest elements with them, by up to a^steps (485).  In the
-    Frobenius norm, relative, before the rounding to ``out_dtype``, with the default steps and coefficients: below 2.5e-3 for
-    gradients that are mostly noise (with sixteen strong directions as well), 6e-3 for singular values that fall off as 1 / i,
-    3e-2 as 1 / i^2, 6e-2 for four strong directions over noise of a hundredth of their size.  Storing such a grad as
-    bfloat16 costs at least four times as much in the last three cases.
+    Accuracy (relative, Frobenius, default steps and coefficients).  The norm is summed in 64 bits and products in float32;
+    the iterates have the bits that the result needs.  For a float16 result they are pairs of fp16 (22 bits): the result
+    is the exact steps rounded once, 2.1e-4 off, 3e-4 at most, at 1.5 to 4 times the time of a bfloat16 one.  For a bfloat16
+    result they have eleven bits (fp16, scaled clear of its subnormals), and what that costs depends on grad, because the steps
+    multiply its smallest singular values, and the rounding of its largest elements with them, by up to a^steps (485): before the
+    rounding to bfloat16 (1.7e-3) below 2.5e-3 for gradients that are mostly noise (with sixteen strong directions as well), 6e-3 for
+    singular values that fall off as 1 / i, 3e-2 as 1 / i^2, 6e-2 for four strong directions over noise of a hundredth of their
+    size (7e-4 as float16).  Storing such a grad as bfloat16 costs at least four times as much in the last three cases.
     """
     if len(coefficients) != 3:
         raise _lib.SruB200Error("coefficients must be (a, b, c), got %r" % (coefficients,))

@@ -18,11 +18,11 @@ def test_form(batch, rows, cols, cluster):
     g = torch.randn(batch, rows, cols, generator=torch.Generator().manual_seed(rows + cols))
     dev = g.to(DEV)
     before = _lib.launch_count
-    got = orthogonalize(dev, out_dtype=torch.float16)
+    got = orthogonalize(dev)
     n = _lib.launch_count - before
     assert n <= 4 if cluster else n >= 17
     before = _lib.launch_count
-    turned = orthogonalize(dev.mT.contiguous(), out_dtype=torch.float16)
+    turned = orthogonalize(dev.mT.contiguous())
     assert (_lib.launch_count - before <= 4) == cluster         # the rule looks at the smaller and the larger side
     _lib.check_device_error()
     x = g[batch - 1].double()
@@ -31,6 +31,7 @@ def test_form(batch, rows, cols, cluster):
     for _ in range(5):
         a = x @ x.mT
         x = (3.4445 * eye - 4.7750 * a + 2.0315 * (a @ a)) @ x
+    rounding = float((x.bfloat16().double() - x).norm())
     for out in (got[batch - 1].cpu().double(), turned[batch - 1].cpu().double().mT):
-        # the documented 2.5e-3 for gradients that are mostly noise, and half a step of fp16
-        assert float((out - x).norm()) <= (2.5e-3 + 2.0 ** -11) * float(x.norm())
+        # the documented 2.5e-3 for gradients that are mostly noise, and what rounding the exact result does
+        assert float((out - x).norm()) <= 2.5e-3 * float(x.norm()) + rounding

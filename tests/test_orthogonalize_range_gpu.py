@@ -55,15 +55,17 @@ def steps64(g, rounded, abc=(3.4445, -4.7750, 2.0315), steps=5):
 @pytest.mark.parametrize("rows,cols", [(128, 384), (384, 128), (256, 1024), (500, 500), (900, 700), (64, 4200), (1024, 1536)])
 @pytest.mark.parametrize("large", [1e4, 1e5])
 def test_one_row_far_above_the_others(rows, cols, large):
-    """The elements of the other rows lie where fp16 is subnormal and has a few bits left; 2^12 X keeps all eleven.  Allowed: 1.5
-    times what the roundings do to 64-bit steps without a range (0.8e-3 to 2.2e-3 of the norm), and half a step of fp16."""
+    """The elements of the other rows lie where fp16 is subnormal and has a few bits left; 2^12 X keeps all eleven.  bfloat16 result:
+    1.5 times what the roundings do to 64-bit steps without a range (0.8e-3 to 2.2e-3 of the norm), and what rounding the exact
+    result does.  float16 result: half as much again as rounding the exact result."""
     g = torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows + cols))
     g[3] *= large
     want, model = steps64(g, False), steps64(g, True)
-    norm = float(want.norm())
+    assert float((model - want).norm()) <= 2.3e-3 * float(want.norm())
+    got = orthogonalize(g.to(DEV)).cpu().double()
+    assert float((got - want).norm()) <= 1.5 * float((model - want).norm()) + float((want.bfloat16().double() - want).norm())
     got = orthogonalize(g.to(DEV), out_dtype=F16).cpu().double()
-    assert float((got - want).norm()) <= 1.5 * float((model - want).norm()) + 2.0 ** -11 * norm
-    assert float((model - want).norm()) <= 2.3e-3 * norm
+    assert float((got - want).norm()) <= 1.5 * float((want.half().double() - want).norm())
 
 
 @pytest.mark.parametrize("rows,cols", SHAPES)
@@ -71,13 +73,15 @@ def test_one_row_far_above_the_others(rows, cols, large):
 def test_coefficients_that_let_the_iterates_grow(rows, cols, a):
     """X <- a X three times: |a|^3 X_0 whatever power of two is held (9, 11, 5 and 3 of the usual 12).  X_0, each of
     three steps and the result round to eleven bits (relative 2^-11; where fp16 is subnormal, half of its smallest step, which
-    later steps multiply), and nothing overflows (A = X X^T is at most 12^4)."""
+    later steps multiply; a bfloat16 result by 2^-8 at the end), and nothing overflows (A = X X^T is at most 12^4).  The bound holds
+    for a float16 result, whose iterates have more bits, too."""
     g = torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows))
-    got = orthogonalize(g.to(DEV), steps=3, coefficients=(a, 0.0, 0.0), out_dtype=F16).cpu().double()
     want = a ** 3 * g.double() / (g.double().norm() + 1e-7)
-    assert got.isfinite().all()
     tiny = 2.0 ** -25 * (abs(a) ** 3 + a ** 2 + abs(a) + 2)
-    assert bool(((got - want).abs() <= 5.05 * 2.0 ** -11 * want.abs() + tiny).all())
+    for out, rounding in ((F16, 0.0), (BF16, 2.0 ** -8)):
+        got = orthogonalize(g.to(DEV), steps=3, coefficients=(a, 0.0, 0.0), out_dtype=out).cpu().double()
+        assert got.isfinite().all()
+        assert bool(((got - want).abs() <= (5.05 * 2.0 ** -11 + rounding * 1.01) * want.abs() + tiny).all())
     _lib.check_device_error()
 
 
