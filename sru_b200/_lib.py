@@ -127,7 +127,7 @@ def call_native(op, name, backward_name, *args):
     like those of ``call``: the forward pass here, the backward pass by hooks on the operator's node of the graph."""
     fn = _native_ops.get(op) or native_op(op)
     try:
-        if (timer is None and not nvtx_ranges) or not args[0].is_cuda:
+        if (timer is None and not nvtx_ranges) or not getattr(args[0], "is_cuda", False):
             return fn(*args)
         with torch.cuda.device(args[0].device):
             out = _watched(name, fn, *args)
