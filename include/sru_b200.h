@@ -392,7 +392,7 @@ int sru_b200_embedding_backward(
  *
  * on the tensor cores, with float32 accumulation.  The iterates have the bits that the result's type needs.
  *   out SRU_BF16 (eight bits): iterates of eleven bits, fp16 scaled by a power of two.  Off the exact steps (relative, Frobenius;
- *     five steps with the usual a, b, c = 3.4445, -4.7750, 2.0315; before the rounding to bf16): below 2.5e-3 for matrices that are
+ *     five steps with the usual a, b, c = 3.4445, -4.7750, 2.0315; before the rounding to bf16): below 2e-3 for matrices that are
  *     mostly noise, 6e-3 for singular values that fall off as 1 / i, 3e-2 as 1 / i^2, 6e-2 for four strong directions over noise
  *     of a hundredth of their size; the steps multiply small singular values, and the roundings beside them, by up to a^steps
  *   out SRU_F16 (eleven bits): pairs of fp16, 22 bits, and three products for each, at 1.5 to 4 times the time.  The exact steps

@@ -13,14 +13,15 @@
 // the start and about 1.2 later, |M| below 10), so fp16's eleven bits are worth more than bf16's range.  But X has small
 // elements (1 / sqrt(mn) at the start, 2.8e-4 at 2048 x 6144, and far less beside a few large rows), and fp16 is subnormal
 // below 6.1e-5: what is held is 2^k X, k = 12 with the usual coefficients (iterate_exponent).  The powers of two come in with
-// the norm and go out where A and the result are rounded, so they cost no rounding.  Off exact steps (64-bit steps with these
-// roundings; with bf16 iterates; 768 x 2304): normal 1.1e-3; 9.0e-3, singular values as 1 / i 4.0e-3; 3.2e-2, as 1 / i^2 2.1e-2;
-// 1.7e-1.  Most of it is X_0's rounding, which the steps multiply by up to a^steps along the smallest singular directions.
+// the norm and go out where A and the result are rounded, so they cost no rounding.  M's diagonal, which is most of M in the
+// last steps, keeps float32's bits as a factor per row (row_factor).  Off exact steps (64-bit steps with these roundings; with bf16
+// iterates; 768 x 2304): normal 0.8e-3; 9.0e-3, singular values as 1 / i 4.0e-3; 3.2e-2, as 1 / i^2 2.1e-2; 1.7e-1.  Most of the latter
+// is X_0's rounding, which the steps multiply by up to a^steps along the smallest singular directions.
 //
 // That is enough for a result in bf16, not for one in fp16, which has as many bits as such iterates.  There X, A and M are pairs of
 // fp16 (PAIR: the value rounded, and the rest rounded), 22 bits; each product is three, lower times lower left out, in one
 // accumulator, and an epilogue stores both parts.  The result is the exact steps rounded once: 2.1e-4 off where eleven bits
-// gave 1.0e-3 (2.1e-4 and 2e-2 for 1 / i^2).  2048 x 6144 1366 us instead of 495, 256 x 1024 145 instead of 87.  Pairs take a launch
+// give 0.8e-3 (2.1e-4 and 2e-2 for 1 / i^2).  2048 x 6144 1366 us instead of 495, 256 x 1024 145 instead of 87.  Pairs take a launch
 // per product: the one-SM and the one-cluster form below have neither the shared memory nor the bits for them.
 //
 // The products run on pairs of SMs (cta_group::2, 256 x BN tiles) in a persistent grid over (matrix, tile).  A product costs
@@ -53,6 +54,8 @@ struct NsArgs {
     float ca, cb, cc;
     float by;                       // a plain product's factor: 2^-2k for A, 2^-k for the result
     int last;                       // it writes the caller's matrix
+    float *fix;                     // row factors of M (batch, fix_pitch): written with M, applied to M X; pairs have none
+    int fix_pitch;
     int *err;
 };
 
@@ -121,6 +124,28 @@ __device__ __forceinline__ void shared_turn(uint32_t turned, int j0, int lane, c
 #pragma unroll
     for (int j = 0; j < 8; ++j)
         asm volatile("st.shared.u16 [%0], %1;" ::"r"(turned + (j0 + j) * 64 + lane * 2), "h"((uint16_t)(w[j >> 1] >> (16 * (j & 1)))) : "memory");
+}
+
+// M = a I + b A + c A A is near a multiple of I in the last steps, so most of what its rounding does is done on the diagonal, where an
+// element's error of up to 2^-11 scales its row of M X.  The ratio of the diagonal element to its rounding is kept in
+// float32 and applied where M X is rounded: 16 x 300 to 24 x 1000 1.5e-3 to 1.8e-3 off exact steps without, 1.2e-3 to 1.4e-3 with it, 768
+// x 2304 1.1e-3 and 0.8e-3; in bf16 results over 200 shapes at most 1.36 times what rounding alone does, 1.7 times without.  It costs
+// nothing in one SM, six 2048 x 512 165.4 -> 168.2 us in clusters, 2048 x 6144 0.4 %.
+__device__ __forceinline__ float row_factor(float v) {
+    const float h = __half2float(__float2half_rn(v));
+    return h == 0.0f || isinf(h) ? 1.0f : __fdividef(v, h);
+}
+
+// Element i mod N of N values, by halves: log2 N selections deep where a chain of N cost a cluster's product 1 us.
+template <int N> __device__ __forceinline__ float pick(const float (&v)[N], int i) {
+    float p[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) p[j] = v[j];
+#pragma unroll
+    for (int w = N / 2; w > 0; w >>= 1)
+#pragma unroll
+        for (int j = 0; j < w; ++j) p[j] = i & w ? p[j + w] : p[j];
+    return p[0];
 }
 
 // Pairs: a product of sums of two is three products, the small ones first, while the accumulator is small and its own
@@ -297,6 +322,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 }
             }
             __syncwarp();
+            const float by = !PAIR && BMN && row < g.M ? g.by * __ldcg(g.fix + (int64_t)z * g.fix_pitch + row) : g.by;
             bool ok = mbar_wait_bounded(bar_tfull + 8 * acc, (it >> 1) & 1);
             if (MODE == kCombine) ok = mbar_wait_bounded(bar_mine, it & 1) && ok;
             if (!ok) { if (lane == 0) atomicExch(g.err, 34); break; }
@@ -309,6 +335,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + first + cc * 32, r);
                 tmem_ld_wait();
                 const uint32_t line = out + (cc >> 1) * 4096 + lane * 128;
+                float diagonal = 1.0f;
 #pragma unroll
                 for (int j0 = 0; j0 < 32; j0 += 8) {
                     const uint32_t at = line + ((((cc & 1) * 4 + j0 / 8) ^ (lane & 7)) << 4);
@@ -327,8 +354,16 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                             if (PAIR) a += (j & 1) ? __high2float(lo2[j >> 1]) : __low2float(lo2[j >> 1]);
                             v[j] = fmaf(g.cc, v[j], fmaf(g.cb, a, row == col0 + j0 + j ? g.ca : 0.0f));
                         }
-                    } else if (g.by != 1.0f) {
+                        // in the block of 32 x 32 on the diagonal
+                        if (!PAIR && col0 == row0) diagonal = lane >> 3 == j0 / 8 ? pick(v, lane) : diagonal;
+                    } else if (!PAIR && AMN) {      // X^T M: M's rows are the result's columns
+                        const float4 *f = reinterpret_cast<const float4 *>(g.fix + (int64_t)z * g.fix_pitch + col0 + j0);
+                        const float4 f0 = __ldcg(f), f1 = __ldcg(f + 1);
                         times(v, g.by);
+                        v[0] *= f0.x; v[1] *= f0.y; v[2] *= f0.z; v[3] *= f0.w;
+                        v[4] *= f1.x; v[5] *= f1.y; v[6] *= f1.z; v[7] *= f1.w;
+                    } else if ((!PAIR && BMN) || g.by != 1.0f) {
+                        times(v, by);
                     }
                     uint32_t w[4];
                     if (MODE == kPlain && !PAIR && g.last) {    // bf16; of pairs the result is fp16, like all before it
@@ -349,6 +384,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                         if (TURN && mirror) shared_turn(turned + S::kTurned, cc * 32 + j0, lane, lo);
                     }
                 }
+                if (MODE == kCombine && !PAIR && col0 == row0 && row < g.M) g.fix[(int64_t)z * g.fix_pitch + row] = row_factor(diagonal);
             }
             tc_fence_before();
             fence_proxy_async();                // the staged values become visible to the copy engine
@@ -560,6 +596,8 @@ struct NsCluster {
     void *out;                      // the last product's, (m, n) or, turned, (n, m), contiguous; NULL: it goes to x like the others
     int turned, turned_wide;        // turned_wide: its rows are 16-byte aligned
     float gram_by, out_by;          // 2^-2k, 2^-k
+    float *fix;                     // row factors of M (batch, fix_pitch)
+    int fix_pitch;
     int *err;
 };
 
@@ -725,6 +763,8 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
                     }
                     __syncwarp();
                 }
+                // written by another CTA of the cluster: past L1, and asked for before the accumulator is ready
+                const float row_by = kind == 2 && row < g.m ? by * __ldcg(g.fix + (int64_t)z * g.fix_pitch + row) : by;
                 bool ok = dead || mbar_wait_bounded(bar_tfull + 8 * acc, (it >> 1) & 1);
                 if (kind == 1) {
                     ok = (dead || mbar_wait_bounded(bar_mine, d_phase)) && ok;
@@ -746,6 +786,16 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster_relaxed(tempty_leader + 8 * acc);
                     }
+                    if (kind == 1 && (row0 & ~63) == first && row < g.m) {      // the diagonal's elements are among these: one per lane
+                        const int at = (row0 & 32) + lane;
+                        uint16_t a;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(a) : "r"(out + lane * 128 + (((at >> 3) ^ (lane & 7)) << 4) + (at & 7) * 2));
+                        float sums[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sums[j] = __uint_as_float(row0 & 32 ? both_r[1][j] : both_r[0][j]);
+                        const float m = fmaf(g.cc, pick(sums, lane), fmaf(g.cb, __half2float(__ushort_as_half(a)), g.ca));
+                        g.fix[(int64_t)z * g.fix_pitch + row] = row_factor(m);
+                    }
 #pragma unroll
                     for (int cc = 0; cc < 2; ++cc) {
                         const int col0 = first + cc * 32;
@@ -766,7 +816,7 @@ ns_cluster_kernel(const __grid_constant__ CUtensorMap map_x0a, const __grid_cons
                                 }
                             } else {
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) v[j] *= by;
+                                for (int j = 0; j < 8; ++j) v[j] *= row_by;
                             }
                             uint32_t w[4];
 #pragma unroll
@@ -1133,6 +1183,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
     __shared__ double sums[kSmallThreads / 32];
     __shared__ uint64_t bars[2];
     __shared__ uint32_t tmem_slot;
+    __shared__ float fix[kSmallM];      // row factors of M
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const NsEdge &e = a.e;
     const int tiles = (e.n + 63) / 64;
@@ -1268,6 +1319,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
         if (!ok) break;
         tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + 128 + part * 32, r);
         tmem_ld_wait();
+        float diagonal = 1.0f;
 #pragma unroll
         for (int j0 = 0; j0 < 32; j0 += 8) {
             const int col = part * 32 + j0;
@@ -1284,9 +1336,11 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
             if (part == q) {                        // the diagonal's block
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] += lane == j0 + j ? a.ca : 0.0f;
+                diagonal = lane >> 3 == j0 / 8 ? pick(v, lane) : diagonal;
             }
             store_halves(at, v);
         }
+        if (part == q) fix[row] = row_factor(diagonal);
         settle();
         // X = M X, 256 columns at a time; a column of the product needs that column of X alone, so it is replaced in place
         auto multiply = [&](int group) {
@@ -1302,6 +1356,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
         };
         multiply(0);
         if (groups > 1) multiply(1);
+        const float row_by = fix[row];
         for (int group = 0; group < groups && ok; ++group) {
             arrive(group & 1);
             if (!ok) break;
@@ -1316,6 +1371,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
                         float v[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[j0 + j]);
+                        times(v, row_by);
                         store_halves(x + tile_at(row, col0 + half + j0), v);
                     }
                 }
@@ -1376,8 +1432,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const NsSmal
 struct NsPlan {
     int64_t m, n, batch, ldx, ldm;
     int parts;                                // of an iterate, A and M: 2 for pairs
-    size_t part_bytes, x_bytes, a_bytes;      // each rounded to 256
-    size_t total() const { return part_bytes + 2 * x_bytes + 2 * a_bytes; }
+    int64_t fix_pitch;                        // whole tiles, so that factors behind the last row can be read
+    size_t part_bytes, x_bytes, a_bytes, fix_bytes;      // each rounded to 256
+    size_t total() const { return part_bytes + 2 * x_bytes + 2 * a_bytes + fix_bytes; }
 };
 
 NsPlan ns_plan(int64_t batch, int64_t rows, int64_t cols, bool pairs) {
@@ -1389,6 +1446,8 @@ NsPlan ns_plan(int64_t batch, int64_t rows, int64_t cols, bool pairs) {
     p.parts = pairs ? 2 : 1;
     p.x_bytes = round((size_t)p.parts * batch * p.m * p.ldx * 2);
     p.a_bytes = round((size_t)p.parts * batch * p.m * p.ldm * 2);
+    p.fix_pitch = (p.m + 255) / 256 * 256;
+    p.fix_bytes = pairs ? 0 : round((size_t)batch * p.fix_pitch * sizeof(float));
     return p;
 }
 
@@ -1673,6 +1732,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
     __half *x[2] = {reinterpret_cast<__half *>(ws + p.part_bytes), reinterpret_cast<__half *>(ws + p.part_bytes + p.x_bytes)};
     __half *a_buf = reinterpret_cast<__half *>(ws + p.part_bytes + 2 * p.x_bytes);
     __half *m_buf = reinterpret_cast<__half *>(ws + p.part_bytes + 2 * p.x_bytes + p.a_bytes);
+    float *fix = reinterpret_cast<float *>(ws + p.part_bytes + 2 * p.x_bytes + 2 * p.a_bytes);
 
     const bool tall = rows > cols;
     NsEdge e;
@@ -1736,7 +1796,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc;
         g.x0 = x[0]; g.x1 = x[1]; g.a = a_buf; g.mm = m_buf; g.ldx = p.ldx; g.ldm = p.ldm;
         g.out = direct ? out : nullptr; g.turned = tall; g.turned_wide = aligned; g.err = err;
-        g.gram_by = gram_by; g.out_by = e.down;
+        g.gram_by = gram_by; g.out_by = e.down; g.fix = fix; g.fix_pitch = (int)p.fix_pitch;
         if (int rc = ns_cluster(xm[0], xm[1], am, mm, g, batch, ctas, st)) return rc;
     }
     for (int s = 0; s < steps && !ctas; ++s) {
@@ -1744,7 +1804,7 @@ int sru_b200_orthogonalize(void *out, const void *grad, int64_t batch, int64_t r
         NsArgs g;
         memset(&g, 0, sizeof(g));
         g.batch = (int)batch; g.err = err;
-        g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc;
+        g.ca = (float)ca; g.cb = (float)cb; g.cc = (float)cc; g.fix = fix; g.fix_pitch = (int)p.fix_pitch;
         const NsMaps *to = s == steps - 1 && direct ? &om : nullptr;
         const int rc = pairs ? ns_step<true>(xm[cur], xm[cur ^ 1], am, mm, to, a_buf, p, g, gram_by, e.down, tall, sms, st)
                              : ns_step<false>(xm[cur], xm[cur ^ 1], am, mm, to, a_buf, p, g, gram_by, e.down, tall, sms, st);

@@ -29,7 +29,7 @@ def orthogonalize(grad: Tensor, steps: int = 5, coefficients: Tuple[float, float
     is the exact steps rounded once, 2.1e-4 off, 3e-4 at most, at 1.5 to 4 times the time of a bfloat16 one.  For a bfloat16
     result they have eleven bits (fp16, scaled clear of its subnormals), and what that costs depends on grad, because the steps
     multiply its smallest singular values, and the rounding of its largest elements with them, by up to a^steps (485): before the
-    rounding to bfloat16 (1.7e-3) below 2.5e-3 for gradients that are mostly noise (with sixteen strong directions as well), 6e-3 for
+    rounding to bfloat16 (1.7e-3) below 2e-3 for gradients that are mostly noise (with sixteen strong directions as well), 6e-3 for
     singular values that fall off as 1 / i, 3e-2 as 1 / i^2, 6e-2 for four strong directions over noise of a hundredth of their
     size (7e-4 as float16).  Storing such a grad as bfloat16 costs at least four times as much in the last three cases.
     """

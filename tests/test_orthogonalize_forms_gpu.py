@@ -33,5 +33,5 @@ def test_form(batch, rows, cols, cluster):
         x = (3.4445 * eye - 4.7750 * a + 2.0315 * (a @ a)) @ x
     rounding = float((x.bfloat16().double() - x).norm())
     for out in (got[batch - 1].cpu().double(), turned[batch - 1].cpu().double().mT):
-        # the documented 2.5e-3 for gradients that are mostly noise, and what rounding the exact result does
-        assert float((out - x).norm()) <= 2.5e-3 * float(x.norm()) + rounding
+        # the documented 2e-3 for gradients that are mostly noise, and what rounding the exact result does
+        assert float((out - x).norm()) <= 2e-3 * float(x.norm()) + rounding
