@@ -396,7 +396,8 @@ int sru_b200_embedding_backward(
  *     mostly noise, 6e-3 for singular values that fall off as 1 / i, 3e-2 as 1 / i^2, 6e-2 for four strong directions over noise
  *     of a hundredth of their size; the steps multiply small singular values, and the roundings beside them, by up to a^steps
  *   out SRU_F16 (eleven bits): pairs of fp16, 22 bits, and three products for each, at 1.5 to 4 times the time.  The exact steps
- *     rounded once: 2.1e-4 (at most 3e-4, and 7e-4 for the four directions)
+ *     rounded once: 2.1e-4 (at most 3e-4, and 7e-4 for the four directions), and 1e-8 more per column of the longer side, for
+ *     the tensor cores' float32 sums
  * Coefficients that let X or X X^T leave fp16's range give infinities or NaN.
  *   grad   `batch` matrices (rows, cols), SRU_F32, SRU_F16 or SRU_BF16, element (z, i, j) at
  *          z * stride_batch + i * stride_row + j * stride_col, one of stride_row, stride_col being 1

@@ -26,7 +26,8 @@ def orthogonalize(grad: Tensor, steps: int = 5, coefficients: Tuple[float, float
 
     Accuracy (relative, Frobenius, default steps and coefficients).  The norm is summed in 64 bits and products in float32;
     the iterates have the bits that the result needs.  For a float16 result they are pairs of fp16 (22 bits): the result
-    is the exact steps rounded once, 2.1e-4 off, 3e-4 at most, at 1.5 to 4 times the time of a bfloat16 one.  For a bfloat16
+    is the exact steps rounded once, 2.1e-4 off, 3e-4 at most (and 1e-8 more per column of the longer side,
+    for the tensor cores' float32 sums), at 1.5 to 4 times the time of a bfloat16 one.  For a bfloat16
     result they have eleven bits (fp16, scaled clear of its subnormals), and what that costs depends on grad, because the steps
     multiply its smallest singular values, and the rounding of its largest elements with them, by up to a^steps (485): before the
     rounding to bfloat16 (1.7e-3) below 2e-3 for gradients that are mostly noise (with sixteen strong directions as well), 6e-3 for

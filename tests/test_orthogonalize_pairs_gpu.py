@@ -145,3 +145,31 @@ def test_no_write_outside_the_outputs(batch, rows, cols, out):
     for k, t in bufs.items():
         assert (t[:256] == 0xA5).all() and (t[256 + sizes[k]:] == 0xA5).all(), k
     assert torch.equal(bufs["out"][256:256 + sizes["out"]].view(out).view(batch, rows, cols), orthogonalize(g, out_dtype=out))
+
+
+def test_offsets_past_32_bits():
+    """A batch whose pairs have more than 2^32 elements, its first and its last matrix; wide, and tall.
+
+    On top of the rounding, float32 sums over n = 60000: the tensor cores add 16 columns at a time and cut the sum off, by 2^-23 of
+    it at most, so that A is off by at most e = n / 16 * 2^-23.  A step takes that to sigma |b sigma^2 + 2 c sigma^4| e, at most 1.2 e for
+    sigma up to 1.2, and later steps, whose slope is about 0.7 around 1, to a third of that again and again: 2.5 e."""
+    torch.manual_seed(1)
+    batch, rows, cols = 300, 130, 60_000
+    g = torch.empty(batch, rows, cols, device=DEV, dtype=BF16).normal_()
+    assert g.numel() > 2 ** 31
+    eye = torch.eye(rows, dtype=torch.float64, device=DEV)
+    for grad in (g, g.view(batch, cols, rows)):
+        got = orthogonalize(grad, out_dtype=F16)
+        for z in (0, batch - 1):
+            x = grad[z].double()
+            x = x.mT if x.size(0) > x.size(1) else x
+            x = x / (x.norm() + 1e-7)
+            for _ in range(5):
+                a = x @ x.T
+                x = (3.4445 * eye - 4.7750 * a + 2.0315 * (a @ a)) @ x
+            own = got[z].double()
+            own = own.mT if own.size(0) > own.size(1) else own
+            # elements near 1 / sqrt(60000): fp16 has its eleven bits there
+            assert float((own - x).norm()) <= 1.5 * float((x.half().double() - x).norm()) + 2.5 * cols / 16 * 2.0 ** -23 * float(x.norm())
+        del got
+    _lib.check_device_error()
