@@ -243,7 +243,8 @@ def call(name, fn, *args):
 
 def _watched(name, fn, *args):
     """fn(*args), in an NVTX range and between a pair of events where those are asked for."""
-    if nvtx_ranges:
+    ranged = nvtx_ranges
+    if ranged:
         torch.cuda.nvtx.range_push(name)
     try:
         if timer is None:
@@ -255,7 +256,7 @@ def _watched(name, fn, *args):
         timer.add(name, start, end)
         return out
     finally:
-        if nvtx_ranges:
+        if ranged:
             torch.cuda.nvtx.range_pop()
 
 
